@@ -835,6 +835,41 @@ int pgk_seq_decode_heads_per_block(void);
 int pgk_seq_heads_per_block(int heads, int kv_heads);
 int pgk_seq_queries_per_tile(int heads, int kv_heads);
 
+/* ------------------------------------------------------------------ keys and values in four bits, and beam search (net-new)
+ * A cache of one side: `pages` pages [kv_heads][page_size x dim / 2 bytes of codes, page_size x dim / 32 16-bit words]; dim 64, 96, 128, 192 or
+ * 256, pages of a multiple of 16 positions, the base on a 16-byte boundary; page_table int32 [slots][max_pages].  A group of 32 elements of a
+ * row stands for s (c - z): lo = min(0, x), hi = max(0, x), s = (hi - lo) / 15 rounded up to four significant bits, z = rint(-lo / s), c =
+ * clip(rint(x / s) + z, 0, 15); its word has s as a bfloat16 in bits 4 to 14 and z in bits 0 to 3.  s < 2^-40: zeros.  A group with a NaN, an
+ * infinity or a magnitude of 2^56: NaN.  The 32-bit word t (dim / 32) + g of a row's codes holds elements 32 g + 8 t ... + 7, lowest bits first.
+ * Slots, positions and page numbers are data of the device: rows that they place outside the arrays are skipped.
+ *   append: q [tokens][heads][dim] (rows of q_ld elements; NULL with heads = 0) is rotated in place, k and v [tokens][kv_heads][dim] go to
+ *           (row_slots[t], positions[t]), k rotated; cos / sin float32 [table_rows][rot], pairs (i, i + rot / 2) or, interleaved, (2 i, 2 i + 1); rot 0: no
+ *           rotation.  Rows name different positions.
+ *   read:   the values at (row_slots[t], positions[t]) as [tokens][kv_heads][dim], zeros for skipped rows.
+ *   attention: sequence s has rows row_starts[s] ... row_starts[s + 1] - 1 of q (row s without row_starts), the last of its context_lens[s]
+ *           positions; max_rows and max_context bound both.  window, softcap: 0 for none; sinks float32 [heads] or NULL; scale 0: 1 / sqrt(dim).
+ * dtype: 0 float32, 1 float16, 2 bfloat16 (q, k, v, out). */
+int pgk_kv4_append(void* q, const void* k, const void* v, long q_ld, long k_ld, long v_ld, const float* cos_table, const float* sin_table,
+                   int table_rows, int rot, int interleaved, void* k_cache, void* v_cache, int pages, int page_size, const int32_t* page_table,
+                   int slots, int max_pages, const int32_t* row_slots, const int32_t* positions, int tokens, int heads, int kv_heads, int dim,
+                   int dtype, void* stream);
+int pgk_kv4_read(const void* cache, int pages, int page_size, const int32_t* page_table, int slots, int max_pages, const int32_t* row_slots,
+                 const int32_t* positions, void* out, int tokens, int kv_heads, int dim, int dtype, void* stream);
+int pgk_kv4_attention(const void* q, long q_ld, const void* k_cache, const void* v_cache, void* out, long o_ld, int pages, int page_size,
+                      const int32_t* page_table, int slots, int max_pages, const int32_t* seq_slots, const int32_t* context_lens,
+                      const int32_t* row_starts, int seqs, int tokens, int max_rows, int max_context, int heads, int kv_heads, int dim,
+                      float scale, int window, float softcap, const float* sinks, int dtype, void* stream);
+/* The n best of every group's beams x vocab candidates score[k] + log_softmax(logits[k])[v] (rows of ld elements), best first, ties to the lower
+ * beam, then the lower token.  finished (or NULL): such a beam keeps its score and has the one candidate pad_token.  Candidates at -infinity
+ * come last: logits of -infinity, beams whose score is NaN or below -1e30, rows with a NaN or +infinity.  beams, n <= 64. */
+int pgk_beam_select(const void* logits, long ld, int dtype, const float* scores, const int32_t* finished, int pad_token, int groups, int beams,
+                    int vocab, int n, float* out_scores, int32_t* out_parents, int32_t* out_tokens, void* stream);
+/* Rows of many arrays [rows][host_row_bytes[a]].  dst NULL: in groups of `group` rows, row i of a group becomes, in place, what row src[i] of it
+ * was (pairs = rows that take part).  Otherwise row dst[i] becomes row src[i]; destinations differ from one another and from every source.
+ * Indexes outside are skipped.  group <= 64.  host_arrays and host_row_bytes are read before the call returns. */
+int pgk_copy_rows(void* const* host_arrays, const int64_t* host_row_bytes, int n_arrays, int rows, const int32_t* src, const int32_t* dst,
+                  int pairs, int group, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

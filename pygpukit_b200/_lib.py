@@ -187,6 +187,12 @@ _SIGS = {
     "pgk_seq_mixer_prep": [vp, i32, i32, i32, i32, i32, i32, vp, vp, f32, i32, f32, vp, vp, vp, i32, vp, i32, i32, vp, vp, vp],
     "pgk_seq_attention": [vp, i32, i32, i32, vp, i32, vp, vp, i32, vp, i32, i32, vp, i32, vp, i32, i32, i32, i32, i32, f32,
                           f32, i32, i32, vp, vp, i32, vp],
+    # the paged cache in four bits (kv4_cache.cu, kv4_attention.cu) and beam search (beam.cu)
+    "pgk_kv4_append": [vp, vp, vp, cl, cl, cl, vp, vp, i32, i32, i32, vp, vp, i32, i32, vp, i32, i32, vp, vp, i32, i32, i32, i32, i32, vp],
+    "pgk_kv4_read": [vp, i32, i32, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, vp],
+    "pgk_kv4_attention": [vp, cl, vp, vp, vp, cl, i32, i32, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, i32, f32, vp, i32, vp],
+    "pgk_beam_select": [vp, cl, i32, vp, vp, i32, i32, i32, i32, i32, vp, vp, vp, vp],
+    "pgk_copy_rows": [vp, vp, i32, i32, vp, vp, i32, i32, vp],
 }
 _RESTYPE = {"pgk_last_error": C.c_char_p, "pgk_launch_count": i64, "pgk_launch_count_reset": None,
             "pgk_sdpa_workspace_bytes": sz, "pgk_p2p_handle_bytes": sz, "pgk_p2p_ready": i32,

@@ -61,6 +61,9 @@ SOURCES = {
     "seq_gated.cu": [],
     "seq_mlstm.cu": [],
     "seq_gla.cu": [],
+    "kv4_cache.cu": [],
+    "kv4_attention.cu": [],
+    "beam.cu": [],
 }
 
 # groups of sources that link on their own (runtime.cu is in every library)
