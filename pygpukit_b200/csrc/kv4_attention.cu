@@ -1,10 +1,27 @@
-// kv4_attention.cu -- attention over the four-bit paged cache (kv4.cuh has the format).
+// kv4_attention.cu -- attention over the four-bit paged cache (kv4.cuh has the format): decoded tokens, and a few rows a sequence.
 //
 //   o[t, h, :] = sum_j w_j v_j / (sum_j w_j + exp(sink_h - m)),   w_j = exp(x_j - m),   x_j = scale q[t, h, :] . k_j, capped c tanh(x_j / c)
 //   over the keys j <= pos(t), with a window also j > pos(t) - window;  pos(t) = context - rows + (t's place among its sequence's rows)
 //
+// With k_j = s (c - z) per group of 32 elements, both sums run over codes: q . k = sum_g s_g (q_g . c_g - z_g sum q_g), and of a group's values
+// sum_j w_j v_j = sum_j (w_j s_j) c_j - sum_j (w_j s_j) z_j.  What this makes of the work:
+//   * codes go to the tensor cores (mma.sync m16n8k16) as they are.  Four bits in the lowest places of a float16 are c 2^-24, four bits above them c 2^-20,
+//     of a bfloat16 c 2^-133 and c 2^-129: subnormal numbers, which the products take exactly (tested), so that two elements cost one AND.
+//     The query carries 2^-4 where the code carries 2^4, and a power of two that brings its largest element below 2^15.
+//   * A is 16 keys of codes, B eight query rows: float16 queries (exact for bfloat16 rows; two terms for float32 ones), a group's sum starts at
+//     -z sum q_g, and a group's scale is one multiply-add per (key, row).
+//   * of the values A is 16 elements by 16 keys -- a lane's bytes of two keys, merged by one permutation --, B the weights times the group's scale and 2^64
+//     (which keeps products with c 2^-133 normal), rounded to bfloat16 once; float32 rows have three such terms, 24 bits.  The sum of w s z is
+//     a product over the same rounded weights, so that what rounding does to codes of up to 15 is done to (c - z) only.
+//   * S comes out as [key][row] and is needed as [key][row] operand of the other layout: movmatrix, two cycles for 64 numbers.
+// What bounds it: with 64 and more sequences the issue slots, about 270 instructions for 16 keys of 128 elements and 8 rows, where the cache's bytes
+// leave 350 cycles of a scheduler; with one, the chain of a launch, a page number, the rows and the fold.
+// A warp takes 32 keys at a time through a ring of its own in shared memory (cp.async, no barrier among warps), with its own maximum and sums;
+// the warps fold in shared memory, and where a sequence's keys are cut over the blocks of a cluster, these fold through distributed shared memory.
+//
 // A row that sees no key gives zeros.
 #include "kv4.cuh"
+#include "tc_common.cuh"
 #include "../../include/pgk_b200.h"
 
 namespace pgk {
@@ -19,78 +36,603 @@ struct Kv4AttnParams {
     Kv4Pages k;
     const unsigned char* v_data;
     const int32_t* seq_slots; const int32_t* contexts; const int32_t* starts;      // starts NULL: a row a sequence
-    int seqs, tokens, max_rows, max_keys, heads;
-    float scale, softcap;
+    int seqs, tokens, max_rows, max_keys, heads, rep, tiles, splits;
+    float scale_log2, cap_log2;           // scale log2 e; cap log2 e or 0
     int window;
     const float* sinks;
+    bool wide_o;
 };
 
+constexpr int F_KEYS = 32, F_STAGES = 2, F_CLUSTER = 8;
+constexpr float F_LIFT = 18446744073709551616.f;                   // 2^64
+
+template <int G> struct Few {
+    static constexpr int WARPS = G <= 4 ? 8 : 4, THREADS = WARPS * 32;
+    static constexpr int STAGE = F_KEYS * 36 * G;                  // codes of K, of V, words of K, of V
+};
+template <int G, int NT, int DT> struct FewSmem {                  // the rings, or the warps' sums; queries in fragments; sums of queries
+    static constexpr int RINGS = Few<G>::WARPS * F_STAGES * Few<G>::STAGE, FOLD = Few<G>::WARPS * 8 * NT * (32 * G + 4) * 4;
+    static constexpr int FRAG = RINGS > FOLD ? RINGS : FOLD, QSUM = FRAG + G * 2 * NT * (DT == 0 ? 2 : 1) * 256, BYTES = QSUM + G * NT * 32;
+};
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {       // an 8 x 8 matrix of 16-bit numbers over the warp
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+// A row of codes in the ring is G pieces of 16 bytes, in an order that keeps the lanes of one load off each other's banks: those of a quad's keys
+// (rows r ... r + 7, all pieces) as well as those of a value's (every second row, one place).
+template <int G>
+__device__ __forceinline__ int piece(int row, int i) {
+    if constexpr (G == 2) return i ^ ((row >> 2) & 1);
+    else if constexpr (G == 4) return i ^ ((row >> 1) & 3);
+    else if constexpr (G == 8) return i ^ ((row >> 1) & 3) << 1 ^ (row & 1);
+    else return i;
+}
+// the G words that lane t of a quad has of a row
+template <int G>
+__device__ __forceinline__ void lds_codes(const unsigned char* rows, int row, int t, uint32_t (&w)[G]) {
+    const unsigned char* at = rows + row * 16 * G;
+    if constexpr (G % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < G; i += 4) {
+            const uint4 v = *(const uint4*)(at + 16 * piece<G>(row, t * (G / 4) + i / 4));
+            w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+        }
+    } else if constexpr (G == 2) {
+        const uint2 v = *(const uint2*)(at + 16 * piece<G>(row, t >> 1) + 8 * (t & 1));
+        w[0] = v.x; w[1] = v.y;
+    } else if constexpr (G % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < G; i += 2) {
+            const uint2 v = *(const uint2*)(at + 4 * (t * G + i));
+            w[i] = v.x; w[i + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < G; ++i) w[i] = *(const uint32_t*)(at + 4 * (t * G + i));
+    }
+}
+// the G group words of a row, two to a register
+template <int G>
+__device__ __forceinline__ void lds_groups(const unsigned char* p, uint32_t (&m)[(G + 1) / 2]) {
+    if constexpr (G == 8) {
+        const uint4 v = *(const uint4*)p;
+        m[0] = v.x; m[1] = v.y; m[2] = v.z; m[3] = v.w;
+    } else if constexpr (G == 4) {
+        const uint2 v = *(const uint2*)p;
+        m[0] = v.x; m[1] = v.y;
+    } else if constexpr (G % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < G / 2; ++i) m[i] = *(const uint32_t*)(p + 4 * i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            const uint32_t h = *(const uint16_t*)(p + 2 * i);
+            m[i / 2] = i % 2 ? m[i / 2] | h << 16 : h;
+        }
+    }
+}
+__device__ __forceinline__ float group_scale(uint32_t m, int odd) { return __uint_as_float(odd ? m & 0x7ff00000u : (m << 16) & 0x7ff00000u); }
+__device__ __forceinline__ float group_zero(uint32_t m, int odd) {
+    return __uint_as_float(((odd ? m >> 16 : m) & 15u) | 0x4b000000u) - 8388608.f;
+}
+
 template <int DT>
-__global__ void __launch_bounds__(128) kv4_attention_plain_kernel(const __grid_constant__ Kv4AttnParams p) {
-    __shared__ float qs[4][256];
+__device__ __forceinline__ float row_element(const void* q, size_t i) {
+    if constexpr (DT == 0) return __ldcg((const float*)q + i);
+    else if constexpr (DT == 1) return __half2float(__ushort_as_half(ld_act2((const uint16_t*)q + i)));
+    else return bf16_bits_to_f32(ld_act2((const uint16_t*)q + i));
+}
+__device__ __forceinline__ float finite(float v) { return fabsf(v) < INFINITY ? v : 0.f; }
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t remote(uint32_t at, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float remote_float(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 remote_float4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
+template <int G, int NT, int DT>
+__global__ void __launch_bounds__(Few<G>::THREADS, G * NT <= 4 ? 2 : 1) kv4_few_kernel(const __grid_constant__ Kv4AttnParams p) {
+    constexpr int D = 32 * G, DP = D + 4, ROWS = 8 * NT, WARPS = Few<G>::WARPS, THREADS = Few<G>::THREADS, STAGE = Few<G>::STAGE;
+    constexpr int QT = DT == 0 ? 2 : 1, PT = DT == 0 ? 3 : 1, MW = (G + 1) / 2;
+    using Smem = FewSmem<G, NT, DT>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ float fac_s[ROWS], wm[WARPS][ROWS], wl[WARPS][ROWS], block_m[ROWS], block_l[ROWS];
+    __shared__ int lim_s[ROWS];
     griddep_wait();
     griddep_launch();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.y * 4 + warp;
-    const int seq = blockIdx.x / p.max_rows, r = blockIdx.x - seq * p.max_rows;
-    const int first = p.starts ? __ldcg(p.starts + seq) : seq, last = p.starts ? __ldcg(p.starts + seq + 1) : seq + 1;
-    const int t = first + r;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, t = lane & 3;
+    const int seq = blockIdx.x / p.tiles, f0 = (blockIdx.x - seq * p.tiles) * ROWS, head = blockIdx.y, split = blockIdx.z;
     const int slot = __ldcg(p.seq_slots + seq), ctx = __ldcg(p.contexts + seq);
-    if (h >= p.heads || t >= last || t < 0 || t >= p.tokens || (unsigned)slot >= (unsigned)p.k.slots) return;
-    const int D = p.k.dim, G = D / 32, g = h / (p.heads / p.k.kv_heads);
-    const int pos = ctx - (last - first) + r;
-    for (int i = lane; i < D / 8; i += 32) {
-        float x[8];
-        kv4_load8<DT>(p.q, (size_t)t * p.q_ld + (size_t)h * D + 8 * i, false, x);
-        for (int e = 0; e < 8; ++e) qs[warp][8 * i + e] = x[e];
-    }
-    __syncwarp();
-    float m = p.sinks ? __ldcg(p.sinks + h) : -INFINITY, l = m == -INFINITY ? 0.f : 1.f, acc[8] = {};
-    const int begin = p.window > 0 ? max(0, pos - p.window + 1) : 0, end = min(min(pos + 1, ctx), p.max_keys);
-    for (int j0 = begin; j0 < end; j0 += 32) {
-        const int j = j0 + lane, page = j < end ? kv4_page(p.k, slot, j) : -1, row = j % p.k.page_size;
-        const size_t at = page < 0 ? 0 : ((size_t)page * p.k.kv_heads + g) * ((size_t)p.k.page_size * kv4_row_bytes(D));
-        float x = -INFINITY;
-        if (page >= 0) {
-            const unsigned char* base = p.k.data + at;
-            x = 0.f;
-            for (int gi = 0; gi < G; ++gi) {
-                const uint32_t word = ld_act2((const uint16_t*)(base + (size_t)p.k.page_size * (D / 2)) + (size_t)row * G + gi);
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t codes = __ldcg((const uint32_t*)(base + (size_t)row * (D / 2)) + w * G + gi);
-                    for (int e = 0; e < 8; ++e) x = fmaf(qs[warp][32 * gi + 8 * w + e], kv4_value(codes, e, word), x);
+    const int first = p.starts ? __ldcg(p.starts + seq) : seq, n = p.starts ? __ldcg(p.starts + seq + 1) - first : 1;
+    const int rows = min(min(n, p.max_rows), 0x7fffffff / p.rep) * p.rep;                  // of this head's group
+    if (f0 >= rows || (unsigned)slot >= (unsigned)p.k.slots) return;                       // the whole cluster
+    const int live = min(ROWS, rows - f0), i0 = f0 / p.rep, i1 = (f0 + live - 1) / p.rep;
+    const int pos0 = ctx - n + i0, pos1 = ctx - n + i1;
+    const int begin = p.window > 0 ? max(0, pos0 - p.window + 1) : 0, end = min(min(pos1 + 1, ctx), p.max_keys);
+    const int b0 = begin / F_KEYS, nb = max(0, (end + F_KEYS - 1) / F_KEYS - b0);
+    const int per = (nb + p.splits - 1) / p.splits, bend = min(nb, (split + 1) * per) + b0;
+    const int lo_max = p.window > 0 ? pos1 - p.window + 1 : 0, hi_min = min(pos0 + 1, end);
+
+    // ---------------- the ring: 32 keys of K and V, their words behind them
+    unsigned char* const ring = smem + (size_t)warp * F_STAGES * STAGE;
+    const size_t head_bytes = (size_t)p.k.page_size * kv4_row_bytes(D);
+    const int32_t* table = p.k.table + (size_t)slot * p.k.max_pages;
+    auto pages_of = [&](int b, int (&pg)[2]) {                     // -1: no such page, or nothing to see there
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int key = b * F_KEYS + 16 * u;
+            pg[u] = b < bend && key < end ? __ldcg(table + (unsigned)key / (unsigned)p.k.page_size) : -1;
+        }
+    };
+    auto fetch = [&](int b, int stage, const int (&pg)[2]) {       // returns which halves exist
+        unsigned char* const to = ring + stage * STAGE;
+        uint32_t ok = 0;
+        size_t at[2];
+        int row[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const bool good = (unsigned)pg[u] < (unsigned)p.k.pages;
+            ok |= (uint32_t)good << u;
+            at[u] = ((size_t)(good ? pg[u] : 0) * p.k.kv_heads + head) * head_bytes;
+            row[u] = good ? (int)((unsigned)(b * F_KEYS + 16 * u) % (unsigned)p.k.page_size) : 0;
+        }
+        if (b < bend) {
+#pragma unroll
+            for (int i = 0; i < G; ++i) {                          // 16 G copies a half: of either side G a lane
+                const int c = i * 32 + lane, u = c >= 16 * G, r = c - u * 16 * G, key = c / G, x = key * G + piece<G>(key, c - key * G);
+                const size_t from = (u ? at[1] : at[0]) + (size_t)(u ? row[1] : row[0]) * (16 * G) + r * 16;
+                cp_async16(to + x * 16, p.k.data + from);
+                cp_async16(to + F_KEYS * 16 * G + x * 16, p.v_data + from);
+            }
+#pragma unroll
+            for (int i = 0; i < (8 * G + 31) / 32; ++i) {          // words: 4 G copies a side
+                const int c = i * 32 + lane;
+                if (c < 8 * G) {
+                    const int side = c >= 4 * G, cc = c - side * 4 * G, u = cc >= 2 * G, r = cc - u * 2 * G;
+                    cp_async16(to + F_KEYS * 32 * G + c * 16, (side ? p.v_data : p.k.data) + (u ? at[1] : at[0]) + (size_t)p.k.page_size * (16 * G) + (size_t)(u ? row[1] : row[0]) * (2 * G) + r * 16);
                 }
             }
-            x *= p.scale;
-            if (p.softcap > 0.f) x = p.softcap * tanhf(x / p.softcap);
         }
-        const float top = fmaxf(m, warp_max(x));
-        const bool nan = __any_sync(0xffffffffu, x != x);
-        const float f = m == -INFINITY ? 0.f : expf(m - top);
-        const float w = x == -INFINITY ? 0.f : expf(x - top);
-        l = l * f + warp_sum(w);
-        if (nan) l = NAN;
-        for (int gi = 0; gi < G; ++gi) acc[gi] *= f;
-        m = top;
-        for (int n = 0; n < 32 && j0 + n < end; ++n) {
-            const float wn = __shfl_sync(0xffffffffu, w, n);
-            const size_t atn = __shfl_sync(0xffffffffu, (unsigned long long)at, n);
-            const int pg = __shfl_sync(0xffffffffu, page, n);
-            if (pg < 0) continue;
-            const int rn = (j0 + n) % p.k.page_size;
-            const unsigned char* base = p.v_data + atn;
-            for (int gi = 0; gi < G; ++gi) {
-                const uint32_t word = ld_act2((const uint16_t*)(base + (size_t)p.k.page_size * (D / 2)) + (size_t)rn * G + gi);
-                const uint32_t codes = __ldcg((const uint32_t*)(base + (size_t)rn * (D / 2)) + (lane >> 3) * G + gi);
-                acc[gi] = fmaf(wn, kv4_value(codes, lane & 7, word), acc[gi]);
+        cp_async_commit();
+        return ok;
+    };
+    int block, ahead[2];
+    uint32_t have[F_STAGES];
+    auto start = [&] {
+        int now[2];
+        block = b0 + split * per + warp;
+        pages_of(block, now);
+        pages_of(block + WARPS, ahead);
+        have[0] = fetch(block, 0, now);
+    };
+    start();
+
+    // ---------------- queries into fragments
+    unsigned char* const frag = smem + Smem::FRAG;
+    float* const qsum = (float*)(smem + Smem::QSUM);               // [G][NT][8]
+    for (int c = warp; c < ROWS; c += WARPS) {
+        const int f = f0 + c, i = f / p.rep, tok = first + i;
+        const bool there = c < live && tok >= 0 && tok < p.tokens;
+        float x[G], top = 0.f;
+        bool odd = false;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            x[g] = there ? row_element<DT>(p.q, (size_t)tok * p.q_ld + (size_t)(head * p.rep + f - i * p.rep) * D + 32 * g + lane) : 0.f;
+            top = fmaxf(top, fabsf(x[g]));
+            odd |= x[g] != x[g];
+        }
+        top = warp_max(top);
+        const uint32_t e = min(max(268u - min(__float_as_uint(top) >> 23, 267u), 4u), 250u);        // 2^14 <= top 2^(e - 127) < 2^15
+        const float mult = __uint_as_float(e << 23);
+        const int w = lane, qt = w >> 3, nib = w & 7, pr = nib & 3;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const float y = x[g] * mult * (pr & 1 ? 0.0625f : 1.f);
+            float used = 0.f, rest = y;
+#pragma unroll
+            for (int term = 0; term < QT; ++term) {
+                const __half h = __float2half_rn(rest);
+                *(uint16_t*)(frag + ((((size_t)(g * 2 + (pr >> 1)) * NT + (c >> 3)) * QT + term) * 32 + (c & 7) * 4 + qt) * 8 + (pr & 1) * 4 + (nib >> 2) * 2) =
+                    __half_as_ushort(h);
+                used += __half2float(h);
+                rest -= __half2float(h);
+            }
+            const float sum = warp_sum(used * (pr & 1 ? 16.f : 1.f));
+            if (lane == 0) qsum[(g * NT + (c >> 3)) * 8 + (c & 7)] = sum * 5.9604644775390625e-8f;   // 2^-24
+        }
+        if (lane == 0) {
+            fac_s[c] = p.scale_log2 * __uint_as_float((254u - e) << 23) * 16777216.f;
+            lim_s[c] = there ? ctx - n + i : -1;
+        }
+    }
+    __syncthreads();
+    float fac[NT][2], m[NT][2], l[NT][2], acc[2 * G][NT][4], zac[NT][4];
+    int lim[NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            fac[j][c] = fac_s[8 * j + 2 * t + c];
+            lim[j][c] = lim_s[8 * j + 2 * t + c];
+        }
+    const uint32_t half_sel = gl & 1 ? 0x7632u : 0x5410u;
+    bool careful = false;
+again:
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            m[j][c] = -INFINITY;
+            l[j][c] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) zac[j][i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
+    }
+
+    for (int k = 0; block < bend; ++k, block += WARPS) {
+        const int stage = k % F_STAGES;
+        __syncwarp();                                              // the other stage has been read
+        {
+            int next[2];
+            pages_of(block + 2 * WARPS, next);
+            have[(k + 1) % F_STAGES] = fetch(block + WARPS, (k + 1) % F_STAGES, ahead);
+            ahead[0] = next[0]; ahead[1] = next[1];
+        }
+        cp_async_wait<F_STAGES - 1>();
+        __syncwarp();
+        const unsigned char* const kc = ring + stage * STAGE;
+        const unsigned char* const vc = kc + F_KEYS * 16 * G;
+        const unsigned char* const kwords = kc + F_KEYS * 32 * G;
+        const unsigned char* const vwords = kwords + F_KEYS * 2 * G;
+        const int key0 = block * F_KEYS;
+        const bool edge = key0 < lo_max || key0 + F_KEYS > hi_min || have[stage] != 3u;
+
+        // ---------------- scores
+        float s[2][NT][4];
+        {
+            uint32_t kw[2][2][G], km[2][2][MW];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int row = 16 * u + 8 * r + gl;
+                    lds_codes<G>(kc, row, t, kw[u][r]);
+                    lds_groups<G>(kwords + row * 2 * G, km[u][r]);
+                }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[u][j][i] = 0.f;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const float2 qs = *(const float2*)(qsum + (g * NT + j) * 8 + 2 * t);
+                    uint2 b[2][QT];
+#pragma unroll
+                    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                        for (int term = 0; term < QT; ++term)
+                            b[ks][term] = *(const uint2*)(frag + ((((size_t)(g * 2 + ks) * NT + j) * QT + term) * 32 + lane) * 8);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float z0 = group_zero(km[u][0][g / 2], g & 1), z1 = group_zero(km[u][1][g / 2], g & 1);
+                        const float s0 = group_scale(km[u][0][g / 2], g & 1), s1 = group_scale(km[u][1][g / 2], g & 1);
+                        float c[4] = {-z0 * qs.x, -z0 * qs.y, -z1 * qs.x, -z1 * qs.y};
+#pragma unroll
+                        for (int ks = 0; ks < 2; ++ks) {
+                            const uint32_t w0 = ks ? kw[u][0][g] >> 8 : kw[u][0][g], w1 = ks ? kw[u][1][g] >> 8 : kw[u][1][g];
+#pragma unroll
+                            for (int term = QT - 1; term >= 0; --term)
+                                mma_f16(c, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, b[ks][term].x, b[ks][term].y);
+                        }
+                        s[u][j][0] = fmaf(s0, c[0], s[u][j][0]);
+                        s[u][j][1] = fmaf(s0, c[1], s[u][j][1]);
+                        s[u][j][2] = fmaf(s1, c[2], s[u][j][2]);
+                        s[u][j][3] = fmaf(s1, c[3], s[u][j][3]);
+                    }
+                }
+            }
+        }
+        // ---------------- weights
+        bool up = false;
+        float top[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float best = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        float x = s[u][j][2 * r + c] * fac[j][c];
+                        if (p.cap_log2 > 0.f) {                    // float32 rows: 2^-22 of a cap of 50 would be a weight's 22nd bit
+                            if constexpr (DT == 0) x = p.cap_log2 * tanhf(x / p.cap_log2);
+                            else x = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(x * (2.885390043f / p.cap_log2))));
+                        }
+                        if (edge) {
+                            const int key = key0 + 16 * u + 8 * r + gl;
+                            if (key > lim[j][c] || key >= end || (p.window > 0 && key <= lim[j][c] - p.window) || !((have[stage] >> u) & 1u)) x = -INFINITY;
+                        }
+                        s[u][j][2 * r + c] = x;
+                        best = fmaxf(best, x);
+                    }
+                top[j][c] = best;
+                up |= best > m[j][c] + 8.f;
+            }
+        }
+        if (__any_sync(0xffffffffu, up)) {                         // a reference moves when its maximum has grown by 2^8 (or at all at first)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                float f[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float best = top[j][c];
+#pragma unroll
+                    for (int o = 4; o <= 16; o <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+                    best = fmaxf(best, m[j][c]);
+                    f[c] = m[j][c] == -INFINITY ? 0.f : ex2(m[j][c] - best);
+                    m[j][c] = best;
+                    l[j][c] *= f[c];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) zac[j][i] *= f[i & 1];
+#pragma unroll
+                for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[i][j][c] *= f[c & 1];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const float base = m[j][c] == -INFINITY ? 0.f : m[j][c];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float w = ex2(s[u][j][2 * r + c] - base);
+                        l[j][c] += w;
+                        s[u][j][2 * r + c] = w * F_LIFT;
+                    }
+            }
+        // ---------------- values
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            uint32_t vw[4][G], vz[4][MW], vm[2][MW];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = 16 * u + 2 * t + (i & 1) + 8 * (i >> 1);
+                lds_codes<G>(vc, row, gl >> 1, vw[i]);
+                lds_groups<G>(vwords + row * 2 * G, vz[i]);
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) lds_groups<G>(vwords + (16 * u + 8 * r + gl) * 2 * G, vm[r]);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const uint32_t v0 = __byte_perm(vw[0][g], vw[1][g], half_sel), v1 = __byte_perm(vw[2][g], vw[3][g], half_sel);
+                const uint32_t zmask = gl == g ? 0x000f000fu : 0u;
+                const uint32_t z0 = __byte_perm(vz[0][g / 2], vz[1][g / 2], g & 1 ? 0x7632 : 0x5410) & zmask;
+                const uint32_t z1 = __byte_perm(vz[2][g / 2], vz[3][g / 2], g & 1 ? 0x7632 : 0x5410) & zmask;
+                const float s0 = group_scale(vm[0][g / 2], g & 1), s1 = group_scale(vm[1][g / 2], g & 1);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    float w[4] = {s[u][j][0] * s0, s[u][j][1] * s0, s[u][j][2] * s1, s[u][j][3] * s1};
+                    if (edge) {                                    // a key that is not seen may have any bytes for a scale
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (s[u][j][i] == 0.f) w[i] = 0.f;
+                    }
+#pragma unroll
+                    for (int term = 0; term < PT; ++term) {
+                        const uint32_t lo = pack_bf16x2(w[0], w[1]), hi = pack_bf16x2(w[2], w[3]);
+                        const uint32_t p0 = transposed(lo), p1 = transposed(hi);
+                        mma_bf16(acc[2 * g][j], v0 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x000f000fu, v1 & 0x00f000f0u, p0, p1);
+                        mma_bf16(acc[2 * g + 1][j], (v0 >> 8) & 0x000f000fu, (v0 >> 8) & 0x00f000f0u, (v1 >> 8) & 0x000f000fu, (v1 >> 8) & 0x00f000f0u, p0, p1);
+                        if (careful)
+                            mma_bf16(zac[j], z0, 0u, z1, 0u, transposed(pack_bf16x2(finite(w[0]), finite(w[1]))), transposed(pack_bf16x2(finite(w[2]), finite(w[3]))));
+                        else
+                            mma_bf16(zac[j], z0, 0u, z1, 0u, p0, p1);
+                        if (term + 1 < PT) {
+                            w[0] -= bf16lo(lo); w[1] -= bf16hi(lo);
+                            w[2] -= bf16lo(hi); w[3] -= bf16hi(hi);
+                        }
+                    }
+                }
             }
         }
     }
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    for (int gi = 0; gi < G; ++gi) {
-        const size_t at = (size_t)t * p.o_ld + (size_t)h * D + 32 * gi + lane;
-        const float o = acc[gi] * inv;
-        if constexpr (DT == 0) ((float*)p.out)[at] = o;
-        else ((uint16_t*)p.out)[at] = (uint16_t)kv4_pack2<DT>(o, 0.f);
+    cp_async_wait<0>();
+    // The groups' sums of w s z share a product's rows: a scale that is NaN, in one group, would reach the others as 0 NaN.  Then once more, without it there.
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) bad |= zac[j][0] != zac[j][0] || zac[j][1] != zac[j][1];
+    if (!careful && __any_sync(0xffffffffu, bad)) {
+        careful = true;
+        __syncwarp();
+        start();
+        goto again;
+    }
+
+    // ---------------- the warps' sums into one
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int o = 4; o <= 16; o <<= 1) l[j][c] += __shfl_xor_sync(0xffffffffu, l[j][c], o);
+    __syncthreads();                                               // the rings are read
+    float* const fold = (float*)smem;                              // [WARPS][ROWS][DP]
+    const float even = 5.9029581035870565e20f, odd = 3.6893488147419103e19f;      // 2^133 / 2^64 and 2^129 / 2^64
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int col = 8 * j + 2 * t + c;
+            if (gl == 0) { wm[warp][col] = m[j][c]; wl[warp][col] = l[j][c]; }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const float z = __shfl_sync(0xffffffffu, zac[j][c], g * 4 + t) * even;
+                const float4 o = make_float4(fmaf(acc[2 * g][j][c], even, -z), fmaf(acc[2 * g][j][2 + c], odd, -z), fmaf(acc[2 * g + 1][j][c], even, -z),
+                                       fmaf(acc[2 * g + 1][j][2 + c], odd, -z));
+                *(float4*)(fold + ((size_t)warp * ROWS + col) * DP + 32 * g + 4 * gl) = o;
+            }
+        }
+    }
+    __syncthreads();
+    if (tid < ROWS) {
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, wm[w][tid]);
+        for (int w = 0; w < WARPS; ++w) {
+            // a warp whose scores are all NaN has no maximum and a sum of NaN
+            const float f = wm[w][tid] == -INFINITY ? wl[w][tid] - wl[w][tid] : exp2f(wm[w][tid] - top);
+            sum += wl[w][tid] * f;
+            wm[w][tid] = f;
+        }
+        block_m[tid] = top;
+        block_l[tid] = sum;
+    }
+    __syncthreads();
+    for (int i = tid; i < live * (D / 4); i += THREADS) {
+        const int col = i / (D / 4), d = (i - col * (D / 4)) * 4;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = wm[w][col];
+            const float4 v = *(const float4*)(fold + ((size_t)w * ROWS + col) * DP + d);
+            o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+        }
+        *(float4*)(fold + (size_t)col * DP + d) = o;
+    }
+    // ---------------- the cluster's into one: block r has every `splits`-th piece
+    if (p.splits > 1) cluster_sync();
+    else __syncthreads();
+    const uint32_t fold_at = smem_u32(fold), m_at = smem_u32(block_m), l_at = smem_u32(block_l);
+    for (int i = split * THREADS + tid; i < live * (D / 4); i += p.splits * THREADS) {
+        const int col = i / (D / 4), d = (i - col * (D / 4)) * 4;
+        const int f = f0 + col, row = f / p.rep, tok = first + row, h = head * p.rep + f - row * p.rep;
+        if (tok < 0 || tok >= p.tokens) continue;
+        const float sink = p.sinks ? __ldcg(p.sinks + h) * 1.4426950408889634f : -INFINITY;
+        float top = sink, sum = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p.splits > 1) {
+            for (int s = 0; s < p.splits; ++s) top = fmaxf(top, remote_float(remote(m_at + 4 * col, s)));
+            for (int s = 0; s < p.splits; ++s) {
+                const float ms = remote_float(remote(m_at + 4 * col, s)), ls = remote_float(remote(l_at + 4 * col, s));
+                const float w = ms == -INFINITY ? ls - ls : exp2f(ms - top);
+                const float4 v = remote_float4(remote(fold_at + (col * DP + d) * 4, s));
+                sum = fmaf(w, ls, sum);
+                o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
+            }
+        } else {
+            top = fmaxf(top, block_m[col]);
+            const float w = block_m[col] == -INFINITY ? block_l[col] - block_l[col] : exp2f(block_m[col] - top);
+            const float4 v = *(const float4*)(fold + (size_t)col * DP + d);
+            sum = w * block_l[col];
+            o = make_float4(w * v.x, w * v.y, w * v.z, w * v.w);
+        }
+        if (sink != -INFINITY) sum += exp2f(sink - top);
+        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        const size_t at = (size_t)tok * p.o_ld + (size_t)h * D + d;
+        o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+        if constexpr (DT == 0) {
+            float* dst = (float*)p.out + at;
+            if (p.wide_o) *(float4*)dst = o;
+            else { dst[0] = o.x; dst[1] = o.y; dst[2] = o.z; dst[3] = o.w; }
+        } else {
+            uint16_t* dst = (uint16_t*)p.out + at;
+            const uint32_t a = kv4_pack2<DT>(o.x, o.y), b = kv4_pack2<DT>(o.z, o.w);
+            if (p.wide_o) *(uint2*)dst = make_uint2(a, b);
+            else { dst[0] = (uint16_t)a; dst[1] = (uint16_t)(a >> 16); dst[2] = (uint16_t)b; dst[3] = (uint16_t)(b >> 16); }
+        }
+    }
+    if (p.splits > 1) cluster_sync();                              // nobody leaves while another reads
+}
+
+template <int G, int NT, int DT>
+cudaError_t launch_few(Kv4AttnParams p, cudaStream_t st) {
+    constexpr int bytes = FewSmem<G, NT, DT>::BYTES;
+    static_assert(bytes <= 220 * 1024);
+    static bool configured = false;
+    if (!configured) {
+        if (cudaError_t e = cudaFuncSetAttribute(kv4_few_kernel<G, NT, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+        configured = true;
+    }
+    p.tiles = (int)(((long long)p.max_rows * p.rep + 8 * NT - 1) / (8 * NT));
+    const long long items = (long long)p.seqs * p.tiles * p.k.kv_heads;
+    const int keys = p.window > 0 && p.window + p.max_rows < p.max_keys ? p.window + p.max_rows : p.max_keys;
+    const int nb = (keys + F_KEYS - 1) / F_KEYS, most = (nb + Few<G>::WARPS - 1) / Few<G>::WARPS;
+    p.splits = 1;
+    while (p.splits < F_CLUSTER && p.splits < most && items * p.splits * 2 <= 2 * sm_count()) p.splits *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.seqs * p.tiles), p.k.kv_heads, p.splits);
+    cfg.blockDim = dim3(Few<G>::THREADS);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = (unsigned)p.splits;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    count_launch();
+    return cudaLaunchKernelEx(&cfg, kv4_few_kernel<G, NT, DT>, p);
+}
+
+// Eight rows a column block: as many blocks as the rows of a sequence's group need, up to what the accumulators' registers allow (G NT <= 8)
+template <int G, int DT>
+cudaError_t launch_few_rows(const Kv4AttnParams& p, cudaStream_t st) {
+    const long long rows = (long long)p.max_rows * p.rep;
+    if constexpr (G <= 2) {
+        if (rows > 16) return launch_few<G, 4, DT>(p, st);
+    }
+    if constexpr (G <= 4) {
+        if (rows > 8) return launch_few<G, 2, DT>(p, st);
+    }
+    return launch_few<G, 1, DT>(p, st);
+}
+template <int DT>
+cudaError_t launch_few_dim(const Kv4AttnParams& p, cudaStream_t st) {
+    switch (p.k.dim) {
+        case 64: return launch_few_rows<2, DT>(p, st);
+        case 96: return launch_few_rows<3, DT>(p, st);
+        case 128: return launch_few_rows<4, DT>(p, st);
+        case 192: return launch_few_rows<6, DT>(p, st);
+        default: return launch_few_rows<8, DT>(p, st);
     }
 }
 
@@ -108,9 +650,10 @@ extern "C" int pgk_kv4_attention(const void* q, long q_ld, const void* k_cache, 
     if (int rc = kv4_check(fn, k_cache, pages, page_size, page_table, slots, max_pages, kv_heads, dim)) return rc;
     if (int rc = kv4_check(fn, v_cache, pages, page_size, page_table, slots, max_pages, kv_heads, dim)) return rc;
     PGK_REQUIRE(dtype >= 0 && dtype <= 2, "kv4_attention failed: unknown type %d", dtype);
-    PGK_REQUIRE(heads > 0 && heads % kv_heads == 0 && heads <= 65535 && q_ld >= (long)heads * dim && o_ld >= (long)heads * dim,
+    PGK_REQUIRE(heads > 0 && heads % kv_heads == 0 && kv_heads <= 65535 && q_ld >= (long)heads * dim && o_ld >= (long)heads * dim,
                 "kv4_attention failed: %d query heads over %d, rows of %ld and %ld", heads, kv_heads, q_ld, o_ld);
-    PGK_REQUIRE(seqs >= 0 && tokens >= 0 && max_rows > 0 && max_context >= 0 && (row_starts || (tokens >= seqs && max_rows == 1)) && (long long)seqs * max_rows <= 0x7fffffffll,
+    PGK_REQUIRE(seqs >= 0 && tokens >= 0 && max_rows > 0 && max_context >= 0 && (row_starts || (tokens >= seqs && max_rows == 1)) &&
+                    (long long)seqs * max_rows * (heads / kv_heads) <= 0x7fffffffll,
                 "kv4_attention failed: %d sequences of up to %d rows in %d, %d keys", seqs, max_rows, tokens, max_context);
     PGK_REQUIRE(window >= 0 && softcap >= 0.f && scale == scale, "kv4_attention failed: window %d, cap %g, scale %g", window, softcap, scale);
     if (seqs == 0 || tokens == 0) return 0;
@@ -120,11 +663,15 @@ extern "C" int pgk_kv4_attention(const void* q, long q_ld, const void* k_cache, 
     p.k = {(unsigned char*)k_cache, page_table, pages, page_size, slots, max_pages, kv_heads, dim};
     p.v_data = (const unsigned char*)v_cache;
     p.seq_slots = seq_slots; p.contexts = context_lens; p.starts = row_starts;
-    p.seqs = seqs; p.tokens = tokens; p.max_rows = max_rows; p.heads = heads;
+    p.seqs = seqs; p.tokens = tokens; p.heads = heads; p.rep = heads / kv_heads;
+    p.max_rows = max_rows < tokens ? max_rows : tokens;
     p.max_keys = max_context < max_pages * page_size ? max_context : max_pages * page_size;
-    p.scale = scale > 0.f ? scale : 1.f / sqrtf((float)dim);
-    p.window = window; p.softcap = softcap; p.sinks = sinks;
-    auto kernel = dtype == 0 ? kv4_attention_plain_kernel<0> : (dtype == 1 ? kv4_attention_plain_kernel<1> : kv4_attention_plain_kernel<2>);
-    PGK_CUDA(launch_waiting(kernel, dim3((unsigned)seqs * max_rows, (heads + 3) / 4), dim3(128), 0, (cudaStream_t)stream, p));
+    p.scale_log2 = (scale > 0.f ? scale : 1.f / sqrtf((float)dim)) * 1.4426950408889634f;
+    p.cap_log2 = softcap * 1.4426950408889634f;
+    p.window = window; p.sinks = sinks;
+    const int size = dtype == 0 ? 4 : 2;
+    p.wide_o = (uintptr_t)out % 16 == 0 && o_ld * size % 16 == 0;
+    const cudaStream_t st = (cudaStream_t)stream;
+    PGK_CUDA(dtype == 0 ? launch_few_dim<0>(p, st) : (dtype == 1 ? launch_few_dim<1>(p, st) : launch_few_dim<2>(p, st)));
     return 0;
 }
