@@ -41,18 +41,19 @@ struct Kv4AttnParams {
     int window;
     const float* sinks;
     bool wide_o;
+    uint32_t page_mul, page_shift;        // n / (page_size / 16) = hi(n page_mul) >> page_shift; page_mul 0: pages of 16
+    long long page_bytes, head_bytes;
 };
 
 constexpr int F_KEYS = 32, F_STAGES = 2, F_CLUSTER = 8;
 constexpr float F_LIFT = 18446744073709551616.f;                   // 2^64
 
-template <int G> struct Few {
-    static constexpr int WARPS = G <= 4 ? 8 : 4, THREADS = WARPS * 32;
+// W warps a block; the rings, or the warps' sums; queries in fragments; sums of queries
+template <int G, int NT, int DT, int W> struct Few {
+    static constexpr int THREADS = W * 32, RESIDENT = G * NT <= 4 ? 16 / W : 8 / W;
     static constexpr int STAGE = F_KEYS * 36 * G;                  // codes of K, of V, words of K, of V
-};
-template <int G, int NT, int DT> struct FewSmem {                  // the rings, or the warps' sums; queries in fragments; sums of queries
-    static constexpr int RINGS = Few<G>::WARPS * F_STAGES * Few<G>::STAGE, FOLD = Few<G>::WARPS * 8 * NT * (32 * G + 4) * 4;
-    static constexpr int FRAG = RINGS > FOLD ? RINGS : FOLD, QSUM = FRAG + G * 2 * NT * (DT == 0 ? 2 : 1) * 256, BYTES = QSUM + G * NT * 32;
+    static constexpr int RINGS = W * F_STAGES * STAGE, FOLD = W * 8 * NT * (32 * G + 4) * 4;
+    static constexpr int FRAG = RINGS > FOLD ? RINGS : FOLD, QSUM = FRAG + G * 2 * NT * (DT == 0 ? 2 : 1) * 256, BYTES = QSUM + G * NT * 128;
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -63,9 +64,13 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(b0));
+}
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {       // an 8 x 8 matrix of 16-bit numbers over the warp
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 // A row of codes in the ring is G pieces of 16 bytes, in an order that keeps the lanes of one load off each other's banks: those of a quad's keys
@@ -122,8 +127,8 @@ __device__ __forceinline__ void lds_groups(const unsigned char* p, uint32_t (&m)
     }
 }
 __device__ __forceinline__ float group_scale(uint32_t m, int odd) { return __uint_as_float(odd ? m & 0x7ff00000u : (m << 16) & 0x7ff00000u); }
-__device__ __forceinline__ float group_zero(uint32_t m, int odd) {
-    return __uint_as_float(((odd ? m >> 16 : m) & 15u) | 0x4b000000u) - 8388608.f;
+__device__ __forceinline__ void cp_async16_at(uint32_t smem, const void* g) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(g) : "memory");
 }
 
 template <int DT>
@@ -132,6 +137,8 @@ __device__ __forceinline__ float row_element(const void* q, size_t i) {
     else if constexpr (DT == 1) return __half2float(__ushort_as_half(ld_act2((const uint16_t*)q + i)));
     else return bf16_bits_to_f32(ld_act2((const uint16_t*)q + i));
 }
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
 __device__ __forceinline__ float finite(float v) { return fabsf(v) < INFINITY ? v : 0.f; }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -152,11 +159,15 @@ __device__ __forceinline__ float4 remote_float4(uint32_t at) {
     return v;
 }
 
-template <int G, int NT, int DT>
-__global__ void __launch_bounds__(Few<G>::THREADS, G * NT <= 4 ? 2 : 1) kv4_few_kernel(const __grid_constant__ Kv4AttnParams p) {
-    constexpr int D = 32 * G, DP = D + 4, ROWS = 8 * NT, WARPS = Few<G>::WARPS, THREADS = Few<G>::THREADS, STAGE = Few<G>::STAGE;
+template <int G, int NT, int DT, int W>
+__global__ void __launch_bounds__(Few<G, NT, DT, W>::THREADS, Few<G, NT, DT, W>::RESIDENT) kv4_few_kernel(const __grid_constant__ Kv4AttnParams p) {
+    using Smem = Few<G, NT, DT, W>;
+    constexpr int D = 32 * G, DP = D + 4, ROWS = 8 * NT, WARPS = W, THREADS = Smem::THREADS, STAGE = Smem::STAGE;
     constexpr int QT = DT == 0 ? 2 : 1, PT = DT == 0 ? 3 : 1, MW = (G + 1) / 2;
-    using Smem = FewSmem<G, NT, DT>;
+    // Rows of 16 bits take a byte, c + 16 c' (a bfloat16 too, subnormal or of the first exponent), where they would take its lower four bits, and subtract the
+    // product of the upper ones in the end: one operation in five less.  The difference costs four bits of the sums' 24.
+    constexpr bool BYTES = DT != 0;
+    constexpr uint32_t LOW = BYTES ? 0x00ff00ffu : 0x000f000fu;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float fac_s[ROWS], wm[WARPS][ROWS], wl[WARPS][ROWS], block_m[ROWS], block_l[ROWS];
     __shared__ int lim_s[ROWS];
@@ -177,42 +188,47 @@ __global__ void __launch_bounds__(Few<G>::THREADS, G * NT <= 4 ? 2 : 1) kv4_few_
 
     // ---------------- the ring: 32 keys of K and V, their words behind them
     unsigned char* const ring = smem + (size_t)warp * F_STAGES * STAGE;
-    const size_t head_bytes = (size_t)p.k.page_size * kv4_row_bytes(D);
+    const uint32_t ring_at = smem_u32(ring);
     const int32_t* table = p.k.table + (size_t)slot * p.k.max_pages;
-    auto pages_of = [&](int b, int (&pg)[2]) {                     // -1: no such page, or nothing to see there
+    const unsigned char* const khead = p.k.data + (size_t)head * p.head_bytes + lane * 16;
+    const unsigned char* const vhead = p.v_data + (size_t)head * p.head_bytes + lane * 16;
+    const int code_bytes = p.k.page_size * 16 * G;
+    auto page_of = [&](uint32_t n) { return p.page_mul ? __umulhi(n, p.page_mul) >> p.page_shift : n; };
+    auto pages_of = [&](int b, int (&pg)[2]) {                     // of the block's two halves; -1: nothing to see there
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int key = b * F_KEYS + 16 * u;
-            pg[u] = b < bend && key < end ? __ldcg(table + (unsigned)key / (unsigned)p.k.page_size) : -1;
+            const int n = 2 * b + u;
+            pg[u] = b < bend && 16 * n < end ? __ldcg(table + page_of(n)) : -1;
         }
     };
-    auto fetch = [&](int b, int stage, const int (&pg)[2]) {       // returns which halves exist
-        unsigned char* const to = ring + stage * STAGE;
+    auto fetch = [&](int b, int stage, const int (&pg)[2]) {       // returns which halves have a page
+        const uint32_t to = ring_at + stage * STAGE;
         uint32_t ok = 0;
-        size_t at[2];
-        int row[2];
+        long long at[2];                                           // of the half's codes, and of its words behind the page's codes
+        int words[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const bool good = (unsigned)pg[u] < (unsigned)p.k.pages;
+            const uint32_t n = 2 * b + u;
+            const int row = good ? (int)(16u * n - page_of(n) * (uint32_t)p.k.page_size) : 0;
             ok |= (uint32_t)good << u;
-            at[u] = ((size_t)(good ? pg[u] : 0) * p.k.kv_heads + head) * head_bytes;
-            row[u] = good ? (int)((unsigned)(b * F_KEYS + 16 * u) % (unsigned)p.k.page_size) : 0;
+            at[u] = (good ? pg[u] : 0) * p.page_bytes + row * (16 * G);
+            words[u] = code_bytes - row * (14 * G);
         }
         if (b < bend) {
 #pragma unroll
             for (int i = 0; i < G; ++i) {                          // 16 G copies a half: of either side G a lane
-                const int c = i * 32 + lane, u = c >= 16 * G, r = c - u * 16 * G, key = c / G, x = key * G + piece<G>(key, c - key * G);
-                const size_t from = (u ? at[1] : at[0]) + (size_t)(u ? row[1] : row[0]) * (16 * G) + r * 16;
-                cp_async16(to + x * 16, p.k.data + from);
-                cp_async16(to + F_KEYS * 16 * G + x * 16, p.v_data + from);
+                const int c = i * 32 + lane, key = c / G, x = key * G + piece<G>(key, c - key * G);
+                const bool second = G % 2 == 0 ? i >= G / 2 : c >= 16 * G;
+                const long long from = (second ? at[1] - 256 * G : at[0]) + i * 512;
+                cp_async16_at(to + x * 16, khead + from);
+                cp_async16_at(to + F_KEYS * 16 * G + x * 16, vhead + from);
             }
 #pragma unroll
-            for (int i = 0; i < (8 * G + 31) / 32; ++i) {          // words: 4 G copies a side
-                const int c = i * 32 + lane;
-                if (c < 8 * G) {
-                    const int side = c >= 4 * G, cc = c - side * 4 * G, u = cc >= 2 * G, r = cc - u * 2 * G;
-                    cp_async16(to + F_KEYS * 32 * G + c * 16, (side ? p.v_data : p.k.data) + (u ? at[1] : at[0]) + (size_t)p.k.page_size * (16 * G) + (size_t)(u ? row[1] : row[0]) * (2 * G) + r * 16);
-                }
+            for (int i = 0; i < (8 * G + 31) / 32; ++i) {          // words: 4 G copies a side, 2 G of either half
+                const int c = i * 32 + lane, side = c >= 4 * G, u = (c - side * 4 * G) >= 2 * G;
+                if (c < 8 * G)
+                    cp_async16_at(to + F_KEYS * 32 * G + c * 16, (side ? vhead : khead) + (u ? at[1] + words[1] : at[0] + words[0]) + i * 512 - (side * 4 * G + u * 2 * G) * 16);
             }
         }
         cp_async_commit();
@@ -231,7 +247,7 @@ __global__ void __launch_bounds__(Few<G>::THREADS, G * NT <= 4 ? 2 : 1) kv4_few_
 
     // ---------------- queries into fragments
     unsigned char* const frag = smem + Smem::FRAG;
-    float* const qsum = (float*)(smem + Smem::QSUM);               // [G][NT][8]
+    unsigned char* const qsum = smem + Smem::QSUM;                 // [G][NT][lane]: -sum of the group's queries, in a term of float16 a quad's lane
     for (int c = warp; c < ROWS; c += WARPS) {
         const int f = f0 + c, i = f / p.rep, tok = first + i;
         const bool there = c < live && tok >= 0 && tok < p.tokens;
@@ -244,7 +260,7 @@ __global__ void __launch_bounds__(Few<G>::THREADS, G * NT <= 4 ? 2 : 1) kv4_few_
             odd |= x[g] != x[g];
         }
         top = warp_max(top);
-        const uint32_t e = min(max(268u - min(__float_as_uint(top) >> 23, 267u), 4u), 250u);        // 2^14 <= top 2^(e - 127) < 2^15
+        const uint32_t e = min(max(263u - min(__float_as_uint(top) >> 23, 262u), 4u), 250u);        // 2^9 <= top 2^(e - 127) < 2^10: 32 of them have a sum
         const float mult = __uint_as_float(e << 23);
         const int w = lane, qt = w >> 3, nib = w & 7, pr = nib & 3;
 #pragma unroll
@@ -259,8 +275,13 @@ __global__ void __launch_bounds__(Few<G>::THREADS, G * NT <= 4 ? 2 : 1) kv4_few_
                 used += __half2float(h);
                 rest -= __half2float(h);
             }
-            const float sum = warp_sum(used * (pr & 1 ? 16.f : 1.f));
-            if (lane == 0) qsum[(g * NT + (c >> 3)) * 8 + (c & 7)] = sum * 5.9604644775390625e-8f;   // 2^-24
+            float sum = -warp_sum(used * (pr & 1 ? 16.f : 1.f));
+            // the lane t of a quad multiplies its copy of z by term t; an even group's z is in a word's lower half, an odd one's in the upper
+            for (int term = 0; term < 4; ++term) {
+                const __half h = __float2half_rn(sum);
+                sum -= __half2float(h);
+                if (lane == term) *(uint32_t*)(qsum + ((size_t)(g * NT + (c >> 3)) * 32 + (c & 7) * 4 + term) * 4) = (uint32_t)__half_as_ushort(h) << (g & 1 ? 16 : 0);
+            }
         }
         if (lane == 0) {
             fac_s[c] = p.scale_log2 * __uint_as_float((254u - e) << 23) * 16777216.f;
@@ -274,7 +295,7 @@ __global__ void __launch_bounds__(Few<G>::THREADS, G * NT <= 4 ? 2 : 1) kv4_few_
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            fac[j][c] = fac_s[8 * j + 2 * t + c];
+            fac[j][c] = p.cap_log2 > 0.f ? 1.f : fac_s[8 * j + 2 * t + c];
             lim[j][c] = lim_s[8 * j + 2 * t + c];
         }
     const uint32_t half_sel = gl & 1 ? 0x7632u : 0x5410u;
@@ -316,7 +337,7 @@ again:
         // ---------------- scores
         float s[2][NT][4];
         {
-            uint32_t kw[2][2][G], km[2][2][MW];
+            uint32_t kw[2][2][G], km[2][2][MW], kz[2][2][MW];
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -324,6 +345,8 @@ again:
                     const int row = 16 * u + 8 * r + gl;
                     lds_codes<G>(kc, row, t, kw[u][r]);
                     lds_groups<G>(kwords + row * 2 * G, km[u][r]);
+#pragma unroll
+                    for (int i = 0; i < MW; ++i) kz[u][r][i] = km[u][r][i] & 0x000f000fu;
                 }
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -335,7 +358,7 @@ again:
             for (int g = 0; g < G; ++g) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const float2 qs = *(const float2*)(qsum + (g * NT + j) * 8 + 2 * t);
+                    const uint32_t qs = *(const uint32_t*)(qsum + ((g * NT + j) * 32 + lane) * 4);
                     uint2 b[2][QT];
 #pragma unroll
                     for (int ks = 0; ks < 2; ++ks)
@@ -344,9 +367,9 @@ again:
                             b[ks][term] = *(const uint2*)(frag + ((((size_t)(g * 2 + ks) * NT + j) * QT + term) * 32 + lane) * 8);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const float z0 = group_zero(km[u][0][g / 2], g & 1), z1 = group_zero(km[u][1][g / 2], g & 1);
                         const float s0 = group_scale(km[u][0][g / 2], g & 1), s1 = group_scale(km[u][1][g / 2], g & 1);
-                        float c[4] = {-z0 * qs.x, -z0 * qs.y, -z1 * qs.x, -z1 * qs.y};
+                        float c[4] = {0.f, 0.f, 0.f, 0.f};
+                        mma_f16_k8(c, kz[u][0][g / 2], kz[u][1][g / 2], qs);
 #pragma unroll
                         for (int ks = 0; ks < 2; ++ks) {
                             const uint32_t w0 = ks ? kw[u][0][g] >> 8 : kw[u][0][g], w1 = ks ? kw[u][1][g] >> 8 : kw[u][1][g];
@@ -363,33 +386,39 @@ again:
             }
         }
         // ---------------- weights
+        if (p.cap_log2 > 0.f) {                                    // (fac is 1 then)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {                  // float32 rows: 2^-22 of a cap of 50 would be a weight's 17th bit
+                        float& x = s[u][j][i];
+                        x *= fac_s[8 * j + 2 * t + (i & 1)];
+                        if constexpr (DT == 0) x = p.cap_log2 * tanhf(x / p.cap_log2);
+                        else x = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(x * (2.885390043f / p.cap_log2))));
+                    }
+        }
+        if (edge) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = key0 + 16 * u + 8 * (i >> 1) + gl, last = lim[j][i & 1];
+                        if (key > last || key >= end || (p.window > 0 && key <= last - p.window) || !((have[stage] >> u) & 1u)) s[u][j][i] = -INFINITY;
+                    }
+        }
         bool up = false;
         float top[NT][2];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float best = -INFINITY;
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        float x = s[u][j][2 * r + c] * fac[j][c];
-                        if (p.cap_log2 > 0.f) {                    // float32 rows: 2^-22 of a cap of 50 would be a weight's 22nd bit
-                            if constexpr (DT == 0) x = p.cap_log2 * tanhf(x / p.cap_log2);
-                            else x = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(x * (2.885390043f / p.cap_log2))));
-                        }
-                        if (edge) {
-                            const int key = key0 + 16 * u + 8 * r + gl;
-                            if (key > lim[j][c] || key >= end || (p.window > 0 && key <= lim[j][c] - p.window) || !((have[stage] >> u) & 1u)) x = -INFINITY;
-                        }
-                        s[u][j][2 * r + c] = x;
-                        best = fmaxf(best, x);
-                    }
-                top[j][c] = best;
-                up |= best > m[j][c] + 8.f;
+                top[j][c] = fmaxf(fmaxf(s[0][j][c], s[0][j][2 + c]), fmaxf(s[1][j][c], s[1][j][2 + c])) * fac[j][c];
+                up |= top[j][c] > m[j][c] + 8.f;
             }
-        }
         if (__any_sync(0xffffffffu, up)) {                         // a reference moves when its maximum has grown by 2^8 (or at all at first)
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -416,61 +445,72 @@ again:
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const float base = m[j][c] == -INFINITY ? 0.f : m[j][c];
+                // Weights are 2^64 times theirs.  In rows of 16 bits the exponent has it, whose rounding then is 2^-18.
+                const float base = (m[j][c] == -INFINITY ? 0.f : -m[j][c]) + (DT == 0 ? 0.f : 64.f);
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const float w = ex2(s[u][j][2 * r + c] - base);
+                        float w = ex2(fmaf(s[u][j][2 * r + c], fac[j][c], base));
+                        if constexpr (DT == 0) w *= F_LIFT;
                         l[j][c] += w;
-                        s[u][j][2 * r + c] = w * F_LIFT;
+                        s[u][j][2 * r + c] = w;
                     }
             }
-        // ---------------- values
+        // ---------------- values: one run of instructions for blocks without an edge
+        auto values = [&](auto special) {
+            constexpr bool SPECIAL = decltype(special)::value;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            uint32_t vw[4][G], vz[4][MW], vm[2][MW];
+            for (int u = 0; u < 2; ++u) {
+                uint32_t vw[4][G], vz[4][MW], vm[2][MW];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = 16 * u + 2 * t + (i & 1) + 8 * (i >> 1);
-                lds_codes<G>(vc, row, gl >> 1, vw[i]);
-                lds_groups<G>(vwords + row * 2 * G, vz[i]);
-            }
+                for (int i = 0; i < 4; ++i) {
+                    const int row = 16 * u + 2 * t + (i & 1) + 8 * (i >> 1);
+                    lds_codes<G>(vc, row, gl >> 1, vw[i]);
+                    lds_groups<G>(vwords + row * 2 * G, vz[i]);
+                }
 #pragma unroll
-            for (int r = 0; r < 2; ++r) lds_groups<G>(vwords + (16 * u + 8 * r + gl) * 2 * G, vm[r]);
+                for (int r = 0; r < 2; ++r) lds_groups<G>(vwords + (16 * u + 8 * r + gl) * 2 * G, vm[r]);
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const uint32_t v0 = __byte_perm(vw[0][g], vw[1][g], half_sel), v1 = __byte_perm(vw[2][g], vw[3][g], half_sel);
-                const uint32_t zmask = gl == g ? 0x000f000fu : 0u;
-                const uint32_t z0 = __byte_perm(vz[0][g / 2], vz[1][g / 2], g & 1 ? 0x7632 : 0x5410) & zmask;
-                const uint32_t z1 = __byte_perm(vz[2][g / 2], vz[3][g / 2], g & 1 ? 0x7632 : 0x5410) & zmask;
-                const float s0 = group_scale(vm[0][g / 2], g & 1), s1 = group_scale(vm[1][g / 2], g & 1);
+                for (int g = 0; g < G; ++g) {
+                    const uint32_t v0 = __byte_perm(vw[0][g], vw[1][g], half_sel), v1 = __byte_perm(vw[2][g], vw[3][g], half_sel);
+                    const uint32_t v2 = BYTES ? __byte_perm(v0, 0, 0x4341) : v0 >> 8, v3 = BYTES ? __byte_perm(v1, 0, 0x4341) : v1 >> 8;
+                    const uint32_t zmask = gl == g ? 0x000f000fu : 0u;
+                    const uint32_t z0 = __byte_perm(vz[0][g / 2], vz[1][g / 2], g & 1 ? 0x7632 : 0x5410) & zmask;
+                    const uint32_t z1 = __byte_perm(vz[2][g / 2], vz[3][g / 2], g & 1 ? 0x7632 : 0x5410) & zmask;
+                    const float s0 = group_scale(vm[0][g / 2], g & 1), s1 = group_scale(vm[1][g / 2], g & 1);
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    float w[4] = {s[u][j][0] * s0, s[u][j][1] * s0, s[u][j][2] * s1, s[u][j][3] * s1};
-                    if (edge) {                                    // a key that is not seen may have any bytes for a scale
+                    for (int j = 0; j < NT; ++j) {
+                        float w[4] = {s[u][j][0] * s0, s[u][j][1] * s0, s[u][j][2] * s1, s[u][j][3] * s1};
+                        if constexpr (SPECIAL) {                   // a key that is not seen may have any bytes for a scale
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (s[u][j][i] == 0.f) w[i] = 0.f;
-                    }
+                            for (int i = 0; i < 4; ++i)
+                                if (s[u][j][i] == 0.f) w[i] = 0.f;
+                        }
 #pragma unroll
-                    for (int term = 0; term < PT; ++term) {
-                        const uint32_t lo = pack_bf16x2(w[0], w[1]), hi = pack_bf16x2(w[2], w[3]);
-                        const uint32_t p0 = transposed(lo), p1 = transposed(hi);
-                        mma_bf16(acc[2 * g][j], v0 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x000f000fu, v1 & 0x00f000f0u, p0, p1);
-                        mma_bf16(acc[2 * g + 1][j], (v0 >> 8) & 0x000f000fu, (v0 >> 8) & 0x00f000f0u, (v1 >> 8) & 0x000f000fu, (v1 >> 8) & 0x00f000f0u, p0, p1);
-                        if (careful)
-                            mma_bf16(zac[j], z0, 0u, z1, 0u, transposed(pack_bf16x2(finite(w[0]), finite(w[1]))), transposed(pack_bf16x2(finite(w[2]), finite(w[3]))));
-                        else
-                            mma_bf16(zac[j], z0, 0u, z1, 0u, p0, p1);
-                        if (term + 1 < PT) {
-                            w[0] -= bf16lo(lo); w[1] -= bf16hi(lo);
-                            w[2] -= bf16lo(hi); w[3] -= bf16hi(hi);
+                        for (int term = 0; term < PT; ++term) {
+                            const uint32_t lo = pack_bf16x2(w[0], w[1]), hi = pack_bf16x2(w[2], w[3]);
+                            const uint32_t p0 = transposed(lo), p1 = transposed(hi);
+                            mma_bf16(acc[2 * g][j], v0 & LOW, v0 & 0x00f000f0u, v1 & LOW, v1 & 0x00f000f0u, p0, p1);
+                            mma_bf16(acc[2 * g + 1][j], BYTES ? v2 : v2 & LOW, v2 & 0x00f000f0u, BYTES ? v3 : v3 & LOW, v3 & 0x00f000f0u, p0, p1);
+                            if constexpr (SPECIAL) {
+                                float y[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) y[i] = careful ? finite(w[i]) : w[i];
+                                mma_bf16(zac[j], z0, 0u, z1, 0u, transposed(pack_bf16x2(y[0], y[1])), transposed(pack_bf16x2(y[2], y[3])));
+                            } else
+                                mma_bf16(zac[j], z0, 0u, z1, 0u, p0, p1);
+                            if (term + 1 < PT) {
+                                w[0] -= bf16lo(lo); w[1] -= bf16hi(lo);
+                                w[2] -= bf16lo(hi); w[3] -= bf16hi(hi);
+                            }
                         }
                     }
                 }
             }
-        }
+        };
+        if (edge || careful) values(Yes{});
+        else values(No{});
     }
     cp_async_wait<0>();
     // The groups' sums of w s z share a product's rows: a scale that is NaN, in one group, would reach the others as 0 NaN.  Then once more, without it there.
@@ -499,12 +539,13 @@ again:
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const int col = 8 * j + 2 * t + c;
-            if (gl == 0) { wm[warp][col] = m[j][c]; wl[warp][col] = l[j][c]; }
+            if (gl == 0) { wm[warp][col] = m[j][c]; wl[warp][col] = l[j][c] * (1.f / F_LIFT); }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const float z = __shfl_sync(0xffffffffu, zac[j][c], g * 4 + t) * even;
-                const float4 o = make_float4(fmaf(acc[2 * g][j][c], even, -z), fmaf(acc[2 * g][j][2 + c], odd, -z), fmaf(acc[2 * g + 1][j][c], even, -z),
-                                       fmaf(acc[2 * g + 1][j][2 + c], odd, -z));
+                const float a0 = BYTES ? acc[2 * g][j][c] - acc[2 * g][j][2 + c] : acc[2 * g][j][c];
+                const float a2 = BYTES ? acc[2 * g + 1][j][c] - acc[2 * g + 1][j][2 + c] : acc[2 * g + 1][j][c];
+                const float4 o = make_float4(fmaf(a0, even, -z), fmaf(acc[2 * g][j][2 + c], odd, -z), fmaf(a2, even, -z), fmaf(acc[2 * g + 1][j][2 + c], odd, -z));
                 *(float4*)(fold + ((size_t)warp * ROWS + col) * DP + 32 * g + 4 * gl) = o;
             }
         }
@@ -580,25 +621,38 @@ again:
     if (p.splits > 1) cluster_sync();                              // nobody leaves while another reads
 }
 
-template <int G, int NT, int DT>
+// Blocks of a cluster that share a sequence's keys.  Time in a warp's blocks of 32 keys (2.3 us with all warps at work): a block's own, and what it
+// spends at its two ends, about five of them, or the SMs' share of all blocks.  Measured (us, 1 / 2 / 4 / 8 of four warps): 64 sequences over 8192 keys, 8
+// heads 161 / 146 / 153 / 173; 8 with five rows over 3000 51.7 / 31.9 / 38.3 / 44.2; one over 4096 36.4 / 22.1 / 14.3 / 10.7, of eight warps 9.8.
+struct Cut { int splits; float cost; };
+Cut few_cut(const Kv4AttnParams& p, int rows, int warps, int resident) {
+    const long long tiles = ((long long)p.max_rows * p.rep + rows - 1) / rows, items = p.seqs * tiles * p.k.kv_heads;
+    const int keys = p.window > 0 && p.window < p.max_keys - p.max_rows ? p.window + p.max_rows : p.max_keys;
+    const int nb = (keys + F_KEYS - 1) / F_KEYS;
+    Cut best = {1, 0.f};
+    for (int s = 1; s <= F_CLUSTER; s *= 2) {
+        const float each = (float)(((nb + s - 1) / s + warps - 1) / warps + 5), all = (float)(items * s) * each / (float)(sm_count() * resident);
+        const float cost = each > all ? each : all;
+        if (s == 1 || cost < best.cost) best = {s, cost};
+    }
+    return best;
+}
+
+template <int G, int NT, int DT, int W>
 cudaError_t launch_few(Kv4AttnParams p, cudaStream_t st) {
-    constexpr int bytes = FewSmem<G, NT, DT>::BYTES;
-    static_assert(bytes <= 220 * 1024);
+    using Smem = Few<G, NT, DT, W>;
+    static_assert(Smem::BYTES <= 220 * 1024);
     static bool configured = false;
     if (!configured) {
-        if (cudaError_t e = cudaFuncSetAttribute(kv4_few_kernel<G, NT, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+        if (cudaError_t e = cudaFuncSetAttribute(kv4_few_kernel<G, NT, DT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem::BYTES)) return e;
         configured = true;
     }
     p.tiles = (int)(((long long)p.max_rows * p.rep + 8 * NT - 1) / (8 * NT));
-    const long long items = (long long)p.seqs * p.tiles * p.k.kv_heads;
-    const int keys = p.window > 0 && p.window + p.max_rows < p.max_keys ? p.window + p.max_rows : p.max_keys;
-    const int nb = (keys + F_KEYS - 1) / F_KEYS, most = (nb + Few<G>::WARPS - 1) / Few<G>::WARPS;
-    p.splits = 1;
-    while (p.splits < F_CLUSTER && p.splits < most && items * p.splits * 2 <= 2 * sm_count()) p.splits *= 2;
+    p.splits = few_cut(p, 8 * NT, W, Smem::RESIDENT).splits;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.seqs * p.tiles), p.k.kv_heads, p.splits);
-    cfg.blockDim = dim3(Few<G>::THREADS);
-    cfg.dynamicSmemBytes = bytes;
+    cfg.blockDim = dim3(Smem::THREADS);
+    cfg.dynamicSmemBytes = Smem::BYTES;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -610,7 +664,7 @@ cudaError_t launch_few(Kv4AttnParams p, cudaStream_t st) {
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     count_launch();
-    return cudaLaunchKernelEx(&cfg, kv4_few_kernel<G, NT, DT>, p);
+    return cudaLaunchKernelEx(&cfg, kv4_few_kernel<G, NT, DT, W>, p);
 }
 
 // Eight rows a column block: as many blocks as the rows of a sequence's group need, up to what the accumulators' registers allow (G NT <= 8)
@@ -618,12 +672,13 @@ template <int G, int DT>
 cudaError_t launch_few_rows(const Kv4AttnParams& p, cudaStream_t st) {
     const long long rows = (long long)p.max_rows * p.rep;
     if constexpr (G <= 2) {
-        if (rows > 16) return launch_few<G, 4, DT>(p, st);
+        if (rows > 16) return launch_few<G, 4, DT, 4>(p, st);
     }
     if constexpr (G <= 4) {
-        if (rows > 8) return launch_few<G, 2, DT>(p, st);
+        if (rows > 8) return launch_few<G, 2, DT, 4>(p, st);
+        if (few_cut(p, 8, 8, Few<G, 1, DT, 8>::RESIDENT).cost < few_cut(p, 8, 4, Few<G, 1, DT, 4>::RESIDENT).cost) return launch_few<G, 1, DT, 8>(p, st);
     }
-    return launch_few<G, 1, DT>(p, st);
+    return launch_few<G, 1, DT, 4>(p, st);
 }
 template <int DT>
 cudaError_t launch_few_dim(const Kv4AttnParams& p, cudaStream_t st) {
@@ -669,6 +724,15 @@ extern "C" int pgk_kv4_attention(const void* q, long q_ld, const void* k_cache, 
     p.scale_log2 = (scale > 0.f ? scale : 1.f / sqrtf((float)dim)) * 1.4426950408889634f;
     p.cap_log2 = softcap * 1.4426950408889634f;
     p.window = window; p.sinks = sinks;
+    p.head_bytes = (long long)page_size * kv4_row_bytes(dim);
+    p.page_bytes = p.head_bytes * kv_heads;
+    const uint32_t sub = (uint32_t)page_size / 16;                 // n < 2^27 and sub <= 2^8: exact with a multiplier of 32 bits
+    if (sub > 1) {
+        uint32_t log = 0;
+        while ((1u << log) < sub) ++log;
+        p.page_shift = log > 5 ? log - 5 : 0;
+        p.page_mul = (uint32_t)((1ull << (32 + p.page_shift)) / sub) + 1;
+    }
     const int size = dtype == 0 ? 4 : 2;
     p.wide_o = (uintptr_t)out % 16 == 0 && o_ld * size % 16 == 0;
     const cudaStream_t st = (cudaStream_t)stream;
