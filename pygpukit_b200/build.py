@@ -63,6 +63,7 @@ SOURCES = {
     "seq_gla.cu": [],
     "kv4_cache.cu": [],
     "kv4_attention.cu": [],
+    "kv4_prompt.cu": [],
     "beam.cu": [],
 }
 

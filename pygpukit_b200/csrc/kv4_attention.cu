@@ -20,7 +20,7 @@
 // the warps fold in shared memory, and where a sequence's keys are cut over the blocks of a cluster, these fold through distributed shared memory.
 //
 // A row that sees no key gives zeros.
-#include "kv4.cuh"
+#include "kv4_attention.cuh"
 #include "tc_common.cuh"
 #include "../../include/pgk_b200.h"
 
@@ -29,21 +29,6 @@ namespace pgk {
 int kv4_check(const char* fn, const void* data, int pages, int page_size, const void* table, int slots, int max_pages, int kv_heads, int dim);
 
 namespace {
-
-struct Kv4AttnParams {
-    const void* q; void* out;
-    long q_ld, o_ld;
-    Kv4Pages k;
-    const unsigned char* v_data;
-    const int32_t* seq_slots; const int32_t* contexts; const int32_t* starts;      // starts NULL: a row a sequence
-    int seqs, tokens, max_rows, max_keys, heads, rep, tiles, splits;
-    float scale_log2, cap_log2;           // scale log2 e; cap log2 e or 0
-    int window;
-    const float* sinks;
-    bool wide_o;
-    uint32_t page_mul, page_shift;        // n / (page_size / 16) = hi(n page_mul) >> page_shift; page_mul 0: pages of 16
-    long long page_bytes, head_bytes;
-};
 
 constexpr int F_KEYS = 32, F_STAGES = 2, F_CLUSTER = 8;
 constexpr float F_LIFT = 18446744073709551616.f;                   // 2^64
@@ -140,25 +125,6 @@ __device__ __forceinline__ float row_element(const void* q, size_t i) {
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 __device__ __forceinline__ float finite(float v) { return fabsf(v) < INFINITY ? v : 0.f; }
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t remote(uint32_t at, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ float remote_float(uint32_t at) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-    return v;
-}
-__device__ __forceinline__ float4 remote_float4(uint32_t at) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-    return v;
-}
-
 template <int G, int NT, int DT, int W>
 __global__ void __launch_bounds__(Few<G, NT, DT, W>::THREADS, Few<G, NT, DT, W>::RESIDENT) kv4_few_kernel(const __grid_constant__ Kv4AttnParams p) {
     using Smem = Few<G, NT, DT, W>;
@@ -193,7 +159,7 @@ __global__ void __launch_bounds__(Few<G, NT, DT, W>::THREADS, Few<G, NT, DT, W>:
     const unsigned char* const khead = p.k.data + (size_t)head * p.head_bytes + lane * 16;
     const unsigned char* const vhead = p.v_data + (size_t)head * p.head_bytes + lane * 16;
     const int code_bytes = p.k.page_size * 16 * G;
-    auto page_of = [&](uint32_t n) { return p.page_mul ? __umulhi(n, p.page_mul) >> p.page_shift : n; };
+    auto page_of = [&](uint32_t n) { return kv4_page_of(p, n); };
     auto pages_of = [&](int b, int (&pg)[2]) {                     // of the block's two halves; -1: nothing to see there
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -734,8 +700,13 @@ extern "C" int pgk_kv4_attention(const void* q, long q_ld, const void* k_cache, 
         p.page_mul = (uint32_t)((1ull << (32 + p.page_shift)) / sub) + 1;
     }
     const int size = dtype == 0 ? 4 : 2;
+    p.wide_q = (uintptr_t)q % 16 == 0 && q_ld * size % 16 == 0;
     p.wide_o = (uintptr_t)out % 16 == 0 && o_ld * size % 16 == 0;
     const cudaStream_t st = (cudaStream_t)stream;
+    if (kv4_prompt_serves(p, dtype)) {
+        PGK_CUDA(kv4_prompt(p, dtype, st));
+        return 0;
+    }
     PGK_CUDA(dtype == 0 ? launch_few_dim<0>(p, st) : (dtype == 1 ? launch_few_dim<1>(p, st) : launch_few_dim<2>(p, st)));
     return 0;
 }

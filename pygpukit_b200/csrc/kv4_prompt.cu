@@ -1,0 +1,508 @@
+// kv4_prompt.cu -- attention of many rows a sequence (prompts, portions of them) over the four-bit paged cache on tcgen05; the mathematics of
+// kv4_attention.cu, for rows of 16 bits and heads of 64, 96 and 128 elements.
+//
+// A block has 128 rows (a token's query heads of one key head beside each other) and walks over tiles of 128 keys:
+//   * four warps expand a tile of K, then of V, to bfloat16 in shared memory -- s (c - z) is a bfloat16 number, nothing is rounded: a nibble under
+//     the exponent of 128 is 128 + c, one subtraction and one product for two elements.  Their loads run one tile ahead, in registers;
+//   * one warp issues S = Q K^T (queries in tensor memory, float16 ones as two bfloat16 terms) and O += P V, the scores of tile i + 1 behind the
+//     weights of tile i;
+//   * eight warps, a lane a row and two warps a row, turn scores into weights; a weight is rounded to bfloat16 once (2^-9 of it, independent from
+//     key to key, beside the output's own 2^-9), their sum is float32 of the unrounded ones.  A row's reference moves when its maximum has grown by 2^8.
+// The eight elements of a word of codes keep the order (0, 4, 1, 5, 2, 6, 3, 7) that its nibbles fall into: queries are brought into it, outputs back.
+// What bounds it: for 128 x 128 x 128 the MMAs take 1232 cycles, exponentials 1024 of the special unit, expansion and weights 640 issue slots each.
+// Few blocks share a sequence's keys within a cluster and fold through distributed shared memory.
+//
+// A value of NaN counts as zero in the products (0 NaN would reach rows that do not see it); where any was met, rows look for the ones they see
+// in the end.
+#include "kv4_attention.cuh"
+#include "tc_common.cuh"
+#include "../../include/pgk_b200.h"
+
+namespace pgk {
+
+namespace {
+
+constexpr int P_ROWS = 128, P_KEYS = 128, P_SOFT = 8, P_EXPAND = 4, P_THREADS = (P_SOFT + 1 + P_EXPAND) * 32, P_STAGES = 2, P_CLUSTER = 8;
+constexpr uint32_t P_CHUNK = P_KEYS * 128;                         // 64 elements of 128 keys
+constexpr uint32_t P_O = 0, P_Q = 128, P_S = 256;                  // TMEM columns: outputs, queries (two terms of 64), two tiles of scores
+constexpr float P_LAZY = 8.f;
+
+template <int G> struct Prompt {
+    static constexpr int D = 32 * G, DN = G == 2 ? 64 : 128;       // 96 elements: the products go on to 128 over zeros
+    static constexpr uint32_t TILE = (DN / 64) * P_CHUNK;
+    static constexpr int RING = 2 * P_STAGES * TILE, FOLD = P_ROWS * (D + 4) * 4, BYTES = (RING > FOLD ? RING : FOLD) + 1024;
+};
+
+__device__ __forceinline__ bool all_wait(int* err, uint64_t* bar, uint32_t parity) {
+    const bool ok = bar_wait(err, smem_u32(bar), parity);
+    return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ uint32_t bf2_add(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t bf2_mul(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+template <int G, int DT>
+__global__ void __launch_bounds__(P_THREADS, 1) kv4_prompt_kernel(const __grid_constant__ Kv4AttnParams p, int* err) {
+    using C = Prompt<G>;
+    constexpr int D = C::D, DN = C::DN, QT = DT == 1 ? 2 : 1, MW = (G + 1) / 2;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ __align__(8) uint64_t kfull[P_STAGES], kempty[P_STAGES], vfull[P_STAGES], vempty[P_STAGES], sfull[2], pready, pvdone;
+    __shared__ uint32_t tmem_base_s;
+    __shared__ float wmax[2][2][P_ROWS], row_m[P_ROWS], row_l[P_ROWS];
+    __shared__ int missing, nans;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const uint32_t ks = (smem_u32(smem) + 1023u) & ~1023u, vs = ks + P_STAGES * C::TILE;
+
+    if (warp == P_SOFT) tmem_alloc(&tmem_base_s, 512);
+    if (tid == 0) {
+        for (int s = 0; s < P_STAGES; ++s) {
+            mbar_init(&kfull[s], P_EXPAND); mbar_init(&kempty[s], 1);
+            mbar_init(&vfull[s], P_EXPAND); mbar_init(&vempty[s], 1);
+        }
+        mbar_init(&sfull[0], 1); mbar_init(&sfull[1], 1);
+        mbar_init(&pready, P_SOFT); mbar_init(&pvdone, 1);
+        mbar_fence_init();
+        missing = nans = 0;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_s;
+    griddep_wait();
+    griddep_launch();
+
+    // the longest rows first
+    const int seq = blockIdx.x % p.seqs, f0 = (p.tiles - 1 - (int)(blockIdx.x / p.seqs)) * P_ROWS, head = blockIdx.y, split = blockIdx.z;
+    const int slot = __ldcg(p.seq_slots + seq), ctx = __ldcg(p.contexts + seq);
+    const int first = p.starts ? __ldcg(p.starts + seq) : seq, n_rows = p.starts ? __ldcg(p.starts + seq + 1) - first : 1;
+    const int rows = min(min(n_rows, p.max_rows), 0x7fffffff / p.rep) * p.rep;
+    const bool work = f0 < rows && (unsigned)slot < (unsigned)p.k.slots;                   // the same in all of the cluster
+    const int live_rows = work ? min(P_ROWS, rows - f0) : 0;
+    const int pos0 = ctx - n_rows + f0 / p.rep, pos1 = ctx - n_rows + (f0 + max(live_rows, 1) - 1) / p.rep;
+    const int begin = p.window > 0 ? max(0, pos0 - p.window + 1) : 0, end = work ? min(min(pos1 + 1, ctx), p.max_keys) : 0;
+    const int t0 = begin / P_KEYS, nt = max(0, (end + P_KEYS - 1) / P_KEYS - t0), per = (nt + p.splits - 1) / p.splits;
+    const int tbeg = t0 + split * per, n = max(0, min(nt, (split + 1) * per) - split * per);
+    const int32_t* const table = p.k.table + (work ? (size_t)slot * p.k.max_pages : 0);
+
+    // row r of the block: which one of the sequence's, and what it sees
+    const int quad = warp & 3, half = (warp >> 2) & 1, row = quad * 32 + lane, f = f0 + row, tok = first + f / p.rep;
+    const int h = head * p.rep + f % p.rep, pos = ctx - n_rows + f / p.rep;
+    const bool live = warp < P_SOFT && row < live_rows && tok >= 0 && tok < p.tokens;
+
+    if (warp < 4) {                                // queries to tensor memory
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            uint32_t a[16], b[16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint16_t* src = (const uint16_t*)p.q + (size_t)tok * p.q_ld + (size_t)h * D + c + 8 * i;
+                uint32_t w[4] = {};
+                if (live) {
+                    if (p.wide_q) {
+                        const uint4 v = ld_act16(src);
+                        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = (uint32_t)ld_act2(src + 2 * e) | (uint32_t)ld_act2(src + 2 * e + 1) << 16;
+                    }
+                }
+                uint32_t v[4] = {__byte_perm(w[0], w[2], 0x5410), __byte_perm(w[0], w[2], 0x7632), __byte_perm(w[1], w[3], 0x5410), __byte_perm(w[1], w[3], 0x7632)};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (DT == 1) {
+                        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v[e]));
+                        a[4 * i + e] = pack_bf16x2(x.x, x.y);
+                        b[4 * i + e] = pack_bf16x2(x.x - bf16lo(a[4 * i + e]), x.y - bf16hi(a[4 * i + e]));
+                    } else
+                        a[4 * i + e] = v[e];
+                }
+            }
+            __syncwarp();
+            const uint32_t to = tmem + ((uint32_t)(quad * 32) << 16) + P_Q + (uint32_t)c / 2u;
+            tmem_st16u(to, a);
+            if constexpr (QT == 2) tmem_st16u(to + 64u, b);
+        }
+        tmem_st_wait();
+    } else {                                       // does a page of these keys not exist?
+        bool gone = false;
+        const int last = min(end, (tbeg + n) * P_KEYS);
+        for (int j = tbeg * P_KEYS + 16 * (tid - 128); j < last; j += 16 * (P_THREADS - 128))
+            gone |= (unsigned)__ldcg(table + kv4_page_of(p, (uint32_t)j >> 4)) >= (unsigned)p.k.pages;
+        if (gone) missing = 1;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+
+    if (warp == P_SOFT) {
+        // ---------------- MMAs
+        constexpr uint32_t id_s = umma_idesc_bf16(P_KEYS), id_o = umma_idesc_bf16(DN) | (1u << 16);       // values: the elements are contiguous
+        bool ok = true;
+        auto scores = [&](int i) {                 // where the weights of tile i - 2 were
+            const int s = i % P_STAGES;
+            ok = ok && all_wait(err, &kfull[s], (uint32_t)(i / P_STAGES) & 1u);
+            if (!ok) return;
+            if (elect_one()) {
+                tc_fence_after();
+#pragma unroll
+                for (int term = QT - 1; term >= 0; --term)
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        umma_bf16_ta(tmem + P_S + (uint32_t)(i & 1) * 128u, tmem + P_Q + (uint32_t)term * 64u + (uint32_t)k * 8u,
+                                     desc_sw128(ks + s * C::TILE + (uint32_t)(k >> 2) * P_CHUNK) + (uint64_t)((k & 3) * 2), id_s, k || term < QT - 1 ? 1u : 0u);
+                umma_commit(&sfull[i & 1]);
+                umma_commit(&kempty[s]);
+            }
+            __syncwarp();
+        };
+        if (n > 0) scores(0);
+        for (int i = 0; ok && i < n; ++i) {
+            const int s = i % P_STAGES;
+            if (i > 0) ok = all_wait(err, &pvdone, (uint32_t)((i - 1) & 1));
+            if (ok && i + 1 < n) scores(i + 1);
+            ok = ok && all_wait(err, lane & 1 ? &vfull[s] : &pready, lane & 1 ? (uint32_t)(i / P_STAGES) & 1u : (uint32_t)(i & 1));
+            if (!ok) break;
+            if (elect_one()) {
+                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < P_KEYS / 16; ++k)             // 16 keys: 2048 bytes of V
+                    umma_bf16_ta(tmem + P_O, tmem + P_S + (uint32_t)(i & 1) * 128u + (uint32_t)k * 8u, desc_mn_sw128(vs + s * C::TILE, P_CHUNK) + (uint64_t)(k * 128),
+                                 id_o, (i | k) ? 1u : 0u);
+                umma_commit(&pvdone);
+                umma_commit(&vempty[s]);
+            }
+            __syncwarp();
+        }
+    } else if (warp > P_SOFT) {
+        // ---------------- tiles of K and V, expanded
+        const int w = warp - P_SOFT - 1, q = lane >> 2, t = lane & 3, kq = (q >> 1) + 4 * (q & 1);        // two quads of an access: keys 4 apart, all banks
+        const unsigned char* const khead = p.k.data + (size_t)head * p.head_bytes;
+        const unsigned char* const vhead = p.v_data + (size_t)head * p.head_bytes;
+        const int code_bytes = p.k.page_size * 16 * G;
+        if constexpr (G == 3) {                    // elements 96 ... 127 of V
+            for (int i = tid - (P_SOFT + 1) * 32; i < P_STAGES * P_KEYS * 4; i += P_EXPAND * 32) {
+                const int s = i / (P_KEYS * 4), key = i / 4 % P_KEYS;
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" :: "r"(vs + s * C::TILE + P_CHUNK + key * 128 + (((4 + i % 4) ^ (key & 7)) * 16)), "r"(0) : "memory");
+            }
+        }
+        struct Raw { uint32_t c[4][G], m[4][MW]; };
+        Raw kr, vr;
+        int pg[2], ahead[2];                       // pages of the warp's two runs of 16 keys; of the tile after
+        auto pages = [&](int i, int (&to)[2]) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int j = (tbeg + i) * P_KEYS + 32 * w + 16 * u;
+                to[u] = i < n && j < end ? __ldcg(table + kv4_page_of(p, (uint32_t)j >> 4)) : -1;
+            }
+        };
+        auto load = [&](const unsigned char* base, int i, Raw& r) {
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+                const int j = (tbeg + i) * P_KEYS + 32 * w + 8 * it + kq;
+                const bool there = j >= begin && j < end && (unsigned)pg[it >> 1] < (unsigned)p.k.pages;
+#pragma unroll
+                for (int g = 0; g < G; ++g) r.c[it][g] = 0;
+#pragma unroll
+                for (int g = 0; g < MW; ++g) r.m[it][g] = 0;
+                if (there) {
+                    const int in_page = j - (int)(kv4_page_of(p, (uint32_t)j >> 4) * (uint32_t)p.k.page_size);
+                    const unsigned char* at = base + pg[it >> 1] * p.page_bytes;
+                    const unsigned char* codes = at + in_page * (16 * G) + t * 4 * G;
+                    const unsigned char* words = at + code_bytes + in_page * (2 * G);
+                    if constexpr (G == 4) {
+                        const uint4 v = ld_act16(codes);
+                        r.c[it][0] = v.x; r.c[it][1] = v.y; r.c[it][2] = v.z; r.c[it][3] = v.w;
+                        const uint2 m = __ldcg((const uint2*)words);
+                        r.m[it][0] = m.x; r.m[it][1] = m.y;
+                    } else if constexpr (G == 2) {
+                        const uint2 v = __ldcg((const uint2*)codes);
+                        r.c[it][0] = v.x; r.c[it][1] = v.y;
+                        r.m[it][0] = __ldcg((const uint32_t*)words);
+                    } else {
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            r.c[it][g] = __ldcg((const uint32_t*)codes + g);
+                            r.m[it][g / 2] |= (uint32_t)ld_act2((const uint16_t*)words + g) << (16 * (g & 1));
+                        }
+                    }
+                }
+            }
+        };
+        bool nan = false;
+        auto expand = [&](const Raw& r, uint32_t tile, bool values) {
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+                const int key = 32 * w + 8 * it + kq;
+                const uint32_t to = tile + key * 128;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    uint32_t m = __byte_perm(r.m[it][g / 2], 0, g & 1 ? 0x3232 : 0x1010);
+                    if (values && (m & 0x7f80u) == 0x7f80u) { nan = true; m = 0; }
+                    const uint32_t zero = (m & 0x000f000fu) | 0xc300c300u, scale = m & 0x7ff07ff0u;        // -(128 + z), s
+                    const uint32_t x = r.c[it][g];
+                    uint32_t y[4] = {x, x >> 4, x >> 8, x >> 12};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = bf2_mul(bf2_add((y[e] & 0x000f000fu) | 0x43004300u, zero), scale);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                                 :: "r"(to + (uint32_t)(g >> 1) * P_CHUNK + (((4 * (g & 1) + t) ^ (key & 7)) * 16)), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+        };
+        pages(0, pg);
+        load(khead, 0, kr);
+        load(vhead, 0, vr);
+        pages(1, ahead);
+        bool ok = true;
+        for (int i = 0; i < n; ++i) {
+            const int s = i % P_STAGES;
+            const uint32_t free = (((uint32_t)i / P_STAGES) & 1u) ^ 1u;
+            ok = ok && all_wait(err, &kempty[s], free);
+            if (!ok) break;
+            expand(kr, ks + s * C::TILE, false);
+            if (lane == 0) mbar_arrive(&kfull[s]);
+            pg[0] = ahead[0]; pg[1] = ahead[1];
+            if (i + 1 < n) load(khead, i + 1, kr);
+            pages(i + 2, ahead);
+            ok = ok && all_wait(err, &vempty[s], free);
+            if (!ok) break;
+            expand(vr, vs + s * C::TILE, true);
+            if (lane == 0) mbar_arrive(&vfull[s]);
+            if (i + 1 < n) load(vhead, i + 1, vr);
+        }
+        if (nan) nans = 1;
+    } else {
+        // ---------------- weights
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+        const int limit = live ? min(pos, end - 1) : -1, under = p.window > 0 ? pos - p.window : -1;       // sees (under, limit]
+        const int clean_lo = p.window > 0 ? pos1 - p.window : -1, clean_hi = missing ? -1 : min(pos0, end - 1);
+        const float fac = p.cap_log2 > 0.f ? 1.f : p.scale_log2;
+        float m = -INFINITY, neg = 0.f, l = 0.f;
+        bool ok = true;
+        for (int i = 0; i < n; ++i) {
+            const uint32_t at = lanes + P_S + (uint32_t)(i & 1) * 128u;
+            const int j0 = (tbeg + i) * P_KEYS + half * 64;
+            ok = ok && all_wait(err, &sfull[i & 1], (uint32_t)((i >> 1) & 1));
+            __syncwarp();
+            tc_fence_after();
+            float s[64];
+#pragma unroll
+            for (int c = 0; c < 64; c += 16) tmem_ld16_async(at + (uint32_t)(half * 64 + c), *(float (*)[16])(s + c));
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int c = 0; c < 64; c += 16) tmem_pass(*(float (*)[16])(s + c));
+            if (p.cap_log2 > 0.f) {
+                const float in = p.scale_log2 * 2.885390043f / p.cap_log2;
+#pragma unroll
+                for (int c = 0; c < 64; ++c) s[c] = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(s[c] * in)));
+            }
+            if (j0 <= clean_lo || j0 + 63 > clean_hi) {
+                uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+                if (missing) {                                    // four runs of 16 keys
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (j0 + 16 * u < end && (unsigned)__ldcg(table + kv4_page_of(p, (uint32_t)(j0 + 16 * u) >> 4)) >= (unsigned)p.k.pages) seen[u >> 1] &= ~(0xffffu << (16 * (u & 1)));
+                }
+#pragma unroll
+                for (int c = 0; c < 64; ++c)
+                    if (j0 + c > limit || j0 + c <= under || !((seen[c >> 5] >> (c & 31)) & 1u)) s[c] = -INFINITY;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 64; ++c) top = fmaxf(top, s[c]);
+            top *= fac;
+            wmax[i & 1][half][row] = top;
+            __syncwarp();
+            asm volatile("bar.sync %0, 64;" :: "r"(1 + quad) : "memory");          // the row's two warps; both have read their scores
+            top = fmaxf(top, wmax[i & 1][half ^ 1][row]);
+            const bool up = top > m + P_LAZY;                     // (also the first finite maximum)
+            if (__any_sync(0xffffffffu, up)) {                    // the same in both warps: each has half of the outputs
+                const float fix = !up ? 1.f : (m == -INFINITY ? 0.f : exp2f(m - top));
+                if (up) { m = top; neg = -top; }
+                l *= fix;
+                if (i > 0) {
+                    ok = ok && all_wait(err, &pvdone, (uint32_t)((i - 1) & 1));
+                    __syncwarp();
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < DN / 2; c += 16) {
+                        float o[16];
+                        const uint32_t to = lanes + P_O + (uint32_t)(half * (DN / 2) + c);
+                        tmem_ld16(to, o);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] *= fix;
+                        tmem_st16(to, o);
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 64; c += 32) {                    // 32 keys: 16 columns
+                uint32_t y[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float a = ex2(fmaf(s[c + 2 * e], fac, neg)), b = ex2(fmaf(s[c + 2 * e + 1], fac, neg));
+                    l += a + b;
+                    y[e] = pack_bf16x2(a, b);
+                }
+                __syncwarp();
+                tmem_st16u(at + (uint32_t)(half * 32 + c / 2), y);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pready);
+        }
+        if (n > 0) all_wait(err, &pvdone, (uint32_t)((n - 1) & 1));
+        asm volatile("bar.sync %0, 64;" :: "r"(1 + quad) : "memory");              // the last tile's maxima are read
+        wmax[0][half][row] = l;
+        __syncwarp();
+        asm volatile("bar.sync %0, 64;" :: "r"(1 + quad) : "memory");
+        if (half == 0) { row_m[row] = m; row_l[row] = wmax[0][0][row] + wmax[0][1][row]; }
+    }
+    __syncthreads();                               // nobody's tile is read or written any more
+    tc_fence_after();
+    float* const fold = (float*)smem;              // [128][D + 4], with more than one block a sequence
+    auto finish = [&](int r, float& top, float sum) {              // what the row's outputs are multiplied by, sink and all
+        const int hr = head * p.rep + (f0 + r) % p.rep;
+        const float sink = p.sinks ? __ldcg(p.sinks + hr) * 1.4426950408889634f : -INFINITY, was = top;
+        top = fmaxf(top, sink);
+        sum = was == -INFINITY ? sum - sum : sum * exp2f(was - top);
+        if (sink != -INFINITY) sum += exp2f(sink - top);
+        return sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    };
+    if (warp < P_SOFT) {
+        uint32_t lost = 0;                         // groups of which the row sees a NaN
+        if (nans && live) {
+            const int from = max(begin, tbeg * P_KEYS), last = min(min(pos, end - 1), (tbeg + n) * P_KEYS - 1);
+            const int under = p.window > 0 ? pos - p.window : -1;
+            for (int j = max(from, under + 1); j <= last; ++j) {
+                const int page = __ldcg(table + kv4_page_of(p, (uint32_t)j >> 4));
+                if ((unsigned)page >= (unsigned)p.k.pages) continue;
+                const int in_page = j - (int)(kv4_page_of(p, (uint32_t)j >> 4) * (uint32_t)p.k.page_size);
+                const uint16_t* words = (const uint16_t*)(p.v_data + page * p.page_bytes + (size_t)head * p.head_bytes + (size_t)p.k.page_size * (16 * G)) + (size_t)in_page * G;
+                for (int g = 0; g < G; ++g)
+                    if ((ld_act2(words + g) & 0x7f80u) == 0x7f80u) lost |= 1u << g;
+            }
+        }
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+        float top = row_m[row];
+        const float was = top, inv = finish(row, top, row_l[row]) * (was == -INFINITY ? 1.f : exp2f(was - top));
+#pragma unroll 1
+        for (int c = half * (DN / 2); c < min(D, (half + 1) * (DN / 2)); c += 16) {
+            float o[16], x[16];
+            __syncwarp();
+            if (n > 0) tmem_ld16(lanes + P_O + (uint32_t)c, o);
+            else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = o[(e & 8) + (e & 4 ? 2 * (e & 3) + 1 : 2 * (e & 3))];
+            if ((lost >> (c / 32)) & 1u) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = NAN;
+            }
+            if (p.splits > 1) {
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) *(float4*)(fold + (size_t)row * (D + 4) + c + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+            } else if (live) {
+                uint16_t* dst = (uint16_t*)p.out + (size_t)tok * p.o_ld + (size_t)h * D + c;
+                uint32_t y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = kv4_pack2<DT>(x[2 * e] * inv, x[2 * e + 1] * inv);
+                if (p.wide_o) {
+                    *(uint4*)dst = make_uint4(y[0], y[1], y[2], y[3]);
+                    *(uint4*)(dst + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) { dst[2 * e] = (uint16_t)y[e]; dst[2 * e + 1] = (uint16_t)(y[e] >> 16); }
+                }
+            }
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == P_SOFT) tmem_dealloc(tmem, 512);
+    if (p.splits == 1) return;
+    // ---------------- the cluster's blocks into one: block r has every `splits`-th piece
+    cluster_sync();
+    const uint32_t fold_at = smem_u32(fold), m_at = smem_u32(row_m), l_at = smem_u32(row_l);
+    for (int i = split * P_THREADS + tid; i < live_rows * (D / 4); i += p.splits * P_THREADS) {
+        const int r = i / (D / 4), d = (i - r * (D / 4)) * 4, fr = f0 + r, to = first + fr / p.rep;
+        if (to < 0 || to >= p.tokens) continue;
+        float top = -INFINITY, sum = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < p.splits; ++s) top = fmaxf(top, remote_float(remote(m_at + 4 * r, s)));
+        for (int s = 0; s < p.splits; ++s) {
+            const float ms = remote_float(remote(m_at + 4 * r, s)), ls = remote_float(remote(l_at + 4 * r, s));
+            const float w = ms == -INFINITY ? ls - ls : exp2f(ms - top);
+            const float4 v = remote_float4(remote(fold_at + (r * (D + 4) + d) * 4, s));
+            sum = fmaf(w, ls, sum);
+            o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
+        }
+        const float was = top, inv = finish(r, top, sum) * (was == -INFINITY ? 1.f : exp2f(was - top));
+        const uint32_t a = kv4_pack2<DT>(o.x * inv, o.y * inv), b = kv4_pack2<DT>(o.z * inv, o.w * inv);
+        uint16_t* dst = (uint16_t*)p.out + (size_t)to * p.o_ld + (size_t)(head * p.rep + fr % p.rep) * D + d;
+        if (p.wide_o) *(uint2*)dst = make_uint2(a, b);
+        else { dst[0] = (uint16_t)a; dst[1] = (uint16_t)(a >> 16); dst[2] = (uint16_t)b; dst[3] = (uint16_t)(b >> 16); }
+    }
+    cluster_sync();                                // nobody leaves while another reads
+}
+
+template <int G, int DT>
+cudaError_t launch_prompt(Kv4AttnParams p, cudaStream_t st) {
+    static bool configured = false;
+    if (!configured) {
+        if (cudaError_t e = cudaFuncSetAttribute(kv4_prompt_kernel<G, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Prompt<G>::BYTES)) return e;
+        configured = true;
+    }
+    int* err = wait_word(kWaitKv4);
+    if (!err) return cudaErrorMemoryAllocation;
+    p.tiles = (int)(((long long)p.max_rows * p.rep + P_ROWS - 1) / P_ROWS);
+    // blocks of a cluster that share a sequence's keys: rounds of blocks times (their tiles + what a block costs besides, about four tiles)
+    const int keys = p.window > 0 && p.window < p.max_keys - P_ROWS ? p.window + P_ROWS : p.max_keys, nt = (keys + P_KEYS - 1) / P_KEYS;
+    const long long items = (long long)p.seqs * p.tiles * p.k.kv_heads;
+    long long least = 0;
+    for (int s = 1; s <= P_CLUSTER; s *= 2) {
+        const long long cost = ((items * s + sm_count() - 1) / sm_count()) * ((nt + s - 1) / s + 4);
+        if (s == 1 || cost < least) { p.splits = s; least = cost; }
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.seqs * p.tiles), p.k.kv_heads, p.splits);
+    cfg.blockDim = dim3(P_THREADS);
+    cfg.dynamicSmemBytes = Prompt<G>::BYTES;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = (unsigned)p.splits;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    count_launch();
+    return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<G, DT>, p, err);
+}
+template <int DT>
+cudaError_t launch_prompt_dim(const Kv4AttnParams& p, cudaStream_t st) {
+    return p.k.dim == 64 ? launch_prompt<2, DT>(p, st) : (p.k.dim == 96 ? launch_prompt<3, DT>(p, st) : launch_prompt<4, DT>(p, st));
+}
+
+}  // namespace
+
+bool kv4_prompt_serves(const Kv4AttnParams& p, int dtype) {
+    return dtype != 0 && p.k.dim <= 128 && (long long)p.max_rows * p.rep >= 64;
+}
+cudaError_t kv4_prompt(const Kv4AttnParams& p, int dtype, cudaStream_t st) { return dtype == 1 ? launch_prompt_dim<1>(p, st) : launch_prompt_dim<2>(p, st); }
+
+}  // namespace pgk
