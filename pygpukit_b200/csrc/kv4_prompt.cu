@@ -2,7 +2,7 @@
 // kv4_attention.cu, for rows of 16 bits and heads of 64, 96 and 128 elements.
 //
 // A block has 128 rows (a token's query heads of one key head beside each other) and walks over tiles of 128 keys:
-//   * four warps expand a tile of K, then of V, to bfloat16 in shared memory -- s (c - z) is a bfloat16 number, nothing is rounded: a nibble under
+//   * eight warps expand a tile of K, then of V, to bfloat16 in shared memory -- s (c - z) is a bfloat16 number, nothing is rounded: a nibble under
 //     the exponent of 128 is 128 + c, one subtraction and one product for two elements.  Their loads run one tile ahead, in registers;
 //   * one warp issues S = Q K^T (queries in tensor memory, float16 ones as two bfloat16 terms) and O += P V, the scores of tile i + 1 behind the
 //     weights of tile i;
@@ -22,7 +22,7 @@ namespace pgk {
 
 namespace {
 
-constexpr int P_ROWS = 128, P_KEYS = 128, P_SOFT = 8, P_EXPAND = 4, P_THREADS = (P_SOFT + 1 + P_EXPAND) * 32, P_STAGES = 2, P_CLUSTER = 8;
+constexpr int P_ROWS = 128, P_KEYS = 128, P_SOFT = 8, P_EXPAND = 8, P_THREADS = (P_SOFT + 1 + P_EXPAND) * 32, P_STAGES = 2, P_CLUSTER = 8;
 constexpr uint32_t P_CHUNK = P_KEYS * 128;                         // 64 elements of 128 keys
 constexpr uint32_t P_O = 0, P_Q = 128, P_S = 256;                  // TMEM columns: outputs, queries (two terms of 64), two tiles of scores
 constexpr float P_LAZY = 8.f;
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) kv4_prompt_kernel(const __grid_c
                 tc_fence_after();
 #pragma unroll
                 for (int k = 0; k < P_KEYS / 16; ++k)             // 16 keys: 2048 bytes of V
-                    umma_bf16_ta(tmem + P_O, tmem + P_S + (uint32_t)(i & 1) * 128u + (uint32_t)k * 8u, desc_mn_sw128(vs + s * C::TILE, P_CHUNK) + (uint64_t)(k * 128),
+                    umma_bf16_ta(tmem + P_O, tmem + P_S + (uint32_t)(i & 1) * 128u + (uint32_t)(k >> 2) * 64u + (uint32_t)(k & 3) * 8u, desc_mn_sw128(vs + s * C::TILE, P_CHUNK) + (uint64_t)(k * 128),
                                  id_o, (i | k) ? 1u : 0u);
                 umma_commit(&pvdone);
                 umma_commit(&vempty[s]);
@@ -192,55 +192,58 @@ __global__ void __launch_bounds__(P_THREADS, 1) kv4_prompt_kernel(const __grid_c
                 asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" :: "r"(vs + s * C::TILE + P_CHUNK + key * 128 + (((4 + i % 4) ^ (key & 7)) * 16)), "r"(0) : "memory");
             }
         }
-        struct Raw { uint32_t c[4][G], m[4][MW]; };
+        struct Raw { uint32_t c[2][G], m[2][MW]; };
         Raw kr, vr;
-        int pg[2], ahead[2];                       // pages of the warp's two runs of 16 keys; of the tile after
-        auto pages = [&](int i, int (&to)[2]) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int j = (tbeg + i) * P_KEYS + 32 * w + 16 * u;
-                to[u] = i < n && j < end ? __ldcg(table + kv4_page_of(p, (uint32_t)j >> 4)) : -1;
-            }
+        int page, ahead;                           // of the warp's 16 keys; of the tile after
+        long long codes = 0, words = 0;            // this lane's places in the head's pages
+        bool there[2] = {false, false};
+        auto page_at = [&](int i) {
+            const int j = (tbeg + i) * P_KEYS + 16 * w;
+            return i < n && j < end ? __ldcg(table + kv4_page_of(p, (uint32_t)j >> 4)) : -1;
         };
-        auto load = [&](const unsigned char* base, int i, Raw& r) {
+        auto place = [&](int i) {
+            const int j = (tbeg + i) * P_KEYS + 16 * w + kq;
+            const int in_page = j - (int)(kv4_page_of(p, (uint32_t)j >> 4) * (uint32_t)p.k.page_size);
+            const bool good = (unsigned)page < (unsigned)p.k.pages;
+            there[0] = good && j >= begin && j < end;
+            there[1] = good && j + 8 >= begin && j + 8 < end;
+            codes = page * p.page_bytes + in_page * (16 * G) + t * 4 * G;
+            words = page * p.page_bytes + code_bytes + in_page * (2 * G);
+        };
+        auto load = [&](const unsigned char* base, Raw& r) {
 #pragma unroll
-            for (int it = 0; it < 4; ++it) {
-                const int j = (tbeg + i) * P_KEYS + 32 * w + 8 * it + kq;
-                const bool there = j >= begin && j < end && (unsigned)pg[it >> 1] < (unsigned)p.k.pages;
+            for (int it = 0; it < 2; ++it) {
 #pragma unroll
                 for (int g = 0; g < G; ++g) r.c[it][g] = 0;
 #pragma unroll
                 for (int g = 0; g < MW; ++g) r.m[it][g] = 0;
-                if (there) {
-                    const int in_page = j - (int)(kv4_page_of(p, (uint32_t)j >> 4) * (uint32_t)p.k.page_size);
-                    const unsigned char* at = base + pg[it >> 1] * p.page_bytes;
-                    const unsigned char* codes = at + in_page * (16 * G) + t * 4 * G;
-                    const unsigned char* words = at + code_bytes + in_page * (2 * G);
+                if (there[it]) {
+                    const unsigned char* const c = base + codes + it * 128 * G;
+                    const unsigned char* const m = base + words + it * 16 * G;
                     if constexpr (G == 4) {
-                        const uint4 v = ld_act16(codes);
+                        const uint4 v = ld_act16(c);
                         r.c[it][0] = v.x; r.c[it][1] = v.y; r.c[it][2] = v.z; r.c[it][3] = v.w;
-                        const uint2 m = __ldcg((const uint2*)words);
-                        r.m[it][0] = m.x; r.m[it][1] = m.y;
+                        const uint2 y = __ldcg((const uint2*)m);
+                        r.m[it][0] = y.x; r.m[it][1] = y.y;
                     } else if constexpr (G == 2) {
-                        const uint2 v = __ldcg((const uint2*)codes);
+                        const uint2 v = __ldcg((const uint2*)c);
                         r.c[it][0] = v.x; r.c[it][1] = v.y;
-                        r.m[it][0] = __ldcg((const uint32_t*)words);
+                        r.m[it][0] = __ldcg((const uint32_t*)m);
                     } else {
 #pragma unroll
                         for (int g = 0; g < G; ++g) {
-                            r.c[it][g] = __ldcg((const uint32_t*)codes + g);
-                            r.m[it][g / 2] |= (uint32_t)ld_act2((const uint16_t*)words + g) << (16 * (g & 1));
+                            r.c[it][g] = __ldcg((const uint32_t*)c + g);
+                            r.m[it][g / 2] |= (uint32_t)ld_act2((const uint16_t*)m + g) << (16 * (g & 1));
                         }
                     }
                 }
             }
         };
         bool nan = false;
+        const uint32_t to_even = (16 * w + kq) * 128 + ((t ^ kq) * 16), to_odd = to_even ^ 64u;           // groups of a chunk's first and second half
         auto expand = [&](const Raw& r, uint32_t tile, bool values) {
 #pragma unroll
-            for (int it = 0; it < 4; ++it) {
-                const int key = 32 * w + 8 * it + kq;
-                const uint32_t to = tile + key * 128;
+            for (int it = 0; it < 2; ++it)
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
                     uint32_t m = __byte_perm(r.m[it][g / 2], 0, g & 1 ? 0x3232 : 0x1010);
@@ -251,16 +254,16 @@ __global__ void __launch_bounds__(P_THREADS, 1) kv4_prompt_kernel(const __grid_c
 #pragma unroll
                     for (int e = 0; e < 4; ++e) y[e] = bf2_mul(bf2_add((y[e] & 0x000f000fu) | 0x43004300u, zero), scale);
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                                 :: "r"(to + (uint32_t)(g >> 1) * P_CHUNK + (((4 * (g & 1) + t) ^ (key & 7)) * 16)), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
+                                 :: "r"(tile + (g & 1 ? to_odd : to_even) + (uint32_t)(g >> 1) * P_CHUNK + (uint32_t)it * 1024u), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
                 }
-            }
             fence_proxy_async();
             __syncwarp();
         };
-        pages(0, pg);
-        load(khead, 0, kr);
-        load(vhead, 0, vr);
-        pages(1, ahead);
+        page = page_at(0);
+        place(0);
+        load(khead, kr);
+        load(vhead, vr);
+        ahead = page_at(1);
         bool ok = true;
         for (int i = 0; i < n; ++i) {
             const int s = i % P_STAGES;
@@ -269,14 +272,15 @@ __global__ void __launch_bounds__(P_THREADS, 1) kv4_prompt_kernel(const __grid_c
             if (!ok) break;
             expand(kr, ks + s * C::TILE, false);
             if (lane == 0) mbar_arrive(&kfull[s]);
-            pg[0] = ahead[0]; pg[1] = ahead[1];
-            if (i + 1 < n) load(khead, i + 1, kr);
-            pages(i + 2, ahead);
+            page = ahead;
+            place(i + 1);
+            if (i + 1 < n) load(khead, kr);
+            ahead = page_at(i + 2);
             ok = ok && all_wait(err, &vempty[s], free);
             if (!ok) break;
             expand(vr, vs + s * C::TILE, true);
             if (lane == 0) mbar_arrive(&vfull[s]);
-            if (i + 1 < n) load(vhead, i + 1, vr);
+            if (i + 1 < n) load(vhead, vr);
         }
         if (nan) nans = 1;
     } else {
@@ -293,35 +297,45 @@ __global__ void __launch_bounds__(P_THREADS, 1) kv4_prompt_kernel(const __grid_c
             ok = ok && all_wait(err, &sfull[i & 1], (uint32_t)((i >> 1) & 1));
             __syncwarp();
             tc_fence_after();
-            float s[64];
+            const bool edge = j0 <= clean_lo || j0 + 63 > clean_hi;
+            uint32_t gone = 0;                                    // of four runs of 16 keys, the ones without a page
+            if (edge && missing) {
 #pragma unroll
-            for (int c = 0; c < 64; c += 16) tmem_ld16_async(at + (uint32_t)(half * 64 + c), *(float (*)[16])(s + c));
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-            for (int c = 0; c < 64; c += 16) tmem_pass(*(float (*)[16])(s + c));
-            if (p.cap_log2 > 0.f) {
-                const float in = p.scale_log2 * 2.885390043f / p.cap_log2;
-#pragma unroll
-                for (int c = 0; c < 64; ++c) s[c] = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(s[c] * in)));
+                for (int u = 0; u < 4; ++u)
+                    if (j0 + 16 * u < end && (unsigned)__ldcg(table + kv4_page_of(p, (uint32_t)(j0 + 16 * u) >> 4)) >= (unsigned)p.k.pages) gone |= 1u << u;
             }
-            if (j0 <= clean_lo || j0 + 63 > clean_hi) {
-                uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-                if (missing) {                                    // four runs of 16 keys
+            // 32 scores at a time, looked at twice: the maximum, then the weights.  A loop: straight code for 64 costs its fetch
+            auto look = [&](int c, float (&s)[32]) {
+                tmem_ld16_async(at + (uint32_t)(half * 64 + c), *(float (*)[16])s);
+                tmem_ld16_async(at + (uint32_t)(half * 64 + c + 16), *(float (*)[16])(s + 16));
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                tmem_pass(*(float (*)[16])s);
+                tmem_pass(*(float (*)[16])(s + 16));
+                if (p.cap_log2 > 0.f) {
+                    const float in = p.scale_log2 * 2.885390043f / p.cap_log2;
 #pragma unroll
-                    for (int u = 0; u < 4; ++u)
-                        if (j0 + 16 * u < end && (unsigned)__ldcg(table + kv4_page_of(p, (uint32_t)(j0 + 16 * u) >> 4)) >= (unsigned)p.k.pages) seen[u >> 1] &= ~(0xffffu << (16 * (u & 1)));
+                    for (int e = 0; e < 32; ++e) s[e] = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(s[e] * in)));
                 }
+                if (edge) {
+                    const int hi = limit - j0 - c, lo = under - j0 - c;
+                    const uint32_t off = gone >> (c / 16);
 #pragma unroll
-                for (int c = 0; c < 64; ++c)
-                    if (j0 + c > limit || j0 + c <= under || !((seen[c >> 5] >> (c & 31)) & 1u)) s[c] = -INFINITY;
-            }
+                    for (int e = 0; e < 32; ++e)
+                        if (e > hi || e <= lo || ((off >> (e / 16)) & 1u)) s[e] = -INFINITY;
+                }
+            };
             float top = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < 64; c += 32) {
+                float s[32];
+                look(c, s);
 #pragma unroll
-            for (int c = 0; c < 64; ++c) top = fmaxf(top, s[c]);
+                for (int e = 0; e < 32; ++e) top = fmaxf(top, s[e]);
+            }
             top *= fac;
             wmax[i & 1][half][row] = top;
             __syncwarp();
-            asm volatile("bar.sync %0, 64;" :: "r"(1 + quad) : "memory");          // the row's two warps; both have read their scores
+            asm volatile("bar.sync %0, 64;" :: "r"(1 + quad) : "memory");          // the row's two warps
             top = fmaxf(top, wmax[i & 1][half ^ 1][row]);
             const bool up = top > m + P_LAZY;                     // (also the first finite maximum)
             if (__any_sync(0xffffffffu, up)) {                    // the same in both warps: each has half of the outputs
@@ -343,17 +357,19 @@ __global__ void __launch_bounds__(P_THREADS, 1) kv4_prompt_kernel(const __grid_c
                     }
                 }
             }
-#pragma unroll
-            for (int c = 0; c < 64; c += 32) {                    // 32 keys: 16 columns
+#pragma unroll 1
+            for (int c = 0; c < 64; c += 32) {                    // 32 keys: 16 columns, where the warp's own scores were
+                float s[32];
                 uint32_t y[16];
+                look(c, s);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float a = ex2(fmaf(s[c + 2 * e], fac, neg)), b = ex2(fmaf(s[c + 2 * e + 1], fac, neg));
+                    const float a = ex2(fmaf(s[2 * e], fac, neg)), b = ex2(fmaf(s[2 * e + 1], fac, neg));
                     l += a + b;
                     y[e] = pack_bf16x2(a, b);
                 }
                 __syncwarp();
-                tmem_st16u(at + (uint32_t)(half * 32 + c / 2), y);
+                tmem_st16u(at + (uint32_t)(half * 64 + c / 2), y);
             }
             tmem_st_wait();
             tc_fence_before();
