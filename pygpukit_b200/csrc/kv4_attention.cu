@@ -703,10 +703,7 @@ extern "C" int pgk_kv4_attention(const void* q, long q_ld, const void* k_cache, 
     p.wide_q = (uintptr_t)q % 16 == 0 && q_ld * size % 16 == 0;
     p.wide_o = (uintptr_t)out % 16 == 0 && o_ld * size % 16 == 0;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (kv4_prompt_serves(p, dtype)) {
-        PGK_CUDA(kv4_prompt(p, dtype, st));
-        return 0;
-    }
+    if (kv4_prompt_serves(p, dtype)) return kv4_prompt(p, dtype, st);
     PGK_CUDA(dtype == 0 ? launch_few_dim<0>(p, st) : (dtype == 1 ? launch_few_dim<1>(p, st) : launch_few_dim<2>(p, st)));
     return 0;
 }

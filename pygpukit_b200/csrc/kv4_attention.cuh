@@ -21,7 +21,7 @@ struct Kv4AttnParams {
 
 // kv4_prompt.cu: whether it serves the call, and the call
 bool kv4_prompt_serves(const Kv4AttnParams& p, int dtype);
-cudaError_t kv4_prompt(const Kv4AttnParams& p, int dtype, cudaStream_t st);
+int kv4_prompt(const Kv4AttnParams& p, int dtype, cudaStream_t st);
 
 #ifdef __CUDACC__
 

@@ -26,6 +26,17 @@ constexpr int P_ROWS = 128, P_KEYS = 128, P_SOFT = 8, P_EXPAND = 8, P_THREADS = 
 constexpr uint32_t P_CHUNK = P_KEYS * 128;                         // 64 elements of 128 keys
 constexpr uint32_t P_O = 0, P_Q = 128, P_S = 256;                  // TMEM columns: outputs, queries (two terms of 64), two tiles of scores
 constexpr float P_LAZY = 8.f;
+constexpr int P_IMAGES_FROM = 4;                                   // blocks of rows that read a sequence's tiles
+constexpr long long P_IMAGES_MOST = 1ll << 30;
+
+// Tiles as they lie in shared memory, made ahead of the products: [sequence][head][tile][K, V], and per tile whether a value is NaN.  Tile 0 is the one
+// that holds the first key of the sequence's first row.
+struct Images {
+    unsigned char* data;
+    int32_t* nans;
+    int tiles;
+};
+__device__ __forceinline__ int first_tile(const Kv4AttnParams& p, int ctx, int n_rows) { return p.window > 0 ? max(0, ctx - n_rows - p.window + 1) / P_KEYS : 0; }
 
 template <int G> struct Prompt {
     static constexpr int D = 32 * G, DN = G == 2 ? 64 : 128;       // 96 elements: the products go on to 128 over zeros
@@ -48,10 +59,101 @@ __device__ __forceinline__ uint32_t bf2_mul(uint32_t a, uint32_t b) {
     return r;
 }
 
-template <int G, int DT>
-__global__ void __launch_bounds__(P_THREADS, 1) kv4_prompt_kernel(const __grid_constant__ Kv4AttnParams p, int* err) {
+// Sixteen keys of a warp: this lane's bytes of two of them (keys kq and kq + 8; two quads of an access are keys 4 apart, so that stores meet all banks)
+template <int G> struct Raw {
+    uint32_t c[2][G], m[2][(G + 1) / 2];
+    __device__ __forceinline__ void load(const unsigned char* codes, const unsigned char* words, const bool (&there)[2]) {
+#pragma unroll
+        for (int it = 0; it < 2; ++it) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) c[it][g] = 0;
+#pragma unroll
+            for (int g = 0; g < (G + 1) / 2; ++g) m[it][g] = 0;
+            if (there[it]) {
+                const unsigned char* const x = codes + it * 128 * G;
+                const unsigned char* const y = words + it * 16 * G;
+                if constexpr (G == 4) {
+                    const uint4 v = ld_act16(x);
+                    c[it][0] = v.x; c[it][1] = v.y; c[it][2] = v.z; c[it][3] = v.w;
+                    const uint2 u = __ldcg((const uint2*)y);
+                    m[it][0] = u.x; m[it][1] = u.y;
+                } else if constexpr (G == 2) {
+                    const uint2 v = __ldcg((const uint2*)x);
+                    c[it][0] = v.x; c[it][1] = v.y;
+                    m[it][0] = __ldcg((const uint32_t*)y);
+                } else {
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        c[it][g] = __ldcg((const uint32_t*)x + g);
+                        m[it][g / 2] |= (uint32_t)ld_act2((const uint16_t*)y + g) << (16 * (g & 1));
+                    }
+                }
+            }
+        }
+    }
+    // put(it, g, four words): elements 32 g + 8 t ... + 7 of the lane's key, in the order of its nibbles.  Values that are NaN become zeros: true
+    template <typename Put> __device__ __forceinline__ bool expand(bool values, Put put) const {
+        bool nan = false;
+#pragma unroll
+        for (int it = 0; it < 2; ++it)
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                uint32_t w = __byte_perm(m[it][g / 2], 0, g & 1 ? 0x3232 : 0x1010);
+                if (values && (w & 0x7f80u) == 0x7f80u) { nan = true; w = 0; }
+                const uint32_t zero = (w & 0x000f000fu) | 0xc300c300u, scale = w & 0x7ff07ff0u;        // -(128 + z), s
+                const uint32_t x = c[it][g];
+                uint32_t y[4] = {x, x >> 4, x >> 8, x >> 12};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = bf2_mul(bf2_add((y[e] & 0x000f000fu) | 0x43004300u, zero), scale);
+                put(it, g, make_uint4(y[0], y[1], y[2], y[3]));
+            }
+        return nan;
+    }
+};
+__device__ __forceinline__ int lane_key(int lane) { return (lane >> 3) + 4 * ((lane >> 2) & 1); }
+// where a lane's eight elements of group g of key `key` (16 w + kq, 8 on with it = 1) lie in a tile
+template <int G>
+__device__ __forceinline__ uint32_t tile_place(int key, int t, int it, int g) {
+    return (uint32_t)key * 128u + ((uint32_t)(((4 * (g & 1) + t) ^ (key & 7)) * 16)) + (uint32_t)(g >> 1) * P_CHUNK + (uint32_t)it * 1024u;
+}
+
+// tiles of K and V, a block each
+template <int G>
+__global__ void __launch_bounds__(P_EXPAND * 32) kv4_images_kernel(const __grid_constant__ Kv4AttnParams p, const __grid_constant__ Images im) {
     using C = Prompt<G>;
-    constexpr int D = C::D, DN = C::DN, QT = DT == 1 ? 2 : 1, MW = (G + 1) / 2;
+    griddep_wait();
+    griddep_launch();
+    const int tile = blockIdx.x, head = blockIdx.y, seq = blockIdx.z, tid = threadIdx.x, lane = tid & 31, w = tid >> 5, t = lane & 3;
+    const int slot = __ldcg(p.seq_slots + seq), ctx = __ldcg(p.contexts + seq);
+    const int n_rows = p.starts ? __ldcg(p.starts + seq + 1) - __ldcg(p.starts + seq) : 1;
+    const int base = first_tile(p, ctx, n_rows), end = min(ctx, p.max_keys), j = (base + tile) * P_KEYS + 16 * w + lane_key(lane);
+    if (base + tile >= (end + P_KEYS - 1) / P_KEYS || (unsigned)slot >= (unsigned)p.k.slots) return;
+    const uint32_t run = (uint32_t)((base + tile) * P_KEYS + 16 * w) >> 4, in_slot = kv4_page_of(p, run);
+    const int page = (int)(run << 4) < end ? __ldcg(p.k.table + (size_t)slot * p.k.max_pages + in_slot) : -1, in_page = j - (int)(in_slot * (uint32_t)p.k.page_size);
+    const bool good = (unsigned)page < (unsigned)p.k.pages, there[2] = {good && j < end, good && j + 8 < end};
+    const long long at = page * p.page_bytes + (long long)head * p.head_bytes;
+    Raw<G> k, v;
+    k.load(p.k.data + at + in_page * (16 * G) + t * 4 * G, p.k.data + at + p.k.page_size * (16 * G) + in_page * (2 * G), there);
+    v.load(p.v_data + at + in_page * (16 * G) + t * 4 * G, p.v_data + at + p.k.page_size * (16 * G) + in_page * (2 * G), there);
+    const size_t n = ((size_t)seq * p.k.kv_heads + head) * im.tiles + tile;
+    unsigned char* const to = im.data + n * (2 * C::TILE);
+    const int key = 16 * w + lane_key(lane);
+    k.expand(false, [&](int it, int g, uint4 x) { *(uint4*)(to + tile_place<G>(key, t, it, g)) = x; });
+    const bool nan = v.expand(true, [&](int it, int g, uint4 x) { *(uint4*)(to + C::TILE + tile_place<G>(key, t, it, g)) = x; });
+    if constexpr (G == 3) {                        // elements 96 ... 127 of V
+        for (int i = tid; i < P_KEYS * 4; i += P_EXPAND * 32)
+            *(uint4*)(to + C::TILE + P_CHUNK + (i / 4) * 128 + (((4 + i % 4) ^ (i / 4 & 7)) * 16)) = make_uint4(0, 0, 0, 0);
+    }
+    const int any = __syncthreads_or(nan);
+    if (tid == 0) im.nans[n] = any;
+}
+
+// IMAGES: one warp copies tiles that kv4_images_kernel has made; otherwise P_EXPAND warps make them
+template <int G, int DT, bool IMAGES>
+__global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4_prompt_kernel(const __grid_constant__ Kv4AttnParams p, const __grid_constant__ Images im, int* err) {
+    using C = Prompt<G>;
+    constexpr int THREADS = IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, FILLS = IMAGES ? 1 : P_EXPAND;
+    constexpr int D = C::D, DN = C::DN, QT = DT == 1 ? 2 : 1;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(8) uint64_t kfull[P_STAGES], kempty[P_STAGES], vfull[P_STAGES], vempty[P_STAGES], sfull[2], pready, pvdone;
     __shared__ uint32_t tmem_base_s;
@@ -63,8 +165,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) kv4_prompt_kernel(const __grid_c
     if (warp == P_SOFT) tmem_alloc(&tmem_base_s, 512);
     if (tid == 0) {
         for (int s = 0; s < P_STAGES; ++s) {
-            mbar_init(&kfull[s], P_EXPAND); mbar_init(&kempty[s], 1);
-            mbar_init(&vfull[s], P_EXPAND); mbar_init(&vempty[s], 1);
+            mbar_init(&kfull[s], FILLS); mbar_init(&kempty[s], 1);
+            mbar_init(&vfull[s], FILLS); mbar_init(&vempty[s], 1);
         }
         mbar_init(&sfull[0], 1); mbar_init(&sfull[1], 1);
         mbar_init(&pready, P_SOFT); mbar_init(&pvdone, 1);
@@ -90,6 +192,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) kv4_prompt_kernel(const __grid_c
     const int t0 = begin / P_KEYS, nt = max(0, (end + P_KEYS - 1) / P_KEYS - t0), per = (nt + p.splits - 1) / p.splits;
     const int tbeg = t0 + split * per, n = max(0, min(nt, (split + 1) * per) - split * per);
     const int32_t* const table = p.k.table + (work ? (size_t)slot * p.k.max_pages : 0);
+
+    const size_t image = ((size_t)seq * p.k.kv_heads + head) * im.tiles + (tbeg - first_tile(p, ctx, n_rows));      // the block's first tile
 
     // row r of the block: which one of the sequence's, and what it sees
     const int quad = warp & 3, half = (warp >> 2) & 1, row = quad * 32 + lane, f = f0 + row, tok = first + f / p.rep;
@@ -133,9 +237,13 @@ __global__ void __launch_bounds__(P_THREADS, 1) kv4_prompt_kernel(const __grid_c
     } else {                                       // does a page of these keys not exist?
         bool gone = false;
         const int last = min(end, (tbeg + n) * P_KEYS);
-        for (int j = tbeg * P_KEYS + 16 * (tid - 128); j < last; j += 16 * (P_THREADS - 128))
+        for (int j = tbeg * P_KEYS + 16 * (tid - 128); j < last; j += 16 * (THREADS - 128))
             gone |= (unsigned)__ldcg(table + kv4_page_of(p, (uint32_t)j >> 4)) >= (unsigned)p.k.pages;
         if (gone) missing = 1;
+        if constexpr (IMAGES) {
+            for (int i = tid - 128; i < n; i += THREADS - 128)
+                if (__ldcg(im.nans + image + i)) nans = 1;
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -181,108 +289,94 @@ __global__ void __launch_bounds__(P_THREADS, 1) kv4_prompt_kernel(const __grid_c
             __syncwarp();
         }
     } else if (warp > P_SOFT) {
-        // ---------------- tiles of K and V, expanded
-        const int w = warp - P_SOFT - 1, q = lane >> 2, t = lane & 3, kq = (q >> 1) + 4 * (q & 1);        // two quads of an access: keys 4 apart, all banks
-        const unsigned char* const khead = p.k.data + (size_t)head * p.head_bytes;
-        const unsigned char* const vhead = p.v_data + (size_t)head * p.head_bytes;
-        const int code_bytes = p.k.page_size * 16 * G;
-        if constexpr (G == 3) {                    // elements 96 ... 127 of V
-            for (int i = tid - (P_SOFT + 1) * 32; i < P_STAGES * P_KEYS * 4; i += P_EXPAND * 32) {
-                const int s = i / (P_KEYS * 4), key = i / 4 % P_KEYS;
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" :: "r"(vs + s * C::TILE + P_CHUNK + key * 128 + (((4 + i % 4) ^ (key & 7)) * 16)), "r"(0) : "memory");
-            }
-        }
-        struct Raw { uint32_t c[2][G], m[2][MW]; };
-        Raw kr, vr;
-        int page, ahead;                           // of the warp's 16 keys; of the tile after
-        long long codes = 0, words = 0;            // this lane's places in the head's pages
-        bool there[2] = {false, false};
-        auto page_at = [&](int i) {
-            const int j = (tbeg + i) * P_KEYS + 16 * w;
-            return i < n && j < end ? __ldcg(table + kv4_page_of(p, (uint32_t)j >> 4)) : -1;
-        };
-        auto place = [&](int i) {
-            const int j = (tbeg + i) * P_KEYS + 16 * w + kq;
-            const int in_page = j - (int)(kv4_page_of(p, (uint32_t)j >> 4) * (uint32_t)p.k.page_size);
-            const bool good = (unsigned)page < (unsigned)p.k.pages;
-            there[0] = good && j >= begin && j < end;
-            there[1] = good && j + 8 >= begin && j + 8 < end;
-            codes = page * p.page_bytes + in_page * (16 * G) + t * 4 * G;
-            words = page * p.page_bytes + code_bytes + in_page * (2 * G);
-        };
-        auto load = [&](const unsigned char* base, Raw& r) {
-#pragma unroll
-            for (int it = 0; it < 2; ++it) {
-#pragma unroll
-                for (int g = 0; g < G; ++g) r.c[it][g] = 0;
-#pragma unroll
-                for (int g = 0; g < MW; ++g) r.m[it][g] = 0;
-                if (there[it]) {
-                    const unsigned char* const c = base + codes + it * 128 * G;
-                    const unsigned char* const m = base + words + it * 16 * G;
-                    if constexpr (G == 4) {
-                        const uint4 v = ld_act16(c);
-                        r.c[it][0] = v.x; r.c[it][1] = v.y; r.c[it][2] = v.z; r.c[it][3] = v.w;
-                        const uint2 y = __ldcg((const uint2*)m);
-                        r.m[it][0] = y.x; r.m[it][1] = y.y;
-                    } else if constexpr (G == 2) {
-                        const uint2 v = __ldcg((const uint2*)c);
-                        r.c[it][0] = v.x; r.c[it][1] = v.y;
-                        r.m[it][0] = __ldcg((const uint32_t*)m);
-                    } else {
-#pragma unroll
-                        for (int g = 0; g < G; ++g) {
-                            r.c[it][g] = __ldcg((const uint32_t*)c + g);
-                            r.m[it][g / 2] |= (uint32_t)ld_act2((const uint16_t*)m + g) << (16 * (g & 1));
-                        }
-                    }
+        if constexpr (IMAGES) {
+            // ---------------- tiles of K and V, copied
+            if (elect_one()) {
+                bool ok = true;
+                auto copy = [&](int i, uint64_t* full, uint64_t* empty, uint32_t at, size_t from) {
+                    const int s = i % P_STAGES;
+                    ok = ok && bar_wait(err, smem_u32(&empty[s]), (((uint32_t)i / P_STAGES) & 1u) ^ 1u);
+                    if (!ok) return false;
+                    mbar_arrive_expect_tx(&full[s], C::TILE);
+                    bulk_copy_g2s(smem + (at - smem_u32(smem)) + s * C::TILE, im.data + from, C::TILE, &full[s]);
+                    return true;
+                };
+                int nk = 0, nv = 0;
+                for (int i = 0; ok && i < n; ++i) {
+                    nk += copy(i, kfull, kempty, ks, (image + i) * (2 * C::TILE));
+                    nv += copy(i, vfull, vempty, vs, (image + i) * (2 * C::TILE) + C::TILE);
                 }
+                for (int j = max(0, nk - P_STAGES); j < nk; ++j)      // whoever gave up: do not leave with copies in flight
+                    bar_wait(err, smem_u32(&kfull[j % P_STAGES]), (uint32_t)(j / P_STAGES) & 1u);
+                for (int j = max(0, nv - P_STAGES); j < nv; ++j)
+                    bar_wait(err, smem_u32(&vfull[j % P_STAGES]), (uint32_t)(j / P_STAGES) & 1u);
             }
-        };
-        bool nan = false;
-        const uint32_t to_even = (16 * w + kq) * 128 + ((t ^ kq) * 16), to_odd = to_even ^ 64u;           // groups of a chunk's first and second half
-        auto expand = [&](const Raw& r, uint32_t tile, bool values) {
-#pragma unroll
-            for (int it = 0; it < 2; ++it)
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    uint32_t m = __byte_perm(r.m[it][g / 2], 0, g & 1 ? 0x3232 : 0x1010);
-                    if (values && (m & 0x7f80u) == 0x7f80u) { nan = true; m = 0; }
-                    const uint32_t zero = (m & 0x000f000fu) | 0xc300c300u, scale = m & 0x7ff07ff0u;        // -(128 + z), s
-                    const uint32_t x = r.c[it][g];
-                    uint32_t y[4] = {x, x >> 4, x >> 8, x >> 12};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] = bf2_mul(bf2_add((y[e] & 0x000f000fu) | 0x43004300u, zero), scale);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                                 :: "r"(tile + (g & 1 ? to_odd : to_even) + (uint32_t)(g >> 1) * P_CHUNK + (uint32_t)it * 1024u), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
-                }
-            fence_proxy_async();
             __syncwarp();
-        };
-        page = page_at(0);
-        place(0);
-        load(khead, kr);
-        load(vhead, vr);
-        ahead = page_at(1);
-        bool ok = true;
-        for (int i = 0; i < n; ++i) {
-            const int s = i % P_STAGES;
-            const uint32_t free = (((uint32_t)i / P_STAGES) & 1u) ^ 1u;
-            ok = ok && all_wait(err, &kempty[s], free);
-            if (!ok) break;
-            expand(kr, ks + s * C::TILE, false);
-            if (lane == 0) mbar_arrive(&kfull[s]);
-            page = ahead;
-            place(i + 1);
-            if (i + 1 < n) load(khead, kr);
-            ahead = page_at(i + 2);
-            ok = ok && all_wait(err, &vempty[s], free);
-            if (!ok) break;
-            expand(vr, vs + s * C::TILE, true);
-            if (lane == 0) mbar_arrive(&vfull[s]);
-            if (i + 1 < n) load(vhead, vr);
+        } else {
+            // ---------------- tiles of K and V, expanded
+            const int w = warp - P_SOFT - 1, t = lane & 3, key = 16 * w + lane_key(lane);
+            const unsigned char* const khead = p.k.data + (size_t)head * p.head_bytes;
+            const unsigned char* const vhead = p.v_data + (size_t)head * p.head_bytes;
+            const int code_bytes = p.k.page_size * 16 * G;
+            if constexpr (G == 3) {                    // elements 96 ... 127 of V
+                for (int i = tid - (P_SOFT + 1) * 32; i < P_STAGES * P_KEYS * 4; i += P_EXPAND * 32) {
+                    const int s = i / (P_KEYS * 4), k = i / 4 % P_KEYS;
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" :: "r"(vs + s * C::TILE + P_CHUNK + k * 128 + (((4 + i % 4) ^ (k & 7)) * 16)), "r"(0) : "memory");
+                }
+            }
+            Raw<G> kr, vr;
+            int page, ahead;                           // of the warp's 16 keys; of the tile after
+            long long codes = 0, words = 0;            // this lane's places in the head's pages
+            bool there[2] = {false, false}, nan = false;
+            auto page_at = [&](int i) {
+                const int j = (tbeg + i) * P_KEYS + 16 * w;
+                return i < n && j < end ? __ldcg(table + kv4_page_of(p, (uint32_t)j >> 4)) : -1;
+            };
+            auto place = [&](int i) {
+                const int j = (tbeg + i) * P_KEYS + key;
+                const int in_page = j - (int)(kv4_page_of(p, (uint32_t)j >> 4) * (uint32_t)p.k.page_size);
+                const bool good = (unsigned)page < (unsigned)p.k.pages;
+                there[0] = good && j >= begin && j < end;
+                there[1] = good && j + 8 >= begin && j + 8 < end;
+                codes = page * p.page_bytes + in_page * (16 * G) + t * 4 * G;
+                words = page * p.page_bytes + code_bytes + in_page * (2 * G);
+            };
+            const uint32_t to_even = tile_place<G>(key, t, 0, 0), to_odd = to_even ^ 64u;                 // groups of a chunk's first and second half
+            auto store = [&](uint32_t tile) {
+                return [=](int it, int g, uint4 x) {
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                                 :: "r"(tile + (g & 1 ? to_odd : to_even) + (uint32_t)(g >> 1) * P_CHUNK + (uint32_t)it * 1024u), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+                };
+            };
+            page = page_at(0);
+            place(0);
+            kr.load(khead + codes, khead + words, there);
+            vr.load(vhead + codes, vhead + words, there);
+            ahead = page_at(1);
+            bool ok = true;
+            for (int i = 0; i < n; ++i) {
+                const int s = i % P_STAGES;
+                const uint32_t free = (((uint32_t)i / P_STAGES) & 1u) ^ 1u;
+                ok = ok && all_wait(err, &kempty[s], free);
+                if (!ok) break;
+                kr.expand(false, store(ks + s * C::TILE));
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&kfull[s]);
+                page = ahead;
+                place(i + 1);
+                if (i + 1 < n) kr.load(khead + codes, khead + words, there);
+                ahead = page_at(i + 2);
+                ok = ok && all_wait(err, &vempty[s], free);
+                if (!ok) break;
+                nan |= vr.expand(true, store(vs + s * C::TILE));
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&vfull[s]);
+                if (i + 1 < n) vr.load(vhead + codes, vhead + words, there);
+            }
+            if (nan) nans = 1;
         }
-        if (nan) nans = 1;
     } else {
         // ---------------- weights
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
@@ -452,7 +546,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) kv4_prompt_kernel(const __grid_c
     // ---------------- the cluster's blocks into one: block r has every `splits`-th piece
     cluster_sync();
     const uint32_t fold_at = smem_u32(fold), m_at = smem_u32(row_m), l_at = smem_u32(row_l);
-    for (int i = split * P_THREADS + tid; i < live_rows * (D / 4); i += p.splits * P_THREADS) {
+    for (int i = split * THREADS + tid; i < live_rows * (D / 4); i += p.splits * THREADS) {
         const int r = i / (D / 4), d = (i - r * (D / 4)) * 4, fr = f0 + r, to = first + fr / p.rep;
         if (to < 0 || to >= p.tokens) continue;
         float top = -INFINITY, sum = 0.f;
@@ -474,27 +568,16 @@ __global__ void __launch_bounds__(P_THREADS, 1) kv4_prompt_kernel(const __grid_c
     cluster_sync();                                // nobody leaves while another reads
 }
 
-template <int G, int DT>
-cudaError_t launch_prompt(Kv4AttnParams p, cudaStream_t st) {
+template <int G, int DT, bool IMAGES>
+cudaError_t launch_prompt_kernel(const Kv4AttnParams& p, const Images& im, int* err, cudaStream_t st) {
     static bool configured = false;
     if (!configured) {
-        if (cudaError_t e = cudaFuncSetAttribute(kv4_prompt_kernel<G, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Prompt<G>::BYTES)) return e;
+        if (cudaError_t e = cudaFuncSetAttribute(kv4_prompt_kernel<G, DT, IMAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Prompt<G>::BYTES)) return e;
         configured = true;
-    }
-    int* err = wait_word(kWaitKv4);
-    if (!err) return cudaErrorMemoryAllocation;
-    p.tiles = (int)(((long long)p.max_rows * p.rep + P_ROWS - 1) / P_ROWS);
-    // blocks of a cluster that share a sequence's keys: rounds of blocks times (their tiles + what a block costs besides, about four tiles)
-    const int keys = p.window > 0 && p.window < p.max_keys - P_ROWS ? p.window + P_ROWS : p.max_keys, nt = (keys + P_KEYS - 1) / P_KEYS;
-    const long long items = (long long)p.seqs * p.tiles * p.k.kv_heads;
-    long long least = 0;
-    for (int s = 1; s <= P_CLUSTER; s *= 2) {
-        const long long cost = ((items * s + sm_count() - 1) / sm_count()) * ((nt + s - 1) / s + 4);
-        if (s == 1 || cost < least) { p.splits = s; least = cost; }
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.seqs * p.tiles), p.k.kv_heads, p.splits);
-    cfg.blockDim = dim3(P_THREADS);
+    cfg.blockDim = dim3(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS);
     cfg.dynamicSmemBytes = Prompt<G>::BYTES;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -507,10 +590,49 @@ cudaError_t launch_prompt(Kv4AttnParams p, cudaStream_t st) {
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     count_launch();
-    return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<G, DT>, p, err);
+    return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<G, DT, IMAGES>, p, im, err);
+}
+
+template <int G, int DT>
+int launch_prompt(Kv4AttnParams p, cudaStream_t st) {
+    int* err = wait_word(kWaitKv4);
+    PGK_REQUIRE(err, "kv4_attention failed: no pinned host memory");
+    p.tiles = (int)(((long long)p.max_rows * p.rep + P_ROWS - 1) / P_ROWS);
+    // blocks of a cluster that share a sequence's keys: rounds of blocks times (their tiles + what a block costs besides, about four tiles)
+    const int keys = p.window > 0 && p.window < p.max_keys - P_ROWS ? p.window + P_ROWS : p.max_keys, nt = (keys + P_KEYS - 1) / P_KEYS;
+    const long long items = (long long)p.seqs * p.tiles * p.k.kv_heads;
+    long long least = 0;
+    for (int s = 1; s <= P_CLUSTER; s *= 2) {
+        const long long cost = ((items * s + sm_count() - 1) / sm_count()) * ((nt + s - 1) / s + 4);
+        if (s == 1 || cost < least) { p.splits = s; least = cost; }
+    }
+    Images im = {};
+    im.tiles = (p.max_keys + P_KEYS - 1) / P_KEYS;
+    if (p.window > 0 && (long long)p.window + p.max_rows < p.max_keys) {
+        const int few = (p.window + p.max_rows) / P_KEYS + 2;
+        if (few < im.tiles) im.tiles = few;
+    }
+    const long long count = (long long)p.seqs * p.k.kv_heads * im.tiles, bytes = count * (2 * Prompt<G>::TILE + 4);
+    void* ws = nullptr;
+    if (p.tiles >= P_IMAGES_FROM && im.tiles > 0 && im.tiles <= 65535 && p.seqs <= 65535 && bytes <= P_IMAGES_MOST) {
+        const int rc = scratch_alloc(&ws, (size_t)bytes, st);
+        if (rc == (int)cudaErrorMemoryAllocation) set_error("");      // no room: the blocks make their tiles
+        else if (rc) return rc;
+    }
+    cudaError_t e = cudaSuccess;
+    if (ws) {
+        im.data = (unsigned char*)ws;
+        im.nans = (int32_t*)((unsigned char*)ws + count * (2 * Prompt<G>::TILE));
+        e = launch_waiting(kv4_images_kernel<G>, dim3(im.tiles, p.k.kv_heads, p.seqs), dim3(P_EXPAND * 32), 0, st, p, im);
+        if (e == cudaSuccess) e = launch_prompt_kernel<G, DT, true>(p, im, err, st);
+    } else
+        e = launch_prompt_kernel<G, DT, false>(p, im, err, st);
+    if (int rc = scratch_free(ws, st)) return rc;
+    PGK_CUDA(e);
+    return 0;
 }
 template <int DT>
-cudaError_t launch_prompt_dim(const Kv4AttnParams& p, cudaStream_t st) {
+int launch_prompt_dim(const Kv4AttnParams& p, cudaStream_t st) {
     return p.k.dim == 64 ? launch_prompt<2, DT>(p, st) : (p.k.dim == 96 ? launch_prompt<3, DT>(p, st) : launch_prompt<4, DT>(p, st));
 }
 
@@ -519,6 +641,6 @@ cudaError_t launch_prompt_dim(const Kv4AttnParams& p, cudaStream_t st) {
 bool kv4_prompt_serves(const Kv4AttnParams& p, int dtype) {
     return dtype != 0 && p.k.dim <= 128 && (long long)p.max_rows * p.rep >= 64;
 }
-cudaError_t kv4_prompt(const Kv4AttnParams& p, int dtype, cudaStream_t st) { return dtype == 1 ? launch_prompt_dim<1>(p, st) : launch_prompt_dim<2>(p, st); }
+int kv4_prompt(const Kv4AttnParams& p, int dtype, cudaStream_t st) { return dtype == 1 ? launch_prompt_dim<1>(p, st) : launch_prompt_dim<2>(p, st); }
 
 }  // namespace pgk
