@@ -2,11 +2,12 @@
 //
 //   c[k, v] = score[k] + (x[k, v] - log sum_u exp x[k, u]);  the n largest of a group's beams x vocabulary, ties to the lowest (beam, token)
 //
-// What bounds the selection: the logits, read once.  A block takes up to 8192 logits of a row into registers: their maximum, the sum of their
-// exponentials, and their n best by the key (value, token), which no two share.  The n-th largest of the block's 256 per-thread maxima is a bound
-// that at least n elements reach, and at most n threads' elements (n x 32) can: those few are ranked by counting.  A block per group then
-// forms the rows' logarithms and ranks the survivors in float64, so that beams whose candidates lie within float32 rounding of each other
-// keep their order.
+// What bounds the selection: the logits, read once, and two launches.  A block takes up to 8192 logits of a row into registers: their maximum, the sum of
+// their exponentials, and their n best by the key (value, token), which no two share.  Elements below a bound are left out: with k = ceil(n / 8), the
+// smallest of its eight warps' k-th largest per-thread maxima, which at least n elements reach; what passes, some dozens of random logits, is ranked by
+// counting.  Where more pass than the list holds (logits that are all the same, say) the bound is the n-th largest of the 256 per-thread maxima
+// by key, which n threads' elements at most can reach.  A block per group then forms the rows' logarithms and takes the best of the sorted lists'
+// heads n times, in float64, so that beams whose candidates lie within float32 rounding of each other keep their order.
 #include "common.cuh"
 #include "tc_common.cuh"
 #include "../../include/pgk_b200.h"
@@ -25,6 +26,7 @@ struct BeamParams {
     const void* x; long ld;
     const float* scores; const int32_t* finished;
     int pad, beams, vocab, n, slices;
+    uint32_t beam_mul;                    // i / (slices n) = hi(i beam_mul) for as many entries as fit shared memory
     float2* part;                         // [row][slice]: maximum, sum
     unsigned long long* keys;             // [row][slice][n], best first; 0: none
     float* out_scores; int32_t* parents; int32_t* tokens;
@@ -42,11 +44,36 @@ __device__ __forceinline__ float beam_value(unsigned long long key) {
 
 template <int DT>
 __device__ __forceinline__ float beam_logit(const void* x, size_t i) {
-    float v;
-    if constexpr (DT == 0) v = __ldcg((const float*)x + i);
-    else if constexpr (DT == 1) { const uint16_t h = ld_act2((const uint16_t*)x + i); v = __half2float(__ushort_as_half(h)); }
-    else v = bf16_bits_to_f32(ld_act2((const uint16_t*)x + i));
-    return v;
+    if constexpr (DT == 0) return __ldcg((const float*)x + i);
+    else if constexpr (DT == 1) return __half2float(__ushort_as_half(ld_act2((const uint16_t*)x + i)));
+    else return bf16_bits_to_f32(ld_act2((const uint16_t*)x + i));
+}
+// four neighbouring logits; `wide`: they start on a 16-byte (8-byte, of 16 bits) boundary and all exist
+template <int DT>
+__device__ __forceinline__ void beam_load4(const void* x, size_t i, bool wide, int exist, float (&v)[4]) {
+    if constexpr (DT == 0) {
+        const float* p = (const float*)x + i;
+        if (wide) {
+            const uint4 w = ldg_stream(p);
+            v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] = c < exist ? __ldcg(p + c) : -INFINITY;
+        }
+    } else {
+        const uint16_t* p = (const uint16_t*)x + i;
+        uint16_t h[4] = {};
+        if (wide) {
+            const uint2 w = __ldcg((const uint2*)p);
+            h[0] = (uint16_t)w.x; h[1] = (uint16_t)(w.x >> 16); h[2] = (uint16_t)w.y; h[3] = (uint16_t)(w.y >> 16);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (c < exist) h[c] = ld_act2(p + c);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = c < exist ? (DT == 1 ? __half2float(__ushort_as_half(h[c])) : bf16_bits_to_f32(h[c])) : -INFINITY;
+    }
 }
 
 // the place of `mine` among the block's values: how many are larger (they are all different, or 0)
@@ -57,74 +84,101 @@ __device__ __forceinline__ int rank_of(const unsigned long long* all, int count,
 }
 
 template <int DT>
-__global__ void __launch_bounds__(B_THREADS) beam_rows_kernel(const __grid_constant__ BeamParams p) {
-    __shared__ unsigned long long best[B_THREADS], list[B_LIST];
-    __shared__ float red[B_THREADS / 32];
+__global__ void __launch_bounds__(B_THREADS, 4) beam_rows_kernel(const __grid_constant__ BeamParams p) {
+    constexpr int WARPS = B_THREADS / 32;
+    __shared__ unsigned long long best[B_THREADS], list[B_LIST], bound;
+    __shared__ float red[WARPS];
+    __shared__ uint32_t kth[WARPS];
     __shared__ int count;
-    __shared__ unsigned long long bound;
     griddep_wait();
     griddep_launch();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, slice = blockIdx.x, row = blockIdx.y;
     if (p.finished && __ldcg(p.finished + row) != 0) return;
     const int from = slice * B_SLICE, n_here = min(B_SLICE, p.vocab - from);
     const char* x = (const char*)p.x + (size_t)row * p.ld * (DT == 0 ? 4 : 2);
+    const bool aligned = ((uintptr_t)x & (DT == 0 ? 15 : 7)) == 0;
+    // element 4 (256 e + tid) + c of the slice is v[4 e + c]
     float v[B_EPT];
+#pragma unroll
+    for (int e = 0; e < B_EPT / 4; ++e) {
+        const int i = 4 * (e * B_THREADS + tid);
+        beam_load4<DT>(x, (size_t)from + i, aligned && i + 4 <= n_here, n_here - i, *(float (*)[4])(v + 4 * e));
+    }
     float top = -INFINITY;
     bool bad = false;
-#pragma unroll
-    for (int e = 0; e < B_EPT; ++e) {
-        const int i = e * B_THREADS + tid;
-        v[e] = i < n_here ? beam_logit<DT>(x, (size_t)from + i) : -INFINITY;
-    }
 #pragma unroll
     for (int e = 0; e < B_EPT; ++e) {
         bad |= v[e] != v[e];
         top = fmaxf(top, v[e]);
     }
     if (tid == 0) { count = 0; bound = 0; }
-    const float mine = top;
+    // the warp's k-th largest maximum, as ordered bits; 0 where fewer lanes have an element
+    {
+        const float mine = top;
+        uint32_t left = 4 * tid < n_here ? (uint32_t)(beam_key(mine, 0) >> 32) : 0u, got = 0;
+        const int k = (p.n + WARPS - 1) / WARPS;
+        for (int i = 0; i < k; ++i) {
+            got = __reduce_max_sync(0xffffffffu, left);
+            const uint32_t who = __ballot_sync(0xffffffffu, left == got);
+            if (lane == __ffs(who) - 1) left = 0;
+        }
+        if (lane == 0) kth[warp] = got;
+    }
     top = warp_max(top);
     if (lane == 0) red[warp] = top;
     bad = __syncthreads_or(bad);
+    uint32_t low = 0xffffffffu;
 #pragma unroll
-    for (int w = 0; w < B_THREADS / 32; ++w) top = fmaxf(top, red[w]);
-    // exponentials; the thread's best key
+    for (int w = 0; w < WARPS; ++w) {
+        top = fmaxf(top, red[w]);
+        low = min(low, kth[w]);
+    }
+    __syncthreads();
     float sum = 0.f;
     const float base = top == -INFINITY ? 0.f : top;
-    unsigned long long key = 0;
 #pragma unroll
-    for (int e = 0; e < B_EPT; ++e) {
-        const int i = e * B_THREADS + tid;
-        sum += expf(v[e] - base);
-        if (v[e] == mine && key == 0 && i < n_here) key = beam_key(v[e], (uint32_t)(from + i));
-    }
+    for (int e = 0; e < B_EPT; ++e) sum += ex2((v[e] - base) * 1.4426950408889634f);      // off by 2^-24 of the distance: terms that count lie near the maximum
+    const float cut = low == 0 ? -INFINITY : __uint_as_float(low ^ ((low >> 31) ? 0x80000000u : 0xffffffffu));
+#pragma unroll
+    for (int e = 0; e < B_EPT; ++e)
+        if (v[e] >= cut) {
+            const int i = 4 * (e / 4 * B_THREADS + tid) + (e & 3);
+            if (i < n_here) {
+                const int at = atomicAdd(&count, 1);
+                if (at < B_LIST) list[at] = beam_key(v[e], (uint32_t)(from + i));
+            }
+        }
     sum = warp_sum(sum);
-    __syncthreads();
     if (lane == 0) red[warp] = sum;
-    best[tid] = key;
     __syncthreads();
     if (tid == 0) {
         sum = 0.f;
-        for (int w = 0; w < B_THREADS / 32; ++w) sum += red[w];
-        // a row with a NaN, or with +infinity, has no candidates: its logarithm says so
-        p.part[(size_t)row * p.slices + slice] = make_float2(bad ? NAN : top, sum);
+        for (int w = 0; w < WARPS; ++w) sum += red[w];
+        p.part[(size_t)row * p.slices + slice] = make_float2(bad ? NAN : top, sum);       // a row with a NaN has no candidates: its maximum says so
     }
-    // the n-th largest of the threads' best keys (0 when fewer threads have any)
-    if (key && rank_of(best, B_THREADS, key) == p.n - 1) bound = key;
-    __syncthreads();
-    const unsigned long long cut = bound;
-#pragma unroll
-    for (int e = 0; e < B_EPT; ++e) {
-        const int i = e * B_THREADS + tid;
-        if (i < n_here && v[e] == v[e]) {
-            const unsigned long long k = beam_key(v[e], (uint32_t)(from + i));
-            if (k >= cut) {
+    if (count > B_LIST) {                                          // the whole block; the logits once more, element i by thread i % 256
+        unsigned long long key = 0;
+        __syncthreads();
+        for (int i = tid; i < n_here; i += B_THREADS) {
+            const float y = beam_logit<DT>(x, (size_t)from + i);
+            if (y == y) key = max(key, beam_key(y, (uint32_t)(from + i)));
+        }
+        best[tid] = key;
+        if (tid == 0) count = 0;
+        __syncthreads();
+        if (key && rank_of(best, B_THREADS, key) == p.n - 1) bound = key;
+        __syncthreads();
+        const unsigned long long least = bound;
+        for (int i = tid; i < n_here; i += B_THREADS) {
+            const float y = beam_logit<DT>(x, (size_t)from + i);
+            const unsigned long long k = beam_key(y, (uint32_t)(from + i));
+            if (y == y && k >= least) {
                 const int at = atomicAdd(&count, 1);
                 if (at < B_LIST) list[at] = k;
             }
         }
+        __syncthreads();
     }
-    __syncthreads();
     const int m = min(count, B_LIST);
     unsigned long long* out = p.keys + ((size_t)row * p.slices + slice) * p.n;
     for (int i = tid; i < m; i += B_THREADS) {
@@ -134,20 +188,34 @@ __global__ void __launch_bounds__(B_THREADS) beam_rows_kernel(const __grid_const
     for (int i = m + tid; i < p.n; i += B_THREADS) out[i] = 0;
 }
 
-// A group's candidates, ordered by (score, lower beam, lower token).  A candidate's place: score in float64, then its flat index.
-__device__ __forceinline__ bool ahead(double c, uint32_t beam, uint32_t token, double d, uint32_t beam2, uint32_t token2) {
-    return c > d || (c == d && (beam < beam2 || (beam == beam2 && token < token2)));
+// float64 as ordered bits, 0 below all (NaN is -infinity)
+__device__ __forceinline__ unsigned long long ordered(double c) {
+    const unsigned long long u = (unsigned long long)__double_as_longlong(c == c ? c : -INFINITY);
+    return u ^ ((u >> 63) ? ~0ull : 1ull << 63);
 }
+__device__ __forceinline__ double unordered(unsigned long long k) { return __longlong_as_double((long long)(k ^ ((k >> 63) ? 1ull << 63 : ~0ull))); }
 
+// A list per (beam, slice), best first; lists in the order of their tokens, so that of equal heads the lowest list's wins.  HELD: all scores in shared memory.
+template <bool HELD>
 __global__ void __launch_bounds__(B_THREADS) beam_merge_kernel(const __grid_constant__ BeamParams p) {
-    __shared__ double lse[B_MAX_BEAMS];
+    constexpr int WARPS = B_THREADS / 32;
+    extern __shared__ __align__(16) unsigned char smem[];          // next [lists], then scores [lists][n]
+    __shared__ double lse[B_MAX_BEAMS], base[B_MAX_BEAMS];
     __shared__ int state[B_MAX_BEAMS];             // 0: candidates from the row's lists; 1: finished; 2: nothing but -infinity
-    __shared__ double bc[B_THREADS / 32];
-    __shared__ uint32_t bb[B_THREADS / 32], bt[B_THREADS / 32];
+    __shared__ unsigned long long top_key[2][WARPS], won_key[B_MAX_N];
+    __shared__ int won_list[B_MAX_N], won_at[B_MAX_N];
+    __shared__ int top_list[2][WARPS];
     griddep_wait();
     griddep_launch();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.x, K = p.beams;
-    for (int k = warp; k < K; k += B_THREADS / 32) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.x, K = p.beams, lists = K * p.slices;
+    int* const next = (int*)smem;
+    unsigned long long* const held = (unsigned long long*)(smem + (((size_t)lists * 4 + 15) & ~(size_t)15));
+    if constexpr (HELD) {                          // the lists come while the logarithms are formed (those of beams that have none: anything)
+        for (int i = tid; i < lists * p.n; i += B_THREADS)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(held + i)), "l"(p.keys + (size_t)g * lists * p.n + i) : "memory");
+        cp_async_commit();
+    }
+    for (int k = warp; k < K; k += WARPS) {
         const int row = g * K + k;
         const float score = __ldcg(p.scores + row);
         int st = !(score > -1e30f) ? 2 : 0;
@@ -166,69 +234,91 @@ __global__ void __launch_bounds__(B_THREADS) beam_merge_kernel(const __grid_cons
             double sum = 0.0;
             for (int s = lane; s < p.slices; s += 32) {
                 const float2 q = __ldcg(p.part + (size_t)row * p.slices + s);
-                if (!bad && q.x > -INFINITY) sum += (double)q.y * exp((double)q.x - (double)top);
+                if (!bad && q.x > -INFINITY) sum += (double)q.y * (double)expf(q.x - top);
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             if (bad) st = 2;
             else l = (double)top + log(sum);
         }
-        if (lane == 0) { lse[k] = l; state[k] = st; }
+        if (lane == 0) { lse[k] = l; base[k] = (double)score; state[k] = st; }
+    }
+    for (int i = tid; i < lists; i += B_THREADS) next[i] = 0;
+    __syncthreads();
+    // entry j of list i: its score and its token
+    auto token_of = [&](int i, int j) -> uint32_t {
+        const int st = state[i / p.slices];
+        if (st == 0) return ~(uint32_t)__ldcg(p.keys + ((size_t)g * lists + i) * p.n + j);
+        if (st == 2) return (uint32_t)j;
+        return j == 0 ? (uint32_t)p.pad : (uint32_t)(j - 1 < p.pad ? j - 1 : j);
+    };
+    auto score_of = [&](unsigned long long key, int k, bool first_list, int j) -> unsigned long long {
+        const int st = state[k];
+        if (st == 0) return key ? ordered(base[k] + ((double)beam_value(key) - lse[k])) : 0;
+        if (!first_list || j >= p.vocab) return 0;                 // the first tokens, all at -infinity; a finished beam's pad at its score
+        return ordered(st == 1 && j == 0 ? base[k] : -INFINITY);
+    };
+    if constexpr (HELD) {
+        cp_async_wait<0>();
+        __syncthreads();
+        for (int i = tid; i < lists * p.n; i += B_THREADS) {
+            const int k = p.beam_mul ? (int)__umulhi((uint32_t)i, p.beam_mul) : i, in_beam = i - k * p.slices * p.n;
+            held[i] = score_of(held[i], k, in_beam < p.n, in_beam);
+        }
+        __syncthreads();
+    }
+    auto head = [&](int i) -> unsigned long long {
+        const int j = next[i];
+        if (j >= p.n) return 0;
+        if constexpr (HELD) return held[i * p.n + j];
+        else return score_of(__ldcg(p.keys + ((size_t)g * lists + i) * p.n + j), i / p.slices, i % p.slices == 0, j);
+    };
+    unsigned long long mine = 0;
+    int which = 0;
+    auto look = [&] {                              // the best head of this thread's lists
+        mine = 0;
+        for (int i = tid; i < lists; i += B_THREADS) {
+            const unsigned long long h = head(i);
+            if (h > mine) { mine = h; which = i; }
+        }
+    };
+    look();
+    for (int place = 0; place < p.n; ++place) {
+        unsigned long long k = mine;
+        int list = which;
+        auto best_of = [&](int width) {            // over the lanes below `width`: lowest list among equals
+            const uint32_t hi = __reduce_max_sync(0xffffffffu, lane < width ? (uint32_t)(k >> 32) : 0u);
+            const bool in = lane < width && (uint32_t)(k >> 32) == hi;
+            const uint32_t lo = __reduce_max_sync(0xffffffffu, in ? (uint32_t)k : 0u);
+            list = (int)__reduce_min_sync(0xffffffffu, in && (uint32_t)k == lo ? (uint32_t)list : 0x7fffffffu);
+            k = (unsigned long long)hi << 32 | lo;
+        };
+        best_of(32);
+        if (lane == 0) { top_key[place & 1][warp] = k; top_list[place & 1][warp] = list; }
+        __syncthreads();
+        k = lane < WARPS ? top_key[place & 1][lane] : 0;
+        list = lane < WARPS ? top_list[place & 1][lane] : 0;
+        best_of(WARPS);
+        if (list % B_THREADS == tid) {             // the winner's thread
+            won_key[place] = k;
+            won_list[place] = list;
+            won_at[place] = next[list]++;
+            look();
+        }
     }
     __syncthreads();
-    const int each = p.slices * p.n, total = K * each;
-    double last_c = INFINITY;
-    uint32_t last_b = 0, last_t = 0;
-    for (int place = 0; place < p.n; ++place) {
-        double c = -INFINITY;
-        uint32_t b = 0xffffffffu, t = 0xffffffffu;                 // behind every candidate
-        for (int i = tid; i < total; i += B_THREADS) {
-            const uint32_t k = (uint32_t)(i / each), j = (uint32_t)(i - (int)k * each);
-            const int row = g * K + (int)k;
-            double cc = -INFINITY;
-            uint32_t tt = j;
-            if (state[k] == 0) {
-                const unsigned long long key = __ldcg(p.keys + (size_t)row * each + j);
-                if (key == 0) continue;
-                tt = ~(uint32_t)key;
-                cc = (double)__ldcg(p.scores + row) + ((double)beam_value(key) - lse[k]);
-            } else {                                               // the first tokens, all at -infinity; a finished beam's pad at its score
-                if (j > (uint32_t)p.n) continue;
-                if (state[k] == 1) {
-                    tt = j == 0 ? (uint32_t)p.pad : (j - 1 < (uint32_t)p.pad ? j - 1 : j);
-                    if (j == 0) cc = (double)__ldcg(p.scores + row);
-                }
-                if (tt >= (uint32_t)p.vocab) continue;
-            }
-            if (place > 0 && !ahead(last_c, last_b, last_t, cc, k, tt)) continue;
-            if (ahead(cc, k, tt, c, b, t)) { c = cc; b = k; t = tt; }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const double c2 = __shfl_xor_sync(0xffffffffu, c, o);
-            const uint32_t b2 = __shfl_xor_sync(0xffffffffu, b, o), t2 = __shfl_xor_sync(0xffffffffu, t, o);
-            if (ahead(c2, b2, t2, c, b, t)) { c = c2; b = b2; t = t2; }
-        }
-        __syncthreads();
-        if (lane == 0) { bc[warp] = c; bb[warp] = b; bt[warp] = t; }
-        __syncthreads();
-        c = bc[0]; b = bb[0]; t = bt[0];
-        for (int w = 1; w < B_THREADS / 32; ++w)
-            if (ahead(bc[w], bb[w], bt[w], c, b, t)) { c = bc[w]; b = bb[w]; t = bt[w]; }
-        last_c = c; last_b = b; last_t = t;
-        if (tid == 0) {
-            const size_t at = (size_t)g * p.n + place;
-            p.out_scores[at] = (float)c;
-            p.parents[at] = (int32_t)b;
-            p.tokens[at] = (int32_t)t;
-        }
+    if (tid < p.n) {
+        const size_t at = (size_t)g * p.n + tid;
+        p.out_scores[at] = (float)unordered(won_key[tid]);
+        p.parents[at] = won_list[tid] / p.slices;
+        p.tokens[at] = (int32_t)token_of(won_list[tid], won_at[tid]);
     }
 }
 
 // ---------------------------------------------------------------- rows that follow their beams
 // A thread has one word of every row of its group: it loads them all, then stores the ones that change, so that a row may be parent and
 // child at once, and two children may have one parent.
-constexpr int R_ARRAYS = 64, R_REGS = 16, R_THREADS = 256, R_SMEM_THREADS = 128, R_MAX = 64;
+constexpr int R_ARRAYS = 64, R_REGS = 16, R_THREADS = 256, R_SMEM_THREADS = 128, R_MAX = 64;      // groups of more than R_REGS rows: through shared memory
 
 struct RowsParams {
     unsigned char* data[R_ARRAYS];
@@ -237,13 +327,13 @@ struct RowsParams {
     int rows, pairs, group;
 };
 
-template <typename W, bool SMEM>
-__global__ void __launch_bounds__(SMEM ? R_SMEM_THREADS : R_THREADS) rows_kernel(const __grid_constant__ RowsParams p) {
+template <typename W, int REGS>
+__global__ void __launch_bounds__(REGS ? R_THREADS : R_SMEM_THREADS) rows_kernel(const __grid_constant__ RowsParams p) {
     extern __shared__ __align__(16) unsigned char held[];
     __shared__ int from[R_MAX], to[R_MAX];
     griddep_wait();
     griddep_launch();
-    const int tid = threadIdx.x, T = SMEM ? R_SMEM_THREADS : R_THREADS, first = blockIdx.y * p.group, n = min(p.group, p.pairs - first);
+    const int tid = threadIdx.x, T = REGS ? R_THREADS : R_SMEM_THREADS, first = blockIdx.y * p.group, n = min(p.group, p.pairs - first);
     if (tid < n) {
         int s = __ldcg(p.src + first + tid), d = first + tid;
         if (p.dst) {
@@ -259,19 +349,19 @@ __global__ void __launch_bounds__(SMEM ? R_SMEM_THREADS : R_THREADS) rows_kernel
     const long long words = p.words[blockIdx.z];
     W* data = reinterpret_cast<W*>(p.data[blockIdx.z]);
     for (long long c = (long long)blockIdx.x * T + tid; c < words; c += (long long)gridDim.x * T) {
-        if constexpr (SMEM) {
+        if constexpr (REGS == 0) {
             W* mine = reinterpret_cast<W*>(held) + tid;
             for (int i = 0; i < n; ++i)
                 if (from[i] >= 0) mine[i * T] = __ldcg(data + from[i] * words + c);
             for (int i = 0; i < n; ++i)
                 if (from[i] >= 0) data[to[i] * words + c] = mine[i * T];
         } else {
-            W v[R_REGS];
+            W v[REGS];
 #pragma unroll
-            for (int i = 0; i < R_REGS; ++i)
+            for (int i = 0; i < REGS; ++i)
                 if (i < n && from[i] >= 0) v[i] = __ldcg(data + from[i] * words + c);
 #pragma unroll
-            for (int i = 0; i < R_REGS; ++i)
+            for (int i = 0; i < REGS; ++i)
                 if (i < n && from[i] >= 0) data[to[i] * words + c] = v[i];
         }
     }
@@ -288,10 +378,15 @@ cudaError_t launch_rows(RowsParams& p, int arrays, cudaStream_t st) {
     if (x > 65535) x = 65535;
     const size_t bytes = smem ? (size_t)p.group * T * sizeof(W) : 0;
     if (smem) {
-        if (cudaError_t e = cudaFuncSetAttribute(rows_kernel<W, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((size_t)R_MAX * T * sizeof(W)))) return e;
-        return launch_waiting(rows_kernel<W, true>, dim3((unsigned)x, blocks_y, arrays), dim3(T), bytes, st, p);
+        static bool configured = false;
+        if (!configured) {
+            if (cudaError_t e = cudaFuncSetAttribute(rows_kernel<W, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((size_t)R_MAX * T * sizeof(W)))) return e;
+            configured = true;
+        }
+        return launch_waiting(rows_kernel<W, 0>, dim3((unsigned)x, blocks_y, arrays), dim3(T), bytes, st, p);
     }
-    return launch_waiting(rows_kernel<W, false>, dim3((unsigned)x, blocks_y, arrays), dim3(T), 0, st, p);
+    auto kernel = p.group <= 4 ? rows_kernel<W, 4> : (p.group <= 8 ? rows_kernel<W, 8> : rows_kernel<W, 16>);
+    return launch_waiting(kernel, dim3((unsigned)x, blocks_y, arrays), dim3(T), 0, st, p);
 }
 
 }  // namespace
@@ -310,6 +405,7 @@ int pgk_beam_select(const void* logits, long ld, int dtype, const float* scores,
     PGK_REQUIRE(n > 0 && n <= B_MAX_N && (long long)n <= (long long)beams * vocab, "beam_select failed: %d of %d x %d candidates (64 at most)", n, beams, vocab);
     PGK_REQUIRE(!finished || (pad_token >= 0 && pad_token < vocab), "beam_select failed: pad token %d outside the vocabulary", pad_token);
     PGK_REQUIRE((long long)groups * beams <= 65535, "beam_select failed: %d groups of %d beams (65535 rows at most)", groups, beams);
+    PGK_REQUIRE((long long)vocab <= 400ll * B_SLICE, "beam_select failed: %d tokens (%lld at most)", vocab, 400ll * B_SLICE);
     if (groups == 0) return 0;
     PGK_REQUIRE(logits && scores && out_scores && out_parents && out_tokens, "beam_select failed: no logits, scores or outputs");
     const cudaStream_t st = (cudaStream_t)stream;
@@ -317,6 +413,7 @@ int pgk_beam_select(const void* logits, long ld, int dtype, const float* scores,
     p.x = logits; p.ld = ld; p.scores = scores; p.finished = finished;
     p.pad = pad_token; p.beams = beams; p.vocab = vocab; p.n = n;
     p.slices = (vocab + B_SLICE - 1) / B_SLICE;
+    p.beam_mul = p.slices * n > 1 ? (uint32_t)((1ull << 32) / (unsigned)(p.slices * n)) + 1 : 0;
     p.out_scores = out_scores; p.parents = out_parents; p.tokens = out_tokens;
     const size_t rows = (size_t)groups * beams, parts = rows * p.slices * sizeof(float2), keys = rows * p.slices * n * sizeof(unsigned long long);
     void* ws = nullptr;
@@ -325,7 +422,17 @@ int pgk_beam_select(const void* logits, long ld, int dtype, const float* scores,
     p.part = (float2*)((char*)ws + keys);
     auto kernel = dtype == 0 ? beam_rows_kernel<0> : (dtype == 1 ? beam_rows_kernel<1> : beam_rows_kernel<2>);
     cudaError_t e = launch_waiting(kernel, dim3(p.slices, (unsigned)rows), dim3(B_THREADS), 0, st, p);
-    if (e == cudaSuccess) e = launch_waiting(beam_merge_kernel, dim3(groups), dim3(B_THREADS), 0, st, p);
+    const size_t next = ((size_t)beams * p.slices * 4 + 15) & ~(size_t)15, held = next + (size_t)beams * p.slices * n * 8;
+    const size_t most = 200 * 1024;
+    static bool configured = false;
+    if (!configured && e == cudaSuccess) {
+        e = cudaFuncSetAttribute(beam_merge_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(beam_merge_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+        configured = e == cudaSuccess;
+    }
+    if (e == cudaSuccess)
+        e = held <= most ? launch_waiting(beam_merge_kernel<true>, dim3(groups), dim3(B_THREADS), held, st, p)
+                         : launch_waiting(beam_merge_kernel<false>, dim3(groups), dim3(B_THREADS), next, st, p);
     if (int rc = scratch_free(ws, st)) return rc;
     PGK_CUDA(e);
     return 0;

@@ -71,42 +71,50 @@ __device__ __forceinline__ void kv4_encode(const float (&x)[8], uint32_t& codes,
     for (int e = 0; e < 8; ++e) codes |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x[e], s)) + z, 0.f), 15.f) << (4 * e);
 }
 
-// eight neighbouring elements of type DT (0 f32, 1 f16, 2 bf16); `wide`: they start on a 16-byte boundary
-template <int DT>
-__device__ __forceinline__ void kv4_load8(const void* base, size_t at, bool wide, float (&x)[8]) {
-    if constexpr (DT == 0) {
-        const float* p = (const float*)base + at;
-        if (wide) {
-            const uint4 a = ld_act16(p), b = ld_act16(p + 4);
-            x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y); x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
-            x[4] = __uint_as_float(b.x); x[5] = __uint_as_float(b.y); x[6] = __uint_as_float(b.z); x[7] = __uint_as_float(b.w);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = __ldcg(p + e);
-        }
-    } else {
-        const uint16_t* p = (const uint16_t*)base + at;
-        uint32_t w[4];
-        if (wide) {
-            const uint4 a = ld_act16(p);
-            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = (uint32_t)ld_act2(p + 2 * e) | (uint32_t)ld_act2(p + 2 * e + 1) << 16;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if constexpr (DT == 2) {
-                x[2 * e] = bf16lo(w[e]);
-                x[2 * e + 1] = bf16hi(w[e]);
+// eight neighbouring elements of type DT (0 f32, 1 f16, 2 bf16) as they lie in memory; `wide`: they start on a 16-byte boundary
+template <int DT> struct Kv4Eight {
+    uint32_t w[DT == 0 ? 8 : 4];
+    __device__ __forceinline__ void load(const void* base, size_t at, bool wide) {
+        if constexpr (DT == 0) {
+            const uint32_t* p = (const uint32_t*)base + at;
+            if (wide) {
+                const uint4 a = ld_act16(p), b = ld_act16(p + 4);
+                w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+                w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
             } else {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-                x[2 * e] = f.x;
-                x[2 * e + 1] = f.y;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = __ldcg(p + e);
+            }
+        } else {
+            const uint16_t* p = (const uint16_t*)base + at;
+            if (wide) {
+                const uint4 a = ld_act16(p);
+                w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = (uint32_t)ld_act2(p + 2 * e) | (uint32_t)ld_act2(p + 2 * e + 1) << 16;
             }
         }
     }
-}
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+        if constexpr (DT == 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (DT == 2) {
+                    x[2 * e] = bf16lo(w[e]);
+                    x[2 * e + 1] = bf16hi(w[e]);
+                } else {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                    x[2 * e] = f.x;
+                    x[2 * e + 1] = f.y;
+                }
+            }
+        }
+    }
+};
 template <int DT>
 __device__ __forceinline__ uint32_t kv4_pack2(float lo, float hi) {
     if constexpr (DT == 2) return pack_bf16x2(lo, hi);

@@ -25,54 +25,71 @@ struct AppendParams {
     Kv4Pages kc;
     unsigned char* v_data;
     const int32_t* slots; const int32_t* positions;
-    int tokens, heads, per;               // per: rows of heads that a warp takes one after the other
-    bool wide_q, wide_k, wide_v;
+    int tokens, heads;
+    bool wide_q, wide_k, wide_v, wide_t;
 };
 
-template <int DT>
+template <int DT, int PER>
 __global__ void __launch_bounds__(A_WARPS * 32) kv4_append_kernel(const __grid_constant__ AppendParams p) {
     griddep_wait();
     griddep_launch();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, token = blockIdx.x;
     const int D = p.kc.dim, W = D / 8, G = D / 32, side = 32 / W;         // side: rows of a warp at a time
-    const int w = lane % W, which = lane / W;
-    const int pos = __ldcg(p.positions + token), page = kv4_page(p.kc, __ldcg(p.slots + token), pos);
-    if (page < 0 || (p.rot > 0 && pos >= p.table_rows)) return;
-    const int i0 = 8 * w, half = p.rot / 2;
-    float cs[8], sn[8];
-    const bool turns = i0 < p.rot && which < side;
+    const int w = lane % W, which = lane / W, i0 = 8 * w, half = p.rot / 2;
+    const int rows = p.heads + 2 * p.kc.kv_heads, first = (blockIdx.y * A_WARPS + warp) * PER * side;
+    if (first >= rows) return;                                             // the whole warp
+    const int pos = __ldcg(p.positions + token), slot = __ldcg(p.slots + token);
+    // q heads, then k, then v
+    auto place = [&](int r, int& kind, int& h) -> size_t {
+        kind = r < p.heads ? 0 : (r < p.heads + p.kc.kv_heads ? 1 : 2);
+        h = kind == 0 ? r : r - p.heads - (kind == 2 ? p.kc.kv_heads : 0);
+        return (size_t)token * (kind == 0 ? p.q_ld : (kind == 1 ? p.k_ld : p.v_ld)) + (size_t)h * D + i0;
+    };
+    Kv4Eight<DT> raw[PER];
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+        const int r = first + n * side + which;
+        int kind, h;
+        const size_t at = place(r, kind, h);
+        raw[n] = {};
+        if (which < side && r < rows) raw[n].load(kind == 0 ? p.q : (kind == 1 ? p.k : p.v), at, kind == 0 ? p.wide_q : (kind == 1 ? p.wide_k : p.wide_v));
+    }
+    if (p.rot > 0 && (unsigned)pos >= (unsigned)p.table_rows) return;      // the whole block
+    const bool turns = i0 < p.rot;
     const int other = p.pairs ? lane : (i0 < half ? lane + half / 8 : lane - half / 8);
+    Kv4Eight<0> c8 = {}, s8 = {};                                          // in pairs: the first four
     if (turns) {
-        const float* c = p.cos + (size_t)pos * p.rot;
-        const float* s = p.sin + (size_t)pos * p.rot;
+        const size_t at = (size_t)pos * p.rot + (p.pairs ? i0 / 2 : (i0 < half ? i0 : i0 - half));
         if (p.pairs) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { cs[e] = __ldcg(c + i0 / 2 + e); sn[e] = __ldcg(s + i0 / 2 + e); }
+            for (int e = 0; e < 4; ++e) { c8.w[e] = __ldcg((const uint32_t*)p.cos + at + e); s8.w[e] = __ldcg((const uint32_t*)p.sin + at + e); }
         } else {
-            const int at = i0 < half ? i0 : i0 - half;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) { cs[e] = __ldcg(c + at + e); sn[e] = __ldcg(s + at + e); }
+            c8.load(p.cos, at, p.wide_t);
+            s8.load(p.sin, at, p.wide_t);
         }
     }
-    const int rows = p.heads + 2 * p.kc.kv_heads, row = pos % p.kc.page_size;
-    const int first = (blockIdx.y * A_WARPS + warp) * p.per * side;
-    for (int n = 0; n < p.per; ++n) {
-        const int r = first + n * side + which;                            // q heads, then k, then v
-        if (first + n * side >= rows) break;                               // the whole warp
-        const bool live = which < side && r < rows;
-        const int kind = r < p.heads ? 0 : (r < p.heads + p.kc.kv_heads ? 1 : 2), h = kind == 0 ? r : r - p.heads - (kind == 2 ? p.kc.kv_heads : 0);
-        const void* src = kind == 0 ? p.q : (kind == 1 ? p.k : p.v);
-        const size_t at = (size_t)token * (kind == 0 ? p.q_ld : (kind == 1 ? p.k_ld : p.v_ld)) + (size_t)h * D + i0;
-        const bool wide = kind == 0 ? p.wide_q : (kind == 1 ? p.wide_k : p.wide_v);
-        float x[8], y[8];
+    const int page = kv4_page(p.kc, slot, pos);
+    if (page < 0) return;
+    float cs[8], sn[8];
+    c8.floats(cs);
+    s8.floats(sn);
+    const int row = pos % p.kc.page_size;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.f;
-        if (live) kv4_load8<DT>(src, at, wide, x);
+    for (int n = 0; n < PER; ++n) {
+        if (first + n * side >= rows) break;                               // the whole warp
+        const int r = first + n * side + which;
+        const bool live = which < side && r < rows;
+        int kind, h;
+        const size_t at = place(r, kind, h);
+        float x[8], y[8];
+        Kv4Eight<DT> far = raw[n];
         if (p.rot > 0 && !p.pairs) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], other & 31);
+            for (int e = 0; e < (DT == 0 ? 8 : 4); ++e) far.w[e] = __shfl_sync(0xffffffffu, far.w[e], other & 31);
         }
-        if (live && turns && kind != 2) {
+        raw[n].floats(x);
+        far.floats(y);
+        if (turns && kind != 2) {
             if (p.pairs) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -82,45 +99,57 @@ __global__ void __launch_bounds__(A_WARPS * 32) kv4_append_kernel(const __grid_c
                 }
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    x[e] = i0 < half ? __fsub_rn(__fmul_rn(x[e], cs[e]), __fmul_rn(y[e], sn[e])) : __fadd_rn(__fmul_rn(x[e], cs[e]), __fmul_rn(y[e], sn[e]));
+                for (int e = 0; e < 8; ++e) {
+                    const float a = __fmul_rn(x[e], cs[e]), b = __fmul_rn(y[e], sn[e]);
+                    x[e] = i0 < half ? __fsub_rn(a, b) : __fadd_rn(a, b);
+                }
             }
         }
+        if (live && kind == 0) kv4_store8<DT>(p.q, at, p.wide_q, x);
+        if (!__any_sync(0xffffffffu, live && kind != 0)) continue;
         uint32_t codes, word;
         kv4_encode(x, codes, word);
-        if (!live) continue;
-        if (kind == 0) {
-            if (p.rot > 0) kv4_store8<DT>(p.q, at, wide, x);
-            continue;
+        if (live && kind != 0) {
+            unsigned char* base = (kind == 1 ? p.kc.data : p.v_data) + ((size_t)page * p.kc.kv_heads + h) * ((size_t)p.kc.page_size * kv4_row_bytes(D));
+            const int t = w & 3, g = w >> 2;
+            *(uint32_t*)(base + (size_t)row * (D / 2) + 4 * (t * G + g)) = codes;
+            if (t == 0) *(uint16_t*)(base + (size_t)p.kc.page_size * (D / 2) + ((size_t)row * G + g) * 2) = (uint16_t)word;
         }
-        unsigned char* base = (kind == 1 ? p.kc.data : p.v_data) + ((size_t)page * p.kc.kv_heads + h) * ((size_t)p.kc.page_size * kv4_row_bytes(D));
-        const int t = w & 3, g = w >> 2;
-        *(uint32_t*)(base + (size_t)row * (D / 2) + 4 * (t * G + g)) = codes;
-        if (t == 0) *(uint16_t*)(base + (size_t)p.kc.page_size * (D / 2) + ((size_t)row * G + g) * 2) = (uint16_t)word;
     }
 }
 
-// a lane a word of codes, rows of heads side by side
+// a thread a word of codes of up to R_HEADS heads
+constexpr int R_HEADS = 4;
 template <int DT>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ Kv4Pages c, const int32_t* slots, const int32_t* positions, void* out, int tokens,
                                                        bool wide) {
     griddep_wait();
     griddep_launch();
-    const int D = c.dim, W = D / 8, G = D / 32;
+    const int D = c.dim, W = D / 8, G = D / 32, parts = (c.kv_heads + R_HEADS - 1) / R_HEADS;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (long long)tokens * c.kv_heads * W) return;
-    const int w = (int)(i % W), h = (int)(i / W % c.kv_heads), token = (int)(i / W / c.kv_heads);
+    if (i >= (long long)tokens * parts * W) return;
+    const int w = (int)(i % W), h0 = (int)(i / W % parts) * R_HEADS, token = (int)(i / W / parts);
     const int pos = __ldcg(positions + token), page = kv4_page(c, __ldcg(slots + token), pos);
-    float x[8] = {};
+    uint32_t codes[R_HEADS] = {}, word[R_HEADS] = {};
     if (page >= 0) {
-        const unsigned char* base = kv4_page_head(c, page, h);
+        const unsigned char* base = kv4_page_head(c, page, h0);
         const int row = pos % c.page_size, t = w & 3, g = w >> 2;
-        const uint32_t codes = __ldcg((const uint32_t*)(base + (size_t)row * (D / 2)) + t * G + g);
-        const uint32_t word = ld_act2((const uint16_t*)(base + (size_t)c.page_size * (D / 2)) + (size_t)row * G + g);
+        const size_t head = (size_t)c.page_size * kv4_row_bytes(D), at = (size_t)row * (D / 2) + 4 * (t * G + g), words = (size_t)c.page_size * (D / 2) + 2 * ((size_t)row * G + g);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = kv4_value(codes, e, word);
+        for (int h = 0; h < R_HEADS; ++h)
+            if (h0 + h < c.kv_heads) {
+                codes[h] = __ldcg((const uint32_t*)(base + h * head + at));
+                word[h] = ld_act2((const uint16_t*)(base + h * head + words));
+            }
     }
-    kv4_store8<DT>(out, (size_t)i * 8, wide, x);
+#pragma unroll
+    for (int h = 0; h < R_HEADS; ++h)
+        if (h0 + h < c.kv_heads) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = kv4_value(codes[h], e, word[h]);
+            kv4_store8<DT>(out, (((size_t)token * c.kv_heads + h0 + h) * W + w) * 8, wide, x);
+        }
 }
 
 }  // namespace
@@ -168,9 +197,12 @@ int pgk_kv4_append(void* q, const void* k, const void* v, long q_ld, long k_ld, 
     auto wide = [&](const void* x, long ld) { return (uintptr_t)x % 16 == 0 && ld * size % 16 == 0; };
     p.wide_q = wide(q, q_ld); p.wide_k = wide(k, k_ld); p.wide_v = wide(v, v_ld);
     const int side = 32 / (dim / 8), steps = (p.heads + 2 * kv_heads + side - 1) / side;
-    p.per = tokens >= 512 ? 4 : 1;
-    const dim3 grid(tokens, (steps + A_WARPS * p.per - 1) / (A_WARPS * p.per));
-    auto kernel = dtype == 0 ? kv4_append_kernel<0> : (dtype == 1 ? kv4_append_kernel<1> : kv4_append_kernel<2>);
+    p.wide_t = rot > 0 && ((uintptr_t)cos_table | (uintptr_t)sin_table) % 16 == 0;
+    // prompts: a warp's loads of six steps are on their way together, and share its token's page and angles
+    const int per = tokens >= 256 ? 6 : 1;
+    const dim3 grid(tokens, (steps + A_WARPS * per - 1) / (A_WARPS * per));
+    auto kernel = per == 6 ? (dtype == 0 ? kv4_append_kernel<0, 6> : (dtype == 1 ? kv4_append_kernel<1, 6> : kv4_append_kernel<2, 6>))
+                           : (dtype == 0 ? kv4_append_kernel<0, 1> : (dtype == 1 ? kv4_append_kernel<1, 1> : kv4_append_kernel<2, 1>));
     PGK_CUDA(launch_waiting(kernel, grid, dim3(A_WARPS * 32), 0, (cudaStream_t)stream, p));
     return 0;
 }
@@ -183,7 +215,7 @@ int pgk_kv4_read(const void* cache, int pages, int page_size, const int32_t* pag
     if (tokens == 0) return 0;
     PGK_REQUIRE(row_slots && positions && out, "kv4_read failed: no slots, positions or output");
     const Kv4Pages c = {(unsigned char*)cache, page_table, pages, page_size, slots, max_pages, kv_heads, dim};
-    const long long blocks = ((long long)tokens * kv_heads * (dim / 8) + 255) / 256;
+    const long long blocks = ((long long)tokens * ((kv_heads + R_HEADS - 1) / R_HEADS) * (dim / 8) + 255) / 256;
     PGK_REQUIRE(blocks <= 0x7fffffffll, "kv4_read failed: %d rows", tokens);
     auto kernel = dtype == 0 ? kv4_read_kernel<0> : (dtype == 1 ? kv4_read_kernel<1> : kv4_read_kernel<2>);
     PGK_CUDA(launch_waiting(kernel, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, c, row_slots, positions, out, tokens, (uintptr_t)out % 16 == 0));

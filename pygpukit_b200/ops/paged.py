@@ -14,7 +14,7 @@ from __future__ import annotations
 from .._lib import api
 from ..core.array import GPUArray
 from ..core.dtypes import bfloat16, float32, float_code, int32, uint8
-from ._common import _out, _st, _validate_float_dtype
+from ._common import _st
 
 INT4_DIMS = (64, 96, 128, 192, 256)
 
@@ -26,26 +26,32 @@ def int4_row_bytes(head_dim: int) -> int:
     return head_dim // 2 + head_dim // 16
 
 
+def _is(a: GPUArray, dtype) -> bool:
+    return a._dtype is dtype or a._dtype == dtype
+
+
 def _cache_check(name: str, caches, page_table: GPUArray, kv_heads: int, dim: int) -> tuple[int, int, int, int]:
     """(pages, page size, slots, pages of a slot)"""
     row = int4_row_bytes(dim)
+    shape = caches[0]._shape
     for c in caches:
-        if c.dtype != uint8 or c.ndim != 4:
+        if len(c._shape) != 4 or not _is(c, uint8):
             raise ValueError(f"{name}: a cache is uint8 [pages, kv_heads, page_size, {row}], got {c.dtype} {c.shape}")
-        if c.shape != caches[0].shape:
-            raise ValueError(f"{name}: the caches' shapes differ: {caches[0].shape} and {c.shape}")
-        if c.shape[1] != kv_heads or c.shape[3] != row:
-            raise ValueError(f"{name}: cache {c.shape} does not hold {kv_heads} heads of {dim} elements (rows of {row} bytes)")
-    if page_table.dtype != int32 or page_table.ndim != 2:
+        if c._shape != shape:
+            raise ValueError(f"{name}: the caches' shapes differ: {shape} and {c.shape}")
+    pages, heads, page_size, held = shape
+    if heads != kv_heads or held != row:
+        raise ValueError(f"{name}: cache {shape} does not hold {kv_heads} heads of {dim} elements (rows of {row} bytes)")
+    if len(page_table._shape) != 2 or not _is(page_table, int32):
         raise ValueError(f"{name}: page_table must be int32 [slots, max_pages], got {page_table.dtype} {page_table.shape}")
-    pages, _, page_size, _ = caches[0].shape
     if page_size < 16 or page_size % 16:
         raise ValueError(f"{name}: pages of {page_size} positions (multiples of 16)")
-    return pages, page_size, page_table.shape[0], page_table.shape[1]
+    slots, max_pages = page_table._shape
+    return pages, page_size, slots, max_pages
 
 
 def _index(name: str, what: str, a: GPUArray, n: int) -> None:
-    if a.dtype != int32 or a.ndim != 1 or a.shape[0] != n:
+    if a._shape != (n,) or not _is(a, int32):
         raise ValueError(f"{name}: {what} must be int32 [{n}], got {a.dtype} {a.shape}")
 
 
@@ -58,48 +64,53 @@ def rope_append_paged_int4(q: "GPUArray | None", k: GPUArray, v: GPUArray, cos: 
     cos = sin = None: nothing turns.  q None: only keys and values.  The keys are rounded to four bits from their float32 values.  Rows of a
     call name different positions.  A row whose slot is negative, or whose position the tables do not have, is skipped, its q included."""
     name = "rope_append_paged_int4"
-    _validate_float_dtype(k, name)
-    if k.ndim != 3 or v.shape != k.shape or v.dtype != k.dtype:
+    code = float_code(k._dtype, name)
+    shape = k._shape
+    if len(shape) != 3 or v._shape != shape or not _is(v, k._dtype):
         raise ValueError(f"{name} expects k, v [tokens, kv_heads, dim] of one type, got {k.dtype} {k.shape} and {v.dtype} {v.shape}")
-    T, H, D = k.shape
-    if q is not None and (q.ndim != 3 or q.dtype != k.dtype or q.shape[0] != T or q.shape[2] != D):
-        raise ValueError(f"{name} expects q [{T}, heads, {D}] of type {k.dtype}, got {q.dtype} {q.shape}")
+    T, H, D = shape
+    Hq, q_ptr = 0, None
+    if q is not None:
+        if len(q._shape) != 3 or q._shape[0] != T or q._shape[2] != D or not _is(q, k._dtype):
+            raise ValueError(f"{name} expects q [{T}, heads, {D}] of type {k.dtype}, got {q.dtype} {q.shape}")
+        Hq, q_ptr = q._shape[1], q._ptr
     pages, ps, n_slots, max_pages = _cache_check(name, (k_cache, v_cache), page_table, H, D)
     _index(name, "slots", slots, T)
     _index(name, "positions", positions, T)
-    rot = rows = 0
+    rot, rows, cos_ptr, sin_ptr = 0, 0, None, None
     if (cos is None) != (sin is None):
         raise ValueError(f"{name}: cos and sin come together")
     if cos is not None:
-        if cos.dtype != float32 or sin.dtype != float32 or cos.ndim != 2 or cos.shape != sin.shape:
+        if len(cos._shape) != 2 or sin._shape != cos._shape or not _is(cos, float32) or not _is(sin, float32):
             raise ValueError(f"{name}: cos, sin must be float32 [max positions, R], got {cos.dtype} {cos.shape} and {sin.dtype} {sin.shape}")
-        rows, rot = cos.shape
+        rows, rot = cos._shape
         if rows < 1 or rot < 16 or rot % 16 or rot > D:
             raise ValueError(f"{name}: a rotation of {rot} elements by tables of {rows} positions (R is a multiple of 16 up to {D})")
-    Hq = q.shape[1] if q is not None else 0
-    api.kv4_append(q.device_ptr if q is not None else None, k.device_ptr, v.device_ptr, Hq * D, H * D, H * D, cos.device_ptr if rot else None,
-                   sin.device_ptr if rot else None, rows, rot, 1 if interleaved else 0, k_cache.device_ptr, v_cache.device_ptr, pages, ps,
-                   page_table.device_ptr, n_slots, max_pages, slots.device_ptr, positions.device_ptr, T, Hq, H, D, float_code(k.dtype), _st())
+        cos_ptr, sin_ptr = cos._ptr, sin._ptr
+    api.kv4_append(q_ptr, k._ptr, v._ptr, Hq * D, H * D, H * D, cos_ptr, sin_ptr, rows, rot, 1 if interleaved else 0, k_cache._ptr, v_cache._ptr, pages, ps,
+                   page_table._ptr, n_slots, max_pages, slots._ptr, positions._ptr, T, Hq, H, D, code, _st())
 
 
 def kv_read_paged_int4(cache: GPUArray, page_table: GPUArray, slots: GPUArray, positions: GPUArray, *, out: GPUArray | None = None) -> GPUArray:
     """What the cache holds at (slots[t], positions[t]) as rows [tokens, kv_heads, dim] (of `out`'s type; bfloat16, which is exact, without
     one).  Skipped rows come back as zeros."""
     name = "kv_read_paged_int4"
-    if cache.ndim != 4 or cache.shape[3] % 9 or cache.shape[3] // 9 * 16 not in INT4_DIMS:
+    shape = cache._shape
+    if len(shape) != 4 or shape[3] % 9 or shape[3] // 9 * 16 not in INT4_DIMS:
         raise ValueError(f"{name}: a cache is uint8 [pages, kv_heads, page_size, row bytes], got {cache.dtype} {cache.shape}")
-    H, D = cache.shape[1], cache.shape[3] // 9 * 16
+    H, D = shape[1], shape[3] // 9 * 16
     pages, ps, n_slots, max_pages = _cache_check(name, (cache,), page_table, H, D)
-    if slots.ndim != 1:
+    if len(slots._shape) != 1:
         raise ValueError(f"{name}: slots must be int32 [tokens], got {slots.dtype} {slots.shape}")
-    T = slots.shape[0]
+    T = slots._shape[0]
     _index(name, "slots", slots, T)
     _index(name, "positions", positions, T)
-    if out is not None:
-        _validate_float_dtype(out, name)
-    out = _out(out, (T, H, D), bfloat16 if out is None else out.dtype)
-    api.kv4_read(cache.device_ptr, pages, ps, page_table.device_ptr, n_slots, max_pages, slots.device_ptr, positions.device_ptr, out.device_ptr, T, H, D,
-                 float_code(out.dtype), _st())
+    if out is None:
+        out = GPUArray((T, H, D), bfloat16)
+    elif out._shape != (T, H, D):
+        raise ValueError(f"{name}: out shape {out.shape} does not match expected {(T, H, D)}")
+    code = float_code(out._dtype, name)
+    api.kv4_read(cache._ptr, pages, ps, page_table._ptr, n_slots, max_pages, slots._ptr, positions._ptr, out._ptr, T, H, D, code, _st())
     return out
 
 
@@ -115,33 +126,33 @@ def sdpa_paged_int4(Q: GPUArray, k_cache: GPUArray, v_cache: GPUArray, out: GPUA
     softcap tanh(score / softcap).  sinks float32 [heads]: a logit of each head that joins the softmax and carries no value.  A row that sees no key is
     zeros.  Sums are float32; bfloat16 and float16 rows weigh values by weights of eight bits' rounding, float32 rows by full ones."""
     name = "sdpa_paged_int4"
-    _validate_float_dtype(Q, name)
-    if Q.ndim != 3 or out.shape != Q.shape or out.dtype != Q.dtype:
+    code = float_code(Q._dtype, name)
+    shape = Q._shape
+    if len(shape) != 3 or out._shape != shape or not _is(out, Q._dtype):
         raise ValueError(f"{name} expects Q and out [tokens, heads, dim] of one type, got {Q.dtype} {Q.shape} and {out.dtype} {out.shape}")
-    T, Hq, D = Q.shape
-    H = k_cache.shape[1] if k_cache.ndim == 4 else 0
+    T, Hq, D = shape
+    H = k_cache._shape[1] if len(k_cache._shape) == 4 else 0
     pages, ps, n_slots, max_pages = _cache_check(name, (k_cache, v_cache), page_table, H, D)
-    if H < 1 or Hq % H:
+    if H < 1 or Hq < 1 or Hq % H:
         raise ValueError(f"{name}: n_heads {Hq} must be a multiple of KV heads {H}")
-    if slots.ndim != 1:
+    if len(slots._shape) != 1:
         raise ValueError(f"{name}: slots must be int32 [sequences], got {slots.dtype} {slots.shape}")
-    S = slots.shape[0]
+    S = slots._shape[0]
     _index(name, "slots", slots, S)
     _index(name, "context_lens", context_lens, S)
     if row_starts is not None:
         _index(name, "row_starts", row_starts, S + 1)
     elif S != T or max_rows != 1:
         raise ValueError(f"{name}: {S} sequences and {T} rows need row_starts")
-    if max_rows < 1 or max_context < 0 or max_context > max_pages * ps:
+    if max_rows < 1 or not 0 <= max_context <= max_pages * ps:
         raise ValueError(f"{name}: max_rows {max_rows}, max_context {max_context} out of range ({max_pages} pages of {ps})")
     if window < 0 or not softcap >= 0.0 or not scale >= 0.0:
         raise ValueError(f"{name}: window {window}, softcap {softcap} and scale {scale} must not be negative")
-    if sinks is not None and (sinks.dtype != float32 or sinks.shape != (Hq,)):
+    if sinks is not None and (sinks._shape != (Hq,) or not _is(sinks, float32)):
         raise ValueError(f"{name}: sinks must be float32 [{Hq}], got {sinks.dtype} {sinks.shape}")
-    api.kv4_attention(Q.device_ptr, Hq * D, k_cache.device_ptr, v_cache.device_ptr, out.device_ptr, Hq * D, pages, ps, page_table.device_ptr, n_slots,
-                      max_pages, slots.device_ptr, context_lens.device_ptr, row_starts.device_ptr if row_starts is not None else None, S, T, int(max_rows),
-                      int(max_context), Hq, H, D, float(scale), int(window), float(softcap), sinks.device_ptr if sinks is not None else None,
-                      float_code(Q.dtype), _st())
+    api.kv4_attention(Q._ptr, Hq * D, k_cache._ptr, v_cache._ptr, out._ptr, Hq * D, pages, ps, page_table._ptr, n_slots, max_pages, slots._ptr,
+                      context_lens._ptr, None if row_starts is None else row_starts._ptr, S, T, max_rows, max_context, Hq, H, D, scale, window, softcap,
+                      None if sinks is None else sinks._ptr, code, _st())
 
 
 __all__ = ["int4_row_bytes", "rope_append_paged_int4", "kv_read_paged_int4", "sdpa_paged_int4"]

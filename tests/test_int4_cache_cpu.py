@@ -114,7 +114,7 @@ def test_the_library_refuses_what_the_operators_do():
     assert lib.pgk_kv4_attention(*{**good, "tokens": 0, "seqs": 0}.values()) == 0
     good = dict(x=p, ld=100, dtype=0, scores=p, finished=None, pad=0, groups=2, beams=3, vocab=100, n=6, s=p, b=p, t=p, stream=None)
     for bad in (dict(dtype=3), dict(beams=0), dict(beams=65), dict(n=0), dict(n=65), dict(ld=99), dict(vocab=0), dict(finished=p, pad=100), dict(groups=30000),
-                dict(x=None), dict(t=None), dict(vocab=1, n=4)):
+                dict(x=None), dict(t=None), dict(vocab=1, n=4), dict(vocab=4000000, ld=4000000)):
         assert lib.pgk_beam_select(*{**good, **bad}.values()) != 0, bad
         assert "beam_select failed" in _lib.last_error()
     assert lib.pgk_beam_select(*{**good, "groups": 0}.values()) == 0
