@@ -861,7 +861,7 @@ int pgk_kv4_attention(const void* q, long q_ld, const void* k_cache, const void*
                       float scale, int window, float softcap, const float* sinks, int dtype, void* stream);
 /* The n best of every group's beams x vocab candidates score[k] + log_softmax(logits[k])[v] (rows of ld elements), best first, ties to the lower
  * beam, then the lower token.  finished (or NULL): such a beam keeps its score and has the one candidate pad_token.  Candidates at -infinity
- * come last: logits of -infinity, beams whose score is NaN or below -1e30, rows with a NaN or +infinity.  beams, n <= 64, vocab <= 3276800. */
+ * come last: logits of -infinity, beams whose score is NaN or below -1e30, rows with a NaN or +infinity.  beams, n <= 64, vocab <= 2048000. */
 int pgk_beam_select(const void* logits, long ld, int dtype, const float* scores, const int32_t* finished, int pad_token, int groups, int beams,
                     int vocab, int n, float* out_scores, int32_t* out_parents, int32_t* out_tokens, void* stream);
 /* Rows of many arrays [rows][host_row_bytes[a]].  dst NULL: in groups of `group` rows, row i of a group becomes, in place, what row src[i] of it

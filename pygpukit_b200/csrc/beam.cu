@@ -104,12 +104,11 @@ __global__ void __launch_bounds__(B_THREADS, 4) beam_rows_kernel(const __grid_co
         const int i = 4 * (e * B_THREADS + tid);
         beam_load4<DT>(x, (size_t)from + i, aligned && i + 4 <= n_here, n_here - i, *(float (*)[4])(v + 4 * e));
     }
-    float top = -INFINITY;
-    bool bad = false;
+    float four[B_EPT / 4], top = -INFINITY;                        // the maxima of neighbouring fours
 #pragma unroll
-    for (int e = 0; e < B_EPT; ++e) {
-        bad |= v[e] != v[e];
-        top = fmaxf(top, v[e]);
+    for (int e = 0; e < B_EPT / 4; ++e) {
+        four[e] = fmaxf(fmaxf(v[4 * e], v[4 * e + 1]), fmaxf(v[4 * e + 2], v[4 * e + 3]));
+        top = fmaxf(top, four[e]);
     }
     if (tid == 0) { count = 0; bound = 0; }
     // the warp's k-th largest maximum, as ordered bits; 0 where fewer lanes have an element
@@ -126,7 +125,7 @@ __global__ void __launch_bounds__(B_THREADS, 4) beam_rows_kernel(const __grid_co
     }
     top = warp_max(top);
     if (lane == 0) red[warp] = top;
-    bad = __syncthreads_or(bad);
+    __syncthreads();
     uint32_t low = 0xffffffffu;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
@@ -140,13 +139,15 @@ __global__ void __launch_bounds__(B_THREADS, 4) beam_rows_kernel(const __grid_co
     for (int e = 0; e < B_EPT; ++e) sum += ex2((v[e] - base) * 1.4426950408889634f);      // off by 2^-24 of the distance: terms that count lie near the maximum
     const float cut = low == 0 ? -INFINITY : __uint_as_float(low ^ ((low >> 31) ? 0x80000000u : 0xffffffffu));
 #pragma unroll
-    for (int e = 0; e < B_EPT; ++e)
-        if (v[e] >= cut) {
-            const int i = 4 * (e / 4 * B_THREADS + tid) + (e & 3);
-            if (i < n_here) {
-                const int at = atomicAdd(&count, 1);
-                if (at < B_LIST) list[at] = beam_key(v[e], (uint32_t)(from + i));
-            }
+    for (int e = 0; e < B_EPT / 4; ++e)
+        if (four[e] >= cut) {
+            const int i = 4 * (e * B_THREADS + tid);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (v[4 * e + c] >= cut && i + c < n_here) {
+                    const int at = atomicAdd(&count, 1);
+                    if (at < B_LIST) list[at] = beam_key(v[4 * e + c], (uint32_t)(from + i + c));
+                }
         }
     sum = warp_sum(sum);
     if (lane == 0) red[warp] = sum;
@@ -154,7 +155,8 @@ __global__ void __launch_bounds__(B_THREADS, 4) beam_rows_kernel(const __grid_co
     if (tid == 0) {
         sum = 0.f;
         for (int w = 0; w < WARPS; ++w) sum += red[w];
-        p.part[(size_t)row * p.slices + slice] = make_float2(bad ? NAN : top, sum);       // a row with a NaN has no candidates: its maximum says so
+        // a row with a NaN or +infinity has no candidates: its sum is NaN, and its maximum says so
+        p.part[(size_t)row * p.slices + slice] = make_float2(sum != sum ? NAN : top, sum);
     }
     if (count > B_LIST) {                                          // the whole block; the logits once more, element i by thread i % 256
         unsigned long long key = 0;
@@ -199,17 +201,17 @@ __device__ __forceinline__ double unordered(unsigned long long k) { return __lon
 template <bool HELD>
 __global__ void __launch_bounds__(B_THREADS) beam_merge_kernel(const __grid_constant__ BeamParams p) {
     constexpr int WARPS = B_THREADS / 32;
-    extern __shared__ __align__(16) unsigned char smem[];          // next [lists], then scores [lists][n]
+    extern __shared__ __align__(16) unsigned char smem[];          // heads [lists], next [lists], then scores [lists][n]
     __shared__ double lse[B_MAX_BEAMS], base[B_MAX_BEAMS];
     __shared__ int state[B_MAX_BEAMS];             // 0: candidates from the row's lists; 1: finished; 2: nothing but -infinity
-    __shared__ unsigned long long top_key[2][WARPS], won_key[B_MAX_N];
+    __shared__ unsigned long long won_key[B_MAX_N];
     __shared__ int won_list[B_MAX_N], won_at[B_MAX_N];
-    __shared__ int top_list[2][WARPS];
     griddep_wait();
     griddep_launch();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.x, K = p.beams, lists = K * p.slices;
-    int* const next = (int*)smem;
-    unsigned long long* const held = (unsigned long long*)(smem + (((size_t)lists * 4 + 15) & ~(size_t)15));
+    unsigned long long* const heads = (unsigned long long*)smem;
+    int* const next = (int*)(heads + lists);
+    unsigned long long* const held = (unsigned long long*)(smem + (((size_t)lists * 12 + 15) & ~(size_t)15));
     if constexpr (HELD) {                          // the lists come while the logarithms are formed (those of beams that have none: anything)
         for (int i = tid; i < lists * p.n; i += B_THREADS)
             asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(held + i)), "l"(p.keys + (size_t)g * lists * p.n + i) : "memory");
@@ -273,37 +275,32 @@ __global__ void __launch_bounds__(B_THREADS) beam_merge_kernel(const __grid_cons
         if constexpr (HELD) return held[i * p.n + j];
         else return score_of(__ldcg(p.keys + ((size_t)g * lists + i) * p.n + j), i / p.slices, i % p.slices == 0, j);
     };
-    unsigned long long mine = 0;
-    int which = 0;
-    auto look = [&] {                              // the best head of this thread's lists
-        mine = 0;
-        for (int i = tid; i < lists; i += B_THREADS) {
-            const unsigned long long h = head(i);
-            if (h > mine) { mine = h; which = i; }
-        }
-    };
-    look();
-    for (int place = 0; place < p.n; ++place) {
-        unsigned long long k = mine;
-        int list = which;
-        auto best_of = [&](int width) {            // over the lanes below `width`: lowest list among equals
-            const uint32_t hi = __reduce_max_sync(0xffffffffu, lane < width ? (uint32_t)(k >> 32) : 0u);
-            const bool in = lane < width && (uint32_t)(k >> 32) == hi;
-            const uint32_t lo = __reduce_max_sync(0xffffffffu, in ? (uint32_t)k : 0u);
-            list = (int)__reduce_min_sync(0xffffffffu, in && (uint32_t)k == lo ? (uint32_t)list : 0x7fffffffu);
-            k = (unsigned long long)hi << 32 | lo;
+    for (int i = tid; i < lists; i += B_THREADS) heads[i] = head(i);
+    __syncthreads();
+    if (warp == 0) {                               // one warp: its lanes have every 32nd list, and no barrier stands between two places
+        unsigned long long mine = 0;
+        int which = 0;
+        auto look = [&] {                          // the best head of this lane's lists
+            mine = 0;
+            for (int i = lane; i < lists; i += 32) {
+                const unsigned long long h = heads[i];
+                if (h > mine) { mine = h; which = i; }
+            }
         };
-        best_of(32);
-        if (lane == 0) { top_key[place & 1][warp] = k; top_list[place & 1][warp] = list; }
-        __syncthreads();
-        k = lane < WARPS ? top_key[place & 1][lane] : 0;
-        list = lane < WARPS ? top_list[place & 1][lane] : 0;
-        best_of(WARPS);
-        if (list % B_THREADS == tid) {             // the winner's thread
-            won_key[place] = k;
-            won_list[place] = list;
-            won_at[place] = next[list]++;
-            look();
+        look();
+        for (int place = 0; place < p.n; ++place) {
+            const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32));
+            const bool in = (uint32_t)(mine >> 32) == hi;
+            const uint32_t lo = __reduce_max_sync(0xffffffffu, in ? (uint32_t)mine : 0u);
+            const int list = (int)__reduce_min_sync(0xffffffffu, in && (uint32_t)mine == lo ? (uint32_t)which : 0x7fffffffu);       // of equals the lowest
+            if (in && (uint32_t)mine == lo && which == list) {
+                won_key[place] = mine;
+                won_list[place] = list;
+                won_at[place] = next[list]++;
+                heads[list] = head(list);
+                look();
+            }
+            __syncwarp();
         }
     }
     __syncthreads();
@@ -405,7 +402,7 @@ int pgk_beam_select(const void* logits, long ld, int dtype, const float* scores,
     PGK_REQUIRE(n > 0 && n <= B_MAX_N && (long long)n <= (long long)beams * vocab, "beam_select failed: %d of %d x %d candidates (64 at most)", n, beams, vocab);
     PGK_REQUIRE(!finished || (pad_token >= 0 && pad_token < vocab), "beam_select failed: pad token %d outside the vocabulary", pad_token);
     PGK_REQUIRE((long long)groups * beams <= 65535, "beam_select failed: %d groups of %d beams (65535 rows at most)", groups, beams);
-    PGK_REQUIRE((long long)vocab <= 400ll * B_SLICE, "beam_select failed: %d tokens (%lld at most)", vocab, 400ll * B_SLICE);
+    PGK_REQUIRE((long long)vocab <= 250ll * B_SLICE, "beam_select failed: %d tokens (%lld at most)", vocab, 250ll * B_SLICE);
     if (groups == 0) return 0;
     PGK_REQUIRE(logits && scores && out_scores && out_parents && out_tokens, "beam_select failed: no logits, scores or outputs");
     const cudaStream_t st = (cudaStream_t)stream;
@@ -422,7 +419,7 @@ int pgk_beam_select(const void* logits, long ld, int dtype, const float* scores,
     p.part = (float2*)((char*)ws + keys);
     auto kernel = dtype == 0 ? beam_rows_kernel<0> : (dtype == 1 ? beam_rows_kernel<1> : beam_rows_kernel<2>);
     cudaError_t e = launch_waiting(kernel, dim3(p.slices, (unsigned)rows), dim3(B_THREADS), 0, st, p);
-    const size_t next = ((size_t)beams * p.slices * 4 + 15) & ~(size_t)15, held = next + (size_t)beams * p.slices * n * 8;
+    const size_t next = ((size_t)beams * p.slices * 12 + 15) & ~(size_t)15, held = next + (size_t)beams * p.slices * n * 8;
     const size_t most = 200 * 1024;
     static bool configured = false;
     if (!configured && e == cudaSuccess) {

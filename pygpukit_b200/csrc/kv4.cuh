@@ -65,10 +65,17 @@ __device__ __forceinline__ void kv4_encode(const float (&x)[8], uint32_t& codes,
     word = 0;
     if (bad) { word = kKv4Nan; return; }
     if (!(s >= 9.094947e-13f)) return;                         // 2^-40
-    const float z = rintf(__fdiv_rn(-lo, s));
+    // x / s by a product with the rounded reciprocal and one residual: correctly rounded (Markstein, IBM J. Res. Dev. 34, 1990), 3 operations where a
+    // division of its own takes about ten.  Adding 1.5 2^23 leaves a quotient of 15 at most rounded to the nearest integer in the lowest bits.
+    const float r = __frcp_rn(s), magic = 12582912.f;
+    auto rounded = [&](float x) {
+        const float q = x * r;
+        return __float_as_uint(__fadd_rn(fmaf(fmaf(-s, q, x), r, q), magic)) - 0x4b400000u;
+    };
+    const int z = (int)rounded(-lo);
     word = (__float_as_uint(s) >> 16) | (uint32_t)z;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) codes |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x[e], s)) + z, 0.f), 15.f) << (4 * e);
+    for (int e = 0; e < 8; ++e) codes |= (uint32_t)min(max((int)rounded(x[e]) + z, 0), 15) << (4 * e);
 }
 
 // eight neighbouring elements of type DT (0 f32, 1 f16, 2 bf16) as they lie in memory; `wide`: they start on a 16-byte boundary

@@ -73,6 +73,10 @@ __global__ void __launch_bounds__(A_WARPS * 32) kv4_append_kernel(const __grid_c
     float cs[8], sn[8];
     c8.floats(cs);
     s8.floats(sn);
+    if (!p.pairs && i0 < half) {                                           // a cos - b sin as a cos + b (-sin): the same bits
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sn[e] = -sn[e];
+    }
     const int row = pos % p.kc.page_size;
 #pragma unroll
     for (int n = 0; n < PER; ++n) {
@@ -99,10 +103,7 @@ __global__ void __launch_bounds__(A_WARPS * 32) kv4_append_kernel(const __grid_c
                 }
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float a = __fmul_rn(x[e], cs[e]), b = __fmul_rn(y[e], sn[e]);
-                    x[e] = i0 < half ? __fsub_rn(a, b) : __fadd_rn(a, b);
-                }
+                for (int e = 0; e < 8; ++e) x[e] = __fadd_rn(__fmul_rn(x[e], cs[e]), __fmul_rn(y[e], sn[e]));
             }
         }
         if (live && kind == 0) kv4_store8<DT>(p.q, at, p.wide_q, x);

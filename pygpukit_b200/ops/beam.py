@@ -10,7 +10,7 @@ from ._common import _st
 from .paged import _is
 
 MAX_BEAMS = 64
-MAX_VOCAB = 3276800
+MAX_VOCAB = 2048000
 
 
 def beam_select(logits: GPUArray, scores: GPUArray, n: int | None = None, *, finished: GPUArray | None = None, pad_token: int = 0,
