@@ -1,5 +1,6 @@
 from .base import DecodeStrategy
 from .batch import DecodeBatch
+from .beam import BeamSearch
 from .jacobi import DecodeJacobi
 from .m1 import DecodeM1
 from .m1_graph import DecodeM1Graph
@@ -7,4 +8,4 @@ from .ragged import RaggedScheduler, Request
 from .speculative import DecodeSpeculative
 
 __all__ = ["DecodeStrategy", "DecodeM1", "DecodeM1Graph", "DecodeBatch", "DecodeSpeculative", "DecodeJacobi", "RaggedScheduler",
-           "Request"]
+           "Request", "BeamSearch"]
