@@ -26,7 +26,7 @@ constexpr int P_ROWS = 128, P_KEYS = 128, P_SOFT = 8, P_EXPAND = 8, P_THREADS = 
 constexpr uint32_t P_CHUNK = P_KEYS * 128;                         // 64 elements of 128 keys
 constexpr uint32_t P_O = 0, P_Q = 128, P_S = 256;                  // TMEM columns: outputs, queries (two terms of 64), two tiles of scores
 constexpr float P_LAZY = 8.f;
-constexpr int P_IMAGES_FROM = 4;                                   // blocks of rows that read a sequence's tiles
+constexpr int P_IMAGES_FROM = 512;                                 // rows of a sequence and head that read its tiles
 constexpr long long P_IMAGES_MOST = 1ll << 30;
 
 // Tiles as they lie in shared memory, made ahead of the products: [sequence][head][tile][K, V], and per tile whether a value is NaN.  Tile 0 is the one
@@ -148,6 +148,218 @@ __global__ void __launch_bounds__(P_EXPAND * 32) kv4_images_kernel(const __grid_
     if (tid == 0) im.nans[n] = any;
 }
 
+// A block's rows -- ROWS of one sequence's, a token's query heads of one key head beside each other -- and the tiles that they see between them.  Blocks
+// come with the longest rows first.
+template <int ROWS> struct Block {
+    int seq, head, split, slot, ctx, first, n_rows, f0, live, pos0, pos1, begin, end, tbeg, n;
+    const int32_t* table;
+    __device__ __forceinline__ explicit Block(const Kv4AttnParams& p) {
+        seq = blockIdx.x % p.seqs;
+        f0 = (p.tiles - 1 - (int)(blockIdx.x / p.seqs)) * ROWS;
+        head = blockIdx.y;
+        split = blockIdx.z;
+        slot = __ldcg(p.seq_slots + seq);
+        ctx = __ldcg(p.contexts + seq);
+        first = p.starts ? __ldcg(p.starts + seq) : seq;
+        n_rows = p.starts ? __ldcg(p.starts + seq + 1) - first : 1;
+        const int rows = min(min(n_rows, p.max_rows), 0x7fffffff / p.rep) * p.rep;
+        const bool work = f0 < rows && (unsigned)slot < (unsigned)p.k.slots;               // the same in all of the cluster
+        live = work ? min(ROWS, rows - f0) : 0;
+        pos0 = ctx - n_rows + f0 / p.rep;
+        pos1 = ctx - n_rows + (f0 + max(live, 1) - 1) / p.rep;
+        begin = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
+        end = work ? min(min(pos1 + 1, ctx), p.max_keys) : 0;
+        const int t0 = begin / P_KEYS, nt = max(0, (end + P_KEYS - 1) / P_KEYS - t0), per = (nt + p.splits - 1) / p.splits;
+        tbeg = t0 + split * per;
+        n = max(0, min(nt, (split + 1) * per) - split * per);
+        table = p.k.table + (work ? (size_t)slot * p.k.max_pages : 0);
+    }
+    // whether a page of the keys does not exist, by `count` threads of which this is number i
+    __device__ __forceinline__ bool gone(const Kv4AttnParams& p, int i, int count) const {
+        bool g = false;
+        const int last = min(end, (tbeg + n) * P_KEYS);
+        for (int j = tbeg * P_KEYS + 16 * i; j < last; j += 16 * count) g |= (unsigned)__ldcg(table + kv4_page_of(p, (uint32_t)j >> 4)) >= (unsigned)p.k.pages;
+        return g;
+    }
+};
+// Row r of a block: whose it is, and what it sees: keys in (under, limit]
+struct Row {
+    int tok, h, pos, limit, under;
+    bool live;
+    template <int ROWS> __device__ __forceinline__ Row(const Kv4AttnParams& p, const Block<ROWS>& b, int r) {
+        const int f = b.f0 + r, i = f / p.rep;
+        tok = b.first + i;
+        h = b.head * p.rep + f - i * p.rep;
+        pos = b.ctx - b.n_rows + i;
+        live = r < b.live && tok >= 0 && tok < p.tokens;
+        limit = live ? min(pos, b.end - 1) : -1;
+        under = p.window > 0 ? pos - p.window : -1;
+    }
+};
+// eight query elements in the order of a word's nibbles, as one or two bfloat16 terms
+template <int DT>
+__device__ __forceinline__ void query8(const Kv4AttnParams& p, const Row& r, int at, uint32_t* a, uint32_t* b) {
+    uint32_t w[4] = {};
+    if (r.live) {
+        const uint16_t* src = (const uint16_t*)p.q + (size_t)r.tok * p.q_ld + at;
+        if (p.wide_q) {
+            const uint4 v = ld_act16(src);
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = (uint32_t)ld_act2(src + 2 * e) | (uint32_t)ld_act2(src + 2 * e + 1) << 16;
+        }
+    }
+    const uint32_t v[4] = {__byte_perm(w[0], w[2], 0x5410), __byte_perm(w[0], w[2], 0x7632), __byte_perm(w[1], w[3], 0x5410), __byte_perm(w[1], w[3], 0x7632)};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (DT == 1) {
+            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v[e]));
+            a[e] = pack_bf16x2(x.x, x.y);
+            b[e] = pack_bf16x2(x.x - bf16lo(a[e]), x.y - bf16hi(a[e]));
+        } else
+            a[e] = v[e];
+    }
+}
+// N scores of a row, from TMEM column `at`, key j0: capped, and -infinity where the row does not see; `off`: runs of 16 keys without a page
+template <int N>
+__device__ __forceinline__ void row_scores(const Kv4AttnParams& p, uint32_t at, int j0, bool edge, const Row& r, uint32_t off, float (&s)[N]) {
+#pragma unroll
+    for (int c = 0; c < N; c += 16) tmem_ld16_async(at + (uint32_t)c, *(float (*)[16])(s + c));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < N; c += 16) tmem_pass(*(float (*)[16])(s + c));
+    if (p.cap_log2 > 0.f) {
+        const float in = p.scale_log2 * 2.885390043f / p.cap_log2;
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[e] = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(s[e] * in)));
+    }
+    if (edge) {
+        const int hi = r.limit - j0, lo = r.under - j0;
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (e > hi || e <= lo || ((off >> (e / 16)) & 1u)) s[e] = -INFINITY;
+    }
+}
+// of `runs` runs of 16 keys from j0 on, the ones without a page
+template <int ROWS>
+__device__ __forceinline__ uint32_t runs_gone(const Kv4AttnParams& p, const Block<ROWS>& b, int j0, int runs) {
+    uint32_t off = 0;
+    for (int u = 0; u < runs; ++u)
+        if (j0 + 16 * u < b.end && (unsigned)__ldcg(b.table + kv4_page_of(p, (uint32_t)(j0 + 16 * u) >> 4)) >= (unsigned)p.k.pages) off |= 1u << u;
+    return off;
+}
+// 32 weights, rounded, to TMEM column `to`; their sum is of the unrounded ones
+__device__ __forceinline__ void weights32(const float* s, float fac, float neg, uint32_t to, float& l) {
+    uint32_t y[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const float a = ex2(fmaf(s[2 * e], fac, neg)), b = ex2(fmaf(s[2 * e + 1], fac, neg));
+        l += a + b;
+        y[e] = pack_bf16x2(a, b);
+    }
+    __syncwarp();
+    tmem_st16u(to, y);
+}
+__device__ __forceinline__ void rescale(uint32_t at, int columns, float f) {
+#pragma unroll 1
+    for (int c = 0; c < columns; c += 16) {
+        float o[16];
+        tmem_ld16(at + (uint32_t)c, o);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[e] *= f;
+        tmem_st16(at + (uint32_t)c, o);
+    }
+}
+// what a row's outputs are multiplied by, whose weights have the reference `top` and the sum `sum`: the sink joins
+__device__ __forceinline__ float row_factor(const Kv4AttnParams& p, int h, float top, float sum) {
+    const float sink = p.sinks ? __ldcg(p.sinks + h) * 1.4426950408889634f : -INFINITY, all = fmaxf(top, sink);
+    const float w = top == -INFINITY ? 1.f : exp2f(top - all);             // (no maximum: nothing seen, or all NaN, which the sum knows)
+    sum *= w;
+    if (sink != -INFINITY) sum += exp2f(sink - all);
+    return sum > 0.f || sum != sum ? w / sum : 0.f;
+}
+// groups of which the row sees a value that is NaN, in the block's tiles
+template <int G, int ROWS>
+__device__ __forceinline__ uint32_t lost_groups(const Kv4AttnParams& p, const Block<ROWS>& b, const Row& r) {
+    uint32_t lost = 0;
+    const int last = min(r.limit, (b.tbeg + b.n) * P_KEYS - 1);
+    for (int j = max(max(b.begin, b.tbeg * P_KEYS), r.under + 1); j <= last; ++j) {
+        const uint32_t in_slot = kv4_page_of(p, (uint32_t)j >> 4);
+        const int page = __ldcg(b.table + in_slot);
+        if ((unsigned)page >= (unsigned)p.k.pages) continue;
+        const uint16_t* words = (const uint16_t*)(p.v_data + page * p.page_bytes + (size_t)b.head * p.head_bytes + (size_t)p.k.page_size * (16 * G)) +
+                                (size_t)(j - (int)(in_slot * (uint32_t)p.k.page_size)) * G;
+        for (int g = 0; g < G; ++g)
+            if ((ld_act2(words + g) & 0x7f80u) == 0x7f80u) lost |= 1u << g;
+    }
+    return lost;
+}
+// outputs [from, to) of a row, from TMEM column `at`: to memory, or to the fold
+template <int DT>
+__device__ __forceinline__ void outputs(const Kv4AttnParams& p, const Row& r, int dim, int from, int to, uint32_t at, bool any, uint32_t lost, float factor, float* fold) {
+#pragma unroll 1
+    for (int c = from; c < to; c += 16) {
+        float o[16], x[16];
+        __syncwarp();
+        if (any) tmem_ld16(at + (uint32_t)c, o);
+        else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = o[(e & 8) + (e & 4 ? 2 * (e & 3) + 1 : 2 * (e & 3))];
+        if ((lost >> (c / 32)) & 1u) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = NAN;
+        }
+        if (fold) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) *(float4*)(fold + c + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        } else if (r.live) {
+            uint16_t* dst = (uint16_t*)p.out + (size_t)r.tok * p.o_ld + (size_t)r.h * dim + c;
+            uint32_t y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = kv4_pack2<DT>(x[2 * e] * factor, x[2 * e + 1] * factor);
+            if (p.wide_o) {
+                *(uint4*)dst = make_uint4(y[0], y[1], y[2], y[3]);
+                *(uint4*)(dst + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { dst[2 * e] = (uint16_t)y[e]; dst[2 * e + 1] = (uint16_t)(y[e] >> 16); }
+            }
+        }
+    }
+    __syncwarp();
+}
+// the cluster's blocks into one, rows of D + 4 floats each: block r has every `splits`-th piece
+template <int D, int DT, int ROWS>
+__device__ __forceinline__ void fold_cluster(const Kv4AttnParams& p, const Block<ROWS>& b, const float* fold, const float* row_m, const float* row_l) {
+    cluster_sync();
+    const uint32_t fold_at = smem_u32(fold), m_at = smem_u32(row_m), l_at = smem_u32(row_l);
+    for (int i = b.split * (int)blockDim.x + (int)threadIdx.x; i < b.live * (D / 4); i += p.splits * (int)blockDim.x) {
+        const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+        const Row row(p, b, r);
+        if (!row.live) continue;
+        float top = -INFINITY, sum = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < p.splits; ++s) top = fmaxf(top, remote_float(remote(m_at + 4 * r, s)));
+        for (int s = 0; s < p.splits; ++s) {
+            const float ms = remote_float(remote(m_at + 4 * r, s)), ls = remote_float(remote(l_at + 4 * r, s));
+            const float w = ms == -INFINITY ? ls - ls : exp2f(ms - top);
+            const float4 v = remote_float4(remote(fold_at + (r * (D + 4) + d) * 4, s));
+            sum = fmaf(w, ls, sum);
+            o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
+        }
+        const float factor = row_factor(p, row.h, top, sum);
+        const uint32_t x = kv4_pack2<DT>(o.x * factor, o.y * factor), y = kv4_pack2<DT>(o.z * factor, o.w * factor);
+        uint16_t* dst = (uint16_t*)p.out + (size_t)row.tok * p.o_ld + (size_t)row.h * D + d;
+        if (p.wide_o) *(uint2*)dst = make_uint2(x, y);
+        else { dst[0] = (uint16_t)x; dst[1] = (uint16_t)(x >> 16); dst[2] = (uint16_t)y; dst[3] = (uint16_t)(y >> 16); }
+    }
+    cluster_sync();                                // nobody leaves while another reads
+}
+
 // IMAGES: one warp copies tiles that kv4_images_kernel has made; otherwise P_EXPAND warps make them
 template <int G, int DT, bool IMAGES>
 __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4_prompt_kernel(const __grid_constant__ Kv4AttnParams p, const __grid_constant__ Images im, int* err) {
@@ -155,7 +367,7 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
     constexpr int THREADS = IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, FILLS = IMAGES ? 1 : P_EXPAND;
     constexpr int D = C::D, DN = C::DN, QT = DT == 1 ? 2 : 1;
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ __align__(8) uint64_t kfull[P_STAGES], kempty[P_STAGES], vfull[P_STAGES], vempty[P_STAGES], sfull[2], pready, pvdone;
+    __shared__ __align__(8) uint64_t kfull[P_STAGES], kempty[P_STAGES], vfull[P_STAGES], vempty[P_STAGES], sfull[2], pready[2], pvdone;
     __shared__ uint32_t tmem_base_s;
     __shared__ float wmax[2][2][P_ROWS], row_m[P_ROWS], row_l[P_ROWS];
     __shared__ int missing, nans;
@@ -169,7 +381,7 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
             mbar_init(&vfull[s], FILLS); mbar_init(&vempty[s], 1);
         }
         mbar_init(&sfull[0], 1); mbar_init(&sfull[1], 1);
-        mbar_init(&pready, P_SOFT); mbar_init(&pvdone, 1);
+        mbar_init(&pready[0], P_SOFT); mbar_init(&pready[1], P_SOFT); mbar_init(&pvdone, 1);
         mbar_fence_init();
         missing = nans = 0;
     }
@@ -180,66 +392,27 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
     griddep_wait();
     griddep_launch();
 
-    // the longest rows first
-    const int seq = blockIdx.x % p.seqs, f0 = (p.tiles - 1 - (int)(blockIdx.x / p.seqs)) * P_ROWS, head = blockIdx.y, split = blockIdx.z;
-    const int slot = __ldcg(p.seq_slots + seq), ctx = __ldcg(p.contexts + seq);
-    const int first = p.starts ? __ldcg(p.starts + seq) : seq, n_rows = p.starts ? __ldcg(p.starts + seq + 1) - first : 1;
-    const int rows = min(min(n_rows, p.max_rows), 0x7fffffff / p.rep) * p.rep;
-    const bool work = f0 < rows && (unsigned)slot < (unsigned)p.k.slots;                   // the same in all of the cluster
-    const int live_rows = work ? min(P_ROWS, rows - f0) : 0;
-    const int pos0 = ctx - n_rows + f0 / p.rep, pos1 = ctx - n_rows + (f0 + max(live_rows, 1) - 1) / p.rep;
-    const int begin = p.window > 0 ? max(0, pos0 - p.window + 1) : 0, end = work ? min(min(pos1 + 1, ctx), p.max_keys) : 0;
-    const int t0 = begin / P_KEYS, nt = max(0, (end + P_KEYS - 1) / P_KEYS - t0), per = (nt + p.splits - 1) / p.splits;
-    const int tbeg = t0 + split * per, n = max(0, min(nt, (split + 1) * per) - split * per);
-    const int32_t* const table = p.k.table + (work ? (size_t)slot * p.k.max_pages : 0);
-
-    const size_t image = ((size_t)seq * p.k.kv_heads + head) * im.tiles + (tbeg - first_tile(p, ctx, n_rows));      // the block's first tile
-
-    // row r of the block: which one of the sequence's, and what it sees
-    const int quad = warp & 3, half = (warp >> 2) & 1, row = quad * 32 + lane, f = f0 + row, tok = first + f / p.rep;
-    const int h = head * p.rep + f % p.rep, pos = ctx - n_rows + f / p.rep;
-    const bool live = warp < P_SOFT && row < live_rows && tok >= 0 && tok < p.tokens;
+    const Block<P_ROWS> b(p);
+    const int n = b.n, begin = b.begin, end = b.end, tbeg = b.tbeg, head = b.head;
+    const size_t image = ((size_t)b.seq * p.k.kv_heads + head) * im.tiles + (tbeg - first_tile(p, b.ctx, b.n_rows));        // the block's first tile
+    const int32_t* const table = b.table;
+    const int quad = warp & 3, half = (warp >> 2) & 1, row = quad * 32 + lane;
+    const Row r(p, b, warp < P_SOFT ? row : P_ROWS);
 
     if (warp < 4) {                                // queries to tensor memory
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
-            uint32_t a[16], b[16];
+            uint32_t x[16], y[16];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint16_t* src = (const uint16_t*)p.q + (size_t)tok * p.q_ld + (size_t)h * D + c + 8 * i;
-                uint32_t w[4] = {};
-                if (live) {
-                    if (p.wide_q) {
-                        const uint4 v = ld_act16(src);
-                        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = (uint32_t)ld_act2(src + 2 * e) | (uint32_t)ld_act2(src + 2 * e + 1) << 16;
-                    }
-                }
-                uint32_t v[4] = {__byte_perm(w[0], w[2], 0x5410), __byte_perm(w[0], w[2], 0x7632), __byte_perm(w[1], w[3], 0x5410), __byte_perm(w[1], w[3], 0x7632)};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (DT == 1) {
-                        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v[e]));
-                        a[4 * i + e] = pack_bf16x2(x.x, x.y);
-                        b[4 * i + e] = pack_bf16x2(x.x - bf16lo(a[4 * i + e]), x.y - bf16hi(a[4 * i + e]));
-                    } else
-                        a[4 * i + e] = v[e];
-                }
-            }
+            for (int i = 0; i < 4; ++i) query8<DT>(p, r, r.h * D + c + 8 * i, x + 4 * i, y + 4 * i);
             __syncwarp();
             const uint32_t to = tmem + ((uint32_t)(quad * 32) << 16) + P_Q + (uint32_t)c / 2u;
-            tmem_st16u(to, a);
-            if constexpr (QT == 2) tmem_st16u(to + 64u, b);
+            tmem_st16u(to, x);
+            if constexpr (QT == 2) tmem_st16u(to + 64u, y);
         }
         tmem_st_wait();
-    } else {                                       // does a page of these keys not exist?
-        bool gone = false;
-        const int last = min(end, (tbeg + n) * P_KEYS);
-        for (int j = tbeg * P_KEYS + 16 * (tid - 128); j < last; j += 16 * (THREADS - 128))
-            gone |= (unsigned)__ldcg(table + kv4_page_of(p, (uint32_t)j >> 4)) >= (unsigned)p.k.pages;
-        if (gone) missing = 1;
+    } else {
+        if (b.gone(p, tid - 128, THREADS - 128)) missing = 1;
         if constexpr (IMAGES) {
             for (int i = tid - 128; i < n; i += THREADS - 128)
                 if (__ldcg(im.nans + image + i)) nans = 1;
@@ -250,44 +423,44 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
     tc_fence_after();
 
     if (warp == P_SOFT) {
-        // ---------------- MMAs
-        constexpr uint32_t id_s = umma_idesc_bf16(P_KEYS), id_o = umma_idesc_bf16(DN) | (1u << 16);       // values: the elements are contiguous
-        bool ok = true;
-        auto scores = [&](int i) {                 // where the weights of tile i - 2 were
-            const int s = i % P_STAGES;
-            ok = ok && all_wait(err, &kfull[s], (uint32_t)(i / P_STAGES) & 1u);
-            if (!ok) return;
-            if (elect_one()) {
+        // ---------------- MMAs, from one thread: votes and elections of a whole warp between them took 250 cycles a wait
+        if (elect_one()) {
+            constexpr uint32_t id_s = umma_idesc_bf16(P_KEYS), id_o = umma_idesc_bf16(DN) | (1u << 16);   // values: the elements are contiguous
+            const uint64_t kd[2] = {desc_sw128(ks), desc_sw128(ks + C::TILE)}, vd[2] = {desc_mn_sw128(vs, P_CHUNK), desc_mn_sw128(vs + C::TILE, P_CHUNK)};
+            bool ok = true;
+            auto scores = [&](int i) {             // where the weights of tile i - 2 were
+                const int s = i % P_STAGES;
+                ok = ok && bar_wait(err, smem_u32(&kfull[s]), (uint32_t)(i / P_STAGES) & 1u);
+                if (!ok) return;
                 tc_fence_after();
+                const uint64_t d = s ? kd[1] : kd[0];
+                const uint32_t to = tmem + P_S + (uint32_t)(i & 1) * 128u;
 #pragma unroll
                 for (int term = QT - 1; term >= 0; --term)
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k)
-                        umma_bf16_ta(tmem + P_S + (uint32_t)(i & 1) * 128u, tmem + P_Q + (uint32_t)term * 64u + (uint32_t)k * 8u,
-                                     desc_sw128(ks + s * C::TILE + (uint32_t)(k >> 2) * P_CHUNK) + (uint64_t)((k & 3) * 2), id_s, k || term < QT - 1 ? 1u : 0u);
+                        umma_bf16_ta(to, tmem + P_Q + (uint32_t)term * 64u + (uint32_t)k * 8u, d + (uint64_t)((k >> 2) * (P_CHUNK / 16) + (k & 3) * 2), id_s, k || term < QT - 1 ? 1u : 0u);
                 umma_commit(&sfull[i & 1]);
                 umma_commit(&kempty[s]);
-            }
-            __syncwarp();
-        };
-        if (n > 0) scores(0);
-        for (int i = 0; ok && i < n; ++i) {
-            const int s = i % P_STAGES;
-            if (i > 0) ok = all_wait(err, &pvdone, (uint32_t)((i - 1) & 1));
-            if (ok && i + 1 < n) scores(i + 1);
-            ok = ok && all_wait(err, lane & 1 ? &vfull[s] : &pready, lane & 1 ? (uint32_t)(i / P_STAGES) & 1u : (uint32_t)(i & 1));
-            if (!ok) break;
-            if (elect_one()) {
+            };
+            if (n > 0) scores(0);
+            for (int i = 0; ok && i < n; ++i) {
+                const int s = i % P_STAGES;
+                if (i > 0) ok = bar_wait(err, smem_u32(&pvdone), (uint32_t)((i - 1) & 1));
+                if (ok && i + 1 < n) scores(i + 1);
+                ok = ok && bar_wait(err, smem_u32(&vfull[s]), (uint32_t)(i / P_STAGES) & 1u) && bar_wait(err, smem_u32(&pready[i & 1]), (uint32_t)(i >> 1) & 1u);
+                if (!ok) break;
                 tc_fence_after();
+                const uint64_t d = s ? vd[1] : vd[0];
+                const uint32_t at = tmem + P_S + (uint32_t)(i & 1) * 128u;
 #pragma unroll
-                for (int k = 0; k < P_KEYS / 16; ++k)             // 16 keys: 2048 bytes of V
-                    umma_bf16_ta(tmem + P_O, tmem + P_S + (uint32_t)(i & 1) * 128u + (uint32_t)(k >> 2) * 64u + (uint32_t)(k & 3) * 8u, desc_mn_sw128(vs + s * C::TILE, P_CHUNK) + (uint64_t)(k * 128),
-                                 id_o, (i | k) ? 1u : 0u);
+                for (int k = 0; k < P_KEYS / 16; ++k)              // 16 keys: 2048 bytes of V
+                    umma_bf16_ta(tmem + P_O, at + (uint32_t)(k >> 2) * 64u + (uint32_t)(k & 3) * 8u, d + (uint64_t)(k * 128), id_o, (i | k) ? 1u : 0u);
                 umma_commit(&pvdone);
                 umma_commit(&vempty[s]);
             }
-            __syncwarp();
         }
+        __syncwarp();
     } else if (warp > P_SOFT) {
         if constexpr (IMAGES) {
             // ---------------- tiles of K and V, copied
@@ -296,17 +469,17 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
                 auto copy = [&](int i, uint64_t* full, uint64_t* empty, uint32_t at, size_t from) {
                     const int s = i % P_STAGES;
                     ok = ok && bar_wait(err, smem_u32(&empty[s]), (((uint32_t)i / P_STAGES) & 1u) ^ 1u);
-                    if (!ok) return false;
+                    if (!ok) return 0;
                     mbar_arrive_expect_tx(&full[s], C::TILE);
                     bulk_copy_g2s(smem + (at - smem_u32(smem)) + s * C::TILE, im.data + from, C::TILE, &full[s]);
-                    return true;
+                    return 1;
                 };
                 int nk = 0, nv = 0;
                 for (int i = 0; ok && i < n; ++i) {
                     nk += copy(i, kfull, kempty, ks, (image + i) * (2 * C::TILE));
                     nv += copy(i, vfull, vempty, vs, (image + i) * (2 * C::TILE) + C::TILE);
                 }
-                for (int j = max(0, nk - P_STAGES); j < nk; ++j)      // whoever gave up: do not leave with copies in flight
+                for (int j = max(0, nk - P_STAGES); j < nk; ++j)            // whoever gave up: do not leave with copies in flight
                     bar_wait(err, smem_u32(&kfull[j % P_STAGES]), (uint32_t)(j / P_STAGES) & 1u);
                 for (int j = max(0, nv - P_STAGES); j < nv; ++j)
                     bar_wait(err, smem_u32(&vfull[j % P_STAGES]), (uint32_t)(j / P_STAGES) & 1u);
@@ -380,8 +553,7 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
     } else {
         // ---------------- weights
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
-        const int limit = live ? min(pos, end - 1) : -1, under = p.window > 0 ? pos - p.window : -1;       // sees (under, limit]
-        const int clean_lo = p.window > 0 ? pos1 - p.window : -1, clean_hi = missing ? -1 : min(pos0, end - 1);
+        const int clean_lo = p.window > 0 ? b.pos1 - p.window : -1, clean_hi = missing ? -1 : min(b.pos0, end - 1);
         const float fac = p.cap_log2 > 0.f ? 1.f : p.scale_log2;
         float m = -INFINITY, neg = 0.f, l = 0.f;
         bool ok = true;
@@ -392,40 +564,11 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
             __syncwarp();
             tc_fence_after();
             const bool edge = j0 <= clean_lo || j0 + 63 > clean_hi;
-            uint32_t gone = 0;                                    // of four runs of 16 keys, the ones without a page
-            if (edge && missing) {
+            const uint32_t off = edge && missing ? runs_gone(p, b, j0, 4) : 0u;
+            float s[64], top = -INFINITY;
+            row_scores(p, at + (uint32_t)(half * 64), j0, edge, r, off, s);
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (j0 + 16 * u < end && (unsigned)__ldcg(table + kv4_page_of(p, (uint32_t)(j0 + 16 * u) >> 4)) >= (unsigned)p.k.pages) gone |= 1u << u;
-            }
-            // 32 scores at a time, looked at twice: the maximum, then the weights.  A loop: straight code for 64 costs its fetch
-            auto look = [&](int c, float (&s)[32]) {
-                tmem_ld16_async(at + (uint32_t)(half * 64 + c), *(float (*)[16])s);
-                tmem_ld16_async(at + (uint32_t)(half * 64 + c + 16), *(float (*)[16])(s + 16));
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                tmem_pass(*(float (*)[16])s);
-                tmem_pass(*(float (*)[16])(s + 16));
-                if (p.cap_log2 > 0.f) {
-                    const float in = p.scale_log2 * 2.885390043f / p.cap_log2;
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) s[e] = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(s[e] * in)));
-                }
-                if (edge) {
-                    const int hi = limit - j0 - c, lo = under - j0 - c;
-                    const uint32_t off = gone >> (c / 16);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (e > hi || e <= lo || ((off >> (e / 16)) & 1u)) s[e] = -INFINITY;
-                }
-            };
-            float top = -INFINITY;
-#pragma unroll 1
-            for (int c = 0; c < 64; c += 32) {
-                float s[32];
-                look(c, s);
-#pragma unroll
-                for (int e = 0; e < 32; ++e) top = fmaxf(top, s[e]);
-            }
+            for (int e = 0; e < 64; ++e) top = fmaxf(top, s[e]);
             top *= fac;
             wmax[i & 1][half][row] = top;
             __syncwarp();
@@ -440,35 +583,15 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
                     ok = ok && all_wait(err, &pvdone, (uint32_t)((i - 1) & 1));
                     __syncwarp();
                     tc_fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < DN / 2; c += 16) {
-                        float o[16];
-                        const uint32_t to = lanes + P_O + (uint32_t)(half * (DN / 2) + c);
-                        tmem_ld16(to, o);
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] *= fix;
-                        tmem_st16(to, o);
-                    }
+                    rescale(lanes + P_O + (uint32_t)(half * (DN / 2)), DN / 2, fix);
                 }
             }
-#pragma unroll 1
-            for (int c = 0; c < 64; c += 32) {                    // 32 keys: 16 columns, where the warp's own scores were
-                float s[32];
-                uint32_t y[16];
-                look(c, s);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float a = ex2(fmaf(s[2 * e], fac, neg)), b = ex2(fmaf(s[2 * e + 1], fac, neg));
-                    l += a + b;
-                    y[e] = pack_bf16x2(a, b);
-                }
-                __syncwarp();
-                tmem_st16u(at + (uint32_t)(half * 64 + c / 2), y);
-            }
+            weights32(s, fac, neg, at + (uint32_t)(half * 64), l);                 // to where the warp's own scores were
+            weights32(s + 32, fac, neg, at + (uint32_t)(half * 64 + 16), l);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&pready);
+            if (lane == 0) mbar_arrive(&pready[i & 1]);           // a barrier each: weights of two tiles may be ready before the first is looked for
         }
         if (n > 0) all_wait(err, &pvdone, (uint32_t)((n - 1) & 1));
         asm volatile("bar.sync %0, 64;" :: "r"(1 + quad) : "memory");              // the last tile's maxima are read
@@ -480,105 +603,21 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
     __syncthreads();                               // nobody's tile is read or written any more
     tc_fence_after();
     float* const fold = (float*)smem;              // [128][D + 4], with more than one block a sequence
-    auto finish = [&](int r, float& top, float sum) {              // what the row's outputs are multiplied by, sink and all
-        const int hr = head * p.rep + (f0 + r) % p.rep;
-        const float sink = p.sinks ? __ldcg(p.sinks + hr) * 1.4426950408889634f : -INFINITY, was = top;
-        top = fmaxf(top, sink);
-        sum = was == -INFINITY ? sum - sum : sum * exp2f(was - top);
-        if (sink != -INFINITY) sum += exp2f(sink - top);
-        return sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    };
-    if (warp < P_SOFT) {
-        uint32_t lost = 0;                         // groups of which the row sees a NaN
-        if (nans && live) {
-            const int from = max(begin, tbeg * P_KEYS), last = min(min(pos, end - 1), (tbeg + n) * P_KEYS - 1);
-            const int under = p.window > 0 ? pos - p.window : -1;
-            for (int j = max(from, under + 1); j <= last; ++j) {
-                const int page = __ldcg(table + kv4_page_of(p, (uint32_t)j >> 4));
-                if ((unsigned)page >= (unsigned)p.k.pages) continue;
-                const int in_page = j - (int)(kv4_page_of(p, (uint32_t)j >> 4) * (uint32_t)p.k.page_size);
-                const uint16_t* words = (const uint16_t*)(p.v_data + page * p.page_bytes + (size_t)head * p.head_bytes + (size_t)p.k.page_size * (16 * G)) + (size_t)in_page * G;
-                for (int g = 0; g < G; ++g)
-                    if ((ld_act2(words + g) & 0x7f80u) == 0x7f80u) lost |= 1u << g;
-            }
-        }
-        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
-        float top = row_m[row];
-        const float was = top, inv = finish(row, top, row_l[row]) * (was == -INFINITY ? 1.f : exp2f(was - top));
-#pragma unroll 1
-        for (int c = half * (DN / 2); c < min(D, (half + 1) * (DN / 2)); c += 16) {
-            float o[16], x[16];
-            __syncwarp();
-            if (n > 0) tmem_ld16(lanes + P_O + (uint32_t)c, o);
-            else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = 0.f;
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = o[(e & 8) + (e & 4 ? 2 * (e & 3) + 1 : 2 * (e & 3))];
-            if ((lost >> (c / 32)) & 1u) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = NAN;
-            }
-            if (p.splits > 1) {
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) *(float4*)(fold + (size_t)row * (D + 4) + c + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-            } else if (live) {
-                uint16_t* dst = (uint16_t*)p.out + (size_t)tok * p.o_ld + (size_t)h * D + c;
-                uint32_t y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = kv4_pack2<DT>(x[2 * e] * inv, x[2 * e + 1] * inv);
-                if (p.wide_o) {
-                    *(uint4*)dst = make_uint4(y[0], y[1], y[2], y[3]);
-                    *(uint4*)(dst + 8) = make_uint4(y[4], y[5], y[6], y[7]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) { dst[2 * e] = (uint16_t)y[e]; dst[2 * e + 1] = (uint16_t)(y[e] >> 16); }
-                }
-            }
-        }
-        __syncwarp();
-    }
+    if (warp < P_SOFT)
+        outputs<DT>(p, r, D, half * (DN / 2), min(D, (half + 1) * (DN / 2)), tmem + ((uint32_t)(quad * 32) << 16) + P_O, n > 0, nans && r.live ? lost_groups<G>(p, b, r) : 0u,
+                    p.splits > 1 ? 0.f : row_factor(p, r.h, row_m[row], row_l[row]), p.splits > 1 ? fold + (size_t)row * (D + 4) : nullptr);
     tc_fence_before();
     __syncthreads();
     if (warp == P_SOFT) tmem_dealloc(tmem, 512);
-    if (p.splits == 1) return;
-    // ---------------- the cluster's blocks into one: block r has every `splits`-th piece
-    cluster_sync();
-    const uint32_t fold_at = smem_u32(fold), m_at = smem_u32(row_m), l_at = smem_u32(row_l);
-    for (int i = split * THREADS + tid; i < live_rows * (D / 4); i += p.splits * THREADS) {
-        const int r = i / (D / 4), d = (i - r * (D / 4)) * 4, fr = f0 + r, to = first + fr / p.rep;
-        if (to < 0 || to >= p.tokens) continue;
-        float top = -INFINITY, sum = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < p.splits; ++s) top = fmaxf(top, remote_float(remote(m_at + 4 * r, s)));
-        for (int s = 0; s < p.splits; ++s) {
-            const float ms = remote_float(remote(m_at + 4 * r, s)), ls = remote_float(remote(l_at + 4 * r, s));
-            const float w = ms == -INFINITY ? ls - ls : exp2f(ms - top);
-            const float4 v = remote_float4(remote(fold_at + (r * (D + 4) + d) * 4, s));
-            sum = fmaf(w, ls, sum);
-            o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
-        }
-        const float was = top, inv = finish(r, top, sum) * (was == -INFINITY ? 1.f : exp2f(was - top));
-        const uint32_t a = kv4_pack2<DT>(o.x * inv, o.y * inv), b = kv4_pack2<DT>(o.z * inv, o.w * inv);
-        uint16_t* dst = (uint16_t*)p.out + (size_t)to * p.o_ld + (size_t)(head * p.rep + fr % p.rep) * D + d;
-        if (p.wide_o) *(uint2*)dst = make_uint2(a, b);
-        else { dst[0] = (uint16_t)a; dst[1] = (uint16_t)(a >> 16); dst[2] = (uint16_t)b; dst[3] = (uint16_t)(b >> 16); }
-    }
-    cluster_sync();                                // nobody leaves while another reads
+    if (p.splits > 1) fold_cluster<D, DT>(p, b, fold, row_m, row_l);
 }
 
-template <int G, int DT, bool IMAGES>
-cudaError_t launch_prompt_kernel(const Kv4AttnParams& p, const Images& im, int* err, cudaStream_t st) {
-    static bool configured = false;
-    if (!configured) {
-        if (cudaError_t e = cudaFuncSetAttribute(kv4_prompt_kernel<G, DT, IMAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Prompt<G>::BYTES)) return e;
-        configured = true;
-    }
+template <typename... K>
+cudaError_t launch_blocks(void (*kernel)(K...), const Kv4AttnParams& p, int threads, int smem, cudaStream_t st, K... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.seqs * p.tiles), p.k.kv_heads, p.splits);
-    cfg.blockDim = dim3(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS);
-    cfg.dynamicSmemBytes = Prompt<G>::BYTES;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -590,22 +629,30 @@ cudaError_t launch_prompt_kernel(const Kv4AttnParams& p, const Images& im, int* 
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     count_launch();
-    return cudaLaunchKernelEx(&cfg, kv4_prompt_kernel<G, DT, IMAGES>, p, im, err);
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
-
-template <int G, int DT>
-int launch_prompt(Kv4AttnParams p, cudaStream_t st) {
-    int* err = wait_word(kWaitKv4);
-    PGK_REQUIRE(err, "kv4_attention failed: no pinned host memory");
-    p.tiles = (int)(((long long)p.max_rows * p.rep + P_ROWS - 1) / P_ROWS);
-    // blocks of a cluster that share a sequence's keys: rounds of blocks times (their tiles + what a block costs besides, about four tiles)
-    const int keys = p.window > 0 && p.window < p.max_keys - P_ROWS ? p.window + P_ROWS : p.max_keys, nt = (keys + P_KEYS - 1) / P_KEYS;
+// Blocks of rows, and how many blocks of a cluster share a sequence's keys: rounds of blocks times (their tiles + what a block costs besides, about four)
+void cut_rows(Kv4AttnParams& p, int rows) {
+    p.tiles = (int)(((long long)p.max_rows * p.rep + rows - 1) / rows);
+    const int keys = p.window > 0 && p.window < p.max_keys - rows ? p.window + rows : p.max_keys, nt = (keys + P_KEYS - 1) / P_KEYS;
     const long long items = (long long)p.seqs * p.tiles * p.k.kv_heads;
     long long least = 0;
     for (int s = 1; s <= P_CLUSTER; s *= 2) {
         const long long cost = ((items * s + sm_count() - 1) / sm_count()) * ((nt + s - 1) / s + 4);
         if (s == 1 || cost < least) { p.splits = s; least = cost; }
     }
+}
+
+template <int G, int DT>
+int launch_prompt(Kv4AttnParams p, cudaStream_t st) {
+    static bool configured = false;
+    if (!configured) {
+        PGK_CUDA(cudaFuncSetAttribute(kv4_prompt_kernel<G, DT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Prompt<G>::BYTES));
+        PGK_CUDA(cudaFuncSetAttribute(kv4_prompt_kernel<G, DT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Prompt<G>::BYTES));
+        configured = true;
+    }
+    int* err = wait_word(kWaitKv4);
+    PGK_REQUIRE(err, "kv4_attention failed: no pinned host memory");
     Images im = {};
     im.tiles = (p.max_keys + P_KEYS - 1) / P_KEYS;
     if (p.window > 0 && (long long)p.window + p.max_rows < p.max_keys) {
@@ -614,19 +661,21 @@ int launch_prompt(Kv4AttnParams p, cudaStream_t st) {
     }
     const long long count = (long long)p.seqs * p.k.kv_heads * im.tiles, bytes = count * (2 * Prompt<G>::TILE + 4);
     void* ws = nullptr;
-    if (p.tiles >= P_IMAGES_FROM && im.tiles > 0 && im.tiles <= 65535 && p.seqs <= 65535 && bytes <= P_IMAGES_MOST) {
+    if ((long long)p.max_rows * p.rep >= P_IMAGES_FROM && im.tiles > 0 && p.k.kv_heads <= 65535 && p.seqs <= 65535 && bytes <= P_IMAGES_MOST) {
         const int rc = scratch_alloc(&ws, (size_t)bytes, st);
         if (rc == (int)cudaErrorMemoryAllocation) set_error("");      // no room: the blocks make their tiles
         else if (rc) return rc;
     }
+    cut_rows(p, P_ROWS);
     cudaError_t e = cudaSuccess;
     if (ws) {
         im.data = (unsigned char*)ws;
         im.nans = (int32_t*)((unsigned char*)ws + count * (2 * Prompt<G>::TILE));
         e = launch_waiting(kv4_images_kernel<G>, dim3(im.tiles, p.k.kv_heads, p.seqs), dim3(P_EXPAND * 32), 0, st, p, im);
-        if (e == cudaSuccess) e = launch_prompt_kernel<G, DT, true>(p, im, err, st);
-    } else
-        e = launch_prompt_kernel<G, DT, false>(p, im, err, st);
+        if (e == cudaSuccess) e = launch_blocks(kv4_prompt_kernel<G, DT, true>, p, (P_SOFT + 2) * 32, Prompt<G>::BYTES, st, p, im, err);
+    } else {
+        e = launch_blocks(kv4_prompt_kernel<G, DT, false>, p, P_THREADS, Prompt<G>::BYTES, st, p, im, err);
+    }
     if (int rc = scratch_free(ws, st)) return rc;
     PGK_CUDA(e);
     return 0;
