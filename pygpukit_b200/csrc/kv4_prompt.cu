@@ -249,13 +249,35 @@ __device__ __forceinline__ uint32_t runs_gone(const Kv4AttnParams& p, const Bloc
         if (j0 + 16 * u < b.end && (unsigned)__ldcg(b.table + kv4_page_of(p, (uint32_t)(j0 + 16 * u) >> 4)) >= (unsigned)p.k.pages) off |= 1u << u;
     return off;
 }
-// 32 weights, rounded, to TMEM column `to`; their sum is of the unrounded ones
-__device__ __forceinline__ void weights32(const float* s, float fac, float neg, uint32_t to, float& l) {
+// pairs of float32 in a register pair: one instruction for two products or sums
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 32 weights 2^(s fac + neg), rounded, to TMEM column `to`; their sum is of the unrounded ones
+__device__ __forceinline__ void weights32(const float* s, float fac, float neg, uint32_t to, uint64_t& l) {
     uint32_t y[16];
+    const uint64_t fac2 = pair(fac, fac), neg2 = pair(neg, neg);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-        const float a = ex2(fmaf(s[2 * e], fac, neg)), b = ex2(fmaf(s[2 * e + 1], fac, neg));
-        l += a + b;
+        const uint64_t x = fma2(pair(s[2 * e], s[2 * e + 1]), fac2, neg2);
+        float a, b;
+        unpair(x, a, b);
+        a = ex2(a);
+        b = ex2(b);
+        l = add2(l, pair(a, b));
         y[e] = pack_bf16x2(a, b);
     }
     __syncwarp();
@@ -586,8 +608,12 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
                     rescale(lanes + P_O + (uint32_t)(half * (DN / 2)), DN / 2, fix);
                 }
             }
-            weights32(s, fac, neg, at + (uint32_t)(half * 64), l);                 // to where the warp's own scores were
-            weights32(s + 32, fac, neg, at + (uint32_t)(half * 64 + 16), l);
+            uint64_t l2 = pair(0.f, 0.f);
+            weights32(s, fac, neg, at + (uint32_t)(half * 64), l2);               // to where the warp's own scores were
+            weights32(s + 32, fac, neg, at + (uint32_t)(half * 64 + 16), l2);
+            float la, lb;
+            unpair(l2, la, lb);
+            l += la + lb;
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
