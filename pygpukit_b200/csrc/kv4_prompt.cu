@@ -22,7 +22,7 @@ namespace pgk {
 
 namespace {
 
-constexpr int P_ROWS = 128, P_KEYS = 128, P_SOFT = 8, P_EXPAND = 8, P_THREADS = (P_SOFT + 1 + P_EXPAND) * 32, P_STAGES = 2, P_CLUSTER = 8;
+constexpr int P_ROWS = 128, P_KEYS = 128, P_SOFT = 8, P_EXPAND = 8, P_THREADS = (P_SOFT + 1 + P_EXPAND) * 32, P_STAGES = 3, P_CLUSTER = 8;
 constexpr uint32_t P_CHUNK = P_KEYS * 128;                         // 64 elements of 128 keys
 constexpr uint32_t P_O = 0, P_Q = 128, P_S = 256;                  // TMEM columns: outputs, queries (two terms of 64), two tiles of scores
 constexpr float P_LAZY = 8.f;
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
     constexpr int THREADS = IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, FILLS = IMAGES ? 1 : P_EXPAND;
     constexpr int D = C::D, DN = C::DN, QT = DT == 1 ? 2 : 1;
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ __align__(8) uint64_t kfull[P_STAGES], kempty[P_STAGES], vfull[P_STAGES], vempty[P_STAGES], sfull[2], pready[2], pvdone;
+    __shared__ __align__(8) uint64_t full[P_STAGES], empty[P_STAGES], sfull[2], pready[2], pvdone;
     __shared__ uint32_t tmem_base_s;
     __shared__ float wmax[2][2][P_ROWS], row_m[P_ROWS], row_l[P_ROWS];
     __shared__ int missing, nans;
@@ -399,8 +399,7 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
     if (warp == P_SOFT) tmem_alloc(&tmem_base_s, 512);
     if (tid == 0) {
         for (int s = 0; s < P_STAGES; ++s) {
-            mbar_init(&kfull[s], FILLS); mbar_init(&kempty[s], 1);
-            mbar_init(&vfull[s], FILLS); mbar_init(&vempty[s], 1);
+            mbar_init(&full[s], FILLS); mbar_init(&empty[s], 1);
         }
         mbar_init(&sfull[0], 1); mbar_init(&sfull[1], 1);
         mbar_init(&pready[0], P_SOFT); mbar_init(&pready[1], P_SOFT); mbar_init(&pvdone, 1);
@@ -448,14 +447,14 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
         // ---------------- MMAs, from one thread: votes and elections of a whole warp between them took 250 cycles a wait
         if (elect_one()) {
             constexpr uint32_t id_s = umma_idesc_bf16(P_KEYS), id_o = umma_idesc_bf16(DN) | (1u << 16);   // values: the elements are contiguous
-            const uint64_t kd[2] = {desc_sw128(ks), desc_sw128(ks + C::TILE)}, vd[2] = {desc_mn_sw128(vs, P_CHUNK), desc_mn_sw128(vs + C::TILE, P_CHUNK)};
+            const uint64_t kd = desc_sw128(ks), vd = desc_mn_sw128(vs, P_CHUNK);
             bool ok = true;
             auto scores = [&](int i) {             // where the weights of tile i - 2 were
                 const int s = i % P_STAGES;
-                ok = ok && bar_wait(err, smem_u32(&kfull[s]), (uint32_t)(i / P_STAGES) & 1u);
+                ok = ok && bar_wait(err, smem_u32(&full[s]), (uint32_t)(i / P_STAGES) & 1u);
                 if (!ok) return;
                 tc_fence_after();
-                const uint64_t d = s ? kd[1] : kd[0];
+                const uint64_t d = kd + (uint64_t)(s * (C::TILE / 16));
                 const uint32_t to = tmem + P_S + (uint32_t)(i & 1) * 128u;
 #pragma unroll
                 for (int term = QT - 1; term >= 0; --term)
@@ -463,23 +462,22 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
                     for (int k = 0; k < D / 16; ++k)
                         umma_bf16_ta(to, tmem + P_Q + (uint32_t)term * 64u + (uint32_t)k * 8u, d + (uint64_t)((k >> 2) * (P_CHUNK / 16) + (k & 3) * 2), id_s, k || term < QT - 1 ? 1u : 0u);
                 umma_commit(&sfull[i & 1]);
-                umma_commit(&kempty[s]);
             };
             if (n > 0) scores(0);
             for (int i = 0; ok && i < n; ++i) {
                 const int s = i % P_STAGES;
                 if (i > 0) ok = bar_wait(err, smem_u32(&pvdone), (uint32_t)((i - 1) & 1));
                 if (ok && i + 1 < n) scores(i + 1);
-                ok = ok && bar_wait(err, smem_u32(&vfull[s]), (uint32_t)(i / P_STAGES) & 1u) && bar_wait(err, smem_u32(&pready[i & 1]), (uint32_t)(i >> 1) & 1u);
+                ok = ok && bar_wait(err, smem_u32(&pready[i & 1]), (uint32_t)(i >> 1) & 1u);
                 if (!ok) break;
                 tc_fence_after();
-                const uint64_t d = s ? vd[1] : vd[0];
+                const uint64_t d = vd + (uint64_t)(s * (C::TILE / 16));
                 const uint32_t at = tmem + P_S + (uint32_t)(i & 1) * 128u;
 #pragma unroll
                 for (int k = 0; k < P_KEYS / 16; ++k)              // 16 keys: 2048 bytes of V
                     umma_bf16_ta(tmem + P_O, at + (uint32_t)(k >> 2) * 64u + (uint32_t)(k & 3) * 8u, d + (uint64_t)(k * 128), id_o, (i | k) ? 1u : 0u);
                 umma_commit(&pvdone);
-                umma_commit(&vempty[s]);
+                umma_commit(&empty[s]);
             }
         }
         __syncwarp();
@@ -488,23 +486,18 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
             // ---------------- tiles of K and V, copied
             if (elect_one()) {
                 bool ok = true;
-                auto copy = [&](int i, uint64_t* full, uint64_t* empty, uint32_t at, size_t from) {
-                    const int s = i % P_STAGES;
-                    ok = ok && bar_wait(err, smem_u32(&empty[s]), (((uint32_t)i / P_STAGES) & 1u) ^ 1u);
-                    if (!ok) return 0;
-                    mbar_arrive_expect_tx(&full[s], C::TILE);
-                    bulk_copy_g2s(smem + (at - smem_u32(smem)) + s * C::TILE, im.data + from, C::TILE, &full[s]);
-                    return 1;
-                };
-                int nk = 0, nv = 0;
-                for (int i = 0; ok && i < n; ++i) {
-                    nk += copy(i, kfull, kempty, ks, (image + i) * (2 * C::TILE));
-                    nv += copy(i, vfull, vempty, vs, (image + i) * (2 * C::TILE) + C::TILE);
+                int made = 0;
+                for (; made < n; ++made) {
+                    const int s = made % P_STAGES;
+                    ok = ok && bar_wait(err, smem_u32(&empty[s]), (((uint32_t)made / P_STAGES) & 1u) ^ 1u);
+                    if (!ok) break;
+                    const unsigned char* const from = im.data + (image + made) * (2 * C::TILE);
+                    mbar_arrive_expect_tx(&full[s], 2 * C::TILE);
+                    bulk_copy_g2s(smem + (ks - smem_u32(smem)) + s * C::TILE, from, C::TILE, &full[s]);
+                    bulk_copy_g2s(smem + (vs - smem_u32(smem)) + s * C::TILE, from + C::TILE, C::TILE, &full[s]);
                 }
-                for (int j = max(0, nk - P_STAGES); j < nk; ++j)            // whoever gave up: do not leave with copies in flight
-                    bar_wait(err, smem_u32(&kfull[j % P_STAGES]), (uint32_t)(j / P_STAGES) & 1u);
-                for (int j = max(0, nv - P_STAGES); j < nv; ++j)
-                    bar_wait(err, smem_u32(&vfull[j % P_STAGES]), (uint32_t)(j / P_STAGES) & 1u);
+                for (int j = max(0, made - P_STAGES); j < made; ++j)        // whoever gave up: do not leave with copies in flight
+                    bar_wait(err, smem_u32(&full[j % P_STAGES]), (uint32_t)(j / P_STAGES) & 1u);
             }
             __syncwarp();
         } else {
@@ -552,22 +545,17 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
             for (int i = 0; i < n; ++i) {
                 const int s = i % P_STAGES;
                 const uint32_t free = (((uint32_t)i / P_STAGES) & 1u) ^ 1u;
-                ok = ok && all_wait(err, &kempty[s], free);
+                ok = ok && all_wait(err, &empty[s], free);
                 if (!ok) break;
                 kr.expand(false, store(ks + s * C::TILE));
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&kfull[s]);
                 page = ahead;
                 place(i + 1);
                 if (i + 1 < n) kr.load(khead + codes, khead + words, there);
                 ahead = page_at(i + 2);
-                ok = ok && all_wait(err, &vempty[s], free);
-                if (!ok) break;
                 nan |= vr.expand(true, store(vs + s * C::TILE));
                 fence_proxy_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&vfull[s]);
+                if (lane == 0) mbar_arrive(&full[s]);
                 if (i + 1 < n) vr.load(vhead + codes, vhead + words, there);
             }
             if (nan) nans = 1;
