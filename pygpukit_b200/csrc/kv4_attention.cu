@@ -11,7 +11,8 @@
 //   * A is 16 keys of codes, B eight query rows: float16 queries (exact for bfloat16 rows; two terms for float32 ones), a group's sum starts at
 //     -z sum q_g, and a group's scale is one multiply-add per (key, row).
 //   * of the values A is 16 elements by 16 keys -- a lane's bytes of two keys, merged by one permutation --, B the weights times the group's scale and 2^64
-//     (which keeps products with c 2^-133 normal), rounded to bfloat16 once; float32 rows have three such terms, 24 bits.  The sum of w s z is
+//     (which keeps products with c 2^-133 normal), rounded to bfloat16 once for rows of that type; float16 rows have two such terms, 16 bits (one left
+//     2^-9 of a weight beside an output's own 2^-12), float32 rows three, 24 bits.  The sum of w s z is
 //     a product over the same rounded weights, so that what rounding does to codes of up to 15 is done to (c - z) only.
 //   * S comes out as [key][row] and is needed as [key][row] operand of the other layout: movmatrix, two cycles for 64 numbers.
 // What bounds it: with 64 and more sequences the issue slots, about 270 instructions for 16 keys of 128 elements and 8 rows, where the cache's bytes
@@ -129,7 +130,7 @@ template <int G, int NT, int DT, int W>
 __global__ void __launch_bounds__(Few<G, NT, DT, W>::THREADS, Few<G, NT, DT, W>::RESIDENT) kv4_few_kernel(const __grid_constant__ Kv4AttnParams p) {
     using Smem = Few<G, NT, DT, W>;
     constexpr int D = 32 * G, DP = D + 4, ROWS = 8 * NT, WARPS = W, THREADS = Smem::THREADS, STAGE = Smem::STAGE;
-    constexpr int QT = DT == 0 ? 2 : 1, PT = DT == 0 ? 3 : 1, MW = (G + 1) / 2;
+    constexpr int QT = DT == 0 ? 2 : 1, PT = 3 - DT, MW = (G + 1) / 2;
     // Rows of 16 bits take a byte, c + 16 c' (a bfloat16 too, subnormal or of the first exponent), where they would take its lower four bits, and subtract the
     // product of the upper ones in the end: one operation in five less.  The difference costs four bits of the sums' 24.
     constexpr bool BYTES = DT != 0;

@@ -7,7 +7,8 @@
 //   * one warp issues S = Q K^T (queries in tensor memory, float16 ones as two bfloat16 terms) and O += P V, the scores of tile i + 1 behind the
 //     weights of tile i;
 //   * eight warps, a lane a row and two warps a row, turn scores into weights; a weight is rounded to bfloat16 once (2^-9 of it, independent from
-//     key to key, beside the output's own 2^-9), their sum is float32 of the unrounded ones.  A row's reference moves when its maximum has grown by 2^8.
+//     key to key, beside the output's own 2^-9), for float16 rows to two such terms (2^-17), their sum is float32 of the unrounded ones.  A row's
+//     reference moves when its maximum has grown by 2^8.
 // The eight elements of a word of codes keep the order (0, 4, 1, 5, 2, 6, 3, 7) that its nibbles fall into: queries are brought into it, outputs back.
 // What bounds it: for 128 x 128 x 128 the MMAs take 1232 cycles, exponentials 1024 of the special unit, expansion and weights 640 issue slots each.
 // Few blocks share a sequence's keys within a cluster and fold through distributed shared memory.
@@ -26,7 +27,9 @@ constexpr int P_ROWS = 128, P_KEYS = 128, P_SOFT = 8, P_EXPAND = 8, P_THREADS = 
 constexpr uint32_t P_CHUNK = P_KEYS * 128;                         // 64 elements of 128 keys
 constexpr uint32_t P_O = 0, P_Q = 128, P_S = 256;                  // TMEM columns: outputs, queries (two terms of 64), two tiles of scores
 constexpr float P_LAZY = 8.f;
-constexpr int P_IMAGES_FROM = 512;                                 // rows of a sequence and head that read its tiles
+// Rows of a sequence and head from which its tiles are made once.  Measured (us, made by each block / once, 8 heads of 128 elements): one sequence over 16384
+// keys, 512 rows 58.6 / 62.4, 768 140 / 130, 1024 104 / 95; 8 over 3000, 512 82.9 / 84.2, 768 116 / 111; 32 over 2000, 512 219 / 228, 768 299 / 294.
+constexpr int P_IMAGES_FROM = 768;
 constexpr long long P_IMAGES_MOST = 1ll << 30;
 
 // Tiles as they lie in shared memory, made ahead of the products: [sequence][head][tile][K, V], and per tile whether a value is NaN.  Tile 0 is the one
@@ -266,9 +269,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// 32 weights 2^(s fac + neg), rounded, to TMEM column `to`; their sum is of the unrounded ones
+// 32 weights 2^(s fac + neg) to TMEM column `to`, as one bfloat16 term or two (the second 32 columns on); their sum is of the unrounded ones
+template <int TERMS>
 __device__ __forceinline__ void weights32(const float* s, float fac, float neg, uint32_t to, uint64_t& l) {
-    uint32_t y[16];
+    uint32_t y[16], z[16];
     const uint64_t fac2 = pair(fac, fac), neg2 = pair(neg, neg);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
@@ -279,9 +283,11 @@ __device__ __forceinline__ void weights32(const float* s, float fac, float neg, 
         b = ex2(b);
         l = add2(l, pair(a, b));
         y[e] = pack_bf16x2(a, b);
+        if constexpr (TERMS == 2) z[e] = pack_bf16x2(a - bf16lo(y[e]), b - bf16hi(y[e]));
     }
     __syncwarp();
     tmem_st16u(to, y);
+    if constexpr (TERMS == 2) tmem_st16u(to + 32u, z);
 }
 __device__ __forceinline__ void rescale(uint32_t at, int columns, float f) {
 #pragma unroll 1
@@ -474,8 +480,10 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
                 const uint64_t d = vd + (uint64_t)(s * (C::TILE / 16));
                 const uint32_t at = tmem + P_S + (uint32_t)(i & 1) * 128u;
 #pragma unroll
-                for (int k = 0; k < P_KEYS / 16; ++k)              // 16 keys: 2048 bytes of V
-                    umma_bf16_ta(tmem + P_O, at + (uint32_t)(k >> 2) * 64u + (uint32_t)(k & 3) * 8u, d + (uint64_t)(k * 128), id_o, (i | k) ? 1u : 0u);
+                for (int term = 0; term < QT; ++term)
+#pragma unroll
+                    for (int k = 0; k < P_KEYS / 16; ++k)          // 16 keys: 2048 bytes of V
+                        umma_bf16_ta(tmem + P_O, at + (uint32_t)term * 32u + (uint32_t)(k >> 2) * 64u + (uint32_t)(k & 3) * 8u, d + (uint64_t)(k * 128), id_o, (i | k | term) ? 1u : 0u);
                 umma_commit(&pvdone);
                 umma_commit(&empty[s]);
             }
@@ -597,8 +605,8 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
                 }
             }
             uint64_t l2 = pair(0.f, 0.f);
-            weights32(s, fac, neg, at + (uint32_t)(half * 64), l2);               // to where the warp's own scores were
-            weights32(s + 32, fac, neg, at + (uint32_t)(half * 64 + 16), l2);
+            weights32<QT>(s, fac, neg, at + (uint32_t)(half * 64), l2);               // to where the warp's own scores were
+            weights32<QT>(s + 32, fac, neg, at + (uint32_t)(half * 64 + 16), l2);
             float la, lb;
             unpair(l2, la, lb);
             l += la + lb;
@@ -626,40 +634,50 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
     if (p.splits > 1) fold_cluster<D, DT>(p, b, fold, row_m, row_l);
 }
 
-template <typename... K>
-cudaError_t launch_blocks(void (*kernel)(K...), const Kv4AttnParams& p, int threads, int smem, cudaStream_t st, K... args) {
+// The blocks' launch: Blocks of rows, and how many blocks of a cluster share a sequence's keys: rounds of clusters times (a block's tiles + what it costs
+// besides, about four of them).  How many clusters run at once is asked for: of eight blocks, one a SM, fewer than 148 / 8.  (Taking the SMs for it, 256
+// rows of eight heads over 3000 keys were cut into 16 clusters of eight, two rounds: 34.5 us; four blocks a cluster: @@.)
+template <int THREADS, int SMEM>
+cudaError_t launch_blocks(void (*kernel)(Kv4AttnParams, Images, int*), Kv4AttnParams p, cudaStream_t st, int (&at_once)[4], Images im, int* err) {
+    p.tiles = (int)(((long long)p.max_rows * p.rep + P_ROWS - 1) / P_ROWS);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(p.seqs * p.tiles), p.k.kv_heads, p.splits);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = 1;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = (unsigned)p.splits;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    count_launch();
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-// Blocks of rows, and how many blocks of a cluster share a sequence's keys: rounds of blocks times (their tiles + what a block costs besides, about four)
-void cut_rows(Kv4AttnParams& p, int rows) {
-    p.tiles = (int)(((long long)p.max_rows * p.rep + rows - 1) / rows);
-    const int keys = p.window > 0 && p.window < p.max_keys - rows ? p.window + rows : p.max_keys, nt = (keys + P_KEYS - 1) / P_KEYS;
+    const int keys = p.window > 0 && p.window < p.max_keys - P_ROWS ? p.window + P_ROWS : p.max_keys, nt = (keys + P_KEYS - 1) / P_KEYS;
     const long long items = (long long)p.seqs * p.tiles * p.k.kv_heads;
     long long least = 0;
-    for (int s = 1; s <= P_CLUSTER; s *= 2) {
-        const long long cost = ((items * s + sm_count() - 1) / sm_count()) * ((nt + s - 1) / s + 4);
+    for (int i = 0; 1 << i <= P_CLUSTER; ++i) {
+        const int s = 1 << i;
+        if (at_once[i] == 0) {
+            attr[0].val.clusterDim.z = (unsigned)s;
+            cfg.gridDim = dim3(1, 1, s);
+            cfg.numAttrs = 1;
+            int n = 0;
+            if (cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg)) return e;
+            at_once[i] = n > 0 ? n : 1;
+        }
+        const long long cost = ((items + at_once[i] - 1) / at_once[i]) * ((nt + s - 1) / s + 4);
         if (s == 1 || cost < least) { p.splits = s; least = cost; }
     }
+    attr[0].val.clusterDim.z = (unsigned)p.splits;
+    cfg.gridDim = dim3((unsigned)(p.seqs * p.tiles), p.k.kv_heads, p.splits);
+    cfg.numAttrs = 2;
+    count_launch();
+    return cudaLaunchKernelEx(&cfg, kernel, p, im, err);
 }
 
 template <int G, int DT>
 int launch_prompt(Kv4AttnParams p, cudaStream_t st) {
     static bool configured = false;
+    static int at_once[2][4] = {};
     if (!configured) {
         PGK_CUDA(cudaFuncSetAttribute(kv4_prompt_kernel<G, DT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Prompt<G>::BYTES));
         PGK_CUDA(cudaFuncSetAttribute(kv4_prompt_kernel<G, DT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Prompt<G>::BYTES));
@@ -680,15 +698,14 @@ int launch_prompt(Kv4AttnParams p, cudaStream_t st) {
         if (rc == (int)cudaErrorMemoryAllocation) set_error("");      // no room: the blocks make their tiles
         else if (rc) return rc;
     }
-    cut_rows(p, P_ROWS);
     cudaError_t e = cudaSuccess;
     if (ws) {
         im.data = (unsigned char*)ws;
         im.nans = (int32_t*)((unsigned char*)ws + count * (2 * Prompt<G>::TILE));
         e = launch_waiting(kv4_images_kernel<G>, dim3(im.tiles, p.k.kv_heads, p.seqs), dim3(P_EXPAND * 32), 0, st, p, im);
-        if (e == cudaSuccess) e = launch_blocks(kv4_prompt_kernel<G, DT, true>, p, (P_SOFT + 2) * 32, Prompt<G>::BYTES, st, p, im, err);
+        if (e == cudaSuccess) e = launch_blocks<(P_SOFT + 2) * 32, Prompt<G>::BYTES>(kv4_prompt_kernel<G, DT, true>, p, st, at_once[1], im, err);
     } else {
-        e = launch_blocks(kv4_prompt_kernel<G, DT, false>, p, P_THREADS, Prompt<G>::BYTES, st, p, im, err);
+        e = launch_blocks<P_THREADS, Prompt<G>::BYTES>(kv4_prompt_kernel<G, DT, false>, p, st, at_once[0], im, err);
     }
     if (int rc = scratch_free(ws, st)) return rc;
     PGK_CUDA(e);
@@ -701,8 +718,11 @@ int launch_prompt_dim(const Kv4AttnParams& p, cudaStream_t st) {
 
 }  // namespace
 
+// More rows than a block of the other kernel has (32 of 64 elements, 16 of more).  Measured there / here (us, 8 heads, 16 and 20 rows): 128 elements, one
+// sequence over 3000 keys 14.2 / 15.6 and 15.6 / 15.5, 8 over 3000 21.7 / 28.0 and 32.1 / 27.9, 32 over 2000 39.4 / 60.7 and 66.5 / 60.8; 64 elements,
+// 32 and 48 rows, 8 over 3000 24.8 / 23.6 and 35.8 / 23.8, 32 over 2000 42.4 / 49.7 and 77.3 / 49.4.
 bool kv4_prompt_serves(const Kv4AttnParams& p, int dtype) {
-    return dtype != 0 && p.k.dim <= 128 && (long long)p.max_rows * p.rep >= 64;
+    return dtype != 0 && p.k.dim <= 128 && (long long)p.max_rows * p.rep > (p.k.dim == 64 ? 32 : 16);
 }
 int kv4_prompt(const Kv4AttnParams& p, int dtype, cudaStream_t st) { return dtype == 1 ? launch_prompt_dim<1>(p, st) : launch_prompt_dim<2>(p, st); }
 

@@ -133,11 +133,12 @@ HALF_STEP = {"bfloat16": 2.0 ** -8, "float16": 2.0 ** -11, "float32": 2.0 ** -24
 
 
 def bound(ref, spread, size, D, dtype, softcap):
-    """What an output may be off.  Its own rounding; a weight's: bfloat16 (half a step 2^-8) where rows have 16 bits, three such terms (2^-23) where
-    they have 32, on codes up to 15 scales; and what the score is off moves a weight by as much, relatively, numerator and denominator:
+    """What an output may be off.  Its own rounding; a weight's: bfloat16 (half a step 2^-8) where rows are of that type, two such terms (2^-16) and an
+    exponent of up to 72 in float32 (2^-18) where they are float16, three (2^-23) where they have 32 bits, on codes up to 15 scales; for rows of 16 bits
+    32 float32 additions (truncated, 2^-23) of bytes up to 17 codes; and what the score is off moves a weight by as much, relatively, numerator and denominator:
     D + 8 float32 roundings of a sum of |q k|, the query's own representation (2^-22, two float16 terms; 2^-25 of the largest element below
     float16's range), the exponential (2^-21) and a tanh (2^-21 of the cap)."""
-    weight = 2.0 ** -23 if dtype == "float32" else 2.0 ** -8
+    weight = {"float32": 2.0 ** -23, "float16": 2.0 ** -16 + 2.0 ** -18 + 17 * 32 * 2.0 ** -23, "bfloat16": 2.0 ** -8 + 17 * 32 * 2.0 ** -23}[dtype]
     score = (D + 12) * 2.0 ** -24 * size + 2.0 ** -21 + (2.0 ** -21 * softcap if softcap else 0.0)
     return HALF_STEP[dtype] * np.abs(ref) + spread * (weight + 2 * score[..., None] + (D + 64) * 2.0 ** -24) + 1e-30
 

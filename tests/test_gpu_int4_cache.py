@@ -179,6 +179,8 @@ FORMS = [  # heads, kv heads, D, page, type, options
     dict(Hq=24, H=2, D=256, PS=64, dtype="bfloat16"),
     dict(Hq=40, H=1, D=64, PS=64, dtype="float32"),
     dict(Hq=7, H=7, D=256, PS=16, dtype="float16", window=1, sinks=True),
+    dict(Hq=8, H=2, D=128, PS=64, dtype="float16"),
+    dict(Hq=32, H=4, D=96, PS=32, dtype="float16", window=70, sinks=True),
 ]
 
 
