@@ -39,7 +39,7 @@ template <int G, int NT, int DT, int W> struct Few {
     static constexpr int THREADS = W * 32, RESIDENT = G * NT <= 4 ? 16 / W : 8 / W;
     static constexpr int STAGE = F_KEYS * 36 * G;                  // codes of K, of V, words of K, of V
     static constexpr int RINGS = W * F_STAGES * STAGE, FOLD = W * 8 * NT * (32 * G + 4) * 4;
-    static constexpr int FRAG = RINGS > FOLD ? RINGS : FOLD, QSUM = FRAG + G * 2 * NT * (DT == 0 ? 2 : 1) * 256, BYTES = QSUM + G * NT * 128;
+    static constexpr int FRAG = RINGS > FOLD ? RINGS : FOLD, QSUM = FRAG + G * 2 * NT * (DT == 0 ? 2 : 1) * 256, BYTES = QSUM + G * NT * (DT == 0 ? 2 : 1) * 128;
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -214,40 +214,39 @@ __global__ void __launch_bounds__(Few<G, NT, DT, W>::THREADS, Few<G, NT, DT, W>:
 
     // ---------------- queries into fragments
     unsigned char* const frag = smem + Smem::FRAG;
-    unsigned char* const qsum = smem + Smem::QSUM;                 // [G][NT][lane]: -sum of the group's queries, in a term of float16 a quad's lane
+    unsigned char* const qsum = smem + Smem::QSUM;                 // [G][NT][term][lane]: -sum of the group's queries, in a term of float16 a quad's lane
     for (int c = warp; c < ROWS; c += WARPS) {
         const int f = f0 + c, i = f / p.rep, tok = first + i;
         const bool there = c < live && tok >= 0 && tok < p.tokens;
         float x[G], top = 0.f;
-        bool odd = false;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             x[g] = there ? row_element<DT>(p.q, (size_t)tok * p.q_ld + (size_t)(head * p.rep + f - i * p.rep) * D + 32 * g + lane) : 0.f;
             top = fmaxf(top, fabsf(x[g]));
-            odd |= x[g] != x[g];
         }
         top = warp_max(top);
-        const uint32_t e = min(max(263u - min(__float_as_uint(top) >> 23, 262u), 4u), 250u);        // 2^9 <= top 2^(e - 127) < 2^10: 32 of them have a sum
+        // 2^9 <= top 2^(e - 127) < 2^10: 32 of them have a sum in float16; of float32 rows 2^10 <= ... < 2^11
+        const uint32_t e = min(max((DT == 0 ? 264u : 263u) - min(__float_as_uint(top) >> 23, 262u), 4u), 250u);
         const float mult = __uint_as_float(e << 23);
         const int w = lane, qt = w >> 3, nib = w & 7, pr = nib & 3;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            const float y = x[g] * mult * (pr & 1 ? 0.0625f : 1.f);
-            float used = 0.f, rest = y;
+            // Terms of float32 rows are integers of 11 bits, the second of 2^-12: their products' sums have 20 bits and are exact, each in an accumulator of
+            // its own (sums of floating terms in one, truncated at every product, were off by 2e-6 of a score, ten times float32's own).
+            const float y = x[g] * mult, first = DT == 0 ? rintf(y) : y, f = pr & 1 ? 0.0625f : 1.f;
 #pragma unroll
             for (int term = 0; term < QT; ++term) {
-                const __half h = __float2half_rn(rest);
+                const float part = term == 0 ? first : rintf((y - first) * 4096.f) * (1.f / 4096.f);
+                const __half h = __float2half_rn(part * f);
                 *(uint16_t*)(frag + ((((size_t)(g * 2 + (pr >> 1)) * NT + (c >> 3)) * QT + term) * 32 + (c & 7) * 4 + qt) * 8 + (pr & 1) * 4 + (nib >> 2) * 2) =
                     __half_as_ushort(h);
-                used += __half2float(h);
-                rest -= __half2float(h);
-            }
-            float sum = -warp_sum(used * (pr & 1 ? 16.f : 1.f));
-            // the lane t of a quad multiplies its copy of z by term t; an even group's z is in a word's lower half, an odd one's in the upper
-            for (int term = 0; term < 4; ++term) {
-                const __half h = __float2half_rn(sum);
-                sum -= __half2float(h);
-                if (lane == term) *(uint32_t*)(qsum + ((size_t)(g * NT + (c >> 3)) * 32 + (c & 7) * 4 + term) * 4) = (uint32_t)__half_as_ushort(h) << (g & 1 ? 16 : 0);
+                float sum = -warp_sum(__half2float(h) * (pr & 1 ? 16.f : 1.f));
+                // the lane i of a quad multiplies its copy of z by piece i; an even group's z is in a word's lower half, an odd one's in the upper
+                for (int i = 0; i < 4; ++i) {
+                    const __half piece = __float2half_rn(DT == 0 ? fminf(fmaxf(sum, -32768.f), 32768.f) : sum);
+                    sum -= __half2float(piece);
+                    if (lane == i) *(uint32_t*)(qsum + ((size_t)((g * NT + (c >> 3)) * QT + term) * 32 + (c & 7) * 4 + i) * 4) = (uint32_t)__half_as_ushort(piece) << (g & 1 ? 16 : 0);
+                }
             }
         }
         if (lane == 0) {
@@ -325,8 +324,10 @@ again:
             for (int g = 0; g < G; ++g) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const uint32_t qs = *(const uint32_t*)(qsum + ((g * NT + j) * 32 + lane) * 4);
+                    uint32_t qs[QT];
                     uint2 b[2][QT];
+#pragma unroll
+                    for (int term = 0; term < QT; ++term) qs[term] = *(const uint32_t*)(qsum + (((g * NT + j) * QT + term) * 32 + lane) * 4);
 #pragma unroll
                     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -336,13 +337,17 @@ again:
                     for (int u = 0; u < 2; ++u) {
                         const float s0 = group_scale(km[u][0][g / 2], g & 1), s1 = group_scale(km[u][1][g / 2], g & 1);
                         float c[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma_f16_k8(c, kz[u][0][g / 2], kz[u][1][g / 2], qs);
 #pragma unroll
-                        for (int ks = 0; ks < 2; ++ks) {
-                            const uint32_t w0 = ks ? kw[u][0][g] >> 8 : kw[u][0][g], w1 = ks ? kw[u][1][g] >> 8 : kw[u][1][g];
+                        for (int term = QT - 1; term >= 0; --term) {
+                            float a[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma_f16_k8(a, kz[u][0][g / 2], kz[u][1][g / 2], qs[term]);
 #pragma unroll
-                            for (int term = QT - 1; term >= 0; --term)
-                                mma_f16(c, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, b[ks][term].x, b[ks][term].y);
+                            for (int ks = 0; ks < 2; ++ks) {
+                                const uint32_t w0 = ks ? kw[u][0][g] >> 8 : kw[u][0][g], w1 = ks ? kw[u][1][g] >> 8 : kw[u][1][g];
+                                mma_f16(a, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, b[ks][term].x, b[ks][term].y);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) c[i] = term == QT - 1 ? a[i] : c[i] + a[i];
                         }
                         s[u][j][0] = fmaf(s0, c[0], s[u][j][0]);
                         s[u][j][1] = fmaf(s0, c[1], s[u][j][1]);
