@@ -7,9 +7,9 @@
 // sum_j w_j v_j = sum_j (w_j s_j) c_j - sum_j (w_j s_j) z_j.  What this makes of the work:
 //   * codes go to the tensor cores (mma.sync m16n8k16) as they are.  Four bits in the lowest places of a float16 are c 2^-24, four bits above them c 2^-20,
 //     of a bfloat16 c 2^-133 and c 2^-129: subnormal numbers, which the products take exactly (tested), so that two elements cost one AND.
-//     The query carries 2^-4 where the code carries 2^4, and a power of two that brings its largest element below 2^15.
-//   * A is 16 keys of codes, B eight query rows: float16 queries (exact for bfloat16 rows; two terms for float32 ones), a group's sum starts at
-//     -z sum q_g, and a group's scale is one multiply-add per (key, row).
+//     The query carries 2^-4 where the code carries 2^4, and a power of two that brings its largest element below 2^10 (2^11).
+//   * A is 16 keys of codes, B eight query rows: float16 queries (exact for bfloat16 rows; two terms, 22 bits of the largest, for float32 ones), a
+//     group's sum starts at -z sum q_g, and a group's scale is one multiply-add per (key, row).
 //   * of the values A is 16 elements by 16 keys -- a lane's bytes of two keys, merged by one permutation --, B the weights times the group's scale and 2^64
 //     (which keeps products with c 2^-133 normal), rounded to bfloat16 once for rows of that type; float16 rows have two such terms, 16 bits (one left
 //     2^-9 of a weight beside an output's own 2^-12), float32 rows three, 24 bits.  The sum of w s z is
@@ -453,6 +453,10 @@ again:
                     const float s0 = group_scale(vm[0][g / 2], g & 1), s1 = group_scale(vm[1][g / 2], g & 1);
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
+                        // Float32 rows sum 16 keys here and add these sums: the products' own additions truncate, which made 1.6e-6 of an output over
+                        // 15751 keys, and 3e-7 this way.
+                        float part[3][4] = {};
+                        float (&low)[4] = DT == 0 ? part[0] : acc[2 * g][j], (&high)[4] = DT == 0 ? part[1] : acc[2 * g + 1][j], (&zsum)[4] = DT == 0 ? part[2] : zac[j];
                         float w[4] = {s[u][j][0] * s0, s[u][j][1] * s0, s[u][j][2] * s1, s[u][j][3] * s1};
                         if constexpr (SPECIAL) {                   // a key that is not seen may have any bytes for a scale
 #pragma unroll
@@ -463,18 +467,26 @@ again:
                         for (int term = 0; term < PT; ++term) {
                             const uint32_t lo = pack_bf16x2(w[0], w[1]), hi = pack_bf16x2(w[2], w[3]);
                             const uint32_t p0 = transposed(lo), p1 = transposed(hi);
-                            mma_bf16(acc[2 * g][j], v0 & LOW, v0 & 0x00f000f0u, v1 & LOW, v1 & 0x00f000f0u, p0, p1);
-                            mma_bf16(acc[2 * g + 1][j], BYTES ? v2 : v2 & LOW, v2 & 0x00f000f0u, BYTES ? v3 : v3 & LOW, v3 & 0x00f000f0u, p0, p1);
+                            mma_bf16(low, v0 & LOW, v0 & 0x00f000f0u, v1 & LOW, v1 & 0x00f000f0u, p0, p1);
+                            mma_bf16(high, BYTES ? v2 : v2 & LOW, v2 & 0x00f000f0u, BYTES ? v3 : v3 & LOW, v3 & 0x00f000f0u, p0, p1);
                             if constexpr (SPECIAL) {
                                 float y[4];
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) y[i] = careful ? finite(w[i]) : w[i];
-                                mma_bf16(zac[j], z0, 0u, z1, 0u, transposed(pack_bf16x2(y[0], y[1])), transposed(pack_bf16x2(y[2], y[3])));
+                                mma_bf16(zsum, z0, 0u, z1, 0u, transposed(pack_bf16x2(y[0], y[1])), transposed(pack_bf16x2(y[2], y[3])));
                             } else
-                                mma_bf16(zac[j], z0, 0u, z1, 0u, p0, p1);
+                                mma_bf16(zsum, z0, 0u, z1, 0u, p0, p1);
                             if (term + 1 < PT) {
                                 w[0] -= bf16lo(lo); w[1] -= bf16hi(lo);
                                 w[2] -= bf16lo(hi); w[3] -= bf16hi(hi);
+                            }
+                        }
+                        if constexpr (DT == 0) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                acc[2 * g][j][i] += part[0][i];
+                                acc[2 * g + 1][j][i] += part[1][i];
+                                zac[j][i] += part[2][i];
                             }
                         }
                     }
