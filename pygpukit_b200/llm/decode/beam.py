@@ -100,7 +100,7 @@ class BeamSearch:
         if not over and len(s.done) == self.K:
             over = max(self._counts(b[0], s.generated) for b in s.beams) <= s.done[0][0]
         if over:
-            for score, tokens, _ in s.beams:
+            for score, tokens, _ in s.beams or (() if s.done else old):        # no candidate at all: the beams as they were
                 self._finish(s, score, tokens)
             for b in old:
                 self.model.release(b[2])

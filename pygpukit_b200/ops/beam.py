@@ -63,7 +63,10 @@ def _rows_of(name: str, arrays) -> tuple[int, array, array]:
             if not a._shape or a._shape[0] != rows:
                 raise ValueError(f"{name}: arrays of {rows} rows, got {a.shape}")
         sizes = array("q", [a.nbytes // max(1, rows) for a in arrays])
-    return rows, array("Q", [a._ptr for a in arrays]), sizes
+    ptrs = [a._ptr for a in arrays]
+    if len(set(ptrs)) < len(ptrs) and first.nbytes:
+        raise ValueError(f"{name}: an array is there twice")
+    return rows, array("Q", ptrs), sizes
 
 
 def reorder_rows(arrays: "list[GPUArray]", parents: GPUArray) -> None:

@@ -149,7 +149,9 @@ def search(K, V, table, prompts, n, eos=None, penalty=1.0, monkeypatch=None):
     def select(logits, scores, n):
         B, k = scores.shape
         x = logits.reshape(B, k, V)
-        c = scores[..., None] + x - np.log(np.exp(x).sum(-1, keepdims=True))
+        with np.errstate(divide="ignore", invalid="ignore"):
+            c = scores[..., None] + x - np.log(np.exp(x).sum(-1, keepdims=True))
+        c[np.isnan(c)] = -np.inf
         flat = c.reshape(B, -1)
         o = np.argsort(-flat, 1, kind="stable")[:, :n]
         return [np.take_along_axis(flat, o, 1), o // V, o % V]
@@ -221,6 +223,16 @@ def test_one_beam_is_greedy(monkeypatch):
         for _ in range(5):
             seq.append(int(np.argmax(table(tuple(seq)))))
         assert got[i][0][1] == seq
+
+
+@pytest.mark.parametrize("dead", [0, 2])
+def test_a_model_without_continuations_ends_where_it_is(monkeypatch, dead):
+    """logits that leave no candidate (masked, or not numbers): the beams as far as they came"""
+    table = random_table(5, 1)
+    got = search(5, 5, lambda seq: np.full(5, -np.inf) if len(seq) >= 1 + dead else table(seq), [[2]], 6, None, 1.0, monkeypatch)
+    assert len(got[0]) == (5 if dead else 1) and all(len(t) == 1 + dead for _, t in got[0])
+    want = every(table, 5, [2], dead, None, 1.0) if dead else [(0.0, [2])]
+    assert got[0][0][1] == want[0][1]
 
 
 def test_requests_and_refusals(monkeypatch):

@@ -89,6 +89,9 @@ def test_rows_refuse():
     for arrays in ([x, arr((5, 4))], [x, arr(())]):
         with pytest.raises(ValueError, match="reorder_rows"):
             ops.reorder_rows(arrays, arr((2, 3), int32))
+    for call in (lambda a: ops.reorder_rows(a, arr((2, 3), int32)), lambda a: ops.copy_rows(a, arr((2,), int32), arr((2,), int32))):
+        with pytest.raises(ValueError, match="twice"):              # its rows would move twice, at once
+            call([x, arr((6, 2)), x])
     for src, dst in ((arr((3,), int64), arr((3,), int32)), (arr((3,), int32), arr((4,), int32)), (arr((3, 1), int32), arr((3, 1), int32))):
         with pytest.raises(ValueError, match="copy_rows"):
             ops.copy_rows([x], src, dst)
