@@ -463,6 +463,43 @@ def test_two_calls_at_once_on_two_streams():
         assert np.array_equal(ref.floats(h["out"].to_numpy(), "bfloat16").astype(np.float64), w)
 
 
+@pytest.mark.parametrize("rows,dtype", [(6, "bfloat16"), (6, "float16"), (60, "bfloat16"), (300, "bfloat16"), (300, "float16"), (5, "float32")])
+def test_two_captured_calls_replayed_at_once(rows, dtype):
+    """graphs of two calls, made before either ran, with what work memory they have: side by side on two streams, and then eager calls"""
+    both = [Attend([(700, rows), (400, rows // 2), (90, 1)], 8, 2, 128, 64, dtype, seed=18 + i) for i in (0, 1)]
+    held = [dict(q=from_numpy(x.q), out=zeros(x.q.shape, TYPES[dtype]), slots=i32(x.slots), ctx=i32([c for c, _ in x.portions]), starts=i32(x.starts)) for x in both]
+
+    def call(x, h):
+        ops.sdpa_paged_int4(h["q"], x.c.kd, x.c.vd, h["out"], x.c.td, h["slots"], h["ctx"], x.top, row_starts=h["starts"], max_rows=rows)
+
+    streams, graphs = [Stream(), Stream()], [CudaGraph(), CudaGraph()]
+    synchronize()
+    for s, g, x, h in zip(streams, graphs, both, held):
+        with g.capture(s):
+            call(x, h)
+    for _ in range(10):
+        for s, g in zip(streams, graphs):
+            with use_stream(s):
+                g.replay(s)
+    for s in streams:
+        s.synchronize()
+    got = [h["out"].to_numpy()[:x.T] for x, h in zip(both, held)]
+    for x, h, g in zip(both, held, got):
+        x.check(x.run())
+        call(x, h)
+        synchronize()
+        assert np.array_equal(h["out"].to_numpy()[:x.T], g)
+
+
+def test_outputs_over_their_queries():
+    """out may be Q: a block has read all of its rows before one of them is written"""
+    for rows, dtype in ((1, "float32"), (4, "bfloat16"), (70, "bfloat16"), (250, "float16")):
+        x = Attend([(900, rows), (300, rows)], 8, 2, 128, 64, dtype, seed=30 + rows)
+        want, q = x.run(), from_numpy(x.q)
+        ops.sdpa_paged_int4(q, x.c.kd, x.c.vd, q, x.c.td, i32(x.slots), i32([c for c, _ in x.portions]), x.top, row_starts=i32(x.starts), max_rows=rows)
+        assert np.array_equal(ref.floats(q.to_numpy(), dtype).astype(np.float64)[:x.T], want[:x.T])
+
+
 def test_offsets_past_32_bits():
     """a cache of more than 4 GB: the last page is where it should be"""
     H, D, PS = 16, 256, 64
