@@ -315,7 +315,11 @@ __global__ void __launch_bounds__(B_THREADS) beam_merge_kernel(const __grid_cons
 // ---------------------------------------------------------------- rows that follow their beams
 // A thread has one word of every row of its group: it loads them all, then stores the ones that change, so that a row may be parent and
 // child at once, and two children may have one parent.
-constexpr int R_ARRAYS = 64, R_REGS = 16, R_THREADS = 256, R_SMEM_THREADS = 128, R_MAX = 64;      // groups of more than R_REGS rows: through shared memory
+// What bounds it: memory (16 arrays of 32 rows of 1 MB in groups of 8: 84.3 us, 6.0 TB/s of what is read and written).  Groups of up to 16 rows go through
+// registers, as many as a group of 4, 8 or 16 needs, larger ones through shared memory, which is slower where both would do (us, 8 arrays of 32 rows of 1 MB,
+// groups of 8 58.9 / 68, of 16 65 / 104); its copies are asynchronous, all of a thread's on their way at once (64 rows, 815 waited for one by one, 144 so), in
+// small blocks, so that a block's loads run beside another's stores (64 rows in blocks of 128 / 64 / 32 threads 183 / 144 / 152).
+constexpr int R_ARRAYS = 64, R_REGS = 16, R_THREADS = 256, R_SMEM_THREADS = 64, R_MAX = 64;
 
 struct RowsParams {
     unsigned char* data[R_ARRAYS];
@@ -331,16 +335,16 @@ __global__ void __launch_bounds__(REGS ? R_THREADS : R_SMEM_THREADS) rows_kernel
     griddep_wait();
     griddep_launch();
     const int tid = threadIdx.x, T = REGS ? R_THREADS : R_SMEM_THREADS, first = blockIdx.y * p.group, n = min(p.group, p.pairs - first);
-    if (tid < n) {
-        int s = __ldcg(p.src + first + tid), d = first + tid;
+    for (int i = tid; i < n; i += T) {
+        int s = __ldcg(p.src + first + i), d = first + i;
         if (p.dst) {
-            d = __ldcg(p.dst + first + tid);
+            d = __ldcg(p.dst + first + i);
             if ((unsigned)s >= (unsigned)p.rows) s = -1;
         } else
             s = (unsigned)s < (unsigned)p.group ? first + s : -1;
         if ((unsigned)d >= (unsigned)p.rows || s == d) s = -1;
-        from[tid] = s;
-        to[tid] = d;
+        from[i] = s;
+        to[i] = d;
     }
     __syncthreads();
     const long long words = p.words[blockIdx.z];
@@ -348,8 +352,16 @@ __global__ void __launch_bounds__(REGS ? R_THREADS : R_SMEM_THREADS) rows_kernel
     for (long long c = (long long)blockIdx.x * T + tid; c < words; c += (long long)gridDim.x * T) {
         if constexpr (REGS == 0) {
             W* mine = reinterpret_cast<W*>(held) + tid;
-            for (int i = 0; i < n; ++i)
-                if (from[i] >= 0) mine[i * T] = __ldcg(data + from[i] * words + c);
+            for (int i = 0; i < n; ++i) {
+                if (from[i] < 0) continue;
+                if constexpr (sizeof(W) == 16) cp_async16(mine + i * T, data + from[i] * words + c);
+                else if constexpr (sizeof(W) == 4) cp_async4(mine + i * T, data + from[i] * words + c);
+                else mine[i * T] = __ldcg(data + from[i] * words + c);
+            }
+            if constexpr (sizeof(W) >= 4) {
+                cp_async_commit();
+                cp_async_wait<0>();                        // a thread reads what it has copied itself
+            }
             for (int i = 0; i < n; ++i)
                 if (from[i] >= 0) data[to[i] * words + c] = mine[i * T];
         } else {

@@ -3,7 +3,8 @@
 //   q[t, h, :], k[t, h, :] rotated by the angles of positions[t] over their first R elements:  (a, b) -> (a cos - b sin, b cos + a sin)
 //   for the pairs (i, i + R / 2), or (2 i, 2 i + 1);  q in place, k and v rounded to four bits into the page that holds the position.
 //
-// What bounds them: memory for prompts (q read and written, k and v read, 9 / 16 byte an element written), the launch for decoded tokens.
+// What bounds them: for prompts instructions, 61 % of the issue slots (4000 tokens of 32 and 8 heads of 128: 29.9 us, 2.9 TB/s of queries read and written, keys and
+// values read, 9 / 16 byte an element written), for decoded tokens the launch (8: 2.2 us); reading back, memory and the launch (4000 tokens 5.2 us).
 // A lane has eight neighbouring elements, one 32-bit word of codes; four lanes a group, D / 8 lanes a row; a rotation's other half comes
 // from another lane of the warp, so that all of a row is loaded before any of it is written.  A warp keeps its token's angles and takes
 // several of the token's heads.  Products and sums are rounded one by one (no fused multiply-add): a key on the border between two codes then
@@ -199,11 +200,15 @@ int pgk_kv4_append(void* q, const void* k, const void* v, long q_ld, long k_ld, 
     p.wide_q = wide(q, q_ld); p.wide_k = wide(k, k_ld); p.wide_v = wide(v, v_ld);
     const int side = 32 / (dim / 8), steps = (p.heads + 2 * kv_heads + side - 1) / side;
     p.wide_t = rot > 0 && ((uintptr_t)cos_table | (uintptr_t)sin_table) % 16 == 0;
-    // prompts: a warp's loads of six steps are on their way together, and share its token's page and angles
-    const int per = tokens >= 256 ? 6 : 1;
+    // Prompts: a warp takes up to three steps of its token, whose loads are on their way together and share its page and angles; never so many that a block's
+    // warps have none (us, one / two / three / six steps a warp: 32 and 8 heads of 128, 128 tokens 3.3 / 3.2 / 3.7 / 5.4, 512 7.0 / 6.7 / 5.7 / 7.8, 4000
+    // 39.1 / 32.1 / 29.9 / 31.2; keys and values alone, 512 5.2 / 3.8 / 4.0 / 5.9; 8 and 1 heads of 64, 4000 7.3 / 7.8 / 8.8 / 10.2).
+    const int full = (steps + A_WARPS - 1) / A_WARPS, per = (long long)tokens * steps < 4096 ? 1 : (full < 3 ? full : 3);
     const dim3 grid(tokens, (steps + A_WARPS * per - 1) / (A_WARPS * per));
-    auto kernel = per == 6 ? (dtype == 0 ? kv4_append_kernel<0, 6> : (dtype == 1 ? kv4_append_kernel<1, 6> : kv4_append_kernel<2, 6>))
-                           : (dtype == 0 ? kv4_append_kernel<0, 1> : (dtype == 1 ? kv4_append_kernel<1, 1> : kv4_append_kernel<2, 1>));
+    auto of = [&](auto* one, auto* two, auto* three) { return per == 1 ? one : (per == 2 ? two : three); };
+    auto kernel = dtype == 0 ? of(kv4_append_kernel<0, 1>, kv4_append_kernel<0, 2>, kv4_append_kernel<0, 3>)
+                             : (dtype == 1 ? of(kv4_append_kernel<1, 1>, kv4_append_kernel<1, 2>, kv4_append_kernel<1, 3>)
+                                           : of(kv4_append_kernel<2, 1>, kv4_append_kernel<2, 2>, kv4_append_kernel<2, 3>));
     PGK_CUDA(launch_waiting(kernel, grid, dim3(A_WARPS * 32), 0, (cudaStream_t)stream, p));
     return 0;
 }
