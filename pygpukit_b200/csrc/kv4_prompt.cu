@@ -473,6 +473,7 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
                 umma_commit(&sfull[i & 1]);
             };
             if (n > 0) scores(0);
+            int made = 0;
             for (int i = 0; ok && i < n; ++i) {
                 const int s = i % P_STAGES;
                 if (i > 0) ok = bar_wait(err, smem_u32(&pvdone), (uint32_t)((i - 1) & 1));
@@ -489,7 +490,9 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
                         umma_bf16_ta(tmem + P_O, at + (uint32_t)term * 32u + (uint32_t)(k >> 2) * 64u + (uint32_t)(k & 3) * 8u, d + (uint64_t)(k * 128), id_o, (i | k | term) ? 1u : 0u);
                 umma_commit(&pvdone);
                 umma_commit(&empty[s]);
+                made = i + 1;
             }
+            if (made) bar_wait(err, smem_u32(&pvdone), (uint32_t)((made - 1) & 1));           // here, where each was waited for: others might take the last but two for it
         }
         __syncwarp();
     } else if (warp > P_SOFT) {
@@ -618,7 +621,6 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
             __syncwarp();
             if (lane == 0) mbar_arrive(&pready[i & 1]);           // a barrier each: weights of two tiles may be ready before the first is looked for
         }
-        if (n > 0) all_wait(err, &pvdone, (uint32_t)((n - 1) & 1));
         asm volatile("bar.sync %0, 64;" :: "r"(1 + quad) : "memory");              // the last tile's maxima are read
         wmax[0][half][row] = l;
         __syncwarp();
