@@ -17,7 +17,7 @@
 //   * S comes out as [key][row] and is needed as [key][row] operand of the other layout: movmatrix, two cycles for 64 numbers.
 // What bounds it: with 64 and more sequences the issue slots, about 270 instructions for 16 keys of 128 elements and 8 rows, where the cache's bytes
 // leave 350 cycles of a scheduler (64 over 8192 keys, 32 / 8 heads of 128: 148 us, 3.6 TB/s); with one, the chain of a launch, a page number, the rows and the
-// fold (4096 keys: 9.4 us).  Float32 rows cost 30 to 45 % more, float16 rows 10 to 15 %.
+// fold (4096 keys: 9.4 us).  The same 64 with float16 rows 179 us, with float32 ones 277; of 4096 keys 9.5 and 12.4.
 // A warp takes 32 keys at a time through a ring of its own in shared memory (cp.async, no barrier among warps), with its own maximum and sums;
 // the warps fold in shared memory, and where a sequence's keys are cut over the blocks of a cluster, these fold through distributed shared memory.
 //

@@ -13,7 +13,8 @@
 // What bounds it: the chain of a row's warps.  Of 128 x 128 x 128 the products take 512 cycles and the exponentials 1024 of the special unit; measured are 1890 a
 // tile (scores ready, maxima 180 cycles, exchange between a row's warps 240, weights 1160, arrival) where tiles were made before, 2750 where the block
 // makes them (K 800 to 1200, V 800, what lies between 400 each: two warps a scheduler, latency), and 13600 at a block's two ends.  Measured: 512 rows over 16384
-// keys, 32 / 4 heads of 128, 147 to 153 us (0.9 PFLOP/s), 2000 rows over themselves, 32 / 8 heads, 72 to 75 us, 8 sequences of 5 rows over 3000 keys 28 us.
+// keys, 32 / 4 heads of 128, 147 to 153 us (0.9 PFLOP/s), 2000 rows over themselves, 32 / 8 heads, 72 to 75 us, 8 sequences of 5 rows over 3000 keys 28 us;
+// float16 rows, twice the products and a second term a weight, 199, 97 and 34.
 // Few blocks share a sequence's keys within a cluster and fold through distributed shared memory.
 //
 // A value of NaN counts as zero in the products (0 NaN would reach rows that do not see it); where any was met, rows look for the ones they see
