@@ -1,5 +1,5 @@
 """Operators on the paged key / value cache in four bits (net-new: the reference's paged attention kernels,
-native/ops/nn/attention/paged_attention.cuh:46-283, read 16-bit pages).
+native/ops/attention/paged_attention.cuh:46-283, read 16-bit pages).
 
 A cache is two uint8 arrays, keys and values, `[pages, kv_heads, page_size, int4_row_bytes(head_dim)]` -- `llm.PagedKVCache` with dtype "int4"
 makes them -- and an int32 page table `[slots, max_pages]`.  A group of 32 elements of a row is held as codes of four bits, a scale of four
