@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(Few<G, NT, DT, W>::THREADS, Few<G, NT, DT, W>:
             }
         }
         if (lane == 0) {
-            fac_s[c] = p.scale_log2 * __uint_as_float((254u - e) << 23) * 16777216.f;
+            fac_s[c] = fminf(p.scale_log2 * __uint_as_float((254u - e) << 23) * 16777216.f, 3.4028235e38f);       // (scores of 10^36: no infinity that a zero meets)
             lim_s[c] = there ? ctx - n + i : -1;
         }
     }
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(Few<G, NT, DT, W>::THREADS, Few<G, NT, DT, W>:
             lim[j][c] = lim_s[8 * j + 2 * t + c];
         }
     const uint32_t half_sel = gl & 1 ? 0x7632u : 0x5410u;
-    bool careful = false;
+    bool careful = false, huge = false;
 again:
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -404,6 +404,7 @@ again:
                     best = fmaxf(best, m[j][c]);
                     f[c] = m[j][c] == -INFINITY ? 0.f : ex2(m[j][c] - best);
                     m[j][c] = best;
+                    huge |= fabsf(best) > KV4_HUGE && best > -INFINITY;
                     l[j][c] *= f[c];
                 }
 #pragma unroll
@@ -413,6 +414,15 @@ again:
 #pragma unroll
                     for (int c = 0; c < 4; ++c) acc[i][j][c] *= f[c & 1];
             }
+            huge = __any_sync(0xffffffffu, huge);
+        }
+        if (huge) {                                                // x - m of rounded x then: what rounding m left of a multiply-add's exact product may be anything
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[u][j][i] *= fac[j][i & 1];
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j)
@@ -424,7 +434,7 @@ again:
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        float w = ex2(fmaf(s[u][j][2 * r + c], fac[j][c], base));
+                        float w = ex2(fmaf(s[u][j][2 * r + c], huge ? 1.f : fac[j][c], base));
                         if constexpr (DT == 0) w *= F_LIFT;
                         l[j][c] += w;
                         s[u][j][2 * r + c] = w;

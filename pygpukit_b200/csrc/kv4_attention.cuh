@@ -25,6 +25,8 @@ int kv4_prompt(const Kv4AttnParams& p, int dtype, cudaStream_t st);
 
 #ifdef __CUDACC__
 
+constexpr float KV4_HUGE = 268435456.f;                            // a reference of 2^28: float32 has steps of 32 there
+
 // the page that holds the 16 positions n
 __device__ __forceinline__ uint32_t kv4_page_of(const Kv4AttnParams& p, uint32_t n) { return p.page_mul ? __umulhi(n, p.page_mul) >> p.page_shift : n; }
 

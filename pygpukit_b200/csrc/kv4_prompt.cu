@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
         const int clean_lo = p.window > 0 ? b.pos1 - p.window : -1, clean_hi = missing ? -1 : min(b.pos0, end - 1);
         const float fac = p.cap_log2 > 0.f ? 1.f : p.scale_log2;
         float m = -INFINITY, neg = 0.f, l = 0.f;
-        bool ok = true;
+        bool ok = true, huge = false;
         for (int i = 0; i < n; ++i) {
             const uint32_t at = lanes + P_S + (uint32_t)(i & 1) * 128u;
             const int j0 = (tbeg + i) * P_KEYS + half * 64;
@@ -603,6 +603,7 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
             if (__any_sync(0xffffffffu, up)) {                    // the same in both warps: each has half of the outputs
                 const float fix = !up ? 1.f : (m == -INFINITY ? 0.f : exp2f(m - top));
                 if (up) { m = top; neg = -top; }
+                huge = __any_sync(0xffffffffu, fabsf(neg) > KV4_HUGE);
                 l *= fix;
                 if (i > 0) {
                     ok = ok && all_wait(err, &pvdone, (uint32_t)((i - 1) & 1));
@@ -611,9 +612,14 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
                     rescale(lanes + P_O + (uint32_t)(half * (DN / 2)), DN / 2, fix);
                 }
             }
+            if (huge) {                                           // x - m of rounded x then, as in the other kernel
+#pragma unroll
+                for (int e = 0; e < 64; ++e) s[e] *= fac;
+            }
+            const float by = huge ? 1.f : fac;
             uint64_t l2 = pair(0.f, 0.f);
-            weights32<QT>(s, fac, neg, at + (uint32_t)(half * 64), l2);               // to where the warp's own scores were
-            weights32<QT>(s + 32, fac, neg, at + (uint32_t)(half * 64 + 16), l2);
+            weights32<QT>(s, by, neg, at + (uint32_t)(half * 64), l2);               // to where the warp's own scores were
+            weights32<QT>(s + 32, by, neg, at + (uint32_t)(half * 64 + 16), l2);
             float la, lb;
             unpair(l2, la, lb);
             l += la + lb;

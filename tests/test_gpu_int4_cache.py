@@ -380,6 +380,20 @@ def test_queries_and_values_of_any_size(factor, dtype):
     a.check(a.run())
 
 
+@pytest.mark.parametrize("rows", [1, 4, 30])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_scores_near_the_end_of_float32(rows, dtype):
+    """|q . k| of 10^36 and an all-zero key: one key has all of the weight, and nothing becomes infinite"""
+    a = Attend([(70, rows)], 4, 2, 128, 16, dtype, seed=9)
+    a.q = ref.rounded(ref.floats(a.q, dtype) * 1e36 / 1.5, dtype)
+    words, groups = ref.encode(np.zeros((1, 128), np.float32))
+    for h in (0, 1):
+        ref.put(a.c.k, a.c.table[a.slots[0], 0], h, 5, words[0], groups[0])
+    a.c.upload()
+    got, (want, spread, _) = a.run(), a.exact()
+    assert (np.abs(got[:a.T] - want) <= ref.bound(want, spread, np.zeros(want.shape[:2]), 128, dtype, 0.0)).all()
+
+
 def test_scores_far_apart_and_all_the_same():
     """one key that takes all the weight, wherever it lies; and queries of zero, whose output is the mean"""
     for at in (0, 63, 64, 150, 299):
