@@ -13,8 +13,8 @@
 // What bounds it: the chain of a row's warps.  Of 128 x 128 x 128 the products take 512 cycles and the exponentials 1024 of the special unit; measured are 1890 a
 // tile (scores ready, maxima 180 cycles, exchange between a row's warps 240, weights 1160, arrival) where tiles were made before, 2750 where the block
 // makes them (K 800 to 1200, V 800, what lies between 400 each: two warps a scheduler, latency), and 13600 at a block's two ends.  Measured: 512 rows over 16384
-// keys, 32 / 4 heads of 128, 147 to 153 us (0.9 PFLOP/s), 2000 rows over themselves, 32 / 8 heads, 72 to 75 us, 8 sequences of 5 rows over 3000 keys 28 us;
-// float16 rows, twice the products and a second term a weight, 199, 97 and 34.
+// keys, 32 / 4 heads of 128, 147 to 154 us (0.9 PFLOP/s), 2000 rows over themselves, 32 / 8 heads, 73 to 77 us, 8 sequences of 5 rows over 3000 keys 28 us;
+// float16 rows, twice the products and a second term a weight, 200, 97 and 36.
 // Few blocks share a sequence's keys within a cluster and fold through distributed shared memory.
 //
 // A value of NaN counts as zero in the products (0 NaN would reach rows that do not see it); where any was met, rows look for the ones they see
@@ -228,18 +228,23 @@ __device__ __forceinline__ void query8(const Kv4AttnParams& p, const Row& r, int
             a[e] = v[e];
     }
 }
-// N scores of a row, from TMEM column `at`, key j0: capped, and -infinity where the row does not see; `off`: runs of 16 keys without a page
+// N scores of a row, from TMEM column `at`, key j0: capped (or, if they are huge, with their factor), and -infinity where the row does not see; `off`: runs of 16 keys without a page
 template <int N>
-__device__ __forceinline__ void row_scores(const Kv4AttnParams& p, uint32_t at, int j0, bool edge, const Row& r, uint32_t off, float (&s)[N]) {
+__device__ __forceinline__ void row_scores(const Kv4AttnParams& p, uint32_t at, int j0, bool edge, bool huge, const Row& r, uint32_t off, float (&s)[N]) {
 #pragma unroll
     for (int c = 0; c < N; c += 16) tmem_ld16_async(at + (uint32_t)c, *(float (*)[16])(s + c));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int c = 0; c < N; c += 16) tmem_pass(*(float (*)[16])(s + c));
-    if (p.cap_log2 > 0.f) {
-        const float in = p.scale_log2 * 2.885390043f / p.cap_log2;
+    if (p.cap_log2 > 0.f || huge) {
+        if (p.cap_log2 > 0.f) {
+            const float in = p.scale_log2 * 2.885390043f / p.cap_log2;
 #pragma unroll
-        for (int e = 0; e < N; ++e) s[e] = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(s[e] * in)));
+            for (int e = 0; e < N; ++e) s[e] = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(s[e] * in)));
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) s[e] *= p.scale_log2;
+        }
     }
     if (edge) {
         const int hi = r.limit - j0, lo = r.under - j0;
@@ -579,8 +584,7 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
         // ---------------- weights
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
         const int clean_lo = p.window > 0 ? b.pos1 - p.window : -1, clean_hi = missing ? -1 : min(b.pos0, end - 1);
-        const float fac = p.cap_log2 > 0.f ? 1.f : p.scale_log2;
-        float m = -INFINITY, neg = 0.f, l = 0.f;
+        float m = -INFINITY, neg = 0.f, l = 0.f, fac = p.cap_log2 > 0.f ? 1.f : p.scale_log2;
         bool ok = true, huge = false;
         for (int i = 0; i < n; ++i) {
             const uint32_t at = lanes + P_S + (uint32_t)(i & 1) * 128u;
@@ -591,7 +595,7 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
             const bool edge = j0 <= clean_lo || j0 + 63 > clean_hi;
             const uint32_t off = edge && missing ? runs_gone(p, b, j0, 4) : 0u;
             float s[64], top = -INFINITY;
-            row_scores(p, at + (uint32_t)(half * 64), j0, edge, r, off, s);
+            row_scores(p, at + (uint32_t)(half * 64), j0, edge, QT == 1 && huge, r, off, s);
 #pragma unroll
             for (int e = 0; e < 64; ++e) top = fmaxf(top, s[e]);
             top *= fac;
@@ -603,8 +607,17 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
             if (__any_sync(0xffffffffu, up)) {                    // the same in both warps: each has half of the outputs
                 const float fix = !up ? 1.f : (m == -INFINITY ? 0.f : exp2f(m - top));
                 if (up) { m = top; neg = -top; }
-                huge = __any_sync(0xffffffffu, fabsf(neg) > KV4_HUGE);
                 l *= fix;
+                // From here on x - m of rounded x, as in the other kernel: in this place, where nothing is in a hurry, or, where registers are scarce (two terms a
+                // weight: spills, 8 x 5 rows 34 us -> 42, so 36), in a run of weights of their own (whose branch costs one-term rows 3 %).
+                if (!huge && p.cap_log2 <= 0.f && __any_sync(0xffffffffu, fabsf(neg) > KV4_HUGE)) {
+                    huge = true;
+                    if constexpr (QT == 1) {
+#pragma unroll
+                        for (int e = 0; e < 64; ++e) s[e] *= fac;
+                        fac = 1.f;
+                    }
+                }
                 if (i > 0) {
                     ok = ok && all_wait(err, &pvdone, (uint32_t)((i - 1) & 1));
                     __syncwarp();
@@ -612,14 +625,16 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
                     rescale(lanes + P_O + (uint32_t)(half * (DN / 2)), DN / 2, fix);
                 }
             }
-            if (huge) {                                           // x - m of rounded x then, as in the other kernel
+            uint64_t l2 = pair(0.f, 0.f);
+            if (QT == 2 && huge) {
 #pragma unroll
                 for (int e = 0; e < 64; ++e) s[e] *= fac;
+                weights32<QT>(s, 1.f, neg, at + (uint32_t)(half * 64), l2);
+                weights32<QT>(s + 32, 1.f, neg, at + (uint32_t)(half * 64 + 16), l2);
+            } else {
+                weights32<QT>(s, fac, neg, at + (uint32_t)(half * 64), l2);           // to where the warp's own scores were
+                weights32<QT>(s + 32, fac, neg, at + (uint32_t)(half * 64 + 16), l2);
             }
-            const float by = huge ? 1.f : fac;
-            uint64_t l2 = pair(0.f, 0.f);
-            weights32<QT>(s, by, neg, at + (uint32_t)(half * 64), l2);               // to where the warp's own scores were
-            weights32<QT>(s + 32, by, neg, at + (uint32_t)(half * 64 + 16), l2);
             float la, lb;
             unpair(l2, la, lb);
             l += la + lb;

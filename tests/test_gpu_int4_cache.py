@@ -394,6 +394,21 @@ def test_scores_near_the_end_of_float32(rows, dtype):
     assert (np.abs(got[:a.T] - want) <= ref.bound(want, spread, np.zeros(want.shape[:2]), 128, dtype, 0.0)).all()
 
 
+@pytest.mark.parametrize("rows", [1, 30])
+def test_scores_of_large_keys(rows):
+    """float16 rows over keys of 2^40: scores of 2^42 among zeros"""
+    a = Attend([(300, rows)], 4, 2, 128, 16, "float16", seed=10)
+    x = np.random.default_rng(2).standard_normal((a.c.pages, 2, 16, 128)) * 2.0 ** 40
+    x[:, :, 3] = 0.0
+    words, groups = ref.encode(x.astype(np.float32))
+    flat = a.c.k.reshape(a.c.pages, 2, -1)
+    flat[..., :16 * 64] = words.reshape(a.c.pages, 2, -1).view(np.uint8)
+    flat[..., 16 * 64:] = groups.reshape(a.c.pages, 2, -1).view(np.uint8)
+    a.c.upload()
+    got, (want, spread, _) = a.run(), a.exact()
+    assert (np.abs(got[:a.T] - want) <= ref.bound(want, spread, np.zeros(want.shape[:2]), 128, "float16", 0.0)).all()
+
+
 def test_scores_far_apart_and_all_the_same():
     """one key that takes all the weight, wherever it lies; and queries of zero, whose output is the mean"""
     for at in (0, 63, 64, 150, 299):
