@@ -149,10 +149,10 @@ __global__ void __launch_bounds__(Few<G, NT, DT, W>::THREADS, Few<G, NT, DT, W>:
     if (f0 >= rows || (unsigned)slot >= (unsigned)p.k.slots) return;                       // the whole cluster
     const int live = min(ROWS, rows - f0), i0 = f0 / p.rep, i1 = (f0 + live - 1) / p.rep;
     const int pos0 = ctx - n + i0, pos1 = ctx - n + i1;
-    const int begin = p.window > 0 ? max(0, pos0 - p.window + 1) : 0, end = min(min(pos1 + 1, ctx), p.max_keys);
+    const int begin = kv4_first_key(p, pos0), end = min(min(pos1 + 1, ctx), p.max_keys);
     const int b0 = begin / F_KEYS, nb = max(0, (end + F_KEYS - 1) / F_KEYS - b0);
     const int per = (nb + p.splits - 1) / p.splits, bend = min(nb, (split + 1) * per) + b0;
-    const int lo_max = p.window > 0 ? pos1 - p.window + 1 : 0, hi_min = min(pos0 + 1, end);
+    const int lo_max = kv4_first_key(p, pos1), hi_min = min(pos0 + 1, end);
 
     // ---------------- the ring: 32 keys of K and V, their words behind them
     unsigned char* const ring = smem + (size_t)warp * F_STAGES * STAGE;
@@ -380,7 +380,7 @@ again:
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int key = key0 + 16 * u + 8 * (i >> 1) + gl, last = lim[j][i & 1];
-                        if (key > last || key >= end || (p.window > 0 && key <= last - p.window) || !((have[stage] >> u) & 1u)) s[u][j][i] = -INFINITY;
+                        if (key > last || key >= end || (p.window > 0 && last - key >= p.window) || !((have[stage] >> u) & 1u)) s[u][j][i] = -INFINITY;
                     }
         }
         bool up = false;

@@ -27,6 +27,10 @@ int kv4_prompt(const Kv4AttnParams& p, int dtype, cudaStream_t st);
 
 constexpr float KV4_HUGE = 268435456.f;                            // a reference of 2^28: float32 has steps of 32 there
 
+// The first key that the row of position `pos` sees.  Windows and contexts are any 32-bit numbers, and a sequence may have rows before its position 0:
+// pos - window + 1 of such a row may lie below -2^31, and is not formed.
+__device__ __forceinline__ int kv4_first_key(const Kv4AttnParams& p, int pos) { return p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0; }
+
 // the page that holds the 16 positions n
 __device__ __forceinline__ uint32_t kv4_page_of(const Kv4AttnParams& p, uint32_t n) { return p.page_mul ? __umulhi(n, p.page_mul) >> p.page_shift : n; }
 

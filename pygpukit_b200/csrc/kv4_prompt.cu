@@ -43,7 +43,7 @@ struct Images {
     int32_t* nans;
     int tiles;
 };
-__device__ __forceinline__ int first_tile(const Kv4AttnParams& p, int ctx, int n_rows) { return p.window > 0 ? max(0, ctx - n_rows - p.window + 1) / P_KEYS : 0; }
+__device__ __forceinline__ int first_tile(const Kv4AttnParams& p, int ctx, int n_rows) { return kv4_first_key(p, ctx - n_rows) / P_KEYS; }
 
 template <int G> struct Prompt {
     static constexpr int D = 32 * G, DN = G == 2 ? 64 : 128;       // 96 elements: the products go on to 128 over zeros
@@ -174,7 +174,7 @@ template <int ROWS> struct Block {
         live = work ? min(ROWS, rows - f0) : 0;
         pos0 = ctx - n_rows + f0 / p.rep;
         pos1 = ctx - n_rows + (f0 + max(live, 1) - 1) / p.rep;
-        begin = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
+        begin = kv4_first_key(p, pos0);
         end = work ? min(min(pos1 + 1, ctx), p.max_keys) : 0;
         const int t0 = begin / P_KEYS, nt = max(0, (end + P_KEYS - 1) / P_KEYS - t0), per = (nt + p.splits - 1) / p.splits;
         tbeg = t0 + split * per;
@@ -200,7 +200,7 @@ struct Row {
         pos = b.ctx - b.n_rows + i;
         live = r < b.live && tok >= 0 && tok < p.tokens;
         limit = live ? min(pos, b.end - 1) : -1;
-        under = p.window > 0 ? pos - p.window : -1;
+        under = kv4_first_key(p, pos) - 1;
     }
 };
 // eight query elements in the order of a word's nibbles, as one or two bfloat16 terms
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(IMAGES ? (P_SOFT + 2) * 32 : P_THREADS, 1) kv4
     } else {
         // ---------------- weights
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
-        const int clean_lo = p.window > 0 ? b.pos1 - p.window : -1, clean_hi = missing ? -1 : min(b.pos0, end - 1);
+        const int clean_lo = kv4_first_key(p, b.pos1) - 1, clean_hi = missing ? -1 : min(b.pos0, end - 1);
         float m = -INFINITY, neg = 0.f, l = 0.f, fac = p.cap_log2 > 0.f ? 1.f : p.scale_log2;
         bool ok = true, huge = false;
         for (int i = 0; i < n; ++i) {
