@@ -21,19 +21,24 @@ from ...core.dtypes import float32, int32
 from ...ops.beam import MAX_BEAMS, beam_select
 
 
+class _Sequence:
+    """the name of a beam's sequence in the cache, which no other search has"""
+
+
 @dataclass
 class _Search:
     id: object
     prompt: list[int]
     max_new_tokens: int
     eos: int | None
-    beams: list = field(default_factory=list)          # (score, generated tokens, sequence id)
+    beams: list = field(default_factory=list)          # (score, generated tokens, sequence)
     done: list = field(default_factory=list)           # heap of (what it counts, order, tokens): the worst first
     generated: int = 0
 
 
 class BeamSearch:
-    """`add_request`, then `run`: {request id: [(what it counts, prompt + generated tokens), ...] best first}."""
+    """`add_request`, then `run`: {request id: [(what it counts, prompt + generated tokens), ...] best first}.  Where a step raises, the cache gets
+    the search's sequences back, and the requests that had not come to their end wait again: another `run` searches them from their prompts."""
 
     def __init__(self, model, num_beams: int, length_penalty: float = 1.0):
         if not 1 <= num_beams <= MAX_BEAMS // 2:
@@ -43,7 +48,7 @@ class BeamSearch:
         self.model, self.K, self.penalty = model, int(num_beams), float(length_penalty)
         self.waiting: list[_Search] = []
         self.finished: dict = {}
-        self._ids = itertools.count()
+        self._held: dict = {}                          # sequences that the cache may have
         self._order = itertools.count()
         self._scores: GPUArray | None = None
         self._out = None
@@ -81,6 +86,10 @@ class BeamSearch:
         if len(s.done) > self.K:
             heapq.heappop(s.done)
 
+    def _release(self, seq) -> None:
+        self.model.release(seq)
+        del self._held[seq]
+
     def _advance(self, s: _Search, cand, from_prompt: bool) -> dict:
         """The next beams from a step's candidates (scores, beams, tokens of one group); what the cache is asked for."""
         old = s.beams
@@ -103,7 +112,7 @@ class BeamSearch:
             for score, tokens, _ in s.beams or (() if s.done else old):        # no candidate at all: the beams as they were
                 self._finish(s, score, tokens)
             for b in old:
-                self.model.release(b[2])
+                self._release(b[2])
             best = sorted(s.done, reverse=True)
             self.finished[s.id] = [(c, s.prompt + t) for c, _, t in best]
             s.beams = []
@@ -116,23 +125,35 @@ class BeamSearch:
                 used.add(src)
                 beams.append((score, tokens, src))
             else:
-                new = (s.id, "beam", next(self._ids))
+                new = _Sequence()
                 takes[new] = src
                 beams.append((score, tokens, new))
         s.beams = beams
         for b in old:
             if b[2] not in used:
-                self.model.release(b[2])
+                self._release(b[2])
         return takes
 
     # ------------------------------------------------------------------ the search
     def run(self) -> dict:
         """Search every waiting request to its end, side by side."""
         live, self.waiting = self.waiting, []
+        try:
+            return self._run(live)
+        except BaseException:
+            cache = getattr(self.model, "cache", None)
+            for seq in [q for q in self._held if cache is not None and q in cache.pool]:
+                self.model.release(seq)
+            self._held.clear()
+            self.waiting = [_Search(s.id, s.prompt, s.max_new_tokens, s.eos) for s in live if s.id not in self.finished] + self.waiting
+            raise
+
+    def _run(self, live: list) -> dict:
         if not live:
             return self.finished
         for s in live:
-            s.beams = [(0.0, [], (s.id, "beam", next(self._ids)))]
+            s.beams = [(0.0, [], _Sequence())]
+            self._held[s.beams[0][2]] = None
         n0 = min(2 * self.K, self.model.config.vocab_size)
         entries = [(s.beams[0][2], s.prompt, [len(s.prompt) - 1]) for s in live]
         logits, _ = self.model.step_device(entries)
@@ -145,6 +166,7 @@ class BeamSearch:
             if not live:
                 return self.finished
             if takes:
+                self._held.update(dict.fromkeys(takes))
                 self.model.cache.assign(takes)
             first = False
             # beams that are missing (fewer candidates than K) have a row all the same: the first beam's, at -infinity
