@@ -90,7 +90,7 @@ class BeamSearch:
         self.model.release(seq)
         del self._held[seq]
 
-    def _advance(self, s: _Search, cand, from_prompt: bool) -> dict:
+    def _advance(self, s: _Search, cand) -> dict:
         """The next beams from a step's candidates (scores, beams, tokens of one group); what the cache is asked for."""
         old = s.beams
         s.beams, s.generated = [], s.generated + 1
@@ -157,18 +157,17 @@ class BeamSearch:
         n0 = min(2 * self.K, self.model.config.vocab_size)
         entries = [(s.beams[0][2], s.prompt, [len(s.prompt) - 1]) for s in live]
         logits, _ = self.model.step_device(entries)
-        cands, first = self._select(logits, np.zeros((len(live), 1), np.float32), n0), True
+        cands = self._select(logits, np.zeros((len(live), 1), np.float32), n0)
         while True:
             takes = {}
             for i, s in enumerate(live):
-                takes.update(self._advance(s, [c[i] for c in cands], first))
+                takes.update(self._advance(s, [c[i] for c in cands]))
             live = [s for s in live if s.beams]
             if not live:
                 return self.finished
             if takes:
                 self._held.update(dict.fromkeys(takes))
                 self.model.cache.assign(takes)
-            first = False
             # beams that are missing (fewer candidates than K) have a row all the same: the first beam's, at -infinity
             entries, rows, scores = [], [], np.full((len(live), self.K), -np.inf, np.float32)
             for i, s in enumerate(live):

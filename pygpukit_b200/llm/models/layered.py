@@ -389,13 +389,14 @@ class LayeredCausalModel:
     def generate(self, prompts, max_new_tokens: int = 20, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
                  eos_token_id: int | None = None, prefill_chunk: int | None = None, num_beams: int = 1, length_penalty: float = 1.0) -> list[list[int]]:
         """Generate for one prompt (a list of ints) or several (a list of lists) through the batch scheduler; with num_beams > 1 the best
-        sequence of a beam search (llm/decode/beam.py), which takes whole prompts and no temperature."""
+        sequence of a beam search (llm/decode/beam.py), which takes whole prompts and samples nothing: no
+        temperature, top_k or top_p."""
         from ..decode.ragged import RaggedScheduler
         single = bool(prompts) and isinstance(prompts[0], (int, np.integer))
         if num_beams != 1:
             from ..decode.beam import BeamSearch
-            if temperature != 0.0 or prefill_chunk is not None:
-                raise ValueError("beam search takes no temperature and no prefill_chunk")
+            if temperature != 0.0 or top_k != 0 or top_p != 1.0 or prefill_chunk is not None:
+                raise ValueError("beam search takes no temperature, top_k or top_p, and no prefill_chunk")
             search = BeamSearch(self, num_beams, length_penalty)
             for i, p in enumerate([prompts] if single else prompts):
                 search.add_request(i, list(p), max_new_tokens, eos_token_id)

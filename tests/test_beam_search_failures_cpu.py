@@ -1,10 +1,11 @@
-"""A beam search that does not come to its end: nothing of it stays behind, and it can be run again.  No GPU."""
+"""A beam search that does not come to its end: nothing of it stays behind, and it can be run again; what it refuses.  No GPU."""
 from types import SimpleNamespace
 
 import numpy as np
 import pytest
 
 from pygpukit_b200.llm.decode import beam as beam_mod
+from pygpukit_b200.llm.models.layered import LayeredCausalModel
 from pygpukit_b200.llm.paged_cache import PagePool
 
 V = 7
@@ -102,3 +103,9 @@ def test_searches_name_their_sequences_apart(monkeypatch):
     model.held[(0, "beam", 0)] = [9, 9, 9]
     assert search(model, monkeypatch).run() == want
     assert model.pool.live_sequences == 1 and model.pool.length((0, "beam", 0)) == 3
+
+
+@pytest.mark.parametrize("bad", [dict(temperature=0.7), dict(top_k=5), dict(top_p=0.9), dict(prefill_chunk=16)], ids=str)
+def test_generate_refuses_what_a_search_does_not_do(bad):
+    with pytest.raises(ValueError, match="beam search takes no"):
+        LayeredCausalModel.generate(Model(), [[1, 2]], 3, num_beams=2, **bad)
