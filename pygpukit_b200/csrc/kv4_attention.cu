@@ -35,12 +35,14 @@ namespace {
 constexpr int F_KEYS = 32, F_STAGES = 2, F_CLUSTER = 8;
 constexpr float F_LIFT = 18446744073709551616.f;                   // 2^64
 
-// W warps a block; the rings, or the warps' sums; queries in fragments; sums of queries
+// W warps a block; the rings, and behind them (float32 rows: in their place, afterwards) the warps' sums; queries in fragments; sums of queries
 template <int G, int NT, int DT, int W> struct Few {
     static constexpr int THREADS = W * 32, RESIDENT = G * NT <= 4 ? 16 / W : 8 / W;
     static constexpr int STAGE = F_KEYS * 36 * G;                  // codes of K, of V, words of K, of V
     static constexpr int RINGS = W * F_STAGES * STAGE, FOLD = W * 8 * NT * (32 * G + 4) * 4;
-    static constexpr int FRAG = RINGS > FOLD ? RINGS : FOLD, QSUM = FRAG + G * 2 * NT * (DT == 0 ? 2 : 1) * 256, BYTES = QSUM + G * NT * (DT == 0 ? 2 : 1) * 128;
+    static constexpr bool RUNS = DT != 0;
+    static constexpr int RUN = DT == 1 ? 8 : 16;                   // blocks whose values one accumulator sums: 32 products, with two terms or one
+    static constexpr int SUMS = RUNS ? RINGS : 0, FRAG = RUNS ? RINGS + FOLD : (RINGS > FOLD ? RINGS : FOLD), QSUM = FRAG + G * 2 * NT * (DT == 0 ? 2 : 1) * 256, BYTES = QSUM + G * NT * (DT == 0 ? 2 : 1) * 128;
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -133,7 +135,7 @@ __global__ void __launch_bounds__(Few<G, NT, DT, W>::THREADS, Few<G, NT, DT, W>:
     constexpr int D = 32 * G, DP = D + 4, ROWS = 8 * NT, WARPS = W, THREADS = Smem::THREADS, STAGE = Smem::STAGE;
     constexpr int QT = DT == 0 ? 2 : 1, PT = 3 - DT, MW = (G + 1) / 2;
     // Rows of 16 bits take a byte, c + 16 c' (a bfloat16 too, subnormal or of the first exponent), where they would take its lower four bits, and subtract the
-    // product of the upper ones in the end: one operation in five less.  The difference costs four bits of the sums' 24.
+    // product of the upper ones in the end: one operation in five less.  The difference costs four bits of the sums' 24, which therefore are short ones (RUN).
     constexpr bool BYTES = DT != 0;
     constexpr uint32_t LOW = BYTES ? 0x00ff00ffu : 0x000f000fu;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -266,8 +268,48 @@ __global__ void __launch_bounds__(Few<G, NT, DT, W>::THREADS, Few<G, NT, DT, W>:
             lim[j][c] = lim_s[8 * j + 2 * t + c];
         }
     const uint32_t half_sel = gl & 1 ? 0x7632u : 0x5410u;
-    bool careful = false, huge = false;
+    bool careful = false, huge = false, bad, fresh;
+    // The accumulators into the warp's sums.  A lane has columns 8 j + 2 t + c, elements 32 g + 4 gl ... + 3 of them, and nobody else does before the warps fold.
+    float* const fold = (float*)(smem + Smem::SUMS);               // [WARPS][ROWS][DP]
+    auto sum_at = [&](int j, int c, int g) { return (float4*)(fold + ((size_t)warp * ROWS + 8 * j + 2 * t + c) * DP + 32 * g + 4 * gl); };
+    auto put = [&] {
+        const float even = 5.9029581035870565e20f, odd = 3.6893488147419103e19f;  // 2^133 / 2^64 and 2^129 / 2^64
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            bad |= zac[j][0] != zac[j][0] || zac[j][1] != zac[j][1];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const float z = __shfl_sync(0xffffffffu, zac[j][c], g * 4 + t) * even;
+                    const float a0 = BYTES ? acc[2 * g][j][c] - acc[2 * g][j][2 + c] : acc[2 * g][j][c];
+                    const float a2 = BYTES ? acc[2 * g + 1][j][c] - acc[2 * g + 1][j][2 + c] : acc[2 * g + 1][j][c];
+                    float4 o = make_float4(fmaf(a0, even, -z), fmaf(acc[2 * g][j][2 + c], odd, -z), fmaf(a2, even, -z), fmaf(acc[2 * g + 1][j][2 + c], odd, -z));
+                    float4* const at = sum_at(j, c, g);
+                    if (!fresh) {
+                        const float4 v = *at;
+                        o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+                    }
+                    *at = o;
+                }
+                float sum = l[j][c] * (1.f / F_LIFT);
+#pragma unroll
+                for (int o = 4; o <= 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (gl == 0) wl[warp][8 * j + 2 * t + c] = fresh ? sum : wl[warp][8 * j + 2 * t + c] + sum;
+                l[j][c] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) zac[j][i] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
+        }
+        fresh = false;
+    };
 again:
+    bad = false;
+    fresh = true;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -413,6 +455,18 @@ again:
                 for (int i = 0; i < 2 * G; ++i)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) acc[i][j][c] *= f[c & 1];
+                if (Smem::RUNS && !fresh) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            float4* const at = sum_at(j, c, g);
+                            const float4 v = *at;
+                            *at = make_float4(v.x * f[c], v.y * f[c], v.z * f[c], v.w * f[c]);
+                        }
+                        if (gl == 0) wl[warp][8 * j + 2 * t + c] *= f[c];
+                    }
+                }
             }
             huge = __any_sync(0xffffffffu, huge);
         }
@@ -506,12 +560,17 @@ again:
         };
         if (edge || careful) values(Yes{});
         else values(No{});
+        // Products add into their accumulator truncated.  Over all of a warp's keys that was 4e-3 of an output over 131072 keys (48 sequences, rows of 16 bits), what the
+        // upper codes' sums are subtracted for above all; 32 products at a time leave nothing beside the output's own rounding (float16 2.06e-4 for 2.05e-4).
+        // Time: 64 sequences over 8192 keys 148 -> 151 us; 153 with 16 products at a time.
+        if (Smem::RUNS && (k % Smem::RUN == Smem::RUN - 1 || block + WARPS >= bend)) put();
     }
     cp_async_wait<0>();
-    // The groups' sums of w s z share a product's rows: a scale that is NaN, in one group, would reach the others as 0 NaN.  Then once more, without it there.
-    bool bad = false;
+    if constexpr (!Smem::RUNS) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) bad |= zac[j][0] != zac[j][0] || zac[j][1] != zac[j][1];
+        for (int j = 0; j < NT; ++j) bad |= zac[j][0] != zac[j][0] || zac[j][1] != zac[j][1];
+    }
+    // The groups' sums of w s z share a product's rows: a scale that is NaN, in one group, would reach the others as 0 NaN.  Then once more, without it there.
     if (!careful && __any_sync(0xffffffffu, bad)) {
         careful = true;
         __syncwarp();
@@ -520,31 +579,24 @@ again:
     }
 
     // ---------------- the warps' sums into one
+    if constexpr (!Smem::RUNS) {
+        __syncthreads();                                           // the rings are read
+        put();
+    } else if (fresh) {                                            // a warp without keys
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int g = 0; g < G; ++g) *sum_at(j, c, g) = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (gl == 0) wl[warp][8 * j + 2 * t + c] = 0.f;
+            }
+    }
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int o = 4; o <= 16; o <<= 1) l[j][c] += __shfl_xor_sync(0xffffffffu, l[j][c], o);
-    __syncthreads();                                               // the rings are read
-    float* const fold = (float*)smem;                              // [WARPS][ROWS][DP]
-    const float even = 5.9029581035870565e20f, odd = 3.6893488147419103e19f;      // 2^133 / 2^64 and 2^129 / 2^64
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int col = 8 * j + 2 * t + c;
-            if (gl == 0) { wm[warp][col] = m[j][c]; wl[warp][col] = l[j][c] * (1.f / F_LIFT); }
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const float z = __shfl_sync(0xffffffffu, zac[j][c], g * 4 + t) * even;
-                const float a0 = BYTES ? acc[2 * g][j][c] - acc[2 * g][j][2 + c] : acc[2 * g][j][c];
-                const float a2 = BYTES ? acc[2 * g + 1][j][c] - acc[2 * g + 1][j][2 + c] : acc[2 * g + 1][j][c];
-                const float4 o = make_float4(fmaf(a0, even, -z), fmaf(acc[2 * g][j][2 + c], odd, -z), fmaf(a2, even, -z), fmaf(acc[2 * g + 1][j][2 + c], odd, -z));
-                *(float4*)(fold + ((size_t)warp * ROWS + col) * DP + 32 * g + 4 * gl) = o;
-            }
-        }
-    }
+            if (gl == 0) wm[warp][8 * j + 2 * t + c] = m[j][c];
     __syncthreads();
     if (tid < ROWS) {
         float top = -INFINITY, sum = 0.f;

@@ -3,6 +3,7 @@ prompts whose tiles are made once, with pages, rows and values missing."""
 import numpy as np
 import pytest
 
+from tests import kv4_ref as ref
 from tests.test_gpu_int4_cache import Attend
 
 pytestmark = pytest.mark.gpu
@@ -30,3 +31,81 @@ def test_windows_of_any_size(portions, dtype, window):
     if window > 2 ** 29:
         a.window = 0
         assert np.array_equal(a.run(), got)
+
+
+# ---------------------------------------------------------------------------------------------------- long sums
+class Shared(Attend):
+    """64 decoded tokens over one slot's pages, of unequal contexts: sequences enough that few blocks share one's keys, and a warp adds thousands of them"""
+
+    def __init__(self, ctx, D, rep, dtype, H=8, seed=60):
+        super().__init__([(ctx, 1)], H * rep, H, D, 64, dtype, seed=seed)
+        S = 64
+        self.slots, self.portions = np.repeat(self.slots, S), [(ctx - 7 * i, 1) for i in range(S)]
+        self.starts, self.T = np.arange(S + 1, dtype=np.int32), S
+        factor = np.where(np.arange(S) % 2, 1.0, 0.02)[:, None, None]         # weights that differ, and all alike
+        self.q = ref.rounded(np.random.default_rng(seed + 1).standard_normal((S, H * rep, D)) * factor, dtype)
+
+    def rows(self, arr, h):
+        """one head's values and scales"""
+        got = ref.rows_of(arr[:, h:h + 1], self.c.table, self.slots[0], self.top)
+        return tuple(x[:, 0] for x in got)
+
+    def check(self, got, ignore=None):
+        """`ignore`: a group of elements that is not compared"""
+        q, rep = ref.floats(self.q, self.dtype).astype(np.float64), self.Hq // self.c.H
+        seen = np.arange(self.top) < np.array([c for c, _ in self.portions])[:, None]
+        keep = np.ones(self.D, bool)
+        if ignore is not None:
+            keep[32 * ignore:32 * ignore + 32] = False
+        for h in (0, self.Hq - 1):
+            (k, _), (v, s) = self.rows(self.c.k, h // rep), self.rows(self.c.v, h // rep)
+            x = np.where(seen, q[:, h] @ k.T / np.sqrt(self.D), -np.inf)
+            w = np.exp(x - x.max(1, keepdims=True))
+            w /= w.sum(1, keepdims=True)
+            size = np.where(seen, np.abs(q[:, h]) @ np.abs(k).T, 0).max(1) / np.sqrt(self.D)
+            want, spread = w @ v[:, keep], w @ (15 * s[:, keep])
+            off, tol = np.abs(got[:, h][:, keep] - want), ref.bound(want, spread, size, self.D, self.dtype, 0.0)
+            print(f"worst {(off / tol).max():.3f} of the bound, rms {np.sqrt(np.mean(off ** 2)):.3e} of {np.sqrt(np.mean(want ** 2)):.3e}")
+            assert (off <= tol).all()
+
+
+@pytest.mark.parametrize("ctx,D,rep,dtype", [(65536, 64, 1, "float16"), (65536, 64, 1, "bfloat16"), (20011, 96, 2, "float32"), (30000, 128, 4, "float16")])
+def test_sums_over_many_keys(ctx, D, rep, dtype):
+    """the bound has 32 truncated additions, whatever the context"""
+    a = Shared(ctx, D, rep, dtype)
+    a.check(a.run(False))
+
+
+@pytest.mark.parametrize("D,rep,dtype", [(64, 1, "float16"), (128, 2, "bfloat16"), (128, 4, "float32"), (256, 1, "float16")])
+def test_maxima_that_grow_along_the_context(D, rep, dtype):
+    """references move long after the first sums were put aside"""
+    ctx = 9000
+    a = Shared(ctx, D, rep, dtype)
+    for h in range(8):
+        x = (a.rows(a.c.k, h)[0] * (1 + 40 * np.arange(ctx) / ctx)[:, None]).astype(np.float32)
+        words, groups = ref.encode(x)
+        for page in range(-(-ctx // 64)):
+            n = min(64, ctx - 64 * page)
+            flat = a.c.k[a.c.table[a.slots[0], page], h].reshape(-1)
+            flat[:n * D // 2] = words[64 * page:64 * page + n].reshape(-1).view(np.uint8)
+            flat[32 * D:32 * D + n * D // 16] = np.ascontiguousarray(groups[64 * page:64 * page + n]).reshape(-1).view(np.uint8)
+    a.c.upload()
+    a.check(a.run(False))
+
+
+@pytest.mark.parametrize("at", [0, 5990])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+def test_a_value_that_is_nan_in_a_long_sum(dtype, at):
+    a = Shared(6000, 128, 1, dtype)
+    for h in range(8):
+        page, row = a.c.table[a.slots[0], at // 64], at % 64
+        words, groups = ref.get(a.c.v, page, h, row)
+        groups[1] = ref.NAN_WORD
+        ref.put(a.c.v, page, h, row, words, groups)
+    a.c.upload()
+    got = a.run(False)
+    sees = np.array([c for c, _ in a.portions]) > at
+    nan = np.zeros(got.shape, bool)
+    nan[sees, :, 32:64] = True
+    assert np.array_equal(np.isnan(got), nan)
+    a.check(got, ignore=1)
