@@ -414,6 +414,7 @@ again:
                         else x = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(x * (2.885390043f / p.cap_log2))));
                     }
         }
+        uint32_t unseen = 0;                                       // of this lane's 8 NT (key, row)
         if (edge) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -422,7 +423,10 @@ again:
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int key = key0 + 16 * u + 8 * (i >> 1) + gl, last = lim[j][i & 1];
-                        if (key > last || key >= end || (p.window > 0 && last - key >= p.window) || !((have[stage] >> u) & 1u)) s[u][j][i] = -INFINITY;
+                        if (key > last || key >= end || (p.window > 0 && last - key >= p.window) || !((have[stage] >> u) & 1u)) {
+                            s[u][j][i] = -INFINITY;
+                            unseen |= 1u << ((u * NT + j) * 4 + i);
+                        }
                     }
         }
         bool up = false;
@@ -523,10 +527,10 @@ again:
                         float part[3][4] = {};
                         float (&low)[4] = DT == 0 ? part[0] : acc[2 * g][j], (&high)[4] = DT == 0 ? part[1] : acc[2 * g + 1][j], (&zsum)[4] = DT == 0 ? part[2] : zac[j];
                         float w[4] = {s[u][j][0] * s0, s[u][j][1] * s0, s[u][j][2] * s1, s[u][j][3] * s1};
-                        if constexpr (SPECIAL) {                   // a key that is not seen may have any bytes for a scale
+                        if constexpr (SPECIAL) {                   // a key that is not seen may have any bytes for a scale (one that is, with a weight of zero too, has its NaN)
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                if (s[u][j][i] == 0.f) w[i] = 0.f;
+                                if ((unseen >> ((u * NT + j) * 4 + i)) & 1u) w[i] = 0.f;
                         }
 #pragma unroll
                         for (int term = 0; term < PT; ++term) {

@@ -109,3 +109,23 @@ def test_a_value_that_is_nan_in_a_long_sum(dtype, at):
     nan[sees, :, 32:64] = True
     assert np.array_equal(np.isnan(got), nan)
     a.check(got, ignore=1)
+
+
+@pytest.mark.parametrize("rows,dtype", [(1, "bfloat16"), (1, "float32"), (3, "float16"), (3, "float32"), (60, "bfloat16"), (250, "float16")])
+@pytest.mark.parametrize("at", [40, 296])
+def test_a_nan_under_a_weight_of_zero(rows, dtype, at):
+    """A key whose score is some thousand below the largest is seen all the same: its value's NaN shows, as 0 NaN does, in whatever block of keys it lies"""
+    a = Attend([(300, rows)], 4, 2, 128, 16, dtype, seed=65)
+    one = np.sign(np.random.default_rng(66).standard_normal(128))
+    a.q = ref.rounded(np.broadcast_to(one, a.q.shape), dtype)
+    page, row = a.c.table[a.slots[0], at // 16], at % 16
+    words, groups = ref.encode((-300 * one).astype(np.float32)[None])      # a score of -3394
+    for h in (0, 1):
+        ref.put(a.c.k, page, h, row, words[0], groups[0])
+    words, groups = ref.get(a.c.v, page, 1, row)
+    groups[2] = ref.NAN_WORD
+    ref.put(a.c.v, page, 1, row, words, groups)
+    a.c.upload()
+    nan = np.zeros((a.T + 2, 4, 128), bool)
+    nan[max(0, at - (300 - rows)):rows, 2:, 64:96] = True
+    assert np.array_equal(np.isnan(a.run()), nan)
