@@ -411,7 +411,7 @@ again:
                         float& x = s[u][j][i];
                         x *= fac_s[8 * j + 2 * t + (i & 1)];
                         if constexpr (DT == 0) x = p.cap_log2 * tanhf(x / p.cap_log2);
-                        else x = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(x * (2.885390043f / p.cap_log2))));
+                        else x = p.cap_log2 * (p.cap_log2 > KV4_CAP_WIDE ? kv4_tanh_wide(x * kv4_cap_in(1.f, p.cap_log2)) : kv4_tanh(x * kv4_cap_in(1.f, p.cap_log2)));
                     }
         }
         uint32_t unseen = 0;                                       // of this lane's 8 NT (key, row)
@@ -761,7 +761,7 @@ extern "C" int pgk_kv4_attention(const void* q, long q_ld, const void* k_cache, 
     PGK_REQUIRE(seqs >= 0 && tokens >= 0 && max_rows > 0 && max_context >= 0 && (row_starts || (tokens >= seqs && max_rows == 1)) &&
                     (long long)seqs * max_rows * (heads / kv_heads) <= 0x7fffffffll,
                 "kv4_attention failed: %d sequences of up to %d rows in %d, %d keys", seqs, max_rows, tokens, max_context);
-    PGK_REQUIRE(window >= 0 && softcap >= 0.f && scale == scale, "kv4_attention failed: window %d, cap %g, scale %g", window, softcap, scale);
+    PGK_REQUIRE(window >= 0 && softcap >= 0.f && softcap < 1e38f && scale >= 0.f && scale < 1e38f, "kv4_attention failed: window %d, cap %g, scale %g", window, softcap, scale);
     if (seqs == 0 || tokens == 0) return 0;
     PGK_REQUIRE(q && out && seq_slots && context_lens, "kv4_attention failed: no queries, output, slots or contexts");
     Kv4AttnParams p = {};
@@ -773,7 +773,7 @@ extern "C" int pgk_kv4_attention(const void* q, long q_ld, const void* k_cache, 
     p.max_rows = max_rows < tokens ? max_rows : tokens;
     p.max_keys = max_context < max_pages * page_size ? max_context : max_pages * page_size;
     p.scale_log2 = (scale > 0.f ? scale : 1.f / sqrtf((float)dim)) * 1.4426950408889634f;
-    p.cap_log2 = softcap * 1.4426950408889634f;
+    p.cap_log2 = softcap > 0.f ? fmaxf(softcap, 1e-30f) * 1.4426950408889634f : 0.f;          // (scores within 1e-30 of zero, and a weight of 1, in any case)
     p.window = window; p.sinks = sinks;
     p.head_bytes = (long long)page_size * kv4_row_bytes(dim);
     p.page_bytes = p.head_bytes * kv_heads;

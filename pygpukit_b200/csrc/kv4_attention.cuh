@@ -1,6 +1,7 @@
 // kv4_attention.cuh -- what the kernels of attention over the four-bit cache share: kv4_attention.cu (a few rows a sequence), kv4_prompt.cu (many).
 #pragma once
 #include "kv4.cuh"
+#include "tc_common.cuh"
 
 namespace pgk {
 
@@ -19,6 +20,8 @@ struct Kv4AttnParams {
     long long page_bytes, head_bytes;
 };
 
+constexpr float KV4_CAP_WIDE = 256.f;      // a cap (times log2 e) from which tanh is wanted to float32 of itself, not of 1
+
 // kv4_prompt.cu: whether it serves the call, and the call
 bool kv4_prompt_serves(const Kv4AttnParams& p, int dtype);
 int kv4_prompt(const Kv4AttnParams& p, int dtype, cudaStream_t st);
@@ -33,6 +36,16 @@ __device__ __forceinline__ int kv4_first_key(const Kv4AttnParams& p, int pos) { 
 
 // the page that holds the 16 positions n
 __device__ __forceinline__ uint32_t kv4_page_of(const Kv4AttnParams& p, uint32_t n) { return p.page_mul ? __umulhi(n, p.page_mul) >> p.page_shift : n; }
+
+// A capped score is cap tanh(y), y = z ln 2 / 2 with z the score times kv4_cap_in.  As 1 - 2 / (1 + e^2y) tanh is off by 2^-22 whatever y is: of a cap of KV4_CAP_WIDE
+// (in units of log2 e: 177) that is 6e-5 of a weight, and everything of much wider ones, which take its series below y = 0.3 (to y^9: 5e-8 of it).
+__device__ __forceinline__ float kv4_tanh(float z) { return 1.f - __fdividef(2.f, 1.f + ex2(z)); }
+// (a call: inline it costs every kernel's other paths 1 %, 152 -> 154 us)
+static __device__ __noinline__ float kv4_tanh_wide(float z) {
+    const float y = z * 0.34657359f, y2 = y * y;
+    return fabsf(y) < 0.3f ? fmaf(y * y2, fmaf(y2, fmaf(y2, fmaf(y2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), y) : kv4_tanh(z);
+}
+__device__ __forceinline__ float kv4_cap_in(float scale, float cap) { return fminf(scale * 2.885390043f / cap, 3.4028235e38f); }     // (no infinity that a zero meets)
 
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");

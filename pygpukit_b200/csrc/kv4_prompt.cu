@@ -238,9 +238,9 @@ __device__ __forceinline__ void row_scores(const Kv4AttnParams& p, uint32_t at, 
     for (int c = 0; c < N; c += 16) tmem_pass(*(float (*)[16])(s + c));
     if (p.cap_log2 > 0.f || huge) {
         if (p.cap_log2 > 0.f) {
-            const float in = p.scale_log2 * 2.885390043f / p.cap_log2;
+            const float in = kv4_cap_in(p.scale_log2, p.cap_log2);
 #pragma unroll
-            for (int e = 0; e < N; ++e) s[e] = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(s[e] * in)));
+            for (int e = 0; e < N; ++e) s[e] = p.cap_log2 * kv4_tanh(s[e] * in);
         } else {
 #pragma unroll
             for (int e = 0; e < N; ++e) s[e] *= p.scale_log2;
@@ -747,9 +747,10 @@ int launch_prompt_dim(const Kv4AttnParams& p, cudaStream_t st) {
 
 // More rows than a block of the other kernel has (32 of 64 elements, 16 of more).  Measured there / here (us, 8 heads, 16 and 20 rows): 128 elements, one
 // sequence over 3000 keys 14.2 / 15.6 and 15.6 / 15.5, 8 over 3000 21.7 / 28.0 and 32.1 / 27.9, 32 over 2000 39.4 / 60.7 and 66.5 / 60.8; 64 elements,
-// 32 and 48 rows, 8 over 3000 24.8 / 23.6 and 35.8 / 23.8, 32 over 2000 42.4 / 49.7 and 77.3 / 49.4.
+// 32 and 48 rows, 8 over 3000 24.8 / 23.6 and 35.8 / 23.8, 32 over 2000 42.4 / 49.7 and 77.3 / 49.4.  Caps that want the series of tanh stay there: its code
+// would cost every call here 1 % (76.8 -> 77.5 us, 152.9 -> 154.7).
 bool kv4_prompt_serves(const Kv4AttnParams& p, int dtype) {
-    return dtype != 0 && p.k.dim <= 128 && (long long)p.max_rows * p.rep > (p.k.dim == 64 ? 32 : 16);
+    return dtype != 0 && p.k.dim <= 128 && p.cap_log2 <= KV4_CAP_WIDE && (long long)p.max_rows * p.rep > (p.k.dim == 64 ? 32 : 16);
 }
 int kv4_prompt(const Kv4AttnParams& p, int dtype, cudaStream_t st) { return dtype == 1 ? launch_prompt_dim<1>(p, st) : launch_prompt_dim<2>(p, st); }
 

@@ -125,7 +125,8 @@ def sdpa_paged_int4(Q: GPUArray, k_cache: GPUArray, v_cache: GPUArray, out: GPUA
     scale 0: 1 / sqrt(dim).  window > 0: a row sees itself and the window - 1 positions before it.  softcap > 0: scores become
     softcap tanh(score / softcap).  sinks float32 [heads]: a logit of each head that joins the softmax and carries no value.  A row that sees no key is
     zeros.  out may be Q.  Sums are float32; values are weighed by weights rounded to 8 bits for bfloat16 rows, 16 for float16 and 24 for float32 ones.  Heads of up to
-    128 elements run on the tensor cores' large tiles from 17 rows (33 at 64 elements) a sequence and key head on, bfloat16 and float16."""
+    128 elements run on the tensor cores' large tiles from 17 rows (33 at 64 elements) a sequence and key head on, bfloat16 and float16,
+    without a softcap above 177."""
     name = "sdpa_paged_int4"
     code = float_code(Q._dtype, name)
     shape = Q._shape

@@ -129,3 +129,17 @@ def test_a_nan_under_a_weight_of_zero(rows, dtype, at):
     nan = np.zeros((a.T + 2, 4, 128), bool)
     nan[max(0, at - (300 - rows)):rows, 2:, 64:96] = True
     assert np.array_equal(np.isnan(a.run()), nan)
+
+
+# ---------------------------------------------------------------------------------------------------- caps
+@pytest.mark.parametrize("rows,dtype", [(1, "bfloat16"), (3, "float16"), (3, "float32"), (60, "bfloat16"), (60, "float16"), (250, "bfloat16")])
+@pytest.mark.parametrize("cap", [1e-36, 1e-3, 0.5, 170.0, 180.0, 5000.0, 1e6, 1e30])
+def test_caps_of_any_size(rows, dtype, cap):
+    """Up to KV4_CAP_WIDE (256 units of log2 e: 177) a cap is off by 2^-21 of itself; above, by a score's 2^-20, which the score's own bound has"""
+    a = Attend([(300, rows), (70, min(rows, 50))], 4, 2, 128, 16, dtype, softcap=cap, seed=70, scale=0.7)
+    got = a.run()
+    want, spread, size = a.exact()
+    tol = ref.bound(want, spread, size, 128, dtype, cap if cap < 177 else 0.0)
+    off = np.abs(got[:a.T] - want)
+    print(f"worst {(off / tol).max():.3f} of the bound")
+    assert (off <= tol).all()
