@@ -123,7 +123,7 @@ def sdpa_paged_int4(Q: GPUArray, k_cache: GPUArray, v_cache: GPUArray, out: GPUA
     max_rows on of a sequence and rows behind the last sequence keep their outputs, as do those of a sequence with a negative slot.
 
     scale 0: 1 / sqrt(dim).  window > 0: a row sees itself and the window - 1 positions before it.  softcap > 0: scores become
-    softcap tanh(score / softcap).  sinks float32 [heads]: a logit of each head that joins the softmax and carries no value.  A row that sees no key is
+    softcap tanh(score / softcap).  Both are finite numbers, 1e-37 to 1e38 where they are not 0.  sinks float32 [heads]: a logit of each head that joins the softmax and carries no value.  A row that sees no key is
     zeros.  out may be Q.  Sums are float32; values are weighed by weights rounded to 8 bits for bfloat16 rows, 16 for float16 and 24 for float32 ones.  Heads of up to
     128 elements run on the tensor cores' large tiles from 17 rows (33 at 64 elements) a sequence and key head on, bfloat16 and float16,
     without a softcap above 177."""
@@ -150,6 +150,10 @@ def sdpa_paged_int4(Q: GPUArray, k_cache: GPUArray, v_cache: GPUArray, out: GPUA
         raise ValueError(f"{name}: max_rows {max_rows}, max_context {max_context} out of range ({max_pages} pages of {ps})")
     if window < 0 or not softcap >= 0.0 or not scale >= 0.0:
         raise ValueError(f"{name}: window {window}, softcap {softcap} and scale {scale} must not be negative")
+    for what, x in (("softcap", softcap), ("scale", scale)):
+        if x and not 1e-37 < x < 1e38:
+            raise ValueError(f"{name}: {what} {x} is not 0 or a number that float32 keeps (1e-37 ... 1e38)")
+    window, max_rows = min(window, 2**31 - 1), min(max_rows, max(T, 1))        # no position and no row lies behind
     if sinks is not None and (sinks._shape != (Hq,) or not _is(sinks, float32)):
         raise ValueError(f"{name}: sinks must be float32 [{Hq}], got {sinks.dtype} {sinks.shape}")
     api.kv4_attention(Q._ptr, Hq * D, k_cache._ptr, v_cache._ptr, out._ptr, Hq * D, pages, ps, page_table._ptr, n_slots, max_pages, slots._ptr,
