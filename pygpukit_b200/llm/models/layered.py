@@ -347,6 +347,8 @@ class LayeredCausalModel:
             for seq_id in end:
                 self.cache.release(seq_id)
             return None, 0
+        if self.cache.int4:
+            raise ValueError("the layers read pages of 16 or 32 bits; a cache in four bits is read by the operators of ops/paged.py")
         stream = _st()
         if self._last_stream is None or self._last_stream[0] is not stream:
             api.device_sync()                          # the step before ran on another stream, on the same arrays

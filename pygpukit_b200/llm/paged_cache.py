@@ -21,7 +21,7 @@ from one, some end).  Whole pages are shared and counted; a partly filled one go
 state rows are, by `ops.copy_rows`.  A sequence that was cut back into a shared page gets a copy of its own before it grows again.
 
 Four bits: dtype "int4" keeps uint8 arrays `[pages, kv_heads, page_size, ops.int4_row_bytes(dim)]` for the operators of `ops/paged.py` (keys and
-values of one size, pages of a multiple of 16 positions, no pooled rows).
+values of one size, pages of a multiple of 16 positions, no pooled rows).  The models' layers do not read them: `LayeredCausalModel` refuses such a cache.
 
 Growth: when the free list runs dry the pool doubles (device arrays are reallocated and the old pages copied, page
 numbers stay valid); a page table row grows the same way.  Sizing the pool for the expected number of live tokens up

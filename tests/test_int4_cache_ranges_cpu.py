@@ -1,8 +1,11 @@
 """Arguments at the ends of their types: what a 32-bit call would take for another number is refused, or is the number that it means.  No GPU."""
+from types import SimpleNamespace
+
 import pytest
 
 from pygpukit_b200 import _lib, ops
 from pygpukit_b200.core.dtypes import bfloat16, int32, uint8
+from pygpukit_b200.llm.models.layered import LayeredCausalModel
 from pygpukit_b200.ops import paged
 from tests.test_int4_cache_cpu import arr
 
@@ -39,3 +42,10 @@ def test_the_library_refuses_them_too():
     for bad in (dict(scale=float("inf")), dict(scale=-1.0), dict(softcap=float("inf")), dict(softcap=float("nan")), dict(scale=2e38), dict(softcap=3e38)):
         assert lib.pgk_kv4_attention(*{**good, **bad}.values()) != 0, bad
         assert "kv4_attention failed" in _lib.last_error()
+
+
+def test_a_model_refuses_a_cache_that_its_layers_do_not_read():
+    m = LayeredCausalModel.__new__(LayeredCausalModel)
+    m.cache = SimpleNamespace(int4=True, extend=None)              # nothing is appended before the refusal
+    with pytest.raises(ValueError, match="four bits"):
+        m.step_device([("a", [1, 2], [1])])
