@@ -143,3 +143,111 @@ def test_caps_of_any_size(rows, dtype, cap):
     off = np.abs(got[:a.T] - want)
     print(f"worst {(off / tol).max():.3f} of the bound")
     assert (off <= tol).all()
+
+
+# ---------------------------------------------------------------------------------------------------- prompts: what is not there, in both kinds of tiles
+MANY = [  # rows of the longest sequence, elements, page, type, window: tiles made by the blocks, and (768 rows a key head) made once
+    (40, 128, 16, "bfloat16", 0), (60, 64, 48, "float16", 90), (50, 96, 16, "bfloat16", 33),
+    (200, 128, 16, "float16", 0), (210, 64, 80, "bfloat16", 150), (195, 96, 32, "float16", 0), (230, 128, 64, "bfloat16", 70),
+]
+
+
+def many(rows, D, PS, dtype, window, seed=80):
+    return Attend([(300, rows), (260, 30), (19, 19)], 8, 2, D, PS, dtype, window=window, seed=seed)
+
+
+def masked(a, there):
+    """float64 outputs and their bound over the keys j of sequence s with there[s][j]"""
+    want, tol = np.zeros((a.T, a.Hq, a.D)), np.zeros((a.T, a.Hq, a.D))
+    rep = a.Hq // a.c.H
+    for i, ((ctx, n), slot, at) in enumerate(zip(a.portions, a.slots, a.starts)):
+        k, _ = ref.rows_of(a.c.k, a.c.table % a.c.pages, slot, ctx)
+        v, s = ref.rows_of(a.c.v, a.c.table % a.c.pages, slot, ctx)
+        q = ref.floats(a.q[at:at + n], a.dtype).astype(np.float64)
+        pos, j = np.arange(ctx - n, ctx)[:, None], np.arange(ctx)
+        seen = (j <= pos) & (j > pos - (a.window or ctx + 1)) & there[i]
+        for h in range(a.Hq):
+            x = np.where(seen, q[:, h] @ k[:, h // rep].T / np.sqrt(a.D), -np.inf)
+            top = x.max(1, keepdims=True)
+            w = np.where(seen, np.exp(x - np.where(np.isfinite(top), top, 0.0)), 0.0)
+            w /= np.maximum(w.sum(1, keepdims=True), 1e-300)
+            want[at:at + n, h] = w @ v[:, h // rep]
+            size = np.where(seen, np.abs(q[:, h]) @ np.abs(k[:, h // rep]).T, 0).max(1) / np.sqrt(a.D)
+            tol[at:at + n, h] = ref.bound(want[at:at + n, h], w @ (15 * s[:, h // rep]), size, a.D, a.dtype, 0.0)
+    return want, tol
+
+
+@pytest.mark.parametrize("rows,D,PS,dtype,window", MANY)
+def test_prompts_over_pages_that_do_not_exist(rows, D, PS, dtype, window):
+    a = many(rows, D, PS, dtype, window)
+    there = [np.ones(c, bool) for c, _ in a.portions]
+    for i, slot in enumerate(a.slots):
+        for page, number in ((1, -5), (3, a.c.pages), (0, 2 ** 31 - 1)):      # the first page too: early rows see nothing
+            if page < a.c.table.shape[1]:
+                a.c.table[slot, page] = number
+                there[i][page * PS:(page + 1) * PS] = False
+    a.c.upload()
+    got = a.run()
+    want, tol = masked(a, there)
+    assert (np.abs(got[:a.T] - want) <= tol).all() and (got[a.T:] == 77.0).all()
+
+
+@pytest.mark.parametrize("rows,D,PS,dtype,window", MANY)
+def test_prompts_over_stale_bytes(rows, D, PS, dtype, window):
+    """whatever lies behind a context or before a window, NaN scales among it, leaves the output's bits alone"""
+    a = many(rows, D, PS, dtype, window)
+    clean = a.run()
+    a.check(clean)
+    used = np.zeros((a.c.pages, PS), bool)
+    for (ctx, n), slot in zip(a.portions, a.slots):
+        j = np.arange(max(0, ctx - n - window + 1) if window else 0, ctx)
+        used[a.c.table[slot, j // PS], j % PS] = True
+    for arr in (a.c.k, a.c.v):
+        for page, row in zip(*np.nonzero(~used)):
+            for h in range(2):
+                words, groups = ref.get(arr, page, h, row)
+                ref.put(arr, page, h, row, words, np.full_like(groups, ref.NAN_WORD))
+    a.c.upload()
+    assert np.array_equal(a.run(), clean)
+
+
+@pytest.mark.parametrize("rows,D,PS,dtype,window", MANY)
+@pytest.mark.parametrize("where", ["key", "value"])
+def test_prompts_and_a_nan(where, rows, D, PS, dtype, window):
+    """a NaN in the middle of the rows' own keys reaches the rows behind it, within its window, of its head's group; of a value, its elements alone"""
+    a = many(rows, D, PS, dtype, window)
+    at = 300 - rows + rows // 2
+    arr = a.c.k if where == "key" else a.c.v
+    page, row = a.c.table[a.slots[0], at // PS], at % PS
+    words, groups = ref.get(arr, page, 1, row)
+    groups[1] = ref.NAN_WORD
+    ref.put(arr, page, 1, row, words, groups)
+    a.c.upload()
+    nan = np.zeros((a.T + 2, 8, D), bool)
+    last = min(rows, rows // 2 + window) if window else rows
+    if where == "key":
+        nan[rows // 2:last, 4:] = True
+    else:
+        nan[rows // 2:last, 4:, 32:64] = True
+    assert np.array_equal(np.isnan(a.run()), nan)
+
+
+@pytest.mark.parametrize("rows,D,PS,dtype,window", MANY)
+def test_prompts_of_fewer_rows_than_there_are(rows, D, PS, dtype, window):
+    """rows from max_rows on, sequences without a slot and starts that reach outside: outputs stay, and nothing else changes"""
+    a = many(rows, D, PS, dtype, window)
+    full = a.run()
+    few = rows - 3
+    got = a.run(max_rows=few)
+    keep = np.ones(a.T + 2, bool)
+    keep[few:rows] = False
+    assert np.array_equal(got[keep], full[keep]) and (got[few:rows] == 77.0).all()
+    slots = a.slots.copy()
+    for bad in (-1, 99):
+        a.slots[1] = bad
+        got = a.run()
+        assert (got[rows:rows + 30] == 77.0).all() and np.array_equal(np.delete(got, np.s_[rows:rows + 30], 0), np.delete(full, np.s_[rows:rows + 30], 0))
+    a.slots = slots
+    a.starts = np.array([-4, rows, rows + 30, 2 ** 30], np.int32)
+    got = a.run(max_rows=rows + 10)
+    assert np.isfinite(got).all() and np.array_equal(got[rows:rows + 30], full[rows:rows + 30])
