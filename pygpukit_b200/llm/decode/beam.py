@@ -18,7 +18,7 @@ import numpy as np
 
 from ...core.array import GPUArray
 from ...core.dtypes import float32, int32
-from ...ops.beam import MAX_BEAMS, beam_select
+from ...ops.beam import MAX_BEAMS, MAX_ROWS, beam_select
 
 
 class _Sequence:
@@ -136,10 +136,16 @@ class BeamSearch:
 
     # ------------------------------------------------------------------ the search
     def run(self) -> dict:
-        """Search every waiting request to its end, side by side."""
-        live, self.waiting = self.waiting, []
+        """Search every waiting request to its end, side by side: as many at a time as a selection has rows for."""
+        most = max(1, MAX_ROWS // self.K)
+        while self.waiting:
+            live, self.waiting = self.waiting[:most], self.waiting[most:]
+            self._run_or_wait(live)
+        return self.finished
+
+    def _run_or_wait(self, live: list) -> None:
         try:
-            return self._run(live)
+            self._run(live)
         except BaseException:
             cache = getattr(self.model, "cache", None)
             for seq in [q for q in self._held if cache is not None and q in cache.pool]:
@@ -148,9 +154,7 @@ class BeamSearch:
             self.waiting = [_Search(s.id, s.prompt, s.max_new_tokens, s.eos) for s in live if s.id not in self.finished] + self.waiting
             raise
 
-    def _run(self, live: list) -> dict:
-        if not live:
-            return self.finished
+    def _run(self, live: list) -> None:
         for s in live:
             s.beams = [(0.0, [], _Sequence())]
             self._held[s.beams[0][2]] = None
@@ -164,7 +168,7 @@ class BeamSearch:
                 takes.update(self._advance(s, [c[i] for c in cands]))
             live = [s for s in live if s.beams]
             if not live:
-                return self.finished
+                return
             if takes:
                 self._held.update(dict.fromkeys(takes))
                 self.model.cache.assign(takes)

@@ -10,6 +10,7 @@ from ._common import _st
 from .paged import _is
 
 MAX_BEAMS = 64
+MAX_ROWS = 65535             # groups x beams of a selection
 MAX_VOCAB = 2048000
 
 
@@ -17,7 +18,8 @@ def beam_select(logits: GPUArray, scores: GPUArray, n: int | None = None, *, fin
                 out: "tuple[GPUArray, GPUArray, GPUArray] | None" = None) -> tuple[GPUArray, GPUArray, GPUArray]:
     """The n best continuations of every group of beams.  logits [groups * beams, vocab]; scores float32 [groups, beams], the beams' sums of log
     probabilities.  A candidate (beam k, token v) scores scores[k] + log_softmax(logits[k])[v]; returns (scores float32, beams int32, tokens int32), each
-    [groups, n], best first, ties to the lower beam and then the lower token.  n (default: the number of beams) and beams are 64 at most.
+    [groups, n], best first, ties to the lower beam and then the lower token (of one beam the larger logit comes first, also where the scores round to one number).
+    n (default: the number of beams) and beams are 64 at most, groups * beams 65535.
 
     finished int32 [groups, beams]: a beam with a nonzero entry keeps its score and has one candidate, pad_token.  Other candidates at
     -infinity (logits of -infinity, beams whose score is NaN or below -1e30, rows that hold a NaN or +infinity) come last, in order."""
@@ -30,6 +32,8 @@ def beam_select(logits: GPUArray, scores: GPUArray, n: int | None = None, *, fin
         raise ValueError(f"{name}: logits must be [{B} * {K}, vocab], got {logits.shape}")
     V = logits._shape[1]
     n = K if n is None else int(n)
+    if B * K > MAX_ROWS:
+        raise ValueError(f"{name}: {B} groups of {K} beams ({MAX_ROWS} rows at most)")
     if not 1 <= K <= MAX_BEAMS or not 1 <= n <= min(MAX_BEAMS, K * V):
         raise ValueError(f"{name}: {n} of {K} beams x {V} tokens (beams and candidates are 1 ... {MAX_BEAMS})")
     if finished is not None:

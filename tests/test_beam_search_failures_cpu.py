@@ -4,9 +4,11 @@ from types import SimpleNamespace
 import numpy as np
 import pytest
 
+from pygpukit_b200 import ops
 from pygpukit_b200.llm.decode import beam as beam_mod
 from pygpukit_b200.llm.models.layered import LayeredCausalModel
 from pygpukit_b200.llm.paged_cache import PagePool
+from tests.test_int4_cache_cpu import arr
 
 V = 7
 
@@ -103,6 +105,36 @@ def test_searches_name_their_sequences_apart(monkeypatch):
     model.held[(0, "beam", 0)] = [9, 9, 9]
     assert search(model, monkeypatch).run() == want
     assert model.pool.live_sequences == 1 and model.pool.length((0, "beam", 0)) == 3
+
+
+def test_more_requests_than_a_selection_has_rows_for(monkeypatch):
+    prompts = [[1, 2, 3], [4], [0, 6], [5, 5], [2]]
+    want = search(Model(), monkeypatch, prompts).run()
+    monkeypatch.setattr(beam_mod, "MAX_ROWS", 7)                    # two requests of three beams
+    model = Model()
+    s = search(model, monkeypatch, prompts)
+    inner, seen = s._select, []
+    monkeypatch.setattr(s, "_select", lambda logits, scores, n: (seen.append(scores.size), inner(logits, scores, n))[1])
+    assert s.run() == want and max(seen) == 6 and model.pool.live_sequences == 0
+    failed = 0
+    for call in range(1, 60):                                       # whichever step fails: requests are done, or wait
+        model = Model()
+        model.fails = ("step", call)
+        s = search(model, monkeypatch, prompts)
+        try:
+            s.run()
+            continue
+        except RuntimeError:
+            failed += 1
+        assert len(s.finished) + len(s.waiting) == 5 and model.pool.live_sequences == 0
+        model.fails = None
+        assert s.run() == want
+    assert failed >= 10
+
+
+def test_a_selection_of_too_many_rows_is_refused():
+    with pytest.raises(ValueError, match="beam_select"):
+        ops.beam_select(arr((65536, 10)), arr((16384, 4)))
 
 
 @pytest.mark.parametrize("bad", [dict(temperature=0.7), dict(top_k=5), dict(top_p=0.9), dict(prefill_chunk=16)], ids=str)
