@@ -847,7 +847,8 @@ int pgk_seq_queries_per_tile(int heads, int kv_heads);
  *           rotation.  Rows name different positions.
  *   read:   the values at (row_slots[t], positions[t]) as [tokens][kv_heads][dim], zeros for skipped rows.
  *   attention: sequence s has rows row_starts[s] ... row_starts[s + 1] - 1 of q (row s without row_starts), the last of its context_lens[s]
- *           positions; max_rows and max_context bound both.  window, softcap: 0 for none; sinks float32 [heads] or NULL; scale 0: 1 / sqrt(dim).
+ *           positions; max_rows and max_context bound both.  window, softcap: 0 for none; sinks float32 [heads] or NULL; scale 0: 1 / sqrt(dim); softcap and
+ *           scale below 1e38.
  * dtype: 0 float32, 1 float16, 2 bfloat16 (q, k, v, out). */
 int pgk_kv4_append(void* q, const void* k, const void* v, long q_ld, long k_ld, long v_ld, const float* cos_table, const float* sin_table,
                    int table_rows, int rot, int interleaved, void* k_cache, void* v_cache, int pages, int page_size, const int32_t* page_table,

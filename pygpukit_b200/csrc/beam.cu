@@ -6,9 +6,10 @@
 // their exponentials, and their n best by the key (value, token), which no two share.  Elements below a bound are left out: with k = ceil(n / 8), the
 // smallest of its eight warps' k-th largest per-thread maxima, which at least n elements reach; what passes, some dozens of random logits, is ranked by
 // counting.  Where more pass than the list holds (logits that are all the same, say) the bound is the n-th largest of the 256 per-thread maxima
-// by key, which n threads' elements at most can reach.  A block per group then forms the rows' logarithms and takes the best of the sorted lists'
+// by key, which n threads' elements at most can reach.  A slice's sum is float32 (its 8192 terms: 4e-8 of a score).  A block per group then forms the rows' logarithms and takes the best of the sorted lists'
 // heads n times, in float64, so that beams whose candidates lie within float32 rounding of each other keep their order.
-// Measured: 4 beams of 32768 tokens 8.8 us, 128 of 151936 27.6: 17 for the rows (78 MB, 4.6 TB/s; half of the issue slots), the rest one warp a group over the heads.
+// Measured: 4 beams of 32768 tokens 8.8 to 9.3 us, 128 of 151936 27.6 to 28.4: 17 for the rows (78 MB, 4.6 TB/s; half of the issue slots), the rest one warp a group
+// over the heads.
 #include "common.cuh"
 #include "tc_common.cuh"
 #include "../../include/pgk_b200.h"

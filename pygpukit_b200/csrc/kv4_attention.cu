@@ -8,16 +8,18 @@
 //   * codes go to the tensor cores (mma.sync m16n8k16) as they are.  Four bits in the lowest places of a float16 are c 2^-24, four bits above them c 2^-20,
 //     of a bfloat16 c 2^-133 and c 2^-129: subnormal numbers, which the products take exactly (tested), so that two elements cost one AND.
 //     The query carries 2^-4 where the code carries 2^4, and a power of two that brings its largest element below 2^10 (2^11).
-//   * A is 16 keys of codes, B eight query rows: float16 queries (exact for bfloat16 rows; two terms, 22 bits of the largest, for float32 ones), a
-//     group's sum starts at -z sum q_g, and a group's scale is one multiply-add per (key, row).
+//   * A is 16 keys of codes, B eight query rows: float16 queries (rows of 16 bits: exact for elements above 2^-22 of their row's largest, bfloat16, or 2^-19, float16,
+//     and within 2^-30 of it below; float32 rows: two terms, 22 bits of the largest), a group's sum starts at -z sum q_g, and a group's scale is one
+//     multiply-add per (key, row).
 //   * of the values A is 16 elements by 16 keys -- a lane's bytes of two keys, merged by one permutation --, B the weights times the group's scale and 2^64
 //     (which keeps products with c 2^-133 normal), rounded to bfloat16 once for rows of that type; float16 rows have two such terms, 16 bits (one left
 //     2^-9 of a weight beside an output's own 2^-12), float32 rows three, 24 bits.  The sum of w s z is
 //     a product over the same rounded weights, so that what rounding does to codes of up to 15 is done to (c - z) only.
 //   * S comes out as [key][row] and is needed as [key][row] operand of the other layout: movmatrix, two cycles for 64 numbers.
-// What bounds it: with 64 and more sequences the issue slots, about 270 instructions for 16 keys of 128 elements and 8 rows, where the cache's bytes
-// leave 350 cycles of a scheduler (64 over 8192 keys, 32 / 8 heads of 128: 148 us, 3.6 TB/s); with one, the chain of a launch, a page number, the rows and the
-// fold (4096 keys: 9.4 us).  The same 64 with float16 rows 179 us, with float32 ones 277; of 4096 keys 9.5 and 12.4.
+// What bounds it: with 64 and more sequences instructions, 340 for 16 keys of 128 elements and 8 rows, which would alone be issued in the time that the cache's
+// bytes take (64 over 8192 keys, 64 / 8 heads of 128: 81 us), but are in 149 to 152: a scheduler has one to issue in 61 % of a SM's active cycles (latencies of
+// dependent ones, the integer units 59 % taken), and SMs are active 88 % of the time, with 1024 blocks on 592 places.  With one sequence the chain of a
+// launch, a page number, the rows and the fold (4096 keys: 9.6 us).  The same 64 with float16 rows 190 us, with float32 ones 279.
 // A warp takes 32 keys at a time through a ring of its own in shared memory (cp.async, no barrier among warps), with its own maximum and sums;
 // the warps fold in shared memory, and where a sequence's keys are cut over the blocks of a cluster, these fold through distributed shared memory.
 //

@@ -8,12 +8,12 @@
 //     weights of tile i are waited for; three tiles of K and V are in shared memory;
 //   * eight warps, a lane a row and two warps a row, turn scores into weights; a weight is rounded to bfloat16 once (2^-9 of it, independent from
 //     key to key, beside the output's own 2^-9), for float16 rows to two such terms (2^-17), their sum is float32 of the unrounded ones.  A row's
-//     reference moves when its maximum has grown by 2^8.
+//     reference moves when its maximum has grown by 2^8.  Products add into tensor memory truncated: over 131072 keys an output is small by 1e-4 of itself.
 // The eight elements of a word of codes keep the order (0, 4, 1, 5, 2, 6, 3, 7) that its nibbles fall into: queries are brought into it, outputs back.
 // What bounds it: the chain of a row's warps.  Of 128 x 128 x 128 the products take 512 cycles and the exponentials 1024 of the special unit; measured are 1890 a
 // tile (scores ready, maxima 180 cycles, exchange between a row's warps 240, weights 1160, arrival) where tiles were made before, 2750 where the block
 // makes them (K 800 to 1200, V 800, what lies between 400 each: two warps a scheduler, latency), and 13600 at a block's two ends.  Measured: 512 rows over 16384
-// keys, 32 / 4 heads of 128, 147 to 154 us (0.9 PFLOP/s), 2000 rows over themselves, 32 / 8 heads, 73 to 77 us, 8 sequences of 5 rows over 3000 keys 28 us;
+// keys, 32 / 4 heads of 128, 147 to 154 us (0.9 PFLOP/s), 2000 rows over themselves, 32 / 8 heads, 73 to 78 us, 8 sequences of 5 rows over 3000 keys 28 us;
 // float16 rows, twice the products and a second term a weight, 200, 97 and 36.
 // Few blocks share a sequence's keys within a cluster and fold through distributed shared memory.
 //

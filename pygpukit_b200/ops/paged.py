@@ -122,11 +122,14 @@ def sdpa_paged_int4(Q: GPUArray, k_cache: GPUArray, v_cache: GPUArray, out: GPUA
     without row_starts.  max_context and max_rows bound what the two arrays hold: keys from max_context on are not seen, rows from
     max_rows on of a sequence and rows behind the last sequence keep their outputs, as do those of a sequence with a negative slot.
 
-    scale 0: 1 / sqrt(dim).  window > 0: a row sees itself and the window - 1 positions before it.  softcap > 0: scores become
-    softcap tanh(score / softcap).  Both are finite numbers, 1e-37 to 1e38 where they are not 0.  sinks float32 [heads]: a logit of each head that joins the softmax and carries no value.  A row that sees no key is
-    zeros.  out may be Q.  Sums are float32; values are weighed by weights rounded to 8 bits for bfloat16 rows, 16 for float16 and 24 for float32 ones.  Heads of up to
-    128 elements run on the tensor cores' large tiles from 17 rows (33 at 64 elements) a sequence and key head on, bfloat16 and float16,
-    without a softcap above 177."""
+    scale 0: 1 / sqrt(dim).  window > 0: a row sees itself and the window - 1 positions before it.  softcap > 0: scores become softcap
+    tanh(score / softcap).  Both are finite numbers, 1e-37 to 1e38 where they are not 0.  sinks float32 [heads]: a logit of each head that
+    joins the softmax and carries no value.  A row that sees no key is zeros.  out may be Q.
+
+    Sums are float32; values are weighed by weights rounded to 8 bits for bfloat16 rows, 16 for float16 and 24 for float32 ones (the attention
+    on 16-bit pages keeps 24 for bfloat16 rows too), and float32 queries keep 22 bits of their row's largest element.  Heads of up to 128
+    elements run on the tensor cores' large tiles from 17 rows (33 at 64 elements) a sequence and key head on, bfloat16 and float16, without a
+    softcap above 177; the longest sequence of a call decides for all of it, so that a prompt and many decoded tokens are two calls rather than one."""
     name = "sdpa_paged_int4"
     code = float_code(Q._dtype, name)
     shape = Q._shape
