@@ -68,8 +68,10 @@ def _rows_of(name: str, arrays) -> tuple[int, array, array]:
                 raise ValueError(f"{name}: arrays of {rows} rows, got {a.shape}")
         sizes = array("q", [a.nbytes // max(1, rows) for a in arrays])
     ptrs = [a._ptr for a in arrays]
-    if len(set(ptrs)) < len(ptrs) and first.nbytes:
-        raise ValueError(f"{name}: an array is there twice")
+    if len(set(ptrs)) < len(ptrs):
+        held = [p for p, n in zip(ptrs, sizes) if n]               # arrays without bytes may share an address
+        if len(set(held)) < len(held):
+            raise ValueError(f"{name}: an array is there twice")
     return rows, array("Q", ptrs), sizes
 
 

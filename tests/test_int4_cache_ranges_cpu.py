@@ -44,6 +44,14 @@ def test_the_library_refuses_them_too():
         assert "kv4_attention failed" in _lib.last_error()
 
 
+def test_an_array_is_there_twice_behind_one_without_bytes():
+    x, none = arr((6, 4)), arr((6, 0))
+    with pytest.raises(ValueError, match="twice"):
+        ops.reorder_rows([none, x, x], arr((2, 3), int32))
+    with pytest.raises(ValueError, match="twice"):
+        ops.copy_rows([none, x, arr((6, 2)), x], arr((2,), int32), arr((2,), int32))
+
+
 def test_a_model_refuses_a_cache_that_its_layers_do_not_read():
     m = LayeredCausalModel.__new__(LayeredCausalModel)
     m.cache = SimpleNamespace(int4=True, extend=None)              # nothing is appended before the refusal
