@@ -871,6 +871,41 @@ int pgk_beam_select(const void* logits, long ld, int dtype, const float* scores,
 int pgk_copy_rows(void* const* host_arrays, const int64_t* host_row_bytes, int n_arrays, int rows, const int32_t* src, const int32_t* dst,
                   int pairs, int group, void* stream);
 
+/* ------------------------------------------------------------------ pages of 16 and 32 bits: trees of drafts, weights by position, rows that move (net-new)
+ * A cache is two arrays [pages][kv_heads][page_size][dim] of the queries' type (dtype 0 float32, 1 float16, 2 bfloat16) on 16-byte boundaries behind
+ * page_table int32 [slots][max_pages]; dim a multiple of 8 up to 256, pages of any size.  Sequence s has rows row_starts[s] ... row_starts[s + 1] - 1 of q (row s
+ * without row_starts), the last n of its context_lens[s] positions: step row t lies at position context - n + t.  Row i sees every position before
+ * context - n and the step rows whose bits its mask has: masks int32 [tokens][mask_words], bit t % 32 of word t / 32; NULL: the rows 0 ... i.
+ * max_rows and max_context bound the data.  Slots, positions and page numbers are data of the device: what they place outside the arrays is skipped.
+ *   attention: out[t][h] = softmax(scale q . k) v, zeros for rows that see nothing; lse (or NULL) float32 [tokens][heads], the natural logarithm of the
+ *           scores' exponentials' sum, -infinity for such rows.  scale 0: 1 / sqrt(dim).  out may be q.
+ *   weigh:  weights[slot][g][j] += sum over the sequence's rows and the heads h of g of exp(scale q . k_j - lse), weights float32 [slots][kv_heads][weights_ld].
+ *   select_rows: of a sequence's positions the `first`, the `recent` and those of the largest weights, ties to the lower position, `budget` in all (or the context's),
+ *           ascending: kept int32 [seqs][kv_heads][budget], -1 behind them; counts int32 [seqs].  NaN is the smallest weight.
+ *   move_rows: row starts[s] + i (starts NULL: 0) of a sequence's pages becomes, in place, what row starts[s] + from[i] was, i < counts[s]; from int32 [seqs][width], or
+ *           [seqs][kv_heads][width] with by_head; from[i] >= i, others are skipped.  Arrays [pages][kv_heads][page_size][bytes of a row]; weights (or NULL) float32
+ *           [slots][kv_heads][weights_ld] move along, those behind the last row up to context_lens[s] become zero.
+ *   tree_masks: parents int32 [tokens], the number within its sequence of the row that a row hangs on (smaller than its own; others: a root) -> masks, depths int32.
+ *   accept_tree: rows int32 [seqs][max_rows] (-1 behind counts[s]): row 0, then of a row's children the lowest whose token is the one chosen behind it; next_tokens: what
+ *           is chosen behind the last.  chosen int32 [total], or NULL: the largest logit's index, the lowest of equal ones, NaN never. */
+int pgk_paged_attention(const void* q, long q_ld, const void* k_cache, const void* v_cache, void* out, long o_ld, int pages, int page_size,
+                        const int32_t* page_table, int slots, int max_pages, const int32_t* seq_slots, const int32_t* context_lens,
+                        const int32_t* row_starts, int seqs, int tokens, int max_rows, int max_context, int heads, int kv_heads, int dim,
+                        float scale, const int32_t* masks, int mask_words, float* lse, int dtype, void* stream);
+int pgk_paged_weigh(const void* q, long q_ld, const void* k_cache, const float* lse, float* weights, long weights_ld, int pages, int page_size,
+                    const int32_t* page_table, int slots, int max_pages, const int32_t* seq_slots, const int32_t* context_lens,
+                    const int32_t* row_starts, int seqs, int tokens, int max_rows, int max_context, int heads, int kv_heads, int dim, float scale,
+                    const int32_t* masks, int mask_words, int dtype, void* stream);
+int pgk_select_rows(const float* weights, long weights_ld, const int32_t* seq_slots, const int32_t* context_lens, int seqs, int slots, int kv_heads,
+                    int max_context, int budget, int first, int recent, int32_t* kept, int32_t* counts, void* stream);
+int pgk_move_rows(void* const* host_arrays, const int32_t* host_row_bytes, int n_arrays, const int32_t* page_table, int pages, int page_size,
+                  int slots, int max_pages, int kv_heads, const int32_t* seq_slots, const int32_t* starts, const int32_t* from, const int32_t* counts,
+                  int seqs, int width, int by_head, float* weights, long weights_ld, const int32_t* context_lens, void* stream);
+int pgk_tree_masks(const int32_t* parents, const int32_t* row_starts, int seqs, int tokens, int max_rows, int words, int32_t* masks, int32_t* depths,
+                   void* stream);
+int pgk_accept_tree(const void* logits, long ld, int dtype, int vocab, const int32_t* chosen, const int32_t* tokens, const int32_t* parents,
+                    const int32_t* row_starts, int seqs, int total, int max_rows, int32_t* rows, int32_t* counts, int32_t* next_tokens, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -193,6 +193,13 @@ _SIGS = {
     "pgk_kv4_attention": [vp, cl, vp, vp, vp, cl, i32, i32, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, i32, f32, vp, i32, vp],
     "pgk_beam_select": [vp, cl, i32, vp, vp, i32, i32, i32, i32, i32, vp, vp, vp, vp],
     "pgk_copy_rows": [vp, vp, i32, i32, vp, vp, i32, i32, vp],
+    # pages of 16 and 32 bits (paged_few.cu, paged_tc.cu, paged_f32.cu, paged_weigh.cu, paged_rows.cu) and trees of drafts (tree.cu)
+    "pgk_paged_attention": [vp, cl, vp, vp, vp, cl, i32, i32, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, vp, i32, vp, i32, vp],
+    "pgk_paged_weigh": [vp, cl, vp, vp, vp, cl, i32, i32, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, vp, i32, i32, vp],
+    "pgk_select_rows": [vp, cl, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp],
+    "pgk_move_rows": [vp, vp, i32, vp, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, i32, i32, vp, cl, vp, vp],
+    "pgk_tree_masks": [vp, vp, i32, i32, i32, i32, vp, vp, vp],
+    "pgk_accept_tree": [vp, cl, i32, i32, vp, vp, vp, vp, i32, i32, i32, vp, vp, vp, vp],
 }
 _RESTYPE = {"pgk_last_error": C.c_char_p, "pgk_launch_count": i64, "pgk_launch_count_reset": None,
             "pgk_sdpa_workspace_bytes": sz, "pgk_p2p_handle_bytes": sz, "pgk_p2p_ready": i32,

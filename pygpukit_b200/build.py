@@ -65,6 +65,12 @@ SOURCES = {
     "kv4_attention.cu": [],
     "kv4_prompt.cu": [],
     "beam.cu": [],
+    "paged_few.cu": [],
+    "paged_tc.cu": [],
+    "paged_f32.cu": [],
+    "paged_weigh.cu": [],
+    "paged_rows.cu": [],
+    "tree.cu": [],
 }
 
 # groups of sources that link on their own (runtime.cu is in every library)

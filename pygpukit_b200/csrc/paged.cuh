@@ -1,0 +1,233 @@
+// paged.cuh -- a key / value cache of 16 or 32 bits in pages [pages][kv_heads][page_size][dim] behind a page table [slots][pages of a slot], and the steps of
+// sequences that attend over it: what paged_few.cu, paged_tc.cu, paged_f32.cu (attention) and paged_weigh.cu (weights by position) share.
+//
+// A sequence has n rows of the queries, which are the last n of its context's positions: step row t lies at position context - n + t.  Row i sees every position
+// before context - n and, of the step's, those whose bit is set in its mask, or without masks the rows 0 ... i.  Slots, contexts, row starts and page numbers are
+// data of the device: whatever they say, nothing outside the arrays is touched.
+#pragma once
+#include "common.cuh"
+
+namespace pgk {
+
+struct PagedParams {
+    const void* q; void* out;
+    long q_ld, o_ld;                      // elements
+    const void* k_data; const void* v_data;
+    const int32_t* table;
+    int pages, page_size, slots, max_pages, kv_heads, dim;
+    const int32_t* seq_slots; const int32_t* contexts; const int32_t* starts;      // starts NULL: a row a sequence
+    int seqs, tokens, max_rows, max_keys, heads, rep, tiles, splits;
+    float scale_log2;                     // scale log2 e
+    const int32_t* masks;                 // [tokens][words], or NULL
+    int words;
+    float* lse;                           // [tokens][heads] natural logarithms, or NULL
+    float* weights; long weights_ld;      // paged_weigh.cu: [slots][kv_heads][weights_ld]
+    bool wide_q, wide_o;                  // rows on 16-byte boundaries
+    uint32_t page_mul, page_shift;        // n / page_size = hi(n page_mul) >> page_shift for n < 2^31; page_mul 0: pages of one position
+};
+
+// paged_tc.cu: whether it serves the call, and the call; paged_few.cu: what it does not; paged_f32.cu
+bool paged_tc_serves(const PagedParams& p, int dtype);
+int paged_tc(const PagedParams& p, int dtype, cudaStream_t st);
+int paged_few(const PagedParams& p, int dtype, cudaStream_t st);
+int paged_f32(const PagedParams& p, cudaStream_t st);
+
+constexpr int PAGED_CLUSTER = 16;         // blocks that share a sequence's keys, at most
+
+// Blocks of a cluster that share a sequence's keys, `step` of them a warp and turn: time in turns, a block's own with about `ends` of them for what it spends at its
+// two ends, or the SMs' share of all blocks.
+inline int paged_cut(const PagedParams& p, long long items, int step, int warps, int resident, float ends, int most) {
+    const int nb = (p.max_keys + step - 1) / step;
+    int best = 1;
+    float least = 0.f;
+    for (int s = 1; s <= most; s *= 2) {
+        const float each = (float)(((nb + s - 1) / s + warps - 1) / warps) + ends, all = (float)(items * s) * each / (float)(sm_count() * resident);
+        const float cost = each > all ? each : all;
+        if (s == 1 || cost < least) { best = s; least = cost; }
+    }
+    return best;
+}
+
+// blocks of a cluster along z, and the launch that waits for the kernel before it
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_clusters(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = grid.z;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    count_launch();
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+#ifdef __CUDACC__
+
+constexpr float PAGED_LOG2E = 1.4426950408889634f, PAGED_LN2 = 0.6931471805599453f, PAGED_LAZY = 8.f;
+
+__device__ __forceinline__ uint32_t paged_page_of(const PagedParams& p, uint32_t n) { return p.page_mul ? __umulhi(n, p.page_mul) >> p.page_shift : n; }
+
+// A block's rows -- ROWS of one sequence's, a token's query heads of one key head beside each other -- and the keys that they see between them, cut over the blocks of a
+// cluster in units of UNIT keys.
+template <int ROWS, int UNIT> struct PagedBlock {
+    int seq, head, split, slot, ctx, first, n_rows, f0, live, base, end, ubeg, uend;       // base: the position of the step's row 0
+    const int32_t* table;
+    __device__ __forceinline__ PagedBlock(const PagedParams& p, int item, int head_, int split_) : head(head_), split(split_) {
+        seq = item % p.seqs;
+        f0 = (p.tiles - 1 - item / p.seqs) * ROWS;
+        slot = __ldcg(p.seq_slots + seq);
+        ctx = max(0, __ldcg(p.contexts + seq));
+        first = p.starts ? __ldcg(p.starts + seq) : seq;
+        n_rows = p.starts ? max(0, __ldcg(p.starts + seq + 1) - first) : 1;
+        const int rows = min(n_rows, p.max_rows) * p.rep;                                // fits: checked by the host
+        const bool work = f0 < rows && (unsigned)slot < (unsigned)p.slots && ctx > 0;
+        live = f0 < rows && (unsigned)slot < (unsigned)p.slots ? min(ROWS, rows - f0) : 0;
+        base = ctx - n_rows;                                                             // may lie before position 0: those rows have no key
+        const int last = p.masks ? ctx : base + (f0 + max(live, 1) - 1) / p.rep + 1;      // behind the last key that a row sees
+        end = work ? max(0, min(min(last, ctx), p.max_keys)) : 0;
+        const int nu = (end + UNIT - 1) / UNIT, per = (nu + p.splits - 1) / p.splits;
+        ubeg = min(nu, split * per);
+        uend = min(nu, ubeg + per);
+        table = p.table + (work ? (size_t)slot * p.max_pages : 0);
+    }
+    // the cache row (of dim elements) that holds position j of the head, or -1
+    __device__ __forceinline__ int row_of(const PagedParams& p, int j) const {
+        if (j < 0 || j >= end) return -1;
+        const uint32_t pg = paged_page_of(p, (uint32_t)j);
+        const int page = __ldcg(table + pg);
+        if ((unsigned)page >= (unsigned)p.pages) return -1;
+        return (page * p.kv_heads + head) * p.page_size + (j - (int)(pg * (uint32_t)p.page_size));
+    }
+    __device__ __forceinline__ int token(const PagedParams& p, int r) const { return first + (f0 + r) / p.rep; }
+};
+
+// Whether step row i sees step row t
+__device__ __forceinline__ bool paged_sees(const PagedParams& p, int tok, int i, int t) {
+    if (!p.masks) return t <= i;
+    return (unsigned)tok < (unsigned)p.tokens && t < 32 * p.words && ((uint32_t)__ldcg(p.masks + (size_t)tok * p.words + (t >> 5)) >> (t & 31)) & 1u;
+}
+// of step rows t ... t + 31 the ones that row i sees; those before the step (t < 0) all
+__device__ __forceinline__ uint32_t paged_window(const PagedParams& p, int tok, int i, int t) {
+    if (t <= -32) return 0xffffffffu;
+    if (!p.masks) return t > i ? 0u : (i - t >= 31 ? 0xffffffffu : (2u << (i - t)) - 1u);
+    if ((unsigned)tok >= (unsigned)p.tokens) return 0u;        // nobody's row
+    const int32_t* row = p.masks + (size_t)tok * p.words;
+    const int w = t >> 5;                                     // floor
+    const uint32_t lo = w < 0 ? 0xffffffffu : (w < p.words ? (uint32_t)__ldcg(row + w) : 0u);
+    const uint32_t hi = w + 1 < p.words ? (uint32_t)__ldcg(row + w + 1) : 0u;
+    return __funnelshift_r(lo, hi, (uint32_t)t & 31u);
+}
+
+__device__ __forceinline__ void paged_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t paged_remote(uint32_t at, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float paged_remote_float(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 paged_remote_float4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+template <int DT> __device__ __forceinline__ uint32_t paged_pack2(float lo, float hi) {
+    if constexpr (DT == 1) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else
+        return pack_bf16x2(lo, hi);
+}
+template <int DT> __device__ __forceinline__ float paged_float(const void* base, size_t at) {
+    if constexpr (DT == 0) return __ldcg((const float*)base + at);
+    else if constexpr (DT == 1) return __half2float(__ushort_as_half(ld_act2((const uint16_t*)base + at)));
+    else return bf16_bits_to_f32(ld_act2((const uint16_t*)base + at));
+}
+// an infinity or NaN among the two 16-bit numbers of a word: those halves' bits
+template <int DT> __device__ __forceinline__ uint32_t paged_unfinite(uint32_t w) {
+    constexpr uint32_t E = DT == 1 ? 0x7c00u : 0x7f80u;
+    return ((w & E) == E ? 0xffffu : 0u) | ((w & (E << 16)) == (E << 16) ? 0xffff0000u : 0u);
+}
+// 2^(s - m) for a reference that is not there yet (m = -infinity)
+__device__ __forceinline__ float paged_neg(float m) { return m == -INFINITY ? 0.f : -m; }
+
+// The end of every kernel: a row's outputs 4 piece ... 4 piece + 3 are divided by the sum and written; the piece's first thread writes the row's logarithm.  `bad`: values
+// among the step's rows that are not finite were taken as zero, since a weight of zero times them would reach rows that do not see them; the rows that do add them here.
+template <int ROWS, int UNIT, int DT>
+__device__ __forceinline__ void paged_finish(const PagedParams& p, const PagedBlock<ROWS, UNIT>& b, int r, int d, float4 o, float top, float sum, bool bad) {
+    const int f = b.f0 + r, i = f / p.rep, tok = b.first + i, h = b.head * p.rep + f - i * p.rep;
+    if (tok < 0 || tok >= p.tokens) return;
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+    if (d == 0 && p.lse) p.lse[(size_t)tok * p.heads + h] = sum > 0.f || sum != sum ? (top + log2f(sum)) * PAGED_LN2 : -INFINITY;
+    if (d >= p.dim) return;
+    if (bad) {
+        for (int j = max(0, b.base); j < b.end; ++j) {
+            if (!paged_sees(p, tok, i, j - b.base)) continue;
+            const int row = b.row_of(p, j);
+            if (row < 0) continue;
+            float* x = &o.x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float v = paged_float<DT>(p.v_data, (size_t)row * p.dim + d + e);
+                if (!(fabsf(v) < INFINITY)) x[e] += v;
+            }
+        }
+    }
+    const size_t at = (size_t)tok * p.o_ld + (size_t)h * p.dim + d;
+    if constexpr (DT == 0) {
+        float* dst = (float*)p.out + at;
+        if (p.wide_o) *(float4*)dst = o;
+        else { dst[0] = o.x; dst[1] = o.y; dst[2] = o.z; dst[3] = o.w; }
+    } else {
+        uint16_t* dst = (uint16_t*)p.out + at;
+        const uint32_t x = paged_pack2<DT>(o.x, o.y), y = paged_pack2<DT>(o.z, o.w);
+        if (p.wide_o) *(uint2*)dst = make_uint2(x, y);
+        else { dst[0] = (uint16_t)x; dst[1] = (uint16_t)(x >> 16); dst[2] = (uint16_t)y; dst[3] = (uint16_t)(y >> 16); }
+    }
+}
+
+// The cluster's blocks into one: `fold` [ROWS][DF floats] with row_m (log2), row_l, and whether a value was taken as zero; block r has every `splits`-th piece.
+template <int ROWS, int UNIT, int DT>
+__device__ __forceinline__ void paged_fold(const PagedParams& p, const PagedBlock<ROWS, UNIT>& b, const float* fold, int DF, const float* row_m, const float* row_l,
+                                           const int* flag) {
+    if (p.splits > 1) paged_cluster_sync();
+    else __syncthreads();
+    const uint32_t fold_at = smem_u32(fold), m_at = smem_u32(row_m), l_at = smem_u32(row_l), flag_at = smem_u32(flag);
+    const int pieces = (p.dim + 3) / 4;
+    bool bad = false;
+    if (b.live > 0)
+        for (int s = 0; s < p.splits; ++s) bad |= __float_as_int(paged_remote_float(paged_remote(flag_at, s))) != 0;
+    for (int i = b.split * (int)blockDim.x + (int)threadIdx.x; i < b.live * pieces; i += p.splits * (int)blockDim.x) {
+        const int r = i / pieces, d = (i - r * pieces) * 4;
+        float top = -INFINITY, sum = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < p.splits; ++s) top = fmaxf(top, paged_remote_float(paged_remote(m_at + 4 * r, s)));
+        for (int s = 0; s < p.splits; ++s) {
+            const float ms = paged_remote_float(paged_remote(m_at + 4 * r, s)), ls = paged_remote_float(paged_remote(l_at + 4 * r, s));
+            const float w = ms == -INFINITY ? ls - ls : exp2f(ms - top);         // no maximum: nothing seen, or all NaN, which the sum knows
+            const float4 v = paged_remote_float4(paged_remote(fold_at + (r * DF + d) * 4, s));
+            sum = fmaf(w, ls, sum);
+            o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
+        }
+        paged_finish<ROWS, UNIT, DT>(p, b, r, d, o, top, sum, bad);
+    }
+    if (p.splits > 1) paged_cluster_sync();        // nobody leaves while another reads
+}
+
+#endif  // __CUDACC__
+
+}  // namespace pgk

@@ -1,0 +1,277 @@
+// paged_rows.cu -- the positions of a cache that stay when it is cut, and rows of the pages that move together.
+//
+// Selection.  Of a sequence's positions the first, the recent and the ones of the largest weights stay, per key head, `budget` in all, in ascending order.  A block has one head: a
+// weight is an ordered 32-bit number, the least that stays is found digit by digit (11, 11 and 10 bits, a histogram each), then every warp counts what stays of its run of
+// positions and writes it behind what the warps before it have.  Bound by its five passes' latencies, 4 bytes a position being little.
+//
+// Moving.  Row start + i of a sequence becomes, in place, what row start + from[i] was, from[i] >= i.  What is written lies before everything that is still to be read, from[i'] >= i' > i,
+// but for the rows that are moved at the same time: a tile's rows are read by all of the cluster before any is written, and the next tile's are on their way
+// meanwhile.  Bound by memory.
+#include "paged.cuh"
+#include "../../include/pgk_b200.h"
+
+namespace pgk {
+
+namespace {
+
+constexpr int C_THREADS = 1024, C_WARPS = C_THREADS / 32, C_BINS = 2048;
+
+struct SelectParams {
+    const float* weights; long ld;
+    const int32_t* seq_slots; const int32_t* contexts;
+    int slots, kv_heads, budget, first, recent, most;
+    int32_t* kept; int32_t* counts;
+};
+
+// a float's order as a number; the positions that stay in any case above all, NaN below all, one zero
+__device__ __forceinline__ uint32_t ordered(float x) {
+    if (x != x) return 0u;
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(C_THREADS) select_kernel(const __grid_constant__ SelectParams p) {
+    __shared__ int bins[C_BINS], part[C_WARPS], over[C_WARPS], same[C_WARPS];
+    __shared__ int found, left;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.x, seq = blockIdx.y;
+    griddep_wait();
+    griddep_launch();
+    const int slot = __ldcg(p.seq_slots + seq);
+    const bool there = (unsigned)slot < (unsigned)p.slots;
+    const int ctx = there ? min(max(0, __ldcg(p.contexts + seq)), p.most) : 0, count = min(ctx, p.budget);
+    int32_t* const kept = p.kept + ((size_t)seq * p.kv_heads + head) * p.budget;
+    if (head == 0 && tid == 0) p.counts[seq] = count;
+    for (int i = count + tid; i < p.budget; i += C_THREADS) kept[i] = -1;
+    if (ctx <= p.budget) {
+        for (int i = tid; i < count; i += C_THREADS) kept[i] = i;
+        return;
+    }
+    const float* const w = p.weights + ((size_t)slot * p.kv_heads + head) * p.ld;
+    const int recent = ctx - p.recent;
+    auto key = [&](int j) { return j < p.first || j >= recent ? 0xffffffffu : ordered(__ldcg(w + j)); };
+    // the least key that stays: digit by digit, `left` of those that share the digits so far
+    uint32_t least = 0;
+    int need = count;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), width = pass == 2 ? 10 : 11;
+        const uint32_t above = pass == 0 ? 0u : 0xffffffffu << (shift + width);
+        for (int i = tid; i < C_BINS; i += C_THREADS) bins[i] = 0;
+        __syncthreads();
+        for (int j = tid; j < ctx; j += C_THREADS) {
+            const uint32_t x = key(j);
+            if ((x & above) == least) atomicAdd(&bins[(x >> shift) & ((1u << width) - 1u)], 1);
+        }
+        __syncthreads();
+        // the bin with the need-th from above: thread i has bins 2 i and 2 i + 1
+        const int hi = bins[2 * tid + 1], lo = bins[2 * tid], mine = hi + lo;
+        int sum = mine;                                       // of this lane and the ones after it
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const int got = __shfl_down_sync(0xffffffffu, sum, x);
+            if (lane + x < 32) sum += got;
+        }
+        if (lane == 0) part[warp] = sum;
+        __syncthreads();
+        int after = 0;
+        for (int i = warp + 1; i < C_WARPS; ++i) after += part[i];
+        const int over_hi = after + sum - mine;               // keys in higher bins
+        if (over_hi < need && need <= over_hi + mine) {
+            const bool upper = need <= over_hi + hi;
+            found = 2 * tid + (upper ? 1 : 0);
+            left = need - over_hi - (upper ? 0 : hi);
+        }
+        __syncthreads();
+        least |= (uint32_t)found << shift;
+        need = left;
+    }
+    // a warp's run of positions, 32 at a time: those above the least, and the first `need` of its equals
+    const int run = ((ctx + C_WARPS - 1) / C_WARPS + 31) & ~31, from = warp * run, to = min(ctx, from + run);
+    int n_over = 0, n_same = 0;
+    for (int j = from; j < to; j += 32) {
+        const uint32_t x = j + lane < to ? key(j + lane) : 0u;
+        n_over += __popc(__ballot_sync(0xffffffffu, j + lane < to && x > least));
+        n_same += __popc(__ballot_sync(0xffffffffu, j + lane < to && x == least));
+    }
+    if (lane == 0) { over[warp] = n_over; same[warp] = n_same; }
+    __syncthreads();
+    int at = 0, seen = 0;
+    for (int i = 0; i < warp; ++i) {
+        at += over[i] + min(same[i], max(0, need - seen));
+        seen += same[i];
+    }
+    for (int j = from; j < to; j += 32) {
+        const uint32_t x = j + lane < to ? key(j + lane) : 0u;
+        const uint32_t eq = __ballot_sync(0xffffffffu, j + lane < to && x == least), below = (1u << lane) - 1u;
+        const bool stays = j + lane < to && (x > least || (x == least && seen + __popc(eq & below) < need));
+        const uint32_t all = __ballot_sync(0xffffffffu, stays);
+        if (stays) kept[at + __popc(all & below)] = j + lane;
+        at += __popc(all);
+        seen += __popc(eq);
+    }
+}
+
+constexpr int M_THREADS = 256, M_UNITS = 8, M_ARRAYS = 128, M_CLUSTER = 8;
+
+struct MoveParams {
+    void* arrays[M_ARRAYS];
+    int bytes[M_ARRAYS];                  // of a row
+    int n;
+    const int32_t* table;
+    int pages, page_size, slots, max_pages, kv_heads;
+    const int32_t* seq_slots; const int32_t* starts;
+    const int32_t* from; const int32_t* counts;
+    int width, by_head;                   // from [sequences][kv_heads if by_head][width]
+    float* weights; long weights_ld;      // moved as well, [slots][kv_heads][weights_ld]; what is behind the last row up to the context becomes zero
+    const int32_t* contexts;
+    uint32_t page_mul, page_shift;
+};
+
+template <int V> struct Unit;
+template <> struct Unit<16> { using T = uint4; };
+template <> struct Unit<4> { using T = uint32_t; };
+template <> struct Unit<2> { using T = uint16_t; };
+__device__ __forceinline__ uint4 load_unit(const uint4* p) { return ld_act16(p); }
+__device__ __forceinline__ uint32_t load_unit(const uint32_t* p) { return __ldcg(p); }
+__device__ __forceinline__ uint16_t load_unit(const uint16_t* p) { return ld_act2(p); }
+
+template <int V>
+__global__ void __launch_bounds__(M_THREADS) move_kernel(const __grid_constant__ MoveParams p) {
+    using T = typename Unit<V>::T;
+    const int tid = threadIdx.x, rank = blockIdx.x, blocks = gridDim.x, array = blockIdx.y / p.kv_heads, head = blockIdx.y - array * p.kv_heads, seq = blockIdx.z;
+    griddep_wait();
+    griddep_launch();
+    const int slot = __ldcg(p.seq_slots + seq);
+    const bool there = (unsigned)slot < (unsigned)p.slots;                // the same in all of the cluster
+    const int count = there ? max(0, min(__ldcg(p.counts + seq), p.width)) : 0, start = p.starts ? __ldcg(p.starts + seq) : 0;
+    const int32_t* const from = p.from + ((size_t)seq * (p.by_head ? p.kv_heads : 1) + (p.by_head ? head : 0)) * p.width;
+    const int32_t* const table = p.table + (there ? (size_t)slot * p.max_pages : 0);
+    auto gather = [&](auto unit, int units, auto place) {                 // rows of `units` units; place(position): its first unit, or NULL
+        using U = decltype(unit);
+        const long long total = (long long)count * units;
+        const int tiles = (int)((total + (long long)M_THREADS * M_UNITS * blocks - 1) / ((long long)M_THREADS * M_UNITS * blocks));
+        U now[M_UNITS], then[M_UNITS];
+        U* to[M_UNITS];
+        U* to_then[M_UNITS];
+        auto read = [&](int tile, U (&x)[M_UNITS], U* (&at)[M_UNITS]) {
+#pragma unroll
+            for (int q = 0; q < M_UNITS; ++q) {
+                const long long e = (((long long)tile * blocks + rank) * M_UNITS + q) * M_THREADS + tid;
+                at[q] = nullptr;
+                if (e >= total) continue;
+                const int i = (int)(e / units), c = (int)(e - (long long)i * units), f = __ldcg(from + i);
+                if (f <= i) continue;                                     // in its place; or before it, where nothing is moved from
+                U* const src = place((long long)start + f);
+                U* const dst = place((long long)start + i);
+                if (!src || !dst) continue;
+                x[q] = load_unit(src + c);
+                at[q] = dst + c;
+            }
+        };
+        if (tiles > 0) read(0, now, to);
+        for (int t = 0; t < tiles; ++t) {
+            if (t + 1 < tiles) read(t + 1, then, to_then);
+            if (blocks > 1) paged_cluster_sync();
+            else __syncthreads();
+#pragma unroll
+            for (int q = 0; q < M_UNITS; ++q) {
+                if (to[q]) *to[q] = now[q];
+                now[q] = then[q];
+                to[q] = to_then[q];
+            }
+        }
+    };
+    if (array < p.n) {
+        const int bytes = p.bytes[array];
+        char* const base = (char*)p.arrays[array];
+        gather(T{}, bytes / V, [&](long long j) -> T* {
+            if (j < 0 || j >= (long long)p.max_pages * p.page_size) return nullptr;
+            const uint32_t pg = p.page_mul ? __umulhi((uint32_t)j, p.page_mul) >> p.page_shift : (uint32_t)j;
+            const int page = __ldcg(table + pg);
+            if ((unsigned)page >= (unsigned)p.pages) return nullptr;
+            return (T*)(base + (((size_t)page * p.kv_heads + head) * p.page_size + ((int)j - (int)(pg * (uint32_t)p.page_size))) * bytes);
+        });
+        return;
+    }
+    if (!there) return;
+    float* const w = p.weights + ((size_t)slot * p.kv_heads + head) * p.weights_ld;
+    gather(uint32_t{}, 1, [&](long long j) { return j >= 0 && j < p.weights_ld ? (uint32_t*)(w + j) : nullptr; });
+    if (blocks > 1) paged_cluster_sync();          // all rows are read
+    else __syncthreads();
+    const long long end = min((long long)__ldcg(p.contexts + seq), (long long)p.weights_ld);
+    for (long long j = max(0ll, (long long)start + count) + rank * M_THREADS + tid; j < end; j += blocks * M_THREADS) w[j] = 0.f;
+}
+
+}  // namespace
+
+}  // namespace pgk
+
+using namespace pgk;
+
+extern "C" int pgk_select_rows(const float* weights, long weights_ld, const int32_t* seq_slots, const int32_t* context_lens, int seqs, int slots, int kv_heads, int max_context,
+                               int budget, int first, int recent, int32_t* kept, int32_t* counts, void* stream) {
+    PGK_REQUIRE(seqs >= 0 && seqs <= 65535 && slots > 0 && kv_heads > 0 && max_context >= 0 && weights_ld >= max_context, "select_rows failed: %d sequences, %d slots of %d heads, %d of %ld positions",
+                seqs, slots, kv_heads, max_context, weights_ld);
+    PGK_REQUIRE(budget > 0 && first >= 0 && recent >= 0 && (long long)first + recent <= budget, "select_rows failed: a budget of %d with %d first and %d recent positions", budget, first, recent);
+    if (seqs == 0) return 0;
+    PGK_REQUIRE(weights && seq_slots && context_lens && kept && counts, "select_rows failed: an array is missing");
+    SelectParams p = {weights, weights_ld, seq_slots, context_lens, slots, kv_heads, budget, first, recent, max_context, kept, counts};
+    PGK_CUDA(launch_waiting(select_kernel, dim3(kv_heads, seqs), dim3(C_THREADS), 0, (cudaStream_t)stream, p));
+    return 0;
+}
+
+extern "C" int pgk_move_rows(void* const* host_arrays, const int32_t* host_row_bytes, int n_arrays, const int32_t* page_table, int pages, int page_size, int slots, int max_pages,
+                             int kv_heads, const int32_t* seq_slots, const int32_t* starts, const int32_t* from, const int32_t* counts, int seqs, int width, int by_head, float* weights,
+                             long weights_ld, const int32_t* context_lens, void* stream) {
+    PGK_REQUIRE(n_arrays >= 0 && pages > 0 && page_size > 0 && slots > 0 && max_pages > 0 && kv_heads > 0 && seqs >= 0 && seqs <= 65535 && width >= 0 && weights_ld >= 0,
+                "move_rows failed: %d arrays of %d pages of %d positions, %d slots of %d pages, %d heads, %d sequences", n_arrays, pages, page_size, slots, max_pages, kv_heads, seqs);
+    PGK_REQUIRE((long long)pages * kv_heads * page_size <= 0x7fffffffll && (long long)max_pages * page_size <= 0x7fffffffll && (long long)kv_heads * (M_ARRAYS + 1) <= 65535,
+                "move_rows failed: too many rows or heads");
+    if (seqs == 0 || (width == 0 && !weights) || (n_arrays == 0 && !weights)) return 0;
+    PGK_REQUIRE(page_table && seq_slots && from && counts && (n_arrays == 0 || (host_arrays && host_row_bytes)) && (!weights || context_lens), "move_rows failed: an array is missing");
+    MoveParams p = {};
+    p.table = page_table; p.pages = pages; p.page_size = page_size; p.slots = slots; p.max_pages = max_pages; p.kv_heads = kv_heads;
+    p.seq_slots = seq_slots; p.starts = starts; p.from = from; p.counts = counts; p.width = width; p.by_head = by_head;
+    p.weights_ld = weights_ld; p.contexts = context_lens;
+    if (page_size > 1) {
+        uint32_t log = 0;
+        while ((1ull << log) < (uint64_t)page_size) ++log;
+        p.page_shift = log - 1;
+        p.page_mul = (uint32_t)((1ull << (31 + log)) / (uint64_t)page_size + 1);
+    }
+    const cudaStream_t st = (cudaStream_t)stream;
+    for (int a0 = 0; a0 < n_arrays || (a0 == 0 && n_arrays == 0); a0 += M_ARRAYS) {
+        p.n = n_arrays - a0 < M_ARRAYS ? n_arrays - a0 : M_ARRAYS;
+        int unit = 16, most = 0;
+        for (int a = 0; a < p.n; ++a) {
+            p.arrays[a] = host_arrays[a0 + a];
+            p.bytes[a] = host_row_bytes[a0 + a];
+            PGK_REQUIRE(p.arrays[a] && p.bytes[a] > 0 && p.bytes[a] % 2 == 0, "move_rows failed: rows of %d bytes", p.bytes[a]);
+            while ((p.bytes[a] | (uintptr_t)p.arrays[a]) % unit) unit = unit == 16 ? 4 : 2;
+            most = p.bytes[a] > most ? p.bytes[a] : most;
+        }
+        const bool last = a0 + M_ARRAYS >= n_arrays;
+        p.weights = last ? weights : nullptr;
+        // blocks that share a head's rows: as many as there are SMs for, none with less than a tile
+        const long long items = (long long)(p.n + (p.weights ? 1 : 0)) * kv_heads * seqs, tile = (long long)M_THREADS * M_UNITS * unit;
+        int blocks = 1;
+        while (blocks < M_CLUSTER && items * blocks * 2 <= 4 * sm_count() && (long long)width * most > tile * blocks) blocks *= 2;
+        const dim3 grid(blocks, (unsigned)((p.n + (p.weights ? 1 : 0)) * kv_heads), (unsigned)seqs);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(M_THREADS);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = (unsigned)blocks;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+        count_launch();
+        PGK_CUDA(unit == 16 ? cudaLaunchKernelEx(&cfg, move_kernel<16>, p) : (unit == 4 ? cudaLaunchKernelEx(&cfg, move_kernel<4>, p) : cudaLaunchKernelEx(&cfg, move_kernel<2>, p)));
+        if (last) break;
+    }
+    return 0;
+}

@@ -7,5 +7,7 @@ from .matmul import *  # noqa: F401,F403
 from .moe import *  # noqa: F401,F403
 from .nn import *  # noqa: F401,F403
 from .paged import *  # noqa: F401,F403
+from .paged_rows import *  # noqa: F401,F403
 from .sampling import *  # noqa: F401,F403
 from .tensor import *  # noqa: F401,F403
+from .tree import *  # noqa: F401,F403
