@@ -164,30 +164,8 @@ template <int DT> __device__ __forceinline__ uint32_t paged_unfinite(uint32_t w)
 // 2^(s - m) for a reference that is not there yet (m = -infinity)
 __device__ __forceinline__ float paged_neg(float m) { return m == -INFINITY ? 0.f : -m; }
 
-// The end of every kernel: a row's outputs 4 piece ... 4 piece + 3 are divided by the sum and written; the piece's first thread writes the row's logarithm.  `bad`: values
-// among the step's rows that are not finite were taken as zero, since a weight of zero times them would reach rows that do not see them; the rows that do add them here.
-template <int ROWS, int UNIT, int DT>
-__device__ __forceinline__ void paged_finish(const PagedParams& p, const PagedBlock<ROWS, UNIT>& b, int r, int d, float4 o, float top, float sum, bool bad) {
-    const int f = b.f0 + r, i = f / p.rep, tok = b.first + i, h = b.head * p.rep + f - i * p.rep;
-    if (tok < 0 || tok >= p.tokens) return;
-    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
-    if (d == 0 && p.lse) p.lse[(size_t)tok * p.heads + h] = sum > 0.f || sum != sum ? (top + log2f(sum)) * PAGED_LN2 : -INFINITY;
-    if (d >= p.dim) return;
-    if (bad) {
-        for (int j = max(0, b.base); j < b.end; ++j) {
-            if (!paged_sees(p, tok, i, j - b.base)) continue;
-            const int row = b.row_of(p, j);
-            if (row < 0) continue;
-            float* x = &o.x;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float v = paged_float<DT>(p.v_data, (size_t)row * p.dim + d + e);
-                if (!(fabsf(v) < INFINITY)) x[e] += v;
-            }
-        }
-    }
-    const size_t at = (size_t)tok * p.o_ld + (size_t)h * p.dim + d;
+// A row's outputs d ... d + 3, rounded and written
+template <int DT> __device__ __forceinline__ void paged_put(const PagedParams& p, size_t at, float4 o) {
     if constexpr (DT == 0) {
         float* dst = (float*)p.out + at;
         if (p.wide_o) *(float4*)dst = o;
@@ -200,30 +178,89 @@ __device__ __forceinline__ void paged_finish(const PagedParams& p, const PagedBl
     }
 }
 
-// The cluster's blocks into one: `fold` [ROWS][DF floats] with row_m (log2), row_l, and whether a value was taken as zero; block r has every `splits`-th piece.
-template <int ROWS, int UNIT, int DT>
-__device__ __forceinline__ void paged_fold(const PagedParams& p, const PagedBlock<ROWS, UNIT>& b, const float* fold, int DF, const float* row_m, const float* row_l,
-                                           const int* flag) {
+// What the cluster's blocks need to become one: shared memory beside the sums [ROWS][DN + 4]
+template <int ROWS> struct PagedFold {
+    float m[ROWS], l[ROWS];               // a block's references (log2) and sums
+    int bad;                              // whether a value of the step's rows that is not finite was taken as zero
+    float factor[PAGED_CLUSTER][ROWS];    // what a block's sums are multiplied by
+    long long at[ROWS];                   // where a row's outputs go, below 0: nowhere
+};
+
+// The end of every kernel: block r of the cluster has every `splits`-th of its rows' pieces of four elements.  `bad`: values among the step's rows that are not finite were
+// taken as zero, since a weight of zero times them would reach rows that do not see them; the rows that do add them here.
+template <int ROWS, int UNIT, int DT, int DN>
+__device__ __forceinline__ void paged_fold(const PagedParams& p, const PagedBlock<ROWS, UNIT>& b, const float* sums, PagedFold<ROWS>& f) {
+    constexpr int PIECES = DN / 4;
     if (p.splits > 1) paged_cluster_sync();
     else __syncthreads();
-    const uint32_t fold_at = smem_u32(fold), m_at = smem_u32(row_m), l_at = smem_u32(row_l), flag_at = smem_u32(flag);
-    const int pieces = (p.dim + 3) / 4;
     bool bad = false;
-    if (b.live > 0)
-        for (int s = 0; s < p.splits; ++s) bad |= __float_as_int(paged_remote_float(paged_remote(flag_at, s))) != 0;
-    for (int i = b.split * (int)blockDim.x + (int)threadIdx.x; i < b.live * pieces; i += p.splits * (int)blockDim.x) {
-        const int r = i / pieces, d = (i - r * pieces) * 4;
-        float top = -INFINITY, sum = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < p.splits; ++s) top = fmaxf(top, paged_remote_float(paged_remote(m_at + 4 * r, s)));
-        for (int s = 0; s < p.splits; ++s) {
-            const float ms = paged_remote_float(paged_remote(m_at + 4 * r, s)), ls = paged_remote_float(paged_remote(l_at + 4 * r, s));
-            const float w = ms == -INFINITY ? ls - ls : exp2f(ms - top);         // no maximum: nothing seen, or all NaN, which the sum knows
-            const float4 v = paged_remote_float4(paged_remote(fold_at + (r * DF + d) * 4, s));
-            sum = fmaf(w, ls, sum);
-            o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
+    for (int s = 0; s < p.splits; ++s) bad |= __float_as_int(paged_remote_float(paged_remote(smem_u32(&f.bad), s))) != 0;
+    for (int r = (int)threadIdx.x; r < ROWS; r += (int)blockDim.x) {
+        const int x = b.f0 + r, i = x / p.rep, tok = b.first + i, h = b.head * p.rep + x - i * p.rep;
+        const bool live = r < b.live && tok >= 0 && tok < p.tokens;
+        float top = -INFINITY, sum = 0.f, ms[PAGED_CLUSTER], ls[PAGED_CLUSTER];
+        const uint32_t m_at = smem_u32(&f.m[r]), l_at = smem_u32(&f.l[r]);
+#pragma unroll
+        for (int s = 0; s < PAGED_CLUSTER; ++s) {
+            ms[s] = -INFINITY;
+            ls[s] = 0.f;
+            if (s < p.splits) {
+                ms[s] = paged_remote_float(paged_remote(m_at, s));
+                ls[s] = paged_remote_float(paged_remote(l_at, s));
+            }
         }
-        paged_finish<ROWS, UNIT, DT>(p, b, r, d, o, top, sum, bad);
+#pragma unroll
+        for (int s = 0; s < PAGED_CLUSTER; ++s) top = fmaxf(top, ms[s]);
+#pragma unroll
+        for (int s = 0; s < PAGED_CLUSTER; ++s) {
+            ms[s] = ms[s] == -INFINITY ? ls[s] - ls[s] : exp2f(ms[s] - top);           // no maximum: nothing seen, or all NaN, which the sum knows
+            sum = fmaf(ms[s], ls[s], sum);
+        }
+        const bool any = sum > 0.f || sum != sum;
+        const float inv = any ? 1.f / sum : 0.f;
+#pragma unroll
+        for (int s = 0; s < PAGED_CLUSTER; ++s)
+            if (s < p.splits) f.factor[s][r] = ms[s] * inv;
+        f.at[r] = live ? (long long)tok * p.o_ld + (long long)h * p.dim : -1ll;
+        if (live && p.lse && b.split == 0) p.lse[(size_t)tok * p.heads + h] = any ? (top + log2f(sum)) * PAGED_LN2 : -INFINITY;
+    }
+    __syncthreads();
+    const uint32_t sums_at = smem_u32(sums);
+    for (int i = b.split * (int)blockDim.x + (int)threadIdx.x; i < b.live * PIECES; i += p.splits * (int)blockDim.x) {
+        const int r = i / PIECES, d = (i - r * PIECES) * 4;
+        const long long at = f.at[r];
+        if (at < 0 || d >= p.dim) continue;
+        float4 o;
+        if (p.splits == 1) {
+            const float w = f.factor[0][r];
+            const float4 v = *(const float4*)(sums + r * (DN + 4) + d);
+            o = make_float4(w * v.x, w * v.y, w * v.z, w * v.w);
+        } else {
+            o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+            for (int s0 = 0; s0 < p.splits; s0 += 2) {                     // two and more: a power of two
+                const uint32_t from = sums_at + (uint32_t)(r * (DN + 4) + d) * 4u;
+                const float4 u = paged_remote_float4(paged_remote(from, s0)), v = paged_remote_float4(paged_remote(from, s0 + 1));
+                const float wu = f.factor[s0][r], wv = f.factor[s0 + 1][r];
+                o.x = fmaf(wu, u.x, o.x); o.y = fmaf(wu, u.y, o.y); o.z = fmaf(wu, u.z, o.z); o.w = fmaf(wu, u.w, o.w);
+                o.x = fmaf(wv, v.x, o.x); o.y = fmaf(wv, v.y, o.y); o.z = fmaf(wv, v.z, o.z); o.w = fmaf(wv, v.w, o.w);
+            }
+        }
+        if (bad) {
+            const int step = (b.f0 + r) / p.rep;
+            for (int j = max(0, b.base); j < b.end; ++j) {
+                if (!paged_sees(p, b.first + step, step, j - b.base)) continue;
+                const int row = b.row_of(p, j);
+                if (row < 0) continue;
+                float* x = &o.x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float v = paged_float<DT>(p.v_data, (size_t)row * p.dim + d + e);
+                    if (!(fabsf(v) < INFINITY)) x[e] += v;
+                }
+            }
+        }
+        paged_put<DT>(p, (size_t)at + d, o);
     }
     if (p.splits > 1) paged_cluster_sync();        // nobody leaves while another reads
 }

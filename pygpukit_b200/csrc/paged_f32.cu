@@ -24,7 +24,7 @@ __device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, b
 template <int R, int PC, int W> struct Single {
     static int warp_floats(int D) { return S_KEYS * (D + 4) + S_KEYS * D + R * S_KEYS; }
     static int bytes(int D) {
-        const int run = (R * D + W * warp_floats(D)) * 4, fold = W * R * (D + 4) * 4;
+        const int run = (R * D + W * warp_floats(D)) * 4, fold = W * R * (128 * PC + 4) * 4;
         return run > fold ? run : fold;
     }
 };
@@ -32,14 +32,14 @@ template <int R, int PC, int W> struct Single {
 template <int R, int PC, int W>
 __global__ void __launch_bounds__(W * 32, 1) paged_f32_kernel(const __grid_constant__ PagedParams p) {
     extern __shared__ __align__(16) float smf[];
-    __shared__ float wm[W][R], wl[W][R], row_m[R], row_l[R];
-    __shared__ int flag;
+    __shared__ float wm[W][R], wl[W][R];
+    __shared__ PagedFold<R> f;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), D = p.dim, D4 = D / 4, DF = D + 4;
     float* const qs = smf;                                    // [R][D]
     float* const ks = qs + R * D + warp * (S_KEYS * DF + S_KEYS * D + R * S_KEYS);
     float* const vs = ks + S_KEYS * DF;
     float* const ps = vs + S_KEYS * D;                        // [R][32]
-    if (tid == 0) flag = 0;
+    if (tid == 0) f.bad = 0;
     griddep_wait();
     griddep_launch();
     const PagedBlock<R, S_KEYS> b(p, (int)blockIdx.x, (int)blockIdx.y, (int)blockIdx.z);
@@ -66,8 +66,8 @@ __global__ void __launch_bounds__(W * 32, 1) paged_f32_kernel(const __grid_const
         fetch(p.v_data, vs, D, rows);
     }
     for (int i = tid; i < R * D; i += W * 32) {
-        const int r = i / D, f = b.f0 + r, tok = b.first + f / p.rep;
-        qs[i] = r < b.live && tok >= 0 && tok < p.tokens ? __ldcg((const float*)p.q + (size_t)tok * p.q_ld + (size_t)(b.head * p.rep + f % p.rep) * D + (i - r * D)) : 0.f;
+        const int r = i / D, x = b.f0 + r, tok = b.first + x / p.rep;
+        qs[i] = r < b.live && tok >= 0 && tok < p.tokens ? __ldcg((const float*)p.q + (size_t)tok * p.q_ld + (size_t)(b.head * p.rep + x % p.rep) * D + (i - r * D)) : 0.f;
     }
     __syncthreads();
 
@@ -113,11 +113,11 @@ __global__ void __launch_bounds__(W * 32, 1) paged_f32_kernel(const __grid_const
             }
             const float top = warp_max(x);
             if (top > m[r] + PAGED_LAZY) {                    // the same in all lanes; also the first finite maximum
-                const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top);
+                const float fix = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top);
                 m[r] = top;
-                l[r] *= f;
+                l[r] *= fix;
 #pragma unroll
-                for (int c = 0; c < PC; ++c) { o[r][c].x *= f; o[r][c].y *= f; o[r][c].z *= f; o[r][c].w *= f; }
+                for (int c = 0; c < PC; ++c) { o[r][c].x *= fix; o[r][c].y *= fix; o[r][c].z *= fix; o[r][c].w *= fix; }
             }
             const float w = ex2(x + paged_neg(m[r]));
             l[r] += w;
@@ -166,43 +166,44 @@ __global__ void __launch_bounds__(W * 32, 1) paged_f32_kernel(const __grid_const
     cp_async_wait<0>();
 
     // ---------------- the warps' sums into one
-    if (bad) flag = 1;
+    if (bad) f.bad = 1;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         l[r] = warp_sum(l[r]);
         if (lane == 0) { wm[warp][r] = m[r]; wl[warp][r] = l[r]; }
     }
     __syncthreads();
-    float* const fold = smf;                                  // [W][R][DF]
+    float* const fold = smf;                                  // [W][R][FS]
+    constexpr int FS = 128 * PC + 4;
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int c = 0; c < PC; ++c)
-            if (lane + 32 * c < D4) *(float4*)(fold + (warp * R + r) * DF + 4 * (lane + 32 * c)) = o[r][c];
+            if (lane + 32 * c < D4) *(float4*)(fold + (warp * R + r) * FS + 4 * (lane + 32 * c)) = o[r][c];
     __syncthreads();
     if (tid < R) {
         float top = -INFINITY, sum = 0.f;
         for (int w = 0; w < W; ++w) top = fmaxf(top, wm[w][tid]);
         for (int w = 0; w < W; ++w) {
-            const float f = wm[w][tid] == -INFINITY ? wl[w][tid] - wl[w][tid] : exp2f(wm[w][tid] - top);
-            sum = fmaf(wl[w][tid], f, sum);
-            wm[w][tid] = f;
+            const float x = wm[w][tid] == -INFINITY ? wl[w][tid] - wl[w][tid] : exp2f(wm[w][tid] - top);
+            sum = fmaf(wl[w][tid], x, sum);
+            wm[w][tid] = x;
         }
-        row_m[tid] = top;
-        row_l[tid] = sum;
+        f.m[tid] = top;
+        f.l[tid] = sum;
     }
     __syncthreads();
     for (int i = tid; i < b.live * D4; i += W * 32) {
         const int r = i / D4, d = (i - r * D4) * 4;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int w = 0; w < W; ++w) {
-            const float f = wm[w][r];
-            const float4 v = *(const float4*)(fold + (w * R + r) * DF + d);
-            x.x = fmaf(f, v.x, x.x); x.y = fmaf(f, v.y, x.y); x.z = fmaf(f, v.z, x.z); x.w = fmaf(f, v.w, x.w);
+            const float y = wm[w][r];
+            const float4 v = *(const float4*)(fold + (w * R + r) * FS + d);
+            x.x = fmaf(y, v.x, x.x); x.y = fmaf(y, v.y, x.y); x.z = fmaf(y, v.z, x.z); x.w = fmaf(y, v.w, x.w);
         }
-        *(float4*)(fold + r * DF + d) = x;
+        *(float4*)(fold + r * FS + d) = x;
     }
-    paged_fold<R, S_KEYS, 0>(p, b, fold, DF, row_m, row_l, &flag);
+    paged_fold<R, S_KEYS, 0, 128 * PC>(p, b, fold, f);
 }
 
 template <int R, int PC, int W>

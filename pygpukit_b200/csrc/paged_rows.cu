@@ -111,12 +111,11 @@ __global__ void __launch_bounds__(C_THREADS) select_kernel(const __grid_constant
     }
 }
 
-constexpr int M_THREADS = 256, M_UNITS = 8, M_ARRAYS = 128, M_CLUSTER = 8;
+constexpr int M_THREADS = 256, M_UNITS = 8, M_TILE = M_THREADS * M_UNITS, M_ARRAYS = 192, M_CLUSTER = 8;
 
 struct MoveParams {
     void* arrays[M_ARRAYS];
-    int bytes[M_ARRAYS];                  // of a row
-    int n;
+    int n, bytes, chunk;                  // arrays, bytes of a row, arrays of a block
     const int32_t* table;
     int pages, page_size, slots, max_pages, kv_heads;
     const int32_t* seq_slots; const int32_t* starts;
@@ -135,69 +134,107 @@ __device__ __forceinline__ uint4 load_unit(const uint4* p) { return ld_act16(p);
 __device__ __forceinline__ uint32_t load_unit(const uint32_t* p) { return __ldcg(p); }
 __device__ __forceinline__ uint16_t load_unit(const uint16_t* p) { return ld_act2(p); }
 
+// A block has a head of a sequence in `chunk` arrays.  Rows of a tile: their places, looked up while the tile before is on its way, are the same in all arrays, and with
+// few rows several arrays' make a tile.
 template <int V>
-__global__ void __launch_bounds__(M_THREADS) move_kernel(const __grid_constant__ MoveParams p) {
+__global__ void __launch_bounds__(M_THREADS, 3) move_kernel(const __grid_constant__ MoveParams p) {
     using T = typename Unit<V>::T;
-    const int tid = threadIdx.x, rank = blockIdx.x, blocks = gridDim.x, array = blockIdx.y / p.kv_heads, head = blockIdx.y - array * p.kv_heads, seq = blockIdx.z;
+    __shared__ int2 places[2][M_TILE];                        // of a tile's rows: from, to; from below 0: in its place, or not at all
+    const int tid = threadIdx.x, rank = blockIdx.x, blocks = gridDim.x, chunk = blockIdx.y / p.kv_heads, head = blockIdx.y - chunk * p.kv_heads, seq = blockIdx.z;
     griddep_wait();
     griddep_launch();
     const int slot = __ldcg(p.seq_slots + seq);
     const bool there = (unsigned)slot < (unsigned)p.slots;                // the same in all of the cluster
     const int count = there ? max(0, min(__ldcg(p.counts + seq), p.width)) : 0, start = p.starts ? __ldcg(p.starts + seq) : 0;
     const int32_t* const from = p.from + ((size_t)seq * (p.by_head ? p.kv_heads : 1) + (p.by_head ? head : 0)) * p.width;
-    const int32_t* const table = p.table + (there ? (size_t)slot * p.max_pages : 0);
-    auto gather = [&](auto unit, int units, auto place) {                 // rows of `units` units; place(position): its first unit, or NULL
-        using U = decltype(unit);
-        const long long total = (long long)count * units;
-        const int tiles = (int)((total + (long long)M_THREADS * M_UNITS * blocks - 1) / ((long long)M_THREADS * M_UNITS * blocks));
-        U now[M_UNITS], then[M_UNITS];
-        U* to[M_UNITS];
-        U* to_then[M_UNITS];
-        auto read = [&](int tile, U (&x)[M_UNITS], U* (&at)[M_UNITS]) {
-#pragma unroll
-            for (int q = 0; q < M_UNITS; ++q) {
-                const long long e = (((long long)tile * blocks + rank) * M_UNITS + q) * M_THREADS + tid;
-                at[q] = nullptr;
-                if (e >= total) continue;
-                const int i = (int)(e / units), c = (int)(e - (long long)i * units), f = __ldcg(from + i);
-                if (f <= i) continue;                                     // in its place; or before it, where nothing is moved from
-                U* const src = place((long long)start + f);
-                U* const dst = place((long long)start + i);
-                if (!src || !dst) continue;
-                x[q] = load_unit(src + c);
-                at[q] = dst + c;
-            }
-        };
-        if (tiles > 0) read(0, now, to);
-        for (int t = 0; t < tiles; ++t) {
-            if (t + 1 < tiles) read(t + 1, then, to_then);
-            if (blocks > 1) paged_cluster_sync();
-            else __syncthreads();
-#pragma unroll
-            for (int q = 0; q < M_UNITS; ++q) {
-                if (to[q]) *to[q] = now[q];
-                now[q] = then[q];
-                to[q] = to_then[q];
-            }
-        }
+    auto all = [&]() {
+        if (blocks > 1) paged_cluster_sync();
+        else __syncthreads();
     };
-    if (array < p.n) {
-        const int bytes = p.bytes[array];
-        char* const base = (char*)p.arrays[array];
-        gather(T{}, bytes / V, [&](long long j) -> T* {
-            if (j < 0 || j >= (long long)p.max_pages * p.page_size) return nullptr;
+    const int a0 = chunk * p.chunk, arrays = min(p.chunk, p.n - a0);
+    if (arrays > 0) {
+        const int32_t* const table = p.table + (there ? (size_t)slot * p.max_pages : 0);
+        auto row_of = [&](long long j) {
+            if (j < 0 || j >= (long long)p.max_pages * p.page_size) return -1;
             const uint32_t pg = p.page_mul ? __umulhi((uint32_t)j, p.page_mul) >> p.page_shift : (uint32_t)j;
             const int page = __ldcg(table + pg);
-            if ((unsigned)page >= (unsigned)p.pages) return nullptr;
-            return (T*)(base + (((size_t)page * p.kv_heads + head) * p.page_size + ((int)j - (int)(pg * (uint32_t)p.page_size))) * bytes);
-        });
+            return (unsigned)page >= (unsigned)p.pages ? -1 : (page * p.kv_heads + head) * p.page_size + ((int)j - (int)(pg * (uint32_t)p.page_size));
+        };
+        const uint32_t units = (uint32_t)(p.bytes / V);
+        // rows of a tile: of one array as many as it has units for, or all there are and as many arrays
+        const int per = max(1, (int)(M_TILE / units)), rows = min(per, count), group = count <= per && blocks == 1 ? max(1, per / max(1, count)) : 1;
+        const int tiles = rows > 0 ? (count + rows * blocks - 1) / (rows * blocks) : 0;
+        auto look = [&](int tile) {
+            const int i0 = (tile * blocks + rank) * rows;
+            for (int r = tid; r < rows; r += M_THREADS) {
+                const int i = i0 + r, f = i < count ? __ldcg(from + i) : -1;
+                int2 x = make_int2(-1, -1);
+                if (f > i) x = make_int2(row_of((long long)start + f), row_of((long long)start + i));           // (before it nothing is moved from)
+                if (x.y < 0) x.x = -1;
+                places[tile & 1][r] = x;
+            }
+        };
+        if (tiles > 0) look(0);
+        __syncthreads();
+        for (int a = 0; a < arrays; a += group) {
+            const int n = min(group, arrays - a);
+            for (int t = 0; t < tiles; ++t) {
+                // rows of more units than a tile has go piece by piece
+                for (uint32_t c0 = 0; c0 < units; c0 += M_TILE) {
+                    const uint32_t wide = min(units - c0, (uint32_t)M_TILE), total = wide * (uint32_t)rows * (uint32_t)n;
+                    T x[M_UNITS];
+                    T* to[M_UNITS];
+#pragma unroll
+                    for (int q = 0; q < M_UNITS; ++q) {
+                        const uint32_t e = (uint32_t)(q * M_THREADS + tid), ar = e / wide, c = c0 + (e - ar * wide), k = group > 1 ? ar / (uint32_t)rows : 0u;
+                        to[q] = nullptr;
+                        if (e >= total) continue;
+                        const int2 at = places[t & 1][ar - k * (uint32_t)rows];
+                        if (at.x < 0) continue;
+                        T* const base = (T*)p.arrays[a0 + a + (int)k];
+                        x[q] = load_unit(base + (size_t)at.x * units + c);
+                        to[q] = base + (size_t)at.y * units + c;
+                    }
+                    if (c0 + M_TILE >= units) {
+                        if (t + 1 < tiles) look(t + 1);
+                        else if (tiles % 2 == 0) look(0);         // for the next array; this tile is in the other buffer
+                    }
+                    all();
+#pragma unroll
+                    for (int q = 0; q < M_UNITS; ++q)
+                        if (to[q]) *to[q] = x[q];
+                }
+            }
+            if (tiles > 1 && tiles % 2 && a + group < arrays) {           // this tile was in tile 0's buffer
+                __syncthreads();
+                look(0);
+                __syncthreads();
+            }
+        }
         return;
     }
     if (!there) return;
     float* const w = p.weights + ((size_t)slot * p.kv_heads + head) * p.weights_ld;
-    gather(uint32_t{}, 1, [&](long long j) { return j >= 0 && j < p.weights_ld ? (uint32_t*)(w + j) : nullptr; });
-    if (blocks > 1) paged_cluster_sync();          // all rows are read
-    else __syncthreads();
+    for (long long i0 = 0; i0 < count; i0 += (long long)M_TILE * blocks) {
+        float x[M_UNITS];
+        long long to[M_UNITS];
+#pragma unroll
+        for (int q = 0; q < M_UNITS; ++q) {
+            const long long i = i0 + ((long long)rank * M_UNITS + q) * M_THREADS + tid;
+            to[q] = -1;
+            if (i >= count) continue;
+            const int f = __ldcg(from + i);
+            const long long src = (long long)start + f, dst = (long long)start + i;
+            if (f <= i || dst < 0 || src >= p.weights_ld) continue;
+            x[q] = __ldcg(w + src);
+            to[q] = dst;
+        }
+        all();
+#pragma unroll
+        for (int q = 0; q < M_UNITS; ++q)
+            if (to[q] >= 0) w[to[q]] = x[q];
+    }
+    all();                                         // all rows are read
     const long long end = min((long long)__ldcg(p.contexts + seq), (long long)p.weights_ld);
     for (long long j = max(0ll, (long long)start + count) + rank * M_THREADS + tid; j < end; j += blocks * M_THREADS) w[j] = 0.f;
 }
@@ -225,7 +262,7 @@ extern "C" int pgk_move_rows(void* const* host_arrays, const int32_t* host_row_b
                              long weights_ld, const int32_t* context_lens, void* stream) {
     PGK_REQUIRE(n_arrays >= 0 && pages > 0 && page_size > 0 && slots > 0 && max_pages > 0 && kv_heads > 0 && seqs >= 0 && seqs <= 65535 && width >= 0 && weights_ld >= 0,
                 "move_rows failed: %d arrays of %d pages of %d positions, %d slots of %d pages, %d heads, %d sequences", n_arrays, pages, page_size, slots, max_pages, kv_heads, seqs);
-    PGK_REQUIRE((long long)pages * kv_heads * page_size <= 0x7fffffffll && (long long)max_pages * page_size <= 0x7fffffffll && (long long)kv_heads * (M_ARRAYS + 1) <= 65535,
+    PGK_REQUIRE((long long)pages * kv_heads * page_size <= 0x7fffffffll && (long long)max_pages * page_size <= 0x7fffffffll && kv_heads <= 65535,
                 "move_rows failed: too many rows or heads");
     if (seqs == 0 || (width == 0 && !weights) || (n_arrays == 0 && !weights)) return 0;
     PGK_REQUIRE(page_table && seq_slots && from && counts && (n_arrays == 0 || (host_arrays && host_row_bytes)) && (!weights || context_lens), "move_rows failed: an array is missing");
@@ -240,25 +277,23 @@ extern "C" int pgk_move_rows(void* const* host_arrays, const int32_t* host_row_b
         p.page_mul = (uint32_t)((1ull << (31 + log)) / (uint64_t)page_size + 1);
     }
     const cudaStream_t st = (cudaStream_t)stream;
-    for (int a0 = 0; a0 < n_arrays || (a0 == 0 && n_arrays == 0); a0 += M_ARRAYS) {
-        p.n = n_arrays - a0 < M_ARRAYS ? n_arrays - a0 : M_ARRAYS;
-        int unit = 16, most = 0;
-        for (int a = 0; a < p.n; ++a) {
-            p.arrays[a] = host_arrays[a0 + a];
-            p.bytes[a] = host_row_bytes[a0 + a];
-            PGK_REQUIRE(p.arrays[a] && p.bytes[a] > 0 && p.bytes[a] % 2 == 0, "move_rows failed: rows of %d bytes", p.bytes[a]);
-            while ((p.bytes[a] | (uintptr_t)p.arrays[a]) % unit) unit = unit == 16 ? 4 : 2;
-            most = p.bytes[a] > most ? p.bytes[a] : most;
-        }
-        const bool last = a0 + M_ARRAYS >= n_arrays;
-        p.weights = last ? weights : nullptr;
+    for (int a = 0; a < n_arrays; ++a)
+        PGK_REQUIRE(host_arrays[a] && host_row_bytes[a] > 0 && host_row_bytes[a] % 2 == 0, "move_rows failed: rows of %d bytes", host_row_bytes[a]);
+    auto move = [&]() -> int {
+        uintptr_t low = (uintptr_t)p.bytes;
+        for (int a = 0; a < p.n; ++a) low |= (uintptr_t)p.arrays[a];
+        const int unit = low % 16 == 0 ? 16 : (low % 4 == 0 ? 4 : 2);
+        // arrays of a block: as many as leave four blocks a SM, where there are so many
+        p.chunk = (int)((long long)p.n * kv_heads * seqs / (4 * sm_count()));
+        if (p.chunk < 1) p.chunk = 1;
+        const int chunks = (p.n + p.chunk - 1) / p.chunk + (p.weights ? 1 : 0);
+        PGK_REQUIRE((long long)chunks * kv_heads <= 65535, "move_rows failed: too many heads");
         // blocks that share a head's rows: as many as there are SMs for, none with less than a tile
-        const long long items = (long long)(p.n + (p.weights ? 1 : 0)) * kv_heads * seqs, tile = (long long)M_THREADS * M_UNITS * unit;
+        const long long items = (long long)chunks * kv_heads * seqs;
         int blocks = 1;
-        while (blocks < M_CLUSTER && items * blocks * 2 <= 4 * sm_count() && (long long)width * most > tile * blocks) blocks *= 2;
-        const dim3 grid(blocks, (unsigned)((p.n + (p.weights ? 1 : 0)) * kv_heads), (unsigned)seqs);
+        while (blocks < M_CLUSTER && items * blocks * 2 <= 4 * sm_count() && (long long)width * (p.bytes / unit) > (long long)M_TILE * blocks) blocks *= 2;
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = grid;
+        cfg.gridDim = dim3(blocks, (unsigned)(chunks * kv_heads), (unsigned)seqs);
         cfg.blockDim = dim3(M_THREADS);
         cfg.stream = st;
         cudaLaunchAttribute attr[2];
@@ -271,7 +306,29 @@ extern "C" int pgk_move_rows(void* const* host_arrays, const int32_t* host_row_b
         cfg.numAttrs = 2;
         count_launch();
         PGK_CUDA(unit == 16 ? cudaLaunchKernelEx(&cfg, move_kernel<16>, p) : (unit == 4 ? cudaLaunchKernelEx(&cfg, move_kernel<4>, p) : cudaLaunchKernelEx(&cfg, move_kernel<2>, p)));
-        if (last) break;
+        p.weights = nullptr;
+        p.n = 0;
+        return 0;
+    };
+    // a launch has arrays of one row size, the first one the weights as well
+    p.weights = weights;
+    for (int a = 0; a < n_arrays; ++a) {
+        bool before = false;
+        for (int e = 0; e < a && !before; ++e) before = host_row_bytes[e] == host_row_bytes[a];
+        if (before) continue;
+        p.bytes = host_row_bytes[a];
+        for (int e = a; e < n_arrays; ++e) {
+            if (host_row_bytes[e] != p.bytes) continue;
+            p.arrays[p.n++] = host_arrays[e];
+            if (p.n == M_ARRAYS)
+                if (int rc = move()) return rc;
+        }
+        if (p.n > 0)
+            if (int rc = move()) return rc;
+    }
+    if (n_arrays == 0) {
+        p.bytes = 2;
+        return move();
     }
     return 0;
 }

@@ -84,8 +84,9 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(8) uint64_t full[T_STAGES], empty[T_STAGES], land, sfull[2], pready[2], pvdone;
     __shared__ uint32_t tmem_base_s;
-    __shared__ float wmax[2][2][T_ROWS], row_m[T_ROWS], row_l[T_ROWS];
-    __shared__ int missing, flag;
+    __shared__ float wmax[2][2][T_ROWS];
+    __shared__ PagedFold<T_ROWS> f;
+    __shared__ int missing;
     int* const err = cp.err;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), D = p.dim;
     const uint32_t ks = (smem_u32(smem) + 1023u) & ~1023u, vs = ks + T_STAGES * X::BYTES;
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
         mbar_init(&sfull[0], 1); mbar_init(&sfull[1], 1);
         mbar_init(&pready[0], T_SOFT); mbar_init(&pready[1], T_SOFT); mbar_init(&pvdone, 1);
         mbar_fence_init();
-        missing = flag = 0;
+        missing = f.bad = 0;
     }
     tc_fence_before();
     __syncthreads();
@@ -114,13 +115,13 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
 
     if (warp < 4) {                                // queries to tensor memory, zeros behind the head's end
         const uint16_t* const src = (const uint16_t*)p.q + (live ? (size_t)tok * p.q_ld + (size_t)(b.head * p.rep + b.f0 + row - step_row * p.rep) * D : 0);
-#pragma unroll 1
-        for (int c = 0; c < X::DN; c += 32) {
-            uint32_t x[16];
+        uint32_t x[X::DN / 32][16];
+#pragma unroll
+        for (int c = 0; c < X::DN / 32; ++c)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 uint4 v = make_uint4(0, 0, 0, 0);
-                const int d = c + 8 * i;
+                const int d = 32 * c + 8 * i;
                 if (live && d < D) {
                     if (p.wide_q) v = ld_act16(src + d);
                     else {
@@ -130,21 +131,24 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
                         v = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
-                x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+                x[c][4 * i] = v.x; x[c][4 * i + 1] = v.y; x[c][4 * i + 2] = v.z; x[c][4 * i + 3] = v.w;
             }
-            __syncwarp();
-            tmem_st16u(tmem + ((uint32_t)(quad * 32) << 16) + T_Q + (uint32_t)c / 2u, x);
-        }
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < X::DN / 32; ++c) tmem_st16u(tmem + ((uint32_t)(quad * 32) << 16) + T_Q + (uint32_t)c * 16u, x[c]);
         tmem_st_wait();
-    } else {
+    } else if (warp <= T_SOFT) {
         const int last = min(b.end, b.uend * T_KEYS);
         bool gone = false;
-        for (int j = b.ubeg * T_KEYS + cp.bp * (tid - 128); j < last; j += cp.bp * (T_THREADS - 128)) gone |= b.row_of(p, j) < 0;
+        for (int j = b.ubeg * T_KEYS + cp.bp * (tid - 128); j < last; j += cp.bp * (T_SOFT + 1 - 4) * 32) gone |= b.row_of(p, j) < 0;
         if (gone) missing = 1;
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
+    if (warp <= T_SOFT) {                          // the copies are on their way meanwhile
+        tc_fence_before();
+        __syncwarp();
+        asm volatile("bar.sync 5, %0;" :: "n"((T_SOFT + 1) * 32) : "memory");
+        tc_fence_after();
+    }
 
     if (warp == T_SOFT) {
         // ---------------- MMAs, from one thread
@@ -218,32 +222,49 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
                 ok = all_wait(err, &land, landed);
                 landed ^= 1u;
                 if (!ok) break;
-                const int k0 = max(0, from - j0);
-                for (int i = k0 * 8 + lane; i < T_KEYS * 8; i += 32) {
-                    const int key = i >> 3;
+                // values of the step's rows: is any not finite?  The largest exponent of a lane's says
+                const int k0 = max(0, from - j0), k1 = min(T_KEYS, b.end - j0);
+                const uint32_t tile = vs + (uint32_t)s * X::BYTES;
+                auto unit = [&](uint32_t a, uint32_t (&x)[4]) {
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(a) : "memory");
+                };
+                auto put = [&](uint32_t a, const uint32_t (&x)[4]) {
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+                };
+                uint32_t most = 0;
+#pragma unroll 4
+                for (int i = k0 * 8 + lane; i < k1 * 8; i += 32)
 #pragma unroll
                     for (int c = 0; c < C; ++c) {
-                        const uint32_t a = vs + (uint32_t)s * X::BYTES + (uint32_t)c * T_CHUNK + (uint32_t)i * 16u;
                         uint32_t x[4];
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(a) : "memory");
-                        const bool behind = j0 + key >= b.end;
-                        bool change = behind;
+                        unit(tile + (uint32_t)c * T_CHUNK + (uint32_t)i * 16u, x);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t u = paged_unfinite<DT>(x[e]);
-                            if (u && !behind) bad = change = true;
-                            x[e] = behind ? 0u : x[e] & ~u;
-                        }
-                        if (change) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+                        for (int e = 0; e < 4; ++e) most = __vmaxu2(most, x[e] & 0x7fff7fffu);
                     }
+                if (__any_sync(0xffffffffu, paged_unfinite<DT>(most) != 0)) {
+                    bad = true;
+                    for (int i = k0 * 8 + lane; i < k1 * 8; i += 32)
+                        for (int c = 0; c < C; ++c) {
+                            const uint32_t a = tile + (uint32_t)c * T_CHUNK + (uint32_t)i * 16u;
+                            uint32_t x[4];
+                            unit(a, x);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[e] &= ~paged_unfinite<DT>(x[e]);
+                            put(a, x);
+                        }
                 }
+                // what lies behind the end in the last copy (what was not copied is zeros)
+                const uint32_t none[4] = {0, 0, 0, 0};
+                for (int i = max(0, k1) * 8 + lane; i < min(T_KEYS, (max(0, k1) + cp.bp - 1) & ~(cp.bp - 1)) * 8; i += 32)
+#pragma unroll
+                    for (int c = 0; c < C; ++c) put(tile + (uint32_t)c * T_CHUNK + (uint32_t)i * 16u, none);
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[s]);
             }
             at = next;
         }
-        if (bad) flag = 1;
+        if (bad) f.bad = 1;
         if (lane == 0)
             for (int j = max(0, made - T_STAGES); j < made; ++j)          // whoever gave up: do not leave with copies in flight
                 bar_wait(err, smem_u32(&full[j % T_STAGES]), (uint32_t)(j / T_STAGES) & 1u);
@@ -327,11 +348,11 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
         wmax[0][half][row] = l;
         __syncwarp();
         asm volatile("bar.sync %0, 64;" :: "r"(1 + quad) : "memory");
-        if (half == 0) { row_m[row] = m; row_l[row] = wmax[0][0][row] + wmax[0][1][row]; }
+        if (half == 0) { f.m[row] = m; f.l[row] = wmax[0][0][row] + wmax[0][1][row]; }
     }
     __syncthreads();                               // nobody's tile is read or written any more
     tc_fence_after();
-    float* const fold = (float*)smem;              // [128][DN + 4]
+    float* const sums = (float*)smem;              // [128][DN + 4]
     if (warp < T_SOFT) {
 #pragma unroll 1
         for (int c = half * (X::DN / 2); c < (half + 1) * (X::DN / 2); c += 16) {
@@ -342,14 +363,14 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
                 for (int e = 0; e < 16; ++e) o[e] = 0.f;
             }
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) *(float4*)(fold + (size_t)row * (X::DN + 4) + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            for (int e = 0; e < 16; e += 4) *(float4*)(sums + (size_t)row * (X::DN + 4) + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             __syncwarp();
         }
     }
     tc_fence_before();
     __syncthreads();
     if (warp == T_SOFT) tmem_dealloc(tmem, 512);
-    paged_fold<T_ROWS, T_KEYS, DT>(p, b, fold, X::DN + 4, row_m, row_l, &flag);
+    paged_fold<T_ROWS, T_KEYS, DT, X::DN>(p, b, sums, f);
 }
 
 // How many blocks of a cluster share a sequence's keys: rounds of clusters times (a block's tiles + what it costs besides, about four of them).  How many clusters

@@ -1,9 +1,10 @@
 // paged_weigh.cu -- the attention weights that a cached position gets, summed over a step's rows and the query heads of its key head: what decides which positions of a
 // cache stay when it is cut.  weights[slot][g][j] += sum over rows i and heads h of g of exp(scale q_ih . k_j - lse_ih), lse from the attention over the same rows.
 //
-// A block has 128 keys of one head, 16 (32 at 32 bits) a warp, in registers (shared memory) once; all rows of the sequence pass by them, 64 (16) at a time in
-// shared memory.  Scores by mma.sync m16n8k16 with the operands' order of paged_few.cu, in float32 by multiply-adds; a position's sum is one thread's, so that the same
-// call gives the same bits.  Decoding is bound by the bytes of the keys, windows of a prompt's last tokens by the exponentials.
+// Scores by mma.sync m16n8k16 with the keys as its 16, as in paged_few.cu, in float32 by multiply-adds.  A block has the step's rows in shared memory (all of them, or as many
+// as fit at a time) and a share of the positions; a warp walks over its own 16 by 16, the next on their way from memory to registers meanwhile.  A
+// position's sum is one thread's until it is added, so that the same call gives the same bits.  Decoding is bound by the bytes of the keys, windows of a prompt's last tokens by
+// products and exponentials.
 #include "paged.cuh"
 #include "tc_common.cuh"
 #include "../../include/pgk_b200.h"
@@ -13,11 +14,11 @@ namespace pgk {
 namespace {
 
 constexpr int H_ALL = 1 << 30;                                // rows of a "block": all of the sequence's
-constexpr int H_WARPS = 8, H_THREADS = H_WARPS * 32, H_KEYS = H_WARPS * 16, H_TILES = 4;
+constexpr int H_WARPS = 4, H_THREADS = H_WARPS * 32, H_KEYS = 16, H_RESIDENT = 4;
+constexpr int H_QBYTES = 48 * 1024;                           // queries of a block at a time: four blocks a SM
 constexpr int G_WARPS = 4, G_THREADS = G_WARPS * 32, G_KEYS = G_WARPS * 32, G_ROWS = 16;
 
 using Keys = PagedBlock<H_ALL, H_KEYS>;
-static_assert(H_KEYS == G_KEYS);
 
 template <int DT>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -42,41 +43,43 @@ __device__ __forceinline__ void add_weight(const PagedParams& p, const Keys& b, 
 
 // N: 32-element pieces of a head
 template <int N, int DT>
-__global__ void __launch_bounds__(H_THREADS, N <= 4 ? 3 : 2) paged_weigh_kernel(const __grid_constant__ PagedParams p) {
-    __shared__ __align__(16) uint4 qs[H_TILES][2 * N * 32];
-    __shared__ float negs[H_TILES * 16];
+__global__ void __launch_bounds__(H_THREADS, N <= 4 ? H_RESIDENT : 2) paged_weigh_kernel(const __grid_constant__ PagedParams p, int most) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    uint4* const qs = (uint4*)smem;                           // [tiles of eight rows][N][32]: lane (gl, t)'s elements 32 s + 8 t ... + 7 of row 8 n + gl
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), gl = lane >> 2, t = lane & 3, D = p.dim;
     griddep_wait();
     griddep_launch();
-    const Keys b(p, (int)blockIdx.z, (int)blockIdx.y, 0);
-    const int k0 = (int)blockIdx.x * H_KEYS, j0 = k0 + 16 * warp;
-    if (k0 >= b.end || b.live == 0) return;
+    const Keys b(p, (int)blockIdx.z, (int)blockIdx.y, (int)blockIdx.x);
+    float* const negs = (float*)(qs + (size_t)most * N * 32);
+    if (b.ubeg >= b.uend || b.live == 0) return;
 
-    const int rows = b.row_of(p, j0 + (lane & 15));
-    const uint32_t there = __ballot_sync(0xffffffffu, rows >= 0);
-    uint4 kk[N][2];
+    const char* const kb = (const char*)p.k_data;
+    const size_t stride = (size_t)D * 2;
+    uint4 kk[N][2], ahead[N][2];
+    auto load_k = [&](int rows, uint4 (&x)[N][2]) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int row = __shfl_sync(0xffffffffu, rows, 8 * u + gl);
-        const char* const src = (const char*)p.k_data + (size_t)max(row, 0) * (D * 2) + 16 * t;
+        for (int u = 0; u < 2; ++u) {
+            const int row = __shfl_sync(0xffffffffu, rows, 8 * u + gl);
+            const char* const src = kb + (size_t)max(row, 0) * stride + 16 * t;
 #pragma unroll
-        for (int s = 0; s < N; ++s) {
-            kk[s][u] = make_uint4(0, 0, 0, 0);
-            if (row >= 0 && 32 * s + 8 * t < D) kk[s][u] = ld_act16(src + 64 * s);
+            for (int s = 0; s < N; ++s) {
+                x[s][u] = make_uint4(0, 0, 0, 0);
+                if (row >= 0 && 32 * s + 8 * t < D) x[s][u] = ld_act16(src + 64 * s);
+            }
         }
-    }
-    const bool edge = (there & 0xffffu) != 0xffffu || j0 + 16 > b.base;
-    float sum[2][2] = {};
+    };
+    auto look = [&](int k) { return k < b.uend ? b.row_of(p, k * H_KEYS + (lane & 15)) : -1; };
 #pragma unroll 1
-    for (int f0 = 0; f0 < b.live; f0 += 16 * H_TILES) {
-        __syncthreads();
-        const int tiles = min(H_TILES, (b.live - f0 + 15) / 16);
-        for (int i = tid; i < tiles * 2 * N * 32; i += H_THREADS) {
-            const int tile = i / (2 * N * 32), x = i - tile * (2 * N * 32), s = x >> 6, l = x & 31, f = f0 + 16 * tile + (l >> 2) + 8 * ((x >> 5) & 1), d = 32 * s + 8 * (l & 3);
+    for (int f0 = 0; f0 < b.live; f0 += 8 * most) {
+        const int tiles = min(most, (b.live - f0 + 7) / 8);
+        int k = b.ubeg + warp, rows = look(k), next = look(k + H_WARPS);
+        load_k(rows, kk);
+        if (f0 > 0) __syncthreads();
+        for (int i = warp; i < tiles * N; i += H_WARPS) {
+            const int n = i / N, s = i - n * N, x = f0 + 8 * n + gl, d = 32 * s + 8 * t, row = x / p.rep, tok = b.first + row;
             uint4 v = make_uint4(0, 0, 0, 0);
-            const int row = f / p.rep, tok = b.first + row;
-            if (f < b.live && d < D && tok >= 0 && tok < p.tokens) {
-                const uint16_t* src = (const uint16_t*)p.q + (size_t)tok * p.q_ld + (size_t)(b.head * p.rep + f - row * p.rep) * D + d;
+            if (x < b.live && d < D && tok >= 0 && tok < p.tokens) {
+                const uint16_t* src = (const uint16_t*)p.q + (size_t)tok * p.q_ld + (size_t)(b.head * p.rep + x - row * p.rep) * D + d;
                 if (p.wide_q) v = ld_act16(src);
                 else {
                     uint32_t w[4];
@@ -85,48 +88,52 @@ __global__ void __launch_bounds__(H_THREADS, N <= 4 ? 3 : 2) paged_weigh_kernel(
                     v = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
-            qs[tile][x] = v;
+            qs[i * 32 + lane] = v;
         }
-        if (tid < 16 * tiles) negs[tid] = row_neg(p, b, f0 + tid);
+        for (int i = tid; i < 8 * tiles; i += H_THREADS) negs[i] = row_neg(p, b, f0 + i);
         __syncthreads();
 #pragma unroll 1
-        for (int tile = 0; tile < tiles; ++tile) {
-            float s[2][4] = {};
+        for (; k < b.uend; k += H_WARPS) {
+            const int j0 = k * H_KEYS;
+            const uint32_t there = __ballot_sync(0xffffffffu, rows >= 0);
+            const bool edge = (there & 0xffffu) != 0xffffu || j0 + H_KEYS > b.base;
+            rows = next;
+            load_k(rows, ahead);
+            next = look(k + 2 * H_WARPS);
+            float sum0 = 0.f, sum1 = 0.f;                     // of keys gl and gl + 8: this lane's rows
+#pragma unroll 1
+            for (int n = 0; n < tiles; ++n) {
+                float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int q = 0; q < N; ++q) {
-                const uint4 a = qs[tile][(2 * q) * 32 + lane], c = qs[tile][(2 * q + 1) * 32 + lane];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    mma16816<DT>(s[u], a.x, c.x, a.y, c.y, kk[q][u].x, kk[q][u].y);
-                    mma16816<DT>(s[u], a.z, c.z, a.w, c.w, kk[q][u].z, kk[q][u].w);
+                for (int q = 0; q < N; ++q) {
+                    const uint4 a = qs[(n * N + q) * 32 + lane];
+                    mma16816<DT>(s, kk[q][0].x, kk[q][1].x, kk[q][0].y, kk[q][1].y, a.x, a.y);
+                    mma16816<DT>(s, kk[q][0].z, kk[q][1].z, kk[q][0].w, kk[q][1].w, a.z, a.w);
+                }
+                const float2 neg = *(const float2*)(negs + 8 * n + 2 * t);
+                const float w0 = weight(s[0], p.scale_log2, neg.x), w1 = weight(s[1], p.scale_log2, neg.y), w2 = weight(s[2], p.scale_log2, neg.x),
+                            w3 = weight(s[3], p.scale_log2, neg.y);
+                if (edge) {
+                    const int i0 = (f0 + 8 * n + 2 * t) / p.rep, i1 = (f0 + 8 * n + 2 * t + 1) / p.rep, at = j0 - b.base;
+                    const uint32_t see0 = paged_window(p, b.first + i0, i0, at) & there, see1 = paged_window(p, b.first + i1, i1, at) & there;
+                    sum0 += ((see0 >> gl) & 1u ? w0 : 0.f) + ((see1 >> gl) & 1u ? w1 : 0.f);
+                    sum1 += ((see0 >> (gl + 8)) & 1u ? w2 : 0.f) + ((see1 >> (gl + 8)) & 1u ? w3 : 0.f);
+                } else {
+                    sum0 += w0 + w1;
+                    sum1 += w2 + w3;
                 }
             }
-            const float n0 = negs[16 * tile + gl], n1 = negs[16 * tile + gl + 8];
-            uint32_t see0 = 0xffffu, see1 = 0xffffu;
-            if (edge) {
-                const int i0 = (f0 + 16 * tile + gl) / p.rep, i1 = (f0 + 16 * tile + gl + 8) / p.rep;
-                see0 = paged_window(p, b.first + i0, i0, j0 - b.base) & there;
-                see1 = paged_window(p, b.first + i1, i1, j0 - b.base) & there;
+#pragma unroll
+            for (int x = 1; x <= 2; x <<= 1) {
+                sum0 += __shfl_xor_sync(0xffffffffu, sum0, x);
+                sum1 += __shfl_xor_sync(0xffffffffu, sum1, x);
             }
+            const int j = j0 + gl + 8 * t;                    // lanes 0 and 1 of a group write
+            if (t < 2 && j < b.end) add_weight(p, b, j, t ? sum1 : sum0);
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int bit = 8 * u + 2 * t + e;
-                    const float w0 = weight(s[u][e], p.scale_log2, n0), w1 = weight(s[u][2 + e], p.scale_log2, n1);
-                    if ((see0 >> bit) & 1u) sum[u][e] += w0;
-                    if ((see1 >> bit) & 1u) sum[u][e] += w1;
-                }
+            for (int s = 0; s < N; ++s) { kk[s][0] = ahead[s][0]; kk[s][1] = ahead[s][1]; }
         }
     }
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-            for (int x = 4; x <= 16; x <<= 1) sum[u][e] += __shfl_xor_sync(0xffffffffu, sum[u][e], x);
-            if (gl == 0 && j0 + 8 * u + 2 * t + e < b.end) add_weight(p, b, j0 + 8 * u + 2 * t + e, sum[u][e]);
-        }
 }
 
 __global__ void __launch_bounds__(G_THREADS) paged_weigh_f32_kernel(const __grid_constant__ PagedParams p) {
@@ -137,7 +144,7 @@ __global__ void __launch_bounds__(G_THREADS) paged_weigh_f32_kernel(const __grid
     float* const ks = qs + G_ROWS * D + warp * 32 * DF;
     griddep_wait();
     griddep_launch();
-    const Keys b(p, (int)blockIdx.z, (int)blockIdx.y, 0);
+    const Keys b(p, (int)blockIdx.z, (int)blockIdx.y, 0);        // all positions; the block's are the next line's
     const int k0 = (int)blockIdx.x * G_KEYS, j0 = k0 + 32 * warp, j = j0 + lane;
     if (k0 >= b.end || b.live == 0) return;
 
@@ -190,27 +197,37 @@ __global__ void __launch_bounds__(G_THREADS) paged_weigh_f32_kernel(const __grid
     if (j < b.end) add_weight(p, b, j, sum);
 }
 
-template <int N, int DT> int launch_weigh(const PagedParams& p, dim3 grid, cudaStream_t st) {
-    PGK_CUDA(launch_waiting(paged_weigh_kernel<N, DT>, grid, dim3(H_THREADS), 0, st, p));
+template <int N, int DT> int launch_weigh(PagedParams p, cudaStream_t st) {
+    static bool configured = false;
+    if (!configured) {
+        PGK_CUDA(cudaFuncSetAttribute(paged_weigh_kernel<N, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, H_QBYTES));
+        configured = true;
+    }
+    // tiles of eight rows that fit, and blocks that share a sequence's positions: four rounds of all SMs, none with less than two turns of its warps
+    const long long tiles = ((long long)p.max_rows * p.rep + 7) / 8, fit = H_QBYTES / (N * 512 + 32);
+    const int most = (int)(tiles < fit ? tiles : fit);
+    const long long items = (long long)p.kv_heads * p.seqs, wanted = (4ll * H_RESIDENT * sm_count() + items - 1) / items, turns = (p.max_keys + 2 * H_WARPS * H_KEYS - 1) / (2 * H_WARPS * H_KEYS);
+    p.splits = (int)(wanted < turns ? wanted : turns);
+    PGK_CUDA(launch_waiting(paged_weigh_kernel<N, DT>, dim3(p.splits, p.kv_heads, p.seqs), dim3(H_THREADS), (size_t)most * (N * 512 + 32), st, p, most));
     return 0;
 }
-template <int DT> int launch_weigh_dim(const PagedParams& p, dim3 grid, cudaStream_t st) {
+template <int DT> int launch_weigh_dim(const PagedParams& p, cudaStream_t st) {
     switch ((p.dim + 31) / 32) {
-        case 1: case 2: return launch_weigh<2, DT>(p, grid, st);
-        case 3: return launch_weigh<3, DT>(p, grid, st);
-        case 4: return launch_weigh<4, DT>(p, grid, st);
-        case 5: case 6: return launch_weigh<6, DT>(p, grid, st);
-        default: return launch_weigh<8, DT>(p, grid, st);
+        case 1: case 2: return launch_weigh<2, DT>(p, st);
+        case 3: return launch_weigh<3, DT>(p, st);
+        case 4: return launch_weigh<4, DT>(p, st);
+        case 5: case 6: return launch_weigh<6, DT>(p, st);
+        default: return launch_weigh<8, DT>(p, st);
     }
 }
 
 int weigh(PagedParams p, int dtype, cudaStream_t st) {
     p.tiles = 1;
+    if (p.max_keys == 0) return 0;
+    if (dtype == 1) return launch_weigh_dim<1>(p, st);
+    if (dtype == 2) return launch_weigh_dim<2>(p, st);
     p.splits = 1;
-    const dim3 grid((unsigned)((p.max_keys + H_KEYS - 1) / H_KEYS), p.kv_heads, p.seqs);
-    if (grid.x == 0) return 0;
-    if (dtype == 1) return launch_weigh_dim<1>(p, grid, st);
-    if (dtype == 2) return launch_weigh_dim<2>(p, grid, st);
+    const dim3 grid((unsigned)((p.max_keys + G_KEYS - 1) / G_KEYS), p.kv_heads, p.seqs);
     static bool configured = false;
     if (!configured) {
         PGK_CUDA(cudaFuncSetAttribute(paged_weigh_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (G_ROWS * 256 + G_WARPS * 32 * 260) * 4));
