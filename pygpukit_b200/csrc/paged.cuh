@@ -48,6 +48,38 @@ inline int paged_cut(const PagedParams& p, long long items, int step, int warps,
     return best;
 }
 
+// How many clusters of a kernel run at once: of eight blocks, one a SM, fewer than 148 / 8
+template <typename... KArgs>
+inline cudaError_t clusters_at_once(int* out, void (*kernel)(KArgs...), int threads, size_t smem, int blocks) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = (unsigned)blocks;
+    cfg.gridDim = dim3(1, 1, (unsigned)blocks);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    *out = 1;
+    int n = 0;
+    if (cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg)) return e;
+    if (n > 0) *out = n;
+    return cudaSuccess;
+}
+// Blocks of a cluster that share a sequence's tiles, a block a SM: rounds of clusters times (a block's tiles + what it costs besides, about four of them)
+inline int paged_clusters(const PagedParams& p, int keys, const int* at_once, int most) {
+    const int nt = (p.max_keys + keys - 1) / keys;
+    const long long items = (long long)p.seqs * p.tiles * p.kv_heads;
+    long long least = 0;
+    int best = 1;
+    for (int s = 1; s <= most; ++s) {
+        const long long cost = ((items + at_once[s] - 1) / at_once[s]) * ((nt + s - 1) / s + 4);
+        if (s == 1 || cost < least) { best = s; least = cost; }
+    }
+    return best;
+}
+
 // blocks of a cluster along z, and the launch that waits for the kernel before it
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_clusters(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
@@ -237,13 +269,19 @@ __device__ __forceinline__ void paged_fold(const PagedParams& p, const PagedBloc
             o = make_float4(w * v.x, w * v.y, w * v.z, w * v.w);
         } else {
             o = make_float4(0.f, 0.f, 0.f, 0.f);
+            const uint32_t from = sums_at + (uint32_t)(r * (DN + 4) + d) * 4u;
 #pragma unroll 1
-            for (int s0 = 0; s0 < p.splits; s0 += 2) {                     // two and more: a power of two
-                const uint32_t from = sums_at + (uint32_t)(r * (DN + 4) + d) * 4u;
-                const float4 u = paged_remote_float4(paged_remote(from, s0)), v = paged_remote_float4(paged_remote(from, s0 + 1));
-                const float wu = f.factor[s0][r], wv = f.factor[s0 + 1][r];
-                o.x = fmaf(wu, u.x, o.x); o.y = fmaf(wu, u.y, o.y); o.z = fmaf(wu, u.z, o.z); o.w = fmaf(wu, u.w, o.w);
-                o.x = fmaf(wv, v.x, o.x); o.y = fmaf(wv, v.y, o.y); o.z = fmaf(wv, v.z, o.z); o.w = fmaf(wv, v.w, o.w);
+            for (int s0 = 0; s0 < p.splits; s0 += 4) {                     // four loads on their way
+                float4 v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (s0 + u < p.splits) v[u] = paged_remote_float4(paged_remote(from, s0 + u));
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (s0 + u < p.splits) {
+                        const float w = f.factor[s0 + u][r];
+                        o.x = fmaf(w, v[u].x, o.x); o.y = fmaf(w, v[u].y, o.y); o.z = fmaf(w, v[u].z, o.z); o.w = fmaf(w, v[u].w, o.w);
+                    }
             }
         }
         if (bad) {

@@ -1,326 +1,483 @@
-// paged_few.cu -- attention of few rows a sequence over 16-bit pages: decoded tokens, small trees of drafts, and whatever the large tiles of paged_tc.cu do not serve
-// (heads above 128 elements, pages that no copy of eight positions fits).
+// paged_few.cu -- attention of few rows a sequence over 16-bit pages: decoded tokens, small trees of drafts, and whatever the tiles of 128 rows of paged_tc.cu do not serve
+// (heads above 128 elements, small pages).
 //
-// One pass over the keys with the running maximum and sum of a softmax.  A block has 8 or 16 (row, head) rows, each of its warps walks over its own blocks of 16 keys by
-// mma.sync m16n8k16, the keys and then the values' elements as its 16: S^T = K Q^T, O^T += V^T P^T, so that eight rows cost half of what sixteen do.  K and V go straight
-// from memory to registers, sixteen bytes a lane: the order of a head's elements in the score's sum is free, so a lane takes the eight that follow each other in one
-// key; V wants pairs of keys in a register, which byte permutations of two keys' loads make.  The next 16 keys are fetched as soon as a product has read these.
-// Weights become two terms of bfloat16 (2^-17 of each; one left an output 1.4 times as far off), one of float16 (2^-12); their sum is float32 of the unrounded ones.
-// Blocks of a cluster share a sequence's keys and fold through distributed shared memory.
+// One pass over the keys with the running maximum and sum of a softmax, on tcgen05 with the keys as the products' 128 lanes: a block has NR = 16, 32 or 64 (row, head) rows,
+// S^T[128 keys, NR] = K Q^T, and O^T[128 elements, 2 NR] += V^T P^T, so that few rows cost few columns and K and V are read from shared memory as TMA left them.  (With mma.sync
+// and K and V in registers, 64 tokens over 8192 keys took 390 us, 550 instructions for 16 keys of a warp; with rows copied to shared memory one by one 455, 15 cycles a
+// copy of 256 bytes.)
+//   * one warp fetches tiles of K and V by turns into a ring, in pieces of as many positions as divide a page, four rows at a time where that is fewer than eight;
+//   * one thread issues the products, the scores of tile i + 1 before the weights of tile i are waited for;
+//   * eight warps, a lane a key, two halves of the rows: maxima meet by shuffles and one exchange among a half's four warps; a row's reference moves when its
+//     maximum has grown by 2^8.  A weight is two terms of the cache's type (bfloat16 2^-17 of it; one term left an output 1.4 times as far off), whose products have
+//     accumulators of their own; its sum is float32 of the unrounded one.
+// Only tiles that hold the step's rows, or the context's end, look at masks; values there as in paged_tc.cu.  Blocks of a cluster share a sequence's keys.
 // Bound by the bytes of the keys and, for one request, by the chain from launch to fold.
 #include "paged.cuh"
 #include "tc_common.cuh"
+#include "tma.cuh"
 #include "../../include/pgk_b200.h"
 
 namespace pgk {
 
 namespace {
 
-constexpr int W_KEYS = 16, W_WARPS = 4, W_THREADS = W_WARPS * 32;
+constexpr int W_KEYS = 128, W_SOFT = 8, W_THREADS = (W_SOFT + 2) * 32;
+constexpr uint32_t W_CHUNK = W_KEYS * 128;                         // 64 elements of 128 keys
 
-// sixteen bytes of the cache, each read once by a block
-__device__ __forceinline__ uint4 ld_cache16(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-template <int DT>
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (DT == 1)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// an 8 x 8 matrix of 16-bit numbers, a register a lane, transposed
-__device__ __forceinline__ uint32_t transposed(uint32_t x) {
-    uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
-    return r;
-}
-
-// N: 32-element pieces of a head; NT: tiles of eight rows
-template <int N, int NT> struct Few {
-    static constexpr int DP = 32 * N, CH = (DP + 63) / 64, ROWS = 8 * NT, DF = DP + 4;
-    static constexpr int QBYTES = N * NT * 32 * 16, FOLD = W_WARPS * ROWS * DF * 4, BYTES = QBYTES > FOLD ? QBYTES : FOLD;
-    static constexpr int RESIDENT = N <= 2 ? (NT == 1 ? 5 : 4) : (N <= 4 ? 3 : 2);
+struct FewCopies {
+    int bp;                  // positions a copy, a power of two that divides the page; 0: four rows wherever they are
+    int rows;                // of the cache: coordinates from here on read zeros
+    int* err;
 };
 
-template <int N, int NT, int DT>
-__global__ void __launch_bounds__(W_THREADS, Few<N, NT>::RESIDENT) paged_few_kernel(const __grid_constant__ PagedParams p) {
-    using F = Few<N, NT>;
-    constexpr int CH = F::CH, ROWS = F::ROWS, TERMS = DT == 1 ? 1 : 2;
-    // float16 weights: from 2^6 down, so that those 2^-20 of the largest still have all their bits; they grow to 2^14 before the reference moves
-    constexpr float TOP = DT == 1 ? 6.f : 0.f;
-    extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ float wm[W_WARPS][ROWS], wl[W_WARPS][ROWS];
-    __shared__ PagedFold<ROWS> f;
-    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), gl = lane >> 2, t = lane & 3;
-    if (tid == 0) f.bad = 0;
-    griddep_wait();
-    griddep_launch();
-    const PagedBlock<ROWS, W_KEYS> b(p, (int)blockIdx.x, (int)blockIdx.y, (int)blockIdx.z);
-    const int D = p.dim;
-    const char* const kb = (const char*)p.k_data;
-    const char* const vb = (const char*)p.v_data;
-    const size_t stride = (size_t)D * 2;
+// NR: rows; C: 64-element chunks of a head
+template <int NR, int C> struct Few {
+    static constexpr int R = NR / 2, DG = (C + 1) / 2, DN = 64 * C, PBUF = NR == 64 ? 1 : 2;
+    static constexpr uint32_t TILE = C * W_CHUNK, QCHUNK = NR * 128, Q = C * QCHUNK, P = W_KEYS * 4 * NR;
+    static constexpr int ROOM = 218 * 1024 - 1024 - (int)(Q + PBUF * P), FIT = ROOM / (int)TILE, SLOTS = FIT < 8 ? FIT : 8;
+    static constexpr int BYTES = SLOTS * (int)TILE + (int)(Q + PBUF * P) + 1024;
+    static constexpr uint32_t COLUMNS = 2 * NR + DG * 2 * NR, TMEM = COLUMNS <= 64 ? 64 : (COLUMNS <= 128 ? 128 : (COLUMNS <= 256 ? 256 : 512));
+    static_assert(SLOTS >= 2 && COLUMNS <= 512 && NR * (DN + 4) * 4 <= SLOTS * (int)TILE);
+};
 
-    uint4 kk[N][2], vv[CH][4];
-    auto load_k = [&](int rows) {                             // key gl, gl + 8: elements 32 s + 8 t ... + 7
+__device__ __forceinline__ bool all_wait(int* err, uint64_t* bar, uint32_t parity) {
+    const bool ok = bar_wait(err, smem_u32(bar), parity);
+    return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ void tmem_ld8_async(uint32_t taddr, float* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const float* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 :: "r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+}
+// N columns of a warp's lanes
+template <int N> __device__ __forceinline__ void tmem_columns(uint32_t taddr, float (&v)[N]) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int row = __shfl_sync(0xffffffffu, rows, 8 * u + gl);
-            const char* const src = kb + (size_t)max(row, 0) * stride + 16 * t;
+    for (int c = 0; c < N; c += 8) tmem_ld8_async(taddr + (uint32_t)c, v + c);
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-            for (int s = 0; s < N; ++s) {
-                kk[s][u] = make_uint4(0, 0, 0, 0);
-                if (row >= 0 && 32 * s + 8 * t < D) kk[s][u] = ld_cache16(src + 64 * s);
-            }
+    for (int c = 0; c < N; ++c) asm volatile("" : "+f"(v[c]) :: "memory");
+}
+// the lanes' N values (8, 16 or 32) reduced over the warp: lane l ends with value l % N
+template <int N, typename F> __device__ __forceinline__ float reduce_lanes(float (&v)[N], int lane, F f) {
+#pragma unroll
+    for (int w = N / 2; w > 0; w >>= 1) {
+        const bool up = lane & w;
+#pragma unroll
+        for (int j = 0; j < w; ++j) {
+            const float got = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + w], w);
+            v[j] = f(up ? v[j + w] : v[j], got);
         }
-    };
-    auto load_v = [&](int rows) {                             // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9: elements 64 c + 8 gl ... + 7
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int row = __shfl_sync(0xffffffffu, rows, 2 * t + (u & 1) + 8 * (u >> 1));
-            const char* const src = vb + (size_t)max(row, 0) * stride + 16 * gl;
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                vv[c][u] = make_uint4(0, 0, 0, 0);
-                if (row >= 0 && 64 * c + 8 * gl < D) vv[c][u] = ld_cache16(src + 128 * c);
-            }
-        }
-    };
-    int k = b.ubeg + warp;
-    int rows = k < b.uend ? b.row_of(p, k * W_KEYS + (lane & 15)) : -1;
-    int next = k + W_WARPS < b.uend ? b.row_of(p, (k + W_WARPS) * W_KEYS + (lane & 15)) : -1;
-
-    // ---------------- queries: piece s, tile n: this lane's eight elements 32 s + 8 t of row 8 n + gl
-    uint4* const qs = (uint4*)smem;
-    for (int i = warp; i < N * NT; i += W_WARPS) {
-        const int r = gl + 8 * (i % NT), d = 32 * (i / NT) + 8 * t, x = b.f0 + r, tok = b.first + x / p.rep;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < b.live && d < D && tok >= 0 && tok < p.tokens) {
-            const uint16_t* src = (const uint16_t*)p.q + (size_t)tok * p.q_ld + (size_t)(b.head * p.rep + x % p.rep) * D + d;
-            if (p.wide_q) v = ld_act16(src);
-            else {
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = (uint32_t)ld_act2(src + 2 * e) | (uint32_t)ld_act2(src + 2 * e + 1) << 16;
-                v = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
-        qs[i * 32 + lane] = v;
     }
-    if (k < b.uend) {
-        load_k(rows);
-        load_v(rows);
-    }
-    __syncthreads();
-
-    float o[CH][4][NT][4], m[NT][2], l[NT][2];               // of rows 8 n + 2 t, + 1
+    float x = v[0];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        m[n][0] = m[n][1] = -INFINITY;
-        l[n][0] = l[n][1] = 0.f;
-    }
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[c][j][n][e] = 0.f;
-    bool bad = false;
-#pragma unroll 1
-    for (; k < b.uend; k += W_WARPS) {
-        const int j0 = k * W_KEYS;
-        float s[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-#pragma unroll
-        for (int q = 0; q < N; ++q)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const uint4 a = qs[(q * NT + n) * 32 + lane];
-                mma16816<DT>(s[n], kk[q][0].x, kk[q][1].x, kk[q][0].y, kk[q][1].y, a.x, a.y);
-                mma16816<DT>(s[n], kk[q][0].z, kk[q][1].z, kk[q][0].w, kk[q][1].w, a.z, a.w);
-            }
-        const uint32_t there = __ballot_sync(0xffffffffu, rows >= 0);
-        const bool edge = (there & 0xffffu) != 0xffffu || j0 + W_KEYS > b.base;
-        const bool more = k + W_WARPS < b.uend;
-        rows = next;
-        if (more) load_k(rows);
-        next = k + 2 * W_WARPS < b.uend ? b.row_of(p, (k + 2 * W_WARPS) * W_KEYS + (lane & 15)) : -1;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] *= p.scale_log2;
-        if (edge) {
-            const int at = j0 - b.base;                       // the step's row of the block's first key, below 0 before the step
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int i = (b.f0 + 8 * n + 2 * t + e) / p.rep;
-                    const uint32_t see = paged_window(p, b.first + i, i, at) & there;
-                    if (!((see >> gl) & 1u)) s[n][e] = -INFINITY;
-                    if (!((see >> (gl + 8)) & 1u)) s[n][2 + e] = -INFINITY;
-                }
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (at + 2 * t + (u & 1) + 8 * (u >> 1) >= 0) {            // values of the step's rows, which not all rows see
-#pragma unroll
-                    for (int c = 0; c < CH; ++c) {
-                        uint32_t* const w = &vv[c][u].x;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t x = paged_unfinite<DT>(w[e]);
-                            bad |= x != 0;
-                            w[e] &= ~x;
-                        }
-                    }
-                }
-        }
-        float top[NT][2];
-        bool up = false;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float x = fmaxf(s[n][e], s[n][2 + e]);
-#pragma unroll
-                for (int y = 4; y <= 16; y <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, y));
-                top[n][e] = x - TOP;
-                up |= top[n][e] > m[n][e] + PAGED_LAZY;       // (also the first finite maximum)
-            }
-        if (__any_sync(0xffffffffu, up)) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    if (!(top[n][e] > m[n][e] + PAGED_LAZY)) continue;
-                    const float fix = m[n][e] == -INFINITY ? 0.f : exp2f(m[n][e] - top[n][e]);
-                    m[n][e] = top[n][e];
-                    l[n][e] *= fix;
-#pragma unroll
-                    for (int c = 0; c < CH; ++c)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) { o[c][j][n][e] *= fix; o[c][j][n][2 + e] *= fix; }
-                }
-        }
-        uint32_t w[NT][TERMS][2];                             // weights of row 8 n + gl: keys 2 t, 2 t + 1 and 2 t + 8, 2 t + 9
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const float n0 = paged_neg(m[n][0]), n1 = paged_neg(m[n][1]);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const float a = ex2(s[n][2 * u] + n0), c = ex2(s[n][2 * u + 1] + n1);
-                l[n][0] += a;
-                l[n][1] += c;
-                const uint32_t x = paged_pack2<DT>(a, c);
-                w[n][0][u] = transposed(x);
-                if constexpr (TERMS == 2) w[n][1][u] = transposed(pack_bf16x2(a - bf16lo(x), c - bf16hi(x)));
-            }
-        }
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const uint32_t* const v0 = &vv[c][0].x;
-            const uint32_t* const v1 = &vv[c][1].x;
-            const uint32_t* const v2 = &vv[c][2].x;
-            const uint32_t* const v3 = &vv[c][3].x;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {                     // elements 64 c + 8 gl + 2 j, + 1 of the key pairs
-                const uint32_t a0 = __byte_perm(v0[j], v1[j], 0x5410), a1 = __byte_perm(v0[j], v1[j], 0x7632), a2 = __byte_perm(v2[j], v3[j], 0x5410),
-                               a3 = __byte_perm(v2[j], v3[j], 0x7632);
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int x = 0; x < TERMS; ++x) mma16816<DT>(o[c][j][n], a0, a1, a2, a3, w[n][x][0], w[n][x][1]);
-            }
-        }
-        if (more) load_v(rows);
-    }
-
-    // ---------------- the warps' sums into one
-    if (bad) f.bad = 1;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float x = l[n][e];
-#pragma unroll
-            for (int y = 4; y <= 16; y <<= 1) x += __shfl_xor_sync(0xffffffffu, x, y);
-            if (gl == 0) { wm[warp][8 * n + 2 * t + e] = m[n][e]; wl[warp][8 * n + 2 * t + e] = x; }
-        }
-    __syncthreads();                                          // the queries are read
-    float* const sums = (float*)smem;                         // [warps][rows][DF]
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-        if (64 * c + 8 * gl < F::DP) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float* const dst = sums + ((size_t)warp * ROWS + 8 * n + 2 * t + e) * F::DF + 64 * c + 8 * gl;
-                    *(float4*)dst = make_float4(o[c][0][n][e], o[c][0][n][2 + e], o[c][1][n][e], o[c][1][n][2 + e]);
-                    *(float4*)(dst + 4) = make_float4(o[c][2][n][e], o[c][2][n][2 + e], o[c][3][n][e], o[c][3][n][2 + e]);
-                }
-        }
-    if (tid < ROWS) {
-        float top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int x = 0; x < W_WARPS; ++x) top = fmaxf(top, wm[x][tid]);
-#pragma unroll
-        for (int x = 0; x < W_WARPS; ++x) {
-            const float y = wm[x][tid] == -INFINITY ? wl[x][tid] - wl[x][tid] : exp2f(wm[x][tid] - top);
-            sum = fmaf(wl[x][tid], y, sum);
-            wm[x][tid] = y;
-        }
-        f.m[tid] = top;
-        f.l[tid] = sum;
-    }
-    __syncthreads();
-    for (int i = tid; i < b.live * (F::DP / 4); i += W_THREADS) {
-        const int r = i / (F::DP / 4), d = (i - r * (F::DP / 4)) * 4;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int y = 0; y < W_WARPS; ++y) {
-            const float z = wm[y][r];
-            const float4 v = *(const float4*)(sums + ((size_t)y * ROWS + r) * F::DF + d);
-            x.x = fmaf(z, v.x, x.x); x.y = fmaf(z, v.y, x.y); x.z = fmaf(z, v.z, x.z); x.w = fmaf(z, v.w, x.w);
-        }
-        *(float4*)(sums + (size_t)r * F::DF + d) = x;
-    }
-    paged_fold<ROWS, W_KEYS, DT, F::DP>(p, b, sums, f);
+    for (int w = N; w < 32; w <<= 1) x = f(x, __shfl_xor_sync(0xffffffffu, x, w));
+    return x;
 }
 
-template <int N, int NT, int DT>
+template <int NR, int C, int DT>
+__global__ void __launch_bounds__(W_THREADS, 1) paged_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                                                                 const __grid_constant__ PagedParams p, const __grid_constant__ FewCopies cp) {
+    using X = Few<NR, C>;
+    constexpr int R = X::R, SLOTS = X::SLOTS;
+    constexpr float TOP = DT == 1 ? 6.f : 0.f;                     // float16 weights: from 2^6 down, so that small ones keep their bits; they grow to 2^14
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS], land, sfull[2], pready[2], pvdone[2];        // a barrier each: of two tiles both may have come before the first is looked for
+    __shared__ uint32_t tmem_base_s;
+    __shared__ __align__(16) float wmax[2][NR][4];
+    __shared__ PagedFold<NR> f;
+    __shared__ int missing;
+    int* const err = cp.err;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), D = p.dim;
+    const uint32_t ring = (smem_u32(smem) + 1023u) & ~1023u, ps = ring + SLOTS * X::TILE, qs = ps + X::PBUF * X::P;
+
+    if (warp == W_SOFT) tmem_alloc(&tmem_base_s, X::TMEM);
+    if (tid == 0) {
+        for (int s = 0; s < SLOTS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        mbar_init(&land, 1);
+        mbar_init(&sfull[0], 1); mbar_init(&sfull[1], 1);
+        mbar_init(&pready[0], W_SOFT); mbar_init(&pready[1], W_SOFT);
+        mbar_init(&pvdone[0], 1); mbar_init(&pvdone[1], 1);
+        mbar_fence_init();
+        missing = f.bad = 0;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_s, tmem_o = tmem + 2 * NR;
+    griddep_wait();
+    griddep_launch();
+
+    const PagedBlock<NR, W_KEYS> b(p, (int)blockIdx.x, (int)blockIdx.y, (int)blockIdx.z);
+    const int n = b.uend - b.ubeg, steps = (D + 15) / 16;
+    const int quad = warp & 3, half = (warp >> 2) & 1, r0 = half * R;
+
+    if (warp < W_SOFT) {
+        // ---------------- queries: rows of 128 bytes, 64 elements each, zeros behind the head's end
+        for (int i = tid; i < NR * C * 8; i += W_SOFT * 32) {
+            const int r = i / (C * 8), u = i - r * (C * 8), d = u * 8, x = b.f0 + r, row = x / p.rep, tok = b.first + row;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < b.live && d < D && tok >= 0 && tok < p.tokens) {
+                const uint16_t* src = (const uint16_t*)p.q + (size_t)tok * p.q_ld + (size_t)(b.head * p.rep + x - row * p.rep) * D + d;
+                if (p.wide_q) v = ld_act16(src);
+                else {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = (uint32_t)ld_act2(src + 2 * e) | (uint32_t)ld_act2(src + 2 * e + 1) << 16;
+                    v = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                         :: "r"(qs + (uint32_t)(u >> 3) * X::QCHUNK + (uint32_t)r * 128u + (uint32_t)(((u & 7) ^ (r & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+        }
+        const int last = min(b.end, b.uend * W_KEYS), step = cp.bp ? cp.bp : 1;
+        bool gone = false;
+        for (int j = b.ubeg * W_KEYS + step * tid; j < last; j += step * W_SOFT * 32) gone |= b.row_of(p, j) < 0;
+        if (gone) missing = 1;
+        fence_proxy_async();
+    }
+    if (warp <= W_SOFT) {                          // the copies are on their way meanwhile
+        __syncwarp();
+        asm volatile("bar.sync 5, %0;" :: "n"((W_SOFT + 1) * 32) : "memory");
+    }
+
+    if (warp == W_SOFT) {
+        // ---------------- MMAs, from one thread; the ring has K 0, K 1, V 0, K 2, V 1, ...
+        if (elect_one()) {
+            constexpr uint32_t types = DT == 1 ? ~((1u << 7) | (1u << 10)) : ~0u;        // both operands float16, or both bfloat16
+            constexpr uint32_t id_s = umma_idesc_bf16(NR) & types, id_o = umma_idesc_bf16_mn(2 * NR) & types;
+            RingPos at;
+            bool ok = true;
+            auto scores = [&](int i) {
+                ok = ok && bar_wait(err, smem_u32(&full[at.s]), at.round);
+                if (!ok) return;
+                tc_fence_after();
+                const uint64_t dk = desc_sw128(ring + at.s * X::TILE), dq = desc_sw128(qs);
+                const uint32_t to = tmem + (uint32_t)(i & 1) * NR;
+#pragma unroll
+                for (int k = 0; k < 4 * C; ++k)
+                    if (k < steps)
+                        umma_bf16(to, dk + (uint64_t)((k >> 2) * (W_CHUNK / 16) + (k & 3) * 2), dq + (uint64_t)((k >> 2) * (X::QCHUNK / 16) + (k & 3) * 2), id_s, k ? 1u : 0u);
+                umma_commit(&sfull[i & 1]);
+                umma_commit(&empty[at.s]);
+                at.next(SLOTS);
+            };
+            if (n > 0) scores(0);
+            int made = 0;
+            for (int i = 0; ok && i < n; ++i) {
+                if (i + 1 < n) scores(i + 1);      // where the scores of tile i - 1 were, whose weights have been waited for
+                ok = ok && bar_wait(err, smem_u32(&pready[i & 1]), (uint32_t)(i >> 1) & 1u) && bar_wait(err, smem_u32(&full[at.s]), at.round);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t from = ps + (X::PBUF == 2 ? (uint32_t)(i & 1) * X::P : 0u);
+                const uint64_t dv = desc_mn_sw128(ring + at.s * X::TILE, W_CHUNK);
+                const uint64_t dp = NR == 16 ? desc_mn_sw64(from, X::P) : desc_mn_sw128(from, W_CHUNK);
+#pragma unroll
+                for (int g = 0; g < X::DG; ++g)
+#pragma unroll
+                    for (int k = 0; k < W_KEYS / 16; ++k)          // 16 keys: 2048 bytes of V, 1024 or 2048 of the weights
+                        umma_bf16(tmem_o + (uint32_t)g * (2 * NR), dv + (uint64_t)(g * (2 * W_CHUNK / 16) + k * 128), dp + (uint64_t)(k * (NR == 16 ? 64 : 128)), id_o, (i | k) ? 1u : 0u);
+                umma_commit(&pvdone[i & 1]);
+                umma_commit(&empty[at.s]);
+                at.next(SLOTS);
+                made = i + 1;
+            }
+            if (made) bar_wait(err, smem_u32(&pvdone[(made - 1) & 1]), (uint32_t)((made - 1) >> 1) & 1u);
+        }
+        __syncwarp();
+    } else if (warp == W_SOFT + 1) {
+        // ---------------- copies
+        const int pieces = cp.bp ? W_KEYS / cp.bp : 32;
+        bool ok = true, bad = false;
+        int issued = 0;
+        uint32_t landed = 0;
+        RingPos at;
+        const int from = min(b.base, b.end);       // from here on values are looked at
+        // this lane's piece of tile i: no such position or page: zeros
+        auto where = [&](int i, int e) {
+            const int r = lane < pieces && i < n ? b.row_of(p, (b.ubeg + i) * W_KEYS + (cp.bp ? lane * cp.bp : 4 * lane + e)) : -1;
+            return r < 0 ? cp.rows : r;
+        };
+        int even[4], odd[4];                       // of tiles i and i + 1 by turns
+        auto look = [&](int i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e == 0 || !cp.bp) {
+                    const int r = where(i, e);
+                    if (i & 1) odd[e] = r;
+                    else even[e] = r;
+                }
+        };
+        auto fetch = [&](const CUtensorMap* map, int i, bool fix) {
+            ok = ok && all_wait(err, &empty[at.s], at.round ^ 1u);
+            if (!ok) return;
+            const uint32_t bar = smem_u32(fix ? &land : &full[at.s]), tile = ring + at.s * X::TILE;
+            if (lane == 0) mbar_expect_tx(bar, X::TILE);
+            __syncwarp();
+            const int x0 = i & 1 ? odd[0] : even[0];
+            if (cp.bp) {
+                if (lane < pieces)
+#pragma unroll
+                    for (int c = 0; c < C; ++c) tma_load_2d(tile + (uint32_t)c * W_CHUNK + (uint32_t)(lane * cp.bp) * 128u, map, c * 64, x0, bar);
+            } else {
+                const int x1 = i & 1 ? odd[1] : even[1], x2 = i & 1 ? odd[2] : even[2], x3 = i & 1 ? odd[3] : even[3];
+#pragma unroll
+                for (int c = 0; c < C; ++c) tma_gather4(tile + (uint32_t)c * W_CHUNK + (uint32_t)lane * 512u, map, c * 64, x0, x1, x2, x3, bar);
+            }
+            ++issued;
+            if (fix) {
+                ok = all_wait(err, &land, landed);
+                landed ^= 1u;
+                if (!ok) return;
+                // values of the step's rows: is any not finite?  The largest magnitude of a lane's says
+                const int j0 = (b.ubeg + i) * W_KEYS, k0 = max(0, from - j0), k1 = min(W_KEYS, b.end - j0);
+                auto unit = [&](uint32_t a, uint32_t (&x)[4]) {
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(a) : "memory");
+                };
+                auto put = [&](uint32_t a, const uint32_t (&x)[4]) {
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+                };
+                uint32_t most = 0;
+#pragma unroll 4
+                for (int e = k0 * 8 + lane; e < k1 * 8; e += 32)
+#pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        uint32_t x[4];
+                        unit(tile + (uint32_t)c * W_CHUNK + (uint32_t)e * 16u, x);
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) most = __vmaxu2(most, x[y] & 0x7fff7fffu);
+                    }
+                if (__any_sync(0xffffffffu, paged_unfinite<DT>(most) != 0)) {
+                    bad = true;
+                    for (int e = k0 * 8 + lane; e < k1 * 8; e += 32)
+                        for (int c = 0; c < C; ++c) {
+                            const uint32_t a = tile + (uint32_t)c * W_CHUNK + (uint32_t)e * 16u;
+                            uint32_t x[4];
+                            unit(a, x);
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) x[y] &= ~paged_unfinite<DT>(x[y]);
+                            put(a, x);
+                        }
+                }
+                // what lies behind the end in the last copy (what was not copied is zeros)
+                const uint32_t none[4] = {0, 0, 0, 0};
+                const int z1 = cp.bp ? min(W_KEYS, (max(0, k1) + cp.bp - 1) & ~(cp.bp - 1)) : 0;
+                for (int e = max(0, k1) * 8 + lane; e < z1 * 8; e += 32)
+#pragma unroll
+                    for (int c = 0; c < C; ++c) put(tile + (uint32_t)c * W_CHUNK + (uint32_t)e * 16u, none);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[at.s]);
+            }
+            at.next(SLOTS);
+        };
+        if (n > 0) {
+            look(0);
+            fetch(&kmap, 0, false);
+            look(1);
+            for (int i = 0; ok && i < n; ++i) {
+                if (i + 1 < n) fetch(&kmap, i + 1, false);
+                if (ok) fetch(&vmap, i, (b.ubeg + i + 1) * W_KEYS > from);
+                look(i + 2);
+            }
+        }
+        if (bad) f.bad = 1;
+        if (lane == 0)
+            for (int j = max(0, issued - SLOTS); j < issued; ++j)         // whoever gave up: do not leave with copies in flight
+                bar_wait(err, smem_u32(&full[j % SLOTS]), (uint32_t)(j / SLOTS) & 1u);
+        __syncwarp();
+    } else {
+        // ---------------- weights: lane = key, rows r0 ... r0 + R - 1
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+        const int clean = missing ? 0 : min(b.base, b.end);               // keys before this one are seen by all
+        const int key = quad * 32 + lane, mine = r0 + (lane & (R - 1));    // the row whose reference the lane keeps
+        const int step_row = (b.f0 + mine) / p.rep, tok = b.first + step_row;
+        const bool live = mine < b.live && tok >= 0 && tok < p.tokens;
+        float m_r = -INFINITY, nm[R], l[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) nm[r] = l[r] = 0.f;
+        bool ok = true;
+        for (int i = 0; i < n; ++i) {
+            const int j0 = (b.ubeg + i) * W_KEYS + quad * 32, j = j0 + lane;
+            const bool edge = j0 + 32 > clean;
+            uint32_t see = 0;                      // of the warp's keys the ones that the lane's row sees
+            bool there = true;
+            if (edge) {
+                see = live && j0 < b.end ? paged_window(p, tok, step_row, j0 - b.base) : 0u;
+                there = missing ? b.row_of(p, j) >= 0 : j < b.end;
+            }
+            ok = ok && all_wait(err, &sfull[i & 1], (uint32_t)((i >> 1) & 1));
+            __syncwarp();
+            tc_fence_after();
+            float s[R];
+            tmem_columns<R>(lanes + (uint32_t)(i & 1) * NR + (uint32_t)r0, s);
+            if (edge) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const uint32_t bits = __shfl_sync(0xffffffffu, see, r);
+                    if (!there || !((bits >> lane) & 1u)) s[r] = -INFINITY;
+                }
+            }
+            float v[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) v[r] = s[r];
+            const float top = reduce_lanes<R>(v, lane, [](float x, float y) { return fmaxf(x, y); });
+            if (lane < R) wmax[i & 1][r0 + lane][quad] = top;
+            __syncwarp();
+            asm volatile("bar.sync %0, 128;" :: "r"(1 + half) : "memory");
+            const float4 w = *(const float4*)wmax[i & 1][mine];
+            const float mt = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)) * p.scale_log2 - TOP;
+            const bool up = mt > m_r + PAGED_LAZY;                // (also the first finite maximum)
+            bool waited = false;
+            if (__any_sync(0xffffffffu, up)) {                    // the same in the half's four warps: its columns of O^T move along
+                const float f_r = !up ? 1.f : (m_r == -INFINITY ? 0.f : exp2f(m_r - mt));
+                if (up) m_r = mt;
+                float fix[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    nm[r] = paged_neg(__shfl_sync(0xffffffffu, m_r, r));
+                    fix[r] = __shfl_sync(0xffffffffu, f_r, r);
+                    l[r] *= fix[r];
+                }
+                if (i > 0) {
+                    ok = ok && all_wait(err, &pvdone[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u);
+                    __syncwarp();
+                    waited = true;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int g = 0; g < 2 * X::DG; ++g) {
+                        const uint32_t to = lanes + 2 * NR + (uint32_t)g * NR + (uint32_t)r0;
+                        float o[R];
+                        tmem_columns<R>(to, o);
+#pragma unroll
+                        for (int r = 0; r < R; ++r) o[r] *= fix[r];
+#pragma unroll
+                        for (int r = 0; r < R; r += 8) tmem_st8(to + (uint32_t)r, o + r);
+                    }
+                    tmem_st_wait();
+                }
+            }
+            uint32_t hi[R / 2], lo[R / 2];
+#pragma unroll
+            for (int e = 0; e < R / 2; ++e) {
+                const float a = ex2(fmaf(s[2 * e], p.scale_log2, nm[2 * e])), c = ex2(fmaf(s[2 * e + 1], p.scale_log2, nm[2 * e + 1]));
+                l[2 * e] += a;
+                l[2 * e + 1] += c;
+                hi[e] = paged_pack2<DT>(a, c);
+                if constexpr (DT == 1) {
+                    const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+                    lo[e] = paged_pack2<DT>(a - back.x, c - back.y);
+                } else
+                    lo[e] = pack_bf16x2(a - bf16lo(hi[e]), c - bf16hi(hi[e]));
+            }
+            // the product that has read what was here: of the tile before, or the one before that
+            if (i >= X::PBUF && !waited) {
+                ok = ok && all_wait(err, &pvdone[(i - X::PBUF) & 1], (uint32_t)((i - X::PBUF) >> 1) & 1u);
+                __syncwarp();
+            }
+            const uint32_t to = ps + (X::PBUF == 2 ? (uint32_t)(i & 1) * X::P : 0u);
+            auto put = [&](int term, int u, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+                uint32_t a;
+                if constexpr (NR == 16) a = to + (uint32_t)key * 64u + (uint32_t)(((2 * term + half) ^ ((key >> 1) & 3)) << 4);
+                else if constexpr (NR == 32) a = to + (uint32_t)key * 128u + (uint32_t)(((4 * term + 2 * half + u) ^ (key & 7)) << 4);
+                else a = to + (uint32_t)term * W_CHUNK + (uint32_t)key * 128u + (uint32_t)(((4 * half + u) ^ (key & 7)) << 4);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+            };
+#pragma unroll
+            for (int u = 0; u < R / 8; ++u) {
+                put(0, u, hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]);
+                put(1, u, lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]);
+            }
+            fence_proxy_async();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pready[i & 1]);
+        }
+        // ---------------- a row's reference and sum
+        const float sum = reduce_lanes<R>(l, lane, [](float x, float y) { return x + y; });
+        asm volatile("bar.sync %0, 128;" :: "r"(1 + half) : "memory");             // the last tile's maxima are read
+        if (lane < R) wmax[0][r0 + lane][quad] = sum;
+        __syncwarp();
+        asm volatile("bar.sync %0, 128;" :: "r"(1 + half) : "memory");
+        if (quad == 0 && lane < R) {
+            const float4 w = *(const float4*)wmax[0][mine];
+            f.m[mine] = m_r;
+            f.l[mine] = (w.x + w.y) + (w.z + w.w);
+        }
+    }
+    __syncthreads();                               // nobody's tile is read or written any more
+    tc_fence_after();
+    float* const sums = (float*)(smem + (ring - smem_u32(smem)));  // [NR][DN + 4]
+    if (warp < W_SOFT) {
+#pragma unroll 1
+        for (int g = 0; g < X::DG; ++g) {
+            const int d = g * 128 + quad * 32 + lane;
+            const uint32_t at = tmem_o + ((uint32_t)(quad * 32) << 16) + (uint32_t)g * (2 * NR) + (uint32_t)r0;
+            float x[R], y[R];
+            if (n > 0) {
+                tmem_columns<R>(at, x);
+                tmem_columns<R>(at + NR, y);
+            } else {
+#pragma unroll
+                for (int r = 0; r < R; ++r) x[r] = y[r] = 0.f;
+            }
+            if (d < X::DN) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) sums[(r0 + r) * (X::DN + 4) + d] = x[r] + y[r];
+            }
+            __syncwarp();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == W_SOFT) tmem_dealloc(tmem, X::TMEM);
+    paged_fold<NR, W_KEYS, DT, X::DN>(p, b, sums, f);
+}
+
+template <int NR, int C, int DT>
 int launch_few(PagedParams p, cudaStream_t st) {
-    using F = Few<N, NT>;
+    using X = Few<NR, C>;
     static bool configured = false;
+    static int at_once[PAGED_CLUSTER + 1] = {};
+    const auto kernel = paged_few_kernel<NR, C, DT>;
     if (!configured) {
-        PGK_CUDA(cudaFuncSetAttribute(paged_few_kernel<N, NT, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::BYTES));
-        PGK_CUDA(cudaFuncSetAttribute(paged_few_kernel<N, NT, DT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        PGK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, X::BYTES));
+        PGK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        for (int i = 1; i <= PAGED_CLUSTER; ++i) PGK_CUDA(clusters_at_once(&at_once[i], kernel, W_THREADS, X::BYTES, i));
         configured = true;
     }
-    p.tiles = (int)(((long long)p.max_rows * p.rep + F::ROWS - 1) / F::ROWS);
-    p.splits = paged_cut(p, (long long)p.seqs * p.tiles * p.kv_heads, W_KEYS, W_WARPS, F::RESIDENT, 6.f, PAGED_CLUSTER);
-    PGK_CUDA(launch_clusters(paged_few_kernel<N, NT, DT>, dim3((unsigned)(p.seqs * p.tiles), p.kv_heads, p.splits), W_THREADS, F::BYTES, st, p));
+    FewCopies cp = {};
+    cp.bp = p.page_size & -p.page_size;
+    if (cp.bp > W_KEYS) cp.bp = W_KEYS;
+    if (cp.bp < 8) cp.bp = 0;
+    cp.rows = p.pages * p.kv_heads * p.page_size;
+    cp.err = wait_word(kWaitPaged);
+    PGK_REQUIRE(cp.err, "paged_attention failed: no pinned host memory");
+    CUtensorMap kmap{}, vmap{};
+    const uint32_t box = cp.bp ? (uint32_t)cp.bp : 1u;
+    PGK_REQUIRE(tma_encode_fn() && tma_map_bf16_2d(&kmap, p.k_data, (uint64_t)p.dim, (uint64_t)cp.rows, (uint64_t)p.dim * 2, 64, box) &&
+                    tma_map_bf16_2d(&vmap, p.v_data, (uint64_t)p.dim, (uint64_t)cp.rows, (uint64_t)p.dim * 2, 64, box),
+                "paged_attention failed: no tensor map of %d rows of %d elements", cp.rows, p.dim);
+    p.tiles = (int)(((long long)p.max_rows * p.rep + NR - 1) / NR);
+    p.splits = paged_clusters(p, W_KEYS, at_once, PAGED_CLUSTER);
+    PGK_CUDA(launch_clusters(kernel, dim3((unsigned)(p.seqs * p.tiles), p.kv_heads, p.splits), W_THREADS, (size_t)X::BYTES, st, kmap, vmap, p, cp));
     return 0;
+}
+template <int C, int DT>
+int launch_few_rows(const PagedParams& p, cudaStream_t st) {
+    const long long rows = (long long)p.max_rows * p.rep;
+    if (rows <= 16) return launch_few<16, C, DT>(p, st);
+    return rows <= 32 ? launch_few<32, C, DT>(p, st) : launch_few<64, C, DT>(p, st);
 }
 template <int DT>
 int launch_few_dim(const PagedParams& p, cudaStream_t st) {
-    const bool two = (long long)p.max_rows * p.rep > 8;
-    switch ((p.dim + 31) / 32) {
-        case 1: case 2: return two ? launch_few<2, 2, DT>(p, st) : launch_few<2, 1, DT>(p, st);
-        case 3: return two ? launch_few<3, 2, DT>(p, st) : launch_few<3, 1, DT>(p, st);
-        case 4: return two ? launch_few<4, 2, DT>(p, st) : launch_few<4, 1, DT>(p, st);
-        case 5: case 6: return launch_few<6, 1, DT>(p, st);
-        default: return launch_few<8, 1, DT>(p, st);
+    switch ((p.dim + 63) / 64) {
+        case 1: return launch_few_rows<1, DT>(p, st);
+        case 2: return launch_few_rows<2, DT>(p, st);
+        case 3: return launch_few_rows<3, DT>(p, st);
+        default: return launch_few_rows<4, DT>(p, st);
     }
 }
 

@@ -17,7 +17,7 @@ namespace pgk {
 
 namespace {
 
-constexpr int T_ROWS = 128, T_KEYS = 128, T_SOFT = 8, T_THREADS = (T_SOFT + 2) * 32, T_STAGES = 3, T_CLUSTER = 8;
+constexpr int T_ROWS = 128, T_KEYS = 128, T_SOFT = 8, T_THREADS = (T_SOFT + 2) * 32, T_STAGES = 3;
 constexpr uint32_t T_CHUNK = T_KEYS * 128;                         // 64 elements of 128 keys
 constexpr uint32_t T_O = 0, T_Q = 128, T_S = 256;                  // TMEM columns: outputs, queries, two tiles of scores
 
@@ -373,30 +373,15 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
     paged_fold<T_ROWS, T_KEYS, DT, X::DN>(p, b, sums, f);
 }
 
-// How many blocks of a cluster share a sequence's keys: rounds of clusters times (a block's tiles + what it costs besides, about four of them).  How many clusters
-// run at once is asked for: of eight blocks, one a SM, fewer than 148 / 8.
 template <int C, int DT>
 int launch_tiles(PagedParams p, cudaStream_t st) {
     static bool configured = false;
-    static int at_once[4] = {};
+    static int at_once[PAGED_CLUSTER + 1] = {};
     const auto kernel = paged_tc_kernel<C, DT>;
     if (!configured) {
         PGK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<C>::SMEM));
-        for (int i = 0; 1 << i <= T_CLUSTER; ++i) {
-            cudaLaunchConfig_t cfg = {};
-            cudaLaunchAttribute attr[1];
-            attr[0].id = cudaLaunchAttributeClusterDimension;
-            attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
-            attr[0].val.clusterDim.z = 1u << i;
-            cfg.gridDim = dim3(1, 1, 1 << i);
-            cfg.blockDim = dim3(T_THREADS);
-            cfg.dynamicSmemBytes = Tile<C>::SMEM;
-            cfg.attrs = attr;
-            cfg.numAttrs = 1;
-            int n = 0;
-            PGK_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
-            at_once[i] = n > 0 ? n : 1;
-        }
+        PGK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        for (int i = 1; i <= PAGED_CLUSTER; ++i) PGK_CUDA(clusters_at_once(&at_once[i], kernel, T_THREADS, Tile<C>::SMEM, i));
         configured = true;
     }
     Copies cp = {};
@@ -410,13 +395,7 @@ int launch_tiles(PagedParams p, cudaStream_t st) {
                     tma_map_bf16_2d(&vmap, p.v_data, (uint64_t)p.dim, (uint64_t)cp.rows, (uint64_t)p.dim * 2, 64, (uint32_t)cp.bp),
                 "paged_attention failed: no tensor map of %d rows of %d elements", cp.rows, p.dim);
     p.tiles = (int)(((long long)p.max_rows * p.rep + T_ROWS - 1) / T_ROWS);
-    const int nt = (p.max_keys + T_KEYS - 1) / T_KEYS;
-    const long long items = (long long)p.seqs * p.tiles * p.kv_heads;
-    long long least = 0;
-    for (int i = 0; 1 << i <= T_CLUSTER; ++i) {
-        const long long cost = ((items + at_once[i] - 1) / at_once[i]) * ((nt + (1 << i) - 1) / (1 << i) + 4);
-        if (i == 0 || cost < least) { p.splits = 1 << i; least = cost; }
-    }
+    p.splits = paged_clusters(p, T_KEYS, at_once, PAGED_CLUSTER);
     PGK_CUDA(launch_clusters(kernel, dim3((unsigned)(p.seqs * p.tiles), p.kv_heads, p.splits), T_THREADS, (size_t)Tile<C>::SMEM, st, kmap, vmap, p, cp));
     return 0;
 }
@@ -425,7 +404,7 @@ int launch_tiles(PagedParams p, cudaStream_t st) {
 
 // More rows than a block of the other kernel has; copies of eight positions and more, 16 bytes at a time
 bool paged_tc_serves(const PagedParams& p, int dtype) {
-    return dtype != 0 && p.dim >= 64 && p.dim <= 128 && p.page_size % 8 == 0 && (long long)p.max_rows * p.rep > 16 && tma_encode_fn() != nullptr;
+    return dtype != 0 && p.dim >= 64 && p.dim <= 128 && p.page_size % 8 == 0 && (long long)p.max_rows * p.rep > 32 && tma_encode_fn() != nullptr;
 }
 int paged_tc(const PagedParams& p, int dtype, cudaStream_t st) {
     if (p.dim == 64) return dtype == 1 ? launch_tiles<1, 1>(p, st) : launch_tiles<1, 2>(p, st);
