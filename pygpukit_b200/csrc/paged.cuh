@@ -34,20 +34,6 @@ int paged_f32(const PagedParams& p, cudaStream_t st);
 
 constexpr int PAGED_CLUSTER = 16;         // blocks that share a sequence's keys, at most
 
-// Blocks of a cluster that share a sequence's keys, `step` of them a warp and turn: time in turns, a block's own with about `ends` of them for what it spends at its
-// two ends, or the SMs' share of all blocks.
-inline int paged_cut(const PagedParams& p, long long items, int step, int warps, int resident, float ends, int most) {
-    const int nb = (p.max_keys + step - 1) / step;
-    int best = 1;
-    float least = 0.f;
-    for (int s = 1; s <= most; s *= 2) {
-        const float each = (float)(((nb + s - 1) / s + warps - 1) / warps) + ends, all = (float)(items * s) * each / (float)(sm_count() * resident);
-        const float cost = each > all ? each : all;
-        if (s == 1 || cost < least) { best = s; least = cost; }
-    }
-    return best;
-}
-
 // How many clusters of a kernel run at once: of eight blocks, one a SM, fewer than 148 / 8
 template <typename... KArgs>
 inline cudaError_t clusters_at_once(int* out, void (*kernel)(KArgs...), int threads, size_t smem, int blocks) {
@@ -67,14 +53,14 @@ inline cudaError_t clusters_at_once(int* out, void (*kernel)(KArgs...), int thre
     if (n > 0) *out = n;
     return cudaSuccess;
 }
-// Blocks of a cluster that share a sequence's tiles, a block a SM: rounds of clusters times (a block's tiles + what it costs besides, about four of them)
-inline int paged_clusters(const PagedParams& p, int keys, const int* at_once, int most) {
+// Blocks of a cluster that share a sequence's tiles: rounds of clusters times (a block's tiles + what it costs besides, in tiles)
+inline int paged_clusters(const PagedParams& p, int keys, const int* at_once, int most, int ends) {
     const int nt = (p.max_keys + keys - 1) / keys;
     const long long items = (long long)p.seqs * p.tiles * p.kv_heads;
     long long least = 0;
     int best = 1;
     for (int s = 1; s <= most; ++s) {
-        const long long cost = ((items + at_once[s] - 1) / at_once[s]) * ((nt + s - 1) / s + 4);
+        const long long cost = ((items + at_once[s] - 1) / at_once[s]) * ((nt + s - 1) / s + ends);
         if (s == 1 || cost < least) { best = s; least = cost; }
     }
     return best;
@@ -192,6 +178,44 @@ template <int DT> __device__ __forceinline__ float paged_float(const void* base,
 template <int DT> __device__ __forceinline__ uint32_t paged_unfinite(uint32_t w) {
     constexpr uint32_t E = DT == 1 ? 0x7c00u : 0x7f80u;
     return ((w & E) == E ? 0xffffu : 0u) | ((w & (E << 16)) == (E << 16) ? 0xffff0000u : 0u);
+}
+// pairs of float32 in a register pair: one instruction for two products or sums
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// the lanes' N values (a power of two up to 32) reduced over the warp: lane l ends with value l % N
+template <int N, typename F> __device__ __forceinline__ float reduce_lanes(float (&v)[N], int lane, F f) {
+#pragma unroll
+    for (int w = N / 2; w > 0; w >>= 1) {
+        const bool up = lane & w;
+#pragma unroll
+        for (int j = 0; j < w; ++j) {
+            const float got = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + w], w);
+            v[j] = f(up ? v[j + w] : v[j], got);
+        }
+    }
+    float x = v[0];
+#pragma unroll
+    for (int w = N; w < 32; w <<= 1) x = f(x, __shfl_xor_sync(0xffffffffu, x, w));
+    return x;
 }
 // 2^(s - m) for a reference that is not there yet (m = -infinity)
 __device__ __forceinline__ float paged_neg(float m) { return m == -INFINITY ? 0.f : -m; }

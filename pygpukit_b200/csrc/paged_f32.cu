@@ -2,8 +2,8 @@
 //
 // A block has R (row, head) rows (4, 8 or 16: as many as a token's heads need), each of its warps walks over its own blocks of 32 keys, whose K and V it fetches to
 // shared memory by itself, K of the next block while this one's values are summed and V while its scores are formed.  Scores: a lane a key, the queries' elements are
-// broadcast; values: a lane four neighbouring elements (and four 128 on), the weights are broadcast.  A row costs 2 instructions' issue a key and
-// element quartet beside the loads, so that few rows are bound by the cache's bytes and trees by the multiply-adds.  Blocks of a cluster share a sequence's keys.
+// broadcast; values: a lane four neighbouring elements (and four 128 on), the weights are broadcast.  Products are
+// pairs of float32 in one instruction.  Few rows are bound by the instructions that fetch and the chain of a turn, trees by the multiply-adds and what feeds them.  Blocks of a cluster share a sequence's keys.
 #include <type_traits>
 
 #include "paged.cuh"
@@ -22,7 +22,7 @@ __device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, b
 
 // PC: quartets of elements a lane has of an output row; W: warps
 template <int R, int PC, int W> struct Single {
-    static int warp_floats(int D) { return S_KEYS * (D + 4) + S_KEYS * D + R * S_KEYS; }
+    static int warp_floats(int D) { return S_KEYS * (D + 4) + S_KEYS * D + 2 * R * S_KEYS; }
     static int bytes(int D) {
         const int run = (R * D + W * warp_floats(D)) * 4, fold = W * R * (128 * PC + 4) * 4;
         return run > fold ? run : fold;
@@ -36,25 +36,32 @@ __global__ void __launch_bounds__(W * 32, 1) paged_f32_kernel(const __grid_const
     __shared__ PagedFold<R> f;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), D = p.dim, D4 = D / 4, DF = D + 4;
     float* const qs = smf;                                    // [R][D]
-    float* const ks = qs + R * D + warp * (S_KEYS * DF + S_KEYS * D + R * S_KEYS);
+    float* const ks = qs + R * D + warp * (S_KEYS * DF + S_KEYS * D + 2 * R * S_KEYS);
     float* const vs = ks + S_KEYS * DF;
-    float* const ps = vs + S_KEYS * D;                        // [R][32]
+    float2* const ps = (float2*)(vs + S_KEYS * D);            // [R][32], each weight twice
     if (tid == 0) f.bad = 0;
     griddep_wait();
     griddep_launch();
     const PagedBlock<R, S_KEYS> b(p, (int)blockIdx.x, (int)blockIdx.y, (int)blockIdx.z);
 
     auto fetch = [&](const void* base, float* to, int ld, int rows) {
-        const float* const src = (const float*)base;
+        const float* const src = (const float*)base + 4 * (D4 <= 16 ? lane & 15 : lane);
         if (D4 <= 16) {                                       // two keys at a time
-            for (int r = 0; r < S_KEYS; r += 2) {
-                const int key = r + (lane >> 4), c = lane & 15, row = __shfl_sync(0xffffffffu, rows, key);
-                if (c < D4) cp_async16_or_zero(to + key * ld + 4 * c, src + (size_t)max(row, 0) * D + 4 * c, row >= 0);
+            float* dst = to + (lane >> 4) * ld + 4 * (lane & 15);
+#pragma unroll 8
+            for (int r = 0; r < S_KEYS; r += 2, dst += 2 * ld) {
+                const int row = __shfl_sync(0xffffffffu, rows, r + (lane >> 4));
+                if ((lane & 15) < D4) cp_async16_or_zero(dst, src + (size_t)max(row, 0) * D, row >= 0);
             }
         } else {
-            for (int r = 0; r < S_KEYS; ++r) {
+            float* dst = to + 4 * lane;
+#pragma unroll 8
+            for (int r = 0; r < S_KEYS; ++r, dst += ld) {
                 const int row = __shfl_sync(0xffffffffu, rows, r);
-                for (int c = lane; c < D4; c += 32) cp_async16_or_zero(to + r * ld + 4 * c, src + (size_t)max(row, 0) * D + 4 * c, row >= 0);
+                const float* const from = src + (size_t)max(row, 0) * D;
+#pragma unroll
+                for (int c = 0; c < PC; ++c)
+                    if (lane + 32 * c < D4) cp_async16_or_zero(dst + 128 * c, from + 128 * c, row >= 0);
             }
         }
         cp_async_commit();
@@ -71,14 +78,13 @@ __global__ void __launch_bounds__(W * 32, 1) paged_f32_kernel(const __grid_const
     }
     __syncthreads();
 
-    float4 o[R][PC];
-    float m[R], l[R];
+    uint64_t o[R][PC][2];                                     // pairs of elements
+    float m_r = -INFINITY, nm[R], l[R];                      // lane r keeps row r's reference
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        m[r] = -INFINITY;
-        l[r] = 0.f;
+        nm[r] = l[r] = 0.f;
 #pragma unroll
-        for (int c = 0; c < PC; ++c) o[r][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < PC; ++c) o[r][c][0] = o[r][c][1] = pair(0.f, 0.f);
     }
     bool bad = false;
 #pragma unroll 1
@@ -86,17 +92,18 @@ __global__ void __launch_bounds__(W * 32, 1) paged_f32_kernel(const __grid_const
         const int j0 = k * S_KEYS, next = k + W < b.uend ? b.row_of(p, (k + W) * S_KEYS + lane) : -1;
         cp_async_wait<1>();                                   // K is here
         __syncwarp();
-        float s[R];
+        uint64_t s2[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) s[r] = 0.f;
+        for (int r = 0; r < R; ++r) s2[r] = pair(0.f, 0.f);
         const float* const kr = ks + lane * DF;
-#pragma unroll 2
+#pragma unroll 4
         for (int c = 0; c < D4; ++c) {
-            const float4 x = *(const float4*)(kr + 4 * c);
+            const ulonglong2 x = *(const ulonglong2*)(kr + 4 * c);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const float4 q = *(const float4*)(qs + r * D + 4 * c);
-                s[r] = fmaf(q.x, x.x, fmaf(q.y, x.y, fmaf(q.z, x.z, fmaf(q.w, x.w, s[r]))));
+                const ulonglong2 q = *(const ulonglong2*)(qs + r * D + 4 * c);
+                s2[r] = fma2(q.x, x.x, s2[r]);
+                s2[r] = fma2(q.y, x.y, s2[r]);
             }
         }
         __syncwarp();
@@ -104,24 +111,37 @@ __global__ void __launch_bounds__(W * 32, 1) paged_f32_kernel(const __grid_const
         else cp_async_commit();
         const bool edge = __any_sync(0xffffffffu, rows < 0) || j0 + S_KEYS > b.base;
         const int at = j0 - b.base;
+        float s[R], v[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            float x = s[r] * p.scale_log2;
+            float a, c;
+            unpair(s2[r], a, c);
+            s[r] = (a + c) * p.scale_log2;
             if (edge) {
                 const int i = (b.f0 + r) / p.rep, t = at + lane;
-                if (rows < 0 || r >= b.live || (t >= 0 && !paged_sees(p, b.first + i, i, t))) x = -INFINITY;
+                if (rows < 0 || r >= b.live || (t >= 0 && !paged_sees(p, b.first + i, i, t))) s[r] = -INFINITY;
             }
-            const float top = warp_max(x);
-            if (top > m[r] + PAGED_LAZY) {                    // the same in all lanes; also the first finite maximum
-                const float fix = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top);
-                m[r] = top;
+            v[r] = s[r];
+        }
+        const float top = reduce_lanes<R>(v, lane, [](float x, float y) { return fmaxf(x, y); });
+        const bool up = top > m_r + PAGED_LAZY;               // (also the first finite maximum)
+        if (__any_sync(0xffffffffu, up)) {
+            const float f_r = !up ? 1.f : (m_r == -INFINITY ? 0.f : exp2f(m_r - top));
+            if (up) m_r = top;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float fix = __shfl_sync(0xffffffffu, f_r, r);
+                nm[r] = paged_neg(__shfl_sync(0xffffffffu, m_r, r));
                 l[r] *= fix;
 #pragma unroll
-                for (int c = 0; c < PC; ++c) { o[r][c].x *= fix; o[r][c].y *= fix; o[r][c].z *= fix; o[r][c].w *= fix; }
+                for (int c = 0; c < PC; ++c) { o[r][c][0] = mul2(o[r][c][0], pair(fix, fix)); o[r][c][1] = mul2(o[r][c][1], pair(fix, fix)); }
             }
-            const float w = ex2(x + paged_neg(m[r]));
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float w = ex2(s[r] + nm[r]);
             l[r] += w;
-            ps[r * S_KEYS + lane] = w;
+            ps[r * S_KEYS + lane] = make_float2(w, w);
         }
         cp_async_wait<1>();                                   // V is here
         __syncwarp();
@@ -144,14 +164,14 @@ __global__ void __launch_bounds__(W * 32, 1) paged_f32_kernel(const __grid_const
                     }
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const float4 w = *(const float4*)(ps + r * S_KEYS + key);
-                    const float wu[4] = {w.x, w.y, w.z, w.w};
+                    const ulonglong2 w0 = *(const ulonglong2*)(ps + r * S_KEYS + key), w1 = *(const ulonglong2*)(ps + r * S_KEYS + key + 2);
+                    const uint64_t w[4] = {w0.x, w0.y, w1.x, w1.y};
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
 #pragma unroll
                         for (int c = 0; c < PC; ++c) {
-                            o[r][c].x = fmaf(wu[u], v[u][c].x, o[r][c].x); o[r][c].y = fmaf(wu[u], v[u][c].y, o[r][c].y);
-                            o[r][c].z = fmaf(wu[u], v[u][c].z, o[r][c].z); o[r][c].w = fmaf(wu[u], v[u][c].w, o[r][c].w);
+                            o[r][c][0] = fma2(w[u], pair(v[u][c].x, v[u][c].y), o[r][c][0]);
+                            o[r][c][1] = fma2(w[u], pair(v[u][c].z, v[u][c].w), o[r][c][1]);
                         }
                 }
             }
@@ -167,10 +187,11 @@ __global__ void __launch_bounds__(W * 32, 1) paged_f32_kernel(const __grid_const
 
     // ---------------- the warps' sums into one
     if (bad) f.bad = 1;
+    if (lane < R) wm[warp][lane] = m_r;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         l[r] = warp_sum(l[r]);
-        if (lane == 0) { wm[warp][r] = m[r]; wl[warp][r] = l[r]; }
+        if (lane == 0) wl[warp][r] = l[r];
     }
     __syncthreads();
     float* const fold = smf;                                  // [W][R][FS]
@@ -179,7 +200,7 @@ __global__ void __launch_bounds__(W * 32, 1) paged_f32_kernel(const __grid_const
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int c = 0; c < PC; ++c)
-            if (lane + 32 * c < D4) *(float4*)(fold + (warp * R + r) * FS + 4 * (lane + 32 * c)) = o[r][c];
+            if (lane + 32 * c < D4) *(ulonglong2*)(fold + (warp * R + r) * FS + 4 * (lane + 32 * c)) = make_ulonglong2(o[r][c][0], o[r][c][1]);
     __syncthreads();
     if (tid < R) {
         float top = -INFINITY, sum = 0.f;
@@ -214,9 +235,12 @@ int launch_single(PagedParams p, cudaStream_t st) {
         PGK_CUDA(cudaFuncSetAttribute(paged_f32_kernel<R, PC, W>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         configured = true;
     }
-    const int smem = Single<R, PC, W>::bytes(p.dim), resident = smem > 110 * 1024 ? 1 : (smem > 72 * 1024 ? 2 : 3);
+    const int smem = Single<R, PC, W>::bytes(p.dim), kind = smem > 113 * 1024 ? 0 : (smem > 75 * 1024 ? 1 : 2);       // one, two, three blocks a SM
+    static int at_once[3][PAGED_CLUSTER + 1] = {};
+    if (at_once[kind][1] == 0)
+        for (int i = 1; i <= PAGED_CLUSTER; ++i) PGK_CUDA(clusters_at_once(&at_once[kind][i], paged_f32_kernel<R, PC, W>, W * 32, (size_t)smem, i));
     p.tiles = (int)(((long long)p.max_rows * p.rep + R - 1) / R);
-    p.splits = paged_cut(p, (long long)p.seqs * p.tiles * p.kv_heads, S_KEYS, W, resident, 3.f, PAGED_CLUSTER);
+    p.splits = paged_clusters(p, S_KEYS * W, at_once[kind], PAGED_CLUSTER, 2);
     PGK_CUDA(launch_clusters(paged_f32_kernel<R, PC, W>, dim3((unsigned)(p.seqs * p.tiles), p.kv_heads, p.splits), W * 32, (size_t)smem, st, p));
     return 0;
 }

@@ -44,39 +44,10 @@ __device__ __forceinline__ bool all_wait(int* err, uint64_t* bar, uint32_t parit
     const bool ok = bar_wait(err, smem_u32(bar), parity);
     return __all_sync(0xffffffffu, ok);
 }
-__device__ __forceinline__ void tmem_ld8_async(uint32_t taddr, float* v) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(taddr) : "memory");
-}
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const float* v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                  :: "r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
 }
-// N columns of a warp's lanes
-template <int N> __device__ __forceinline__ void tmem_columns(uint32_t taddr, float (&v)[N]) {
-#pragma unroll
-    for (int c = 0; c < N; c += 8) tmem_ld8_async(taddr + (uint32_t)c, v + c);
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int c = 0; c < N; ++c) asm volatile("" : "+f"(v[c]) :: "memory");
-}
-// the lanes' N values (8, 16 or 32) reduced over the warp: lane l ends with value l % N
-template <int N, typename F> __device__ __forceinline__ float reduce_lanes(float (&v)[N], int lane, F f) {
-#pragma unroll
-    for (int w = N / 2; w > 0; w >>= 1) {
-        const bool up = lane & w;
-#pragma unroll
-        for (int j = 0; j < w; ++j) {
-            const float got = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + w], w);
-            v[j] = f(up ? v[j + w] : v[j], got);
-        }
-    }
-    float x = v[0];
-#pragma unroll
-    for (int w = N; w < 32; w <<= 1) x = f(x, __shfl_xor_sync(0xffffffffu, x, w));
-    return x;
-}
-
 template <int NR, int C, int DT>
 __global__ void __launch_bounds__(W_THREADS, 1) paged_few_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                                                                  const __grid_constant__ PagedParams p, const __grid_constant__ FewCopies cp) {
@@ -116,6 +87,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) paged_few_kernel(const __grid_co
 
     if (warp < W_SOFT) {
         // ---------------- queries: rows of 128 bytes, 64 elements each, zeros behind the head's end
+#pragma unroll 4
         for (int i = tid; i < NR * C * 8; i += W_SOFT * 32) {
             const int r = i / (C * 8), u = i - r * (C * 8), d = u * 8, x = b.f0 + r, row = x / p.rep, tok = b.first + row;
             uint4 v = make_uint4(0, 0, 0, 0);
@@ -461,7 +433,7 @@ int launch_few(PagedParams p, cudaStream_t st) {
                     tma_map_bf16_2d(&vmap, p.v_data, (uint64_t)p.dim, (uint64_t)cp.rows, (uint64_t)p.dim * 2, 64, box),
                 "paged_attention failed: no tensor map of %d rows of %d elements", cp.rows, p.dim);
     p.tiles = (int)(((long long)p.max_rows * p.rep + NR - 1) / NR);
-    p.splits = paged_clusters(p, W_KEYS, at_once, PAGED_CLUSTER);
+    p.splits = paged_clusters(p, W_KEYS, at_once, PAGED_CLUSTER, 4);
     PGK_CUDA(launch_clusters(kernel, dim3((unsigned)(p.seqs * p.tiles), p.kv_heads, p.splits), W_THREADS, (size_t)X::BYTES, st, kmap, vmap, p, cp));
     return 0;
 }

@@ -41,23 +41,6 @@ __device__ __forceinline__ bool all_wait(int* err, uint64_t* bar, uint32_t parit
     const bool ok = bar_wait(err, smem_u32(bar), parity);
     return __all_sync(0xffffffffu, ok);
 }
-// pairs of float32 in a register pair: one instruction for two products or sums
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 // 32 weights 2^(s scale + neg) to TMEM column `to`; their sum is of the unrounded ones
 template <int DT>
 __device__ __forceinline__ void weights32(const float* s, float scale, float neg, uint32_t to, uint64_t& l) {
@@ -395,7 +378,7 @@ int launch_tiles(PagedParams p, cudaStream_t st) {
                     tma_map_bf16_2d(&vmap, p.v_data, (uint64_t)p.dim, (uint64_t)cp.rows, (uint64_t)p.dim * 2, 64, (uint32_t)cp.bp),
                 "paged_attention failed: no tensor map of %d rows of %d elements", cp.rows, p.dim);
     p.tiles = (int)(((long long)p.max_rows * p.rep + T_ROWS - 1) / T_ROWS);
-    p.splits = paged_clusters(p, T_KEYS, at_once, PAGED_CLUSTER);
+    p.splits = paged_clusters(p, T_KEYS, at_once, PAGED_CLUSTER, 4);
     PGK_CUDA(launch_clusters(kernel, dim3((unsigned)(p.seqs * p.tiles), p.kv_heads, p.splits), T_THREADS, (size_t)Tile<C>::SMEM, st, kmap, vmap, p, cp));
     return 0;
 }

@@ -1,12 +1,12 @@
 // paged_weigh.cu -- the attention weights that a cached position gets, summed over a step's rows and the query heads of its key head: what decides which positions of a
 // cache stay when it is cut.  weights[slot][g][j] += sum over rows i and heads h of g of exp(scale q_ih . k_j - lse_ih), lse from the attention over the same rows.
 //
-// Scores by mma.sync m16n8k16 with the keys as its 16, as in paged_few.cu, in float32 by multiply-adds.  A block has the step's rows in shared memory (all of them, or as many
-// as fit at a time) and a share of the positions; a warp walks over its own 16 by 16, the next on their way from memory to registers meanwhile.  A
-// position's sum is one thread's until it is added, so that the same call gives the same bits.  Decoding is bound by the bytes of the keys, windows of a prompt's last tokens by
-// products and exponentials.
+// 16-bit pages: scores S^T[128 keys, NR rows] = K Q^T by tcgen05 as in paged_few.cu, tiles of K through a ring, the step's rows in shared memory (as many as 64 KB hold at a
+// time); eight warps, a lane a key and half of the rows each, sum the weights as they come.  32-bit pages: multiply-adds, a lane a key.  A position's sum is one
+// thread's until it is added, so that the same call gives the same bits.  Decoding is bound by the bytes of the keys, windows of a prompt's last tokens by the exponentials.
 #include "paged.cuh"
 #include "tc_common.cuh"
+#include "tma.cuh"
 #include "../../include/pgk_b200.h"
 
 namespace pgk {
@@ -14,126 +14,232 @@ namespace pgk {
 namespace {
 
 constexpr int H_ALL = 1 << 30;                                // rows of a "block": all of the sequence's
-constexpr int H_WARPS = 4, H_THREADS = H_WARPS * 32, H_KEYS = 16, H_RESIDENT = 4;
-constexpr int H_QBYTES = 48 * 1024;                           // queries of a block at a time: four blocks a SM
+constexpr int H_KEYS = 128, H_SOFT = 8, H_THREADS = (H_SOFT + 2) * 32, H_QBYTES = 64 * 1024;
+constexpr uint32_t H_CHUNK = H_KEYS * 128;                    // 64 elements of 128 keys
 constexpr int G_WARPS = 4, G_THREADS = G_WARPS * 32, G_KEYS = G_WARPS * 32, G_ROWS = 16;
 
 using Keys = PagedBlock<H_ALL, H_KEYS>;
+static_assert(H_KEYS == G_KEYS);
 
-template <int DT>
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (DT == 1)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// minus a row's logarithm (log2): -infinity for rows that do not exist or see nothing
+// minus a row's logarithm (log2); for rows that do not exist or see nothing a number that leaves no weight (a key's NaN is in the sums of the rows that see it all the same)
+constexpr float H_NONE = -3e38f;
 __device__ __forceinline__ float row_neg(const PagedParams& p, const Keys& b, int r) {
     const int tok = b.token(p, r);
-    if (r >= b.live || tok < 0 || tok >= p.tokens) return -INFINITY;
+    if (r >= b.live || tok < 0 || tok >= p.tokens) return H_NONE;
     const float z = __ldcg(p.lse + (size_t)tok * p.heads + b.head * p.rep + r % p.rep);
-    return z == -INFINITY ? -INFINITY : -z * PAGED_LOG2E;
+    return z == -INFINITY ? H_NONE : -z * PAGED_LOG2E;
 }
-__device__ __forceinline__ float weight(float s, float scale, float neg) { return neg == -INFINITY ? 0.f : ex2(fmaf(s, scale, neg)); }
 __device__ __forceinline__ void add_weight(const PagedParams& p, const Keys& b, int j, float w) {
     atomicAdd(p.weights + ((size_t)b.slot * p.kv_heads + b.head) * p.weights_ld + j, w);
 }
 
-// N: 32-element pieces of a head
-template <int N, int DT>
-__global__ void __launch_bounds__(H_THREADS, N <= 4 ? H_RESIDENT : 2) paged_weigh_kernel(const __grid_constant__ PagedParams p, int most) {
+struct WeighCopies {
+    int bp, rows;            // as in paged_few.cu
+    int groups;              // of NR rows, in shared memory at a time
+    int* err;
+};
+
+// NR: rows of a product; C: 64-element chunks of a head
+template <int NR, int C> struct Weigh {
+    static constexpr int R = NR / 2, SLOTS = C == 1 ? 4 : (C == 2 ? 3 : 2);
+    static constexpr uint32_t TILE = C * H_CHUNK, QCHUNK = NR * 128, Q = C * QCHUNK, TMEM = 2 * NR < 32 ? 32 : 2 * NR;
+    static constexpr int MOST = H_QBYTES / (int)Q;
+    static int bytes(int groups) { return SLOTS * (int)TILE + groups * ((int)Q + NR * 4) + 1024; }
+};
+
+template <int NR, int C, int DT>
+__global__ void __launch_bounds__(H_THREADS) paged_weigh_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ PagedParams p, const __grid_constant__ WeighCopies cp) {
+    using X = Weigh<NR, C>;
+    constexpr int R = X::R, SLOTS = X::SLOTS;
     extern __shared__ __align__(16) unsigned char smem[];
-    uint4* const qs = (uint4*)smem;                           // [tiles of eight rows][N][32]: lane (gl, t)'s elements 32 s + 8 t ... + 7 of row 8 n + gl
-    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), gl = lane >> 2, t = lane & 3, D = p.dim;
+    __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS], sfull[2], sread[2];
+    __shared__ uint32_t tmem_base_s;
+    __shared__ float other[2][H_KEYS];
+    __shared__ int missing;
+    int* const err = cp.err;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), D = p.dim;
+    const uint32_t ring = (smem_u32(smem) + 1023u) & ~1023u, qs = ring + SLOTS * X::TILE;
+    float* const negs = (float*)(smem + (qs - smem_u32(smem)) + (size_t)cp.groups * X::Q);        // [groups][NR]
+
+    if (warp == H_SOFT) tmem_alloc(&tmem_base_s, X::TMEM);
+    if (tid == 0) {
+        for (int s = 0; s < SLOTS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&sfull[s], 1); mbar_init(&sread[s], H_SOFT); }
+        mbar_fence_init();
+        missing = 0;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_s;
     griddep_wait();
     griddep_launch();
-    const Keys b(p, (int)blockIdx.z, (int)blockIdx.y, (int)blockIdx.x);
-    float* const negs = (float*)(qs + (size_t)most * N * 32);
-    if (b.ubeg >= b.uend || b.live == 0) return;
 
-    const char* const kb = (const char*)p.k_data;
-    const size_t stride = (size_t)D * 2;
-    uint4 kk[N][2], ahead[N][2];
-    auto load_k = [&](int rows, uint4 (&x)[N][2]) {
+    const Keys b(p, (int)blockIdx.z, (int)blockIdx.y, (int)blockIdx.x);
+    const int n = b.live > 0 ? b.uend - b.ubeg : 0, steps = (D + 15) / 16, batch = cp.groups * NR, batches = (b.live + batch - 1) / batch;
+    const int quad = warp & 3, half = (warp >> 2) & 1, r0 = half * R;
+
+    if (warp < H_SOFT) {
+        const int last = min(b.end, b.uend * H_KEYS), step = cp.bp ? cp.bp : 1;
+        bool gone = false;
+        for (int j = b.ubeg * H_KEYS + step * tid; j < last; j += step * H_SOFT * 32) gone |= b.row_of(p, j) < 0;
+        if (gone) missing = 1;
+    }
+    int turns = 0, tiles = 0;                      // of the batches before: score buffers and ring places that were used
+    bool ok = true;
+    for (int y = 0; y < batches; ++y) {
+        const int f0 = y * batch, groups = min(cp.groups, (b.live - f0 + NR - 1) / NR);
+        int turn = turns;
+        RingPos at;
+        at.s = (uint32_t)(tiles % SLOTS);
+        at.round = (uint32_t)(tiles / SLOTS) & 1u;
+        if (warp < H_SOFT) {
+            // ---------------- the batch's rows
+#pragma unroll 4
+            for (int i = tid; i < groups * NR * C * 8; i += H_SOFT * 32) {
+                const int r = i / (C * 8), u = i - r * (C * 8), d = u * 8, x = f0 + r, row = x / p.rep, tok = b.first + row, g = r / NR, rr = r - g * NR;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (x < b.live && d < D && tok >= 0 && tok < p.tokens) {
+                    const uint16_t* src = (const uint16_t*)p.q + (size_t)tok * p.q_ld + (size_t)(b.head * p.rep + x - row * p.rep) * D + d;
+                    if (p.wide_q) v = ld_act16(src);
+                    else {
+                        uint32_t w[4];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int row = __shfl_sync(0xffffffffu, rows, 8 * u + gl);
-            const char* const src = kb + (size_t)max(row, 0) * stride + 16 * t;
-#pragma unroll
-            for (int s = 0; s < N; ++s) {
-                x[s][u] = make_uint4(0, 0, 0, 0);
-                if (row >= 0 && 32 * s + 8 * t < D) x[s][u] = ld_act16(src + 64 * s);
+                        for (int e = 0; e < 4; ++e) w[e] = (uint32_t)ld_act2(src + 2 * e) | (uint32_t)ld_act2(src + 2 * e + 1) << 16;
+                        v = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                             :: "r"(qs + (uint32_t)g * X::Q + (uint32_t)(u >> 3) * X::QCHUNK + (uint32_t)rr * 128u + (uint32_t)(((u & 7) ^ (rr & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                             : "memory");
             }
+            for (int i = tid; i < groups * NR; i += H_SOFT * 32) negs[i] = row_neg(p, b, f0 + i);
+            fence_proxy_async();
         }
-    };
-    auto look = [&](int k) { return k < b.uend ? b.row_of(p, k * H_KEYS + (lane & 15)) : -1; };
-#pragma unroll 1
-    for (int f0 = 0; f0 < b.live; f0 += 8 * most) {
-        const int tiles = min(most, (b.live - f0 + 7) / 8);
-        int k = b.ubeg + warp, rows = look(k), next = look(k + H_WARPS);
-        load_k(rows, kk);
-        if (f0 > 0) __syncthreads();
-        for (int i = warp; i < tiles * N; i += H_WARPS) {
-            const int n = i / N, s = i - n * N, x = f0 + 8 * n + gl, d = 32 * s + 8 * t, row = x / p.rep, tok = b.first + row;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (x < b.live && d < D && tok >= 0 && tok < p.tokens) {
-                const uint16_t* src = (const uint16_t*)p.q + (size_t)tok * p.q_ld + (size_t)(b.head * p.rep + x - row * p.rep) * D + d;
-                if (p.wide_q) v = ld_act16(src);
-                else {
-                    uint32_t w[4];
+        if (warp <= H_SOFT) {                      // the copies are on their way meanwhile
+            __syncwarp();
+            asm volatile("bar.sync 5, %0;" :: "n"((H_SOFT + 1) * 32) : "memory");
+        }
+        if (warp == H_SOFT) {
+            // ---------------- MMAs, from one thread
+            if (elect_one()) {
+                for (int i = 0; ok && i < n; ++i) {
+                    ok = bar_wait(err, smem_u32(&full[at.s]), at.round);
+                    const uint64_t dk = desc_sw128(ring + at.s * X::TILE);
+                    for (int g = 0; ok && g < groups; ++g, ++turn) {
+                        ok = bar_wait(err, smem_u32(&sread[turn & 1]), ((uint32_t)(turn >> 1) & 1u) ^ 1u);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t dq = desc_sw128(qs + (uint32_t)g * X::Q);
+                        constexpr uint32_t types = DT == 1 ? ~((1u << 7) | (1u << 10)) : ~0u, id = umma_idesc_bf16(NR) & types;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = (uint32_t)ld_act2(src + 2 * e) | (uint32_t)ld_act2(src + 2 * e + 1) << 16;
-                    v = make_uint4(w[0], w[1], w[2], w[3]);
+                        for (int k = 0; k < 4 * C; ++k)
+                            if (k < steps)
+                                umma_bf16(tmem + (uint32_t)(turn & 1) * NR, dk + (uint64_t)((k >> 2) * (H_CHUNK / 16) + (k & 3) * 2),
+                                          dq + (uint64_t)((k >> 2) * (X::QCHUNK / 16) + (k & 3) * 2), id, k ? 1u : 0u);
+                        umma_commit(&sfull[turn & 1]);
+                    }
+                    if (ok) umma_commit(&empty[at.s]);
+                    at.next(SLOTS);
                 }
             }
-            qs[i * 32 + lane] = v;
-        }
-        for (int i = tid; i < 8 * tiles; i += H_THREADS) negs[i] = row_neg(p, b, f0 + i);
-        __syncthreads();
-#pragma unroll 1
-        for (; k < b.uend; k += H_WARPS) {
-            const int j0 = k * H_KEYS;
-            const uint32_t there = __ballot_sync(0xffffffffu, rows >= 0);
-            const bool edge = (there & 0xffffu) != 0xffffu || j0 + H_KEYS > b.base;
-            rows = next;
-            load_k(rows, ahead);
-            next = look(k + 2 * H_WARPS);
-            float sum0 = 0.f, sum1 = 0.f;                     // of keys gl and gl + 8: this lane's rows
-#pragma unroll 1
-            for (int n = 0; n < tiles; ++n) {
-                float s[4] = {0.f, 0.f, 0.f, 0.f};
+            __syncwarp();
+        } else if (warp == H_SOFT + 1) {
+            // ---------------- copies, as in paged_few.cu
+            const int pieces = cp.bp ? H_KEYS / cp.bp : 32;
+            int row[4];
+            auto look = [&](int i) {
 #pragma unroll
-                for (int q = 0; q < N; ++q) {
-                    const uint4 a = qs[(n * N + q) * 32 + lane];
-                    mma16816<DT>(s, kk[q][0].x, kk[q][1].x, kk[q][0].y, kk[q][1].y, a.x, a.y);
-                    mma16816<DT>(s, kk[q][0].z, kk[q][1].z, kk[q][0].w, kk[q][1].w, a.z, a.w);
+                for (int e = 0; e < 4; ++e) {
+                    if (e > 0 && cp.bp) continue;
+                    const int r = lane < pieces && i < n ? b.row_of(p, (b.ubeg + i) * H_KEYS + (cp.bp ? lane * cp.bp : 4 * lane + e)) : -1;
+                    row[e] = r < 0 ? cp.rows : r;
                 }
-                const float2 neg = *(const float2*)(negs + 8 * n + 2 * t);
-                const float w0 = weight(s[0], p.scale_log2, neg.x), w1 = weight(s[1], p.scale_log2, neg.y), w2 = weight(s[2], p.scale_log2, neg.x),
-                            w3 = weight(s[3], p.scale_log2, neg.y);
-                if (edge) {
-                    const int i0 = (f0 + 8 * n + 2 * t) / p.rep, i1 = (f0 + 8 * n + 2 * t + 1) / p.rep, at = j0 - b.base;
-                    const uint32_t see0 = paged_window(p, b.first + i0, i0, at) & there, see1 = paged_window(p, b.first + i1, i1, at) & there;
-                    sum0 += ((see0 >> gl) & 1u ? w0 : 0.f) + ((see1 >> gl) & 1u ? w1 : 0.f);
-                    sum1 += ((see0 >> (gl + 8)) & 1u ? w2 : 0.f) + ((see1 >> (gl + 8)) & 1u ? w3 : 0.f);
+            };
+            look(0);
+            for (int i = 0; ok && i < n; ++i) {
+                ok = __all_sync(0xffffffffu, bar_wait(err, smem_u32(&empty[at.s]), at.round ^ 1u));
+                if (!ok) break;
+                const uint32_t bar = smem_u32(&full[at.s]), tile = ring + at.s * X::TILE;
+                if (lane == 0) mbar_expect_tx(bar, X::TILE);
+                __syncwarp();
+                if (cp.bp) {
+                    if (lane < pieces)
+#pragma unroll
+                        for (int c = 0; c < C; ++c) tma_load_2d(tile + (uint32_t)c * H_CHUNK + (uint32_t)(lane * cp.bp) * 128u, &kmap, c * 64, row[0], bar);
                 } else {
-                    sum0 += w0 + w1;
-                    sum1 += w2 + w3;
+#pragma unroll
+                    for (int c = 0; c < C; ++c) tma_gather4(tile + (uint32_t)c * H_CHUNK + (uint32_t)lane * 512u, &kmap, c * 64, row[0], row[1], row[2], row[3], bar);
                 }
+                look(i + 1);
+                at.next(SLOTS);
             }
+        } else {
+            // ---------------- weights: lane = key, rows r0 ... r0 + R - 1 of every group
+            const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+            const int clean = missing ? 0 : min(b.base, b.end), key = quad * 32 + lane;
+            for (int i = 0; i < n; ++i) {
+                const int j0 = (b.ubeg + i) * H_KEYS + quad * 32, j = j0 + lane;
+                const bool edge = j0 + 32 > clean, there = edge && missing ? b.row_of(p, j) >= 0 : j < b.end;
+                float sum = 0.f;
+                for (int g = 0; g < groups; ++g, ++turn) {
+                    uint32_t see = 0;
+                    if (edge) {
+                        const int x = f0 + g * NR + r0 + (lane & (R - 1)), row = x / p.rep;
+                        see = x < b.live && j0 < b.end ? paged_window(p, b.first + row, row, j0 - b.base) : 0u;
+                    }
+                    ok = ok && __all_sync(0xffffffffu, bar_wait(err, smem_u32(&sfull[turn & 1]), (uint32_t)(turn >> 1) & 1u));
+                    __syncwarp();
+                    tc_fence_after();
+                    float s[R];
+                    tmem_columns<R>(lanes + (uint32_t)(turn & 1) * NR + (uint32_t)r0, s);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sread[turn & 1]);
+                    const float4* const neg = (const float4*)(negs + g * NR + r0);
+                    const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
+                    uint64_t sum2 = pair(sum, 0.f);
 #pragma unroll
-            for (int x = 1; x <= 2; x <<= 1) {
-                sum0 += __shfl_xor_sync(0xffffffffu, sum0, x);
-                sum1 += __shfl_xor_sync(0xffffffffu, sum1, x);
+                    for (int r = 0; r < R; r += 4) {
+                        const float4 x = neg[r / 4];
+                        float w[4];
+                        unpair(fma2(pair(s[r], s[r + 1]), scale2, pair(x.x, x.y)), w[0], w[1]);
+                        unpair(fma2(pair(s[r + 2], s[r + 3]), scale2, pair(x.z, x.w)), w[2], w[3]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            w[e] = ex2(w[e]);
+                            if (edge) {
+                                const uint32_t bits = __shfl_sync(0xffffffffu, see, r + e);
+                                if (!there || !((bits >> lane) & 1u)) w[e] = 0.f;
+                            }
+                        }
+                        sum2 = add2(sum2, pair(w[0], w[1]));
+                        sum2 = add2(sum2, pair(w[2], w[3]));
+                    }
+                    float u, v;
+                    unpair(sum2, u, v);
+                    sum = u + v;
+                }
+                if (half == 1) other[i & 1][key] = sum;
+                asm volatile("bar.sync %0, 64;" :: "r"(1 + quad) : "memory");      // a key's two warps; two turns of places, so that none is overwritten unread
+                if (half == 0 && j < b.end) add_weight(p, b, j, sum + other[i & 1][key]);
             }
-            const int j = j0 + gl + 8 * t;                    // lanes 0 and 1 of a group write
-            if (t < 2 && j < b.end) add_weight(p, b, j, t ? sum1 : sum0);
-#pragma unroll
-            for (int s = 0; s < N; ++s) { kk[s][0] = ahead[s][0]; kk[s][1] = ahead[s][1]; }
+        }
+        turns += n * groups;
+        tiles += n;
+        if (warp <= H_SOFT && y + 1 < batches) {   // the rows are read
+            __syncwarp();
+            asm volatile("bar.sync 5, %0;" :: "n"((H_SOFT + 1) * 32) : "memory");
         }
     }
+    if (warp == H_SOFT + 1 && lane == 0 && !ok)    // whoever gave up: do not leave with copies in flight
+        for (int s = 0; s < SLOTS; ++s) {
+            bar_wait(err, smem_u32(&full[s]), 0u);
+            bar_wait(err, smem_u32(&full[s]), 1u);
+        }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == H_SOFT) tmem_dealloc(tmem, X::TMEM);
 }
 
 __global__ void __launch_bounds__(G_THREADS) paged_weigh_f32_kernel(const __grid_constant__ PagedParams p) {
@@ -184,7 +290,7 @@ __global__ void __launch_bounds__(G_THREADS) paged_weigh_f32_kernel(const __grid
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float w = weight(s[r], p.scale_log2, negs[r0 + r]);
+                const float w = ex2(fmaf(s[r], p.scale_log2, negs[r0 + r]));
                 bool sees = true;
                 if (edge) {
                     const int i = (f0 + r0 + r) / p.rep;
@@ -197,27 +303,47 @@ __global__ void __launch_bounds__(G_THREADS) paged_weigh_f32_kernel(const __grid
     if (j < b.end) add_weight(p, b, j, sum);
 }
 
-template <int N, int DT> int launch_weigh(PagedParams p, cudaStream_t st) {
+template <int NR, int C, int DT> int launch_weigh(PagedParams p, cudaStream_t st) {
+    using X = Weigh<NR, C>;
     static bool configured = false;
     if (!configured) {
-        PGK_CUDA(cudaFuncSetAttribute(paged_weigh_kernel<N, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, H_QBYTES));
+        PGK_CUDA(cudaFuncSetAttribute(paged_weigh_kernel<NR, C, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::bytes(X::MOST)));
         configured = true;
     }
-    // tiles of eight rows that fit, and blocks that share a sequence's positions: four rounds of all SMs, none with less than two turns of its warps
-    const long long tiles = ((long long)p.max_rows * p.rep + 7) / 8, fit = H_QBYTES / (N * 512 + 32);
-    const int most = (int)(tiles < fit ? tiles : fit);
-    const long long items = (long long)p.kv_heads * p.seqs, wanted = (4ll * H_RESIDENT * sm_count() + items - 1) / items, turns = (p.max_keys + 2 * H_WARPS * H_KEYS - 1) / (2 * H_WARPS * H_KEYS);
-    p.splits = (int)(wanted < turns ? wanted : turns);
-    PGK_CUDA(launch_waiting(paged_weigh_kernel<N, DT>, dim3(p.splits, p.kv_heads, p.seqs), dim3(H_THREADS), (size_t)most * (N * 512 + 32), st, p, most));
+    WeighCopies cp = {};
+    cp.bp = p.page_size & -p.page_size;
+    if (cp.bp > H_KEYS) cp.bp = H_KEYS;
+    if (cp.bp < 8) cp.bp = 0;
+    cp.rows = p.pages * p.kv_heads * p.page_size;
+    const long long groups = ((long long)p.max_rows * p.rep + NR - 1) / NR;
+    cp.groups = (int)(groups < X::MOST ? groups : X::MOST);
+    cp.err = wait_word(kWaitPaged);
+    PGK_REQUIRE(cp.err, "paged_weigh failed: no pinned host memory");
+    CUtensorMap kmap{};
+    PGK_REQUIRE(tma_encode_fn() && tma_map_bf16_2d(&kmap, p.k_data, (uint64_t)p.dim, (uint64_t)cp.rows, (uint64_t)p.dim * 2, 64, cp.bp ? (uint32_t)cp.bp : 1u),
+                "paged_weigh failed: no tensor map of %d rows of %d elements", cp.rows, p.dim);
+    // blocks that share a sequence's positions: rounds of all SMs times (a block's tiles + what it costs besides, about three of them)
+    const int smem = X::bytes(cp.groups), resident = smem > 112 * 1024 ? 1 : (smem > 74 * 1024 ? 2 : 3), nt = (p.max_keys + H_KEYS - 1) / H_KEYS;
+    const long long items = (long long)p.seqs * p.kv_heads, slots = (long long)resident * sm_count();
+    long long least = 0;
+    for (int s = 1; s <= nt && s <= 1024; ++s) {
+        const long long cost = ((items * s + slots - 1) / slots) * ((nt + s - 1) / s + 3);
+        if (s == 1 || cost < least) { p.splits = s; least = cost; }
+    }
+    PGK_CUDA(launch_waiting(paged_weigh_kernel<NR, C, DT>, dim3(p.splits, p.kv_heads, p.seqs), dim3(H_THREADS), (size_t)smem, st, kmap, p, cp));
     return 0;
 }
+template <int C, int DT> int launch_weigh_rows(const PagedParams& p, cudaStream_t st) {
+    const long long rows = (long long)p.max_rows * p.rep;
+    if (rows <= 16) return launch_weigh<16, C, DT>(p, st);
+    return rows <= 32 ? launch_weigh<32, C, DT>(p, st) : launch_weigh<64, C, DT>(p, st);
+}
 template <int DT> int launch_weigh_dim(const PagedParams& p, cudaStream_t st) {
-    switch ((p.dim + 31) / 32) {
-        case 1: case 2: return launch_weigh<2, DT>(p, st);
-        case 3: return launch_weigh<3, DT>(p, st);
-        case 4: return launch_weigh<4, DT>(p, st);
-        case 5: case 6: return launch_weigh<6, DT>(p, st);
-        default: return launch_weigh<8, DT>(p, st);
+    switch ((p.dim + 63) / 64) {
+        case 1: return launch_weigh_rows<1, DT>(p, st);
+        case 2: return launch_weigh_rows<2, DT>(p, st);
+        case 3: return launch_weigh_rows<3, DT>(p, st);
+        default: return launch_weigh_rows<4, DT>(p, st);
     }
 }
 

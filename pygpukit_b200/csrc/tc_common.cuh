@@ -167,4 +167,17 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) 
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ void tmem_ld8_async(uint32_t taddr, float* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(taddr) : "memory");
+}
+// N columns of a warp's lanes
+template <int N> __device__ __forceinline__ void tmem_columns(uint32_t taddr, float (&v)[N]) {
+#pragma unroll
+    for (int c = 0; c < N; c += 8) tmem_ld8_async(taddr + (uint32_t)c, v + c);
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < N; ++c) asm volatile("" : "+f"(v[c]) :: "memory");
+}
+
 }  // namespace pgk
