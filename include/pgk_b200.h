@@ -901,6 +901,10 @@ int pgk_select_rows(const float* weights, long weights_ld, const int32_t* seq_sl
 int pgk_move_rows(void* const* host_arrays, const int32_t* host_row_bytes, int n_arrays, const int32_t* page_table, int pages, int page_size,
                   int slots, int max_pages, int kv_heads, const int32_t* seq_slots, const int32_t* starts, const int32_t* from, const int32_t* counts,
                   int seqs, int width, int by_head, float* weights, long weights_ld, const int32_t* context_lens, void* stream);
+/* pgk_qk_norm_rope_kv_write for the rows of a tree: row m goes to position pos + m of the cache, turned by pos + depths[m] (0 <= depths[m] <= m). */
+int pgk_qk_norm_rope_kv_write_tree(void* qkv, const void* q_gamma, const void* k_gamma, float eps, const float* cos_table, const float* sin_table,
+                                   void* k_cache, void* v_cache, int M, int n_heads_q, int n_kv, int head_dim, int max_seq, int pos,
+                                   const int32_t* pos_buf, const int32_t* depths, void* stream);
 int pgk_tree_masks(const int32_t* parents, const int32_t* row_starts, int seqs, int tokens, int max_rows, int words, int32_t* masks, int32_t* depths,
                    void* stream);
 int pgk_accept_tree(const void* logits, long ld, int dtype, int vocab, const int32_t* chosen, const int32_t* tokens, const int32_t* parents,

@@ -198,6 +198,7 @@ _SIGS = {
     "pgk_paged_weigh": [vp, cl, vp, vp, vp, cl, i32, i32, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, vp, i32, i32, vp],
     "pgk_select_rows": [vp, cl, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp],
     "pgk_move_rows": [vp, vp, i32, vp, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, i32, i32, vp, cl, vp, vp],
+    "pgk_qk_norm_rope_kv_write_tree": [vp, vp, vp, f32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp],
     "pgk_tree_masks": [vp, vp, i32, i32, i32, i32, vp, vp, vp],
     "pgk_accept_tree": [vp, cl, i32, i32, vp, vp, vp, vp, i32, i32, i32, vp, vp, vp, vp],
 }

@@ -378,7 +378,7 @@ __global__ void qk_norm_rope_kv_kernel(uint16_t* qkv, const uint16_t* qg,
                                        const uint16_t* kg, float eps, const float* cs,
                                        const float* sn, uint16_t* __restrict__ kc,
                                        uint16_t* __restrict__ vc, int M, int hq, int hkv, int hd, int max_seq,
-                                       int pos, const int32_t* pos_buf) {
+                                       int pos, const int32_t* pos_buf, const int32_t* depths) {
     griddep_wait();
     griddep_launch();
     const int lane = threadIdx.x & 31;
@@ -386,7 +386,8 @@ __global__ void qk_norm_rope_kv_kernel(uint16_t* qkv, const uint16_t* qg,
     const int H = hq + 2 * hkv;
     if (gw >= M * H) return;
     const int m = gw / H, h = gw % H;
-    const int p = (pos_buf ? *pos_buf : pos) + m;
+    const int p0 = pos_buf ? *pos_buf : pos, p = p0 + m;
+    const int turn = depths ? p0 + min(max(__ldcg(depths + m), 0), m) : p;        // the position of the rotation: a row of a tree lies behind its siblings
     uint16_t* row = qkv + ((size_t)m * H + h) * hd;
     const int half = hd >> 1;
     if (h >= hq + hkv) {   // V head: straight copy into the cache
@@ -423,7 +424,7 @@ __global__ void qk_norm_rope_kv_kernel(uint16_t* qkv, const uint16_t* qg,
         }
         uint16_t y0, y1;
         if (cs) {
-            float c = cs[(size_t)p * hd + d], s = sn[(size_t)p * hd + d];
+            float c = cs[(size_t)turn * hd + d], s = sn[(size_t)turn * hd + d];
             y0 = f32_to_bf16_bits(x0 * c - x1 * s); y1 = f32_to_bf16_bits(x1 * c + x0 * s);
         } else {                                  // no rotary embedding (GPT-2): plain K/V cache write
             y0 = f32_to_bf16_bits(x0); y1 = f32_to_bf16_bits(x1);
@@ -605,11 +606,15 @@ int pgk_kv_cache_update(const void* new_kv, void* cache, int seq, int n_kv, int 
 int pgk_qk_norm_rope_kv_write(void* qkv, const void* q_gamma, const void* k_gamma, float eps, const float* cos_table,
                               const float* sin_table, void* k_cache, void* v_cache, int M, int n_heads_q, int n_kv,
                               int head_dim, int max_seq, int pos, const int32_t* pos_buf, void* stream) {
+    return pgk_qk_norm_rope_kv_write_tree(qkv, q_gamma, k_gamma, eps, cos_table, sin_table, k_cache, v_cache, M, n_heads_q, n_kv, head_dim, max_seq, pos, pos_buf, nullptr, stream);
+}
+int pgk_qk_norm_rope_kv_write_tree(void* qkv, const void* q_gamma, const void* k_gamma, float eps, const float* cos_table, const float* sin_table, void* k_cache, void* v_cache, int M,
+                                   int n_heads_q, int n_kv, int head_dim, int max_seq, int pos, const int32_t* pos_buf, const int32_t* depths, void* stream) {
     PGK_REQUIRE(head_dim % 2 == 0 && M >= 1, "qk_norm_rope_kv_write failed: invalid shape");
     long warps = (long)M * (n_heads_q + 2 * n_kv);
     PGK_CUDA(launch_waiting(qk_norm_rope_kv_kernel, dim3(blocks_for((size_t)warps * 32, 128)), dim3(128), 0, ST(stream),
                     (uint16_t*)qkv, (const uint16_t*)q_gamma, (const uint16_t*)k_gamma, eps, cos_table, sin_table,
-                    (uint16_t*)k_cache, (uint16_t*)v_cache, M, n_heads_q, n_kv, head_dim, max_seq, pos, pos_buf));
+                    (uint16_t*)k_cache, (uint16_t*)v_cache, M, n_heads_q, n_kv, head_dim, max_seq, pos, pos_buf, depths));
     return 0;
 }
 

@@ -1,8 +1,9 @@
 // paged_rows.cu -- the positions of a cache that stay when it is cut, and rows of the pages that move together.
 //
-// Selection.  Of a sequence's positions the first, the recent and the ones of the largest weights stay, per key head, `budget` in all, in ascending order.  A block has one head: a
-// weight is an ordered 32-bit number, the least that stays is found digit by digit (11, 11 and 10 bits, a histogram each), then every warp counts what stays of its run of
-// positions and writes it behind what the warps before it have.  Bound by its five passes' latencies, 4 bytes a position being little.
+// Selection.  Of a sequence's positions the first, the recent and the ones of the largest weights stay, per key head, `budget` in all, in ascending order.  A block has one head, a
+// warp a run of its positions, a weight as an ordered 32-bit number in a register.  The least that stays is found in four digits of eight bits, a histogram each, in which every lane
+// has a column of its own: weights are alike in their upper digits, and a warp's 32 additions to one place would take turns.  Then a warp counts what stays of its run and writes it
+// behind what the warps before it have.  Bound by its passes' latencies, 4 bytes a position being little.
 //
 // Moving.  Row start + i of a sequence becomes, in place, what row start + from[i] was, from[i] >= i.  What is written lies before everything that is still to be read, from[i'] >= i' > i,
 // but for the rows that are moved at the same time: a tile's rows are read by all of the cluster before any is written, and the next tile's are on their way
@@ -14,7 +15,7 @@ namespace pgk {
 
 namespace {
 
-constexpr int C_THREADS = 1024, C_WARPS = C_THREADS / 32, C_BINS = 2048;
+constexpr int C_THREADS = 1024, C_WARPS = C_THREADS / 32, C_BINS = 256;
 
 struct SelectParams {
     const float* weights; long ld;
@@ -30,8 +31,11 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// K: positions of a lane that stay in registers; 0: looked at anew in every pass
+template <int K>
 __global__ void __launch_bounds__(C_THREADS) select_kernel(const __grid_constant__ SelectParams p) {
-    __shared__ int bins[C_BINS], part[C_WARPS], over[C_WARPS], same[C_WARPS];
+    __shared__ int bins[C_BINS][32];
+    __shared__ int sums[C_BINS], over[C_WARPS], same[C_WARPS];
     __shared__ int found, left;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.x, seq = blockIdx.y;
     griddep_wait();
@@ -48,51 +52,73 @@ __global__ void __launch_bounds__(C_THREADS) select_kernel(const __grid_constant
     }
     const float* const w = p.weights + ((size_t)slot * p.kv_heads + head) * p.ld;
     const int recent = ctx - p.recent;
-    auto key = [&](int j) { return j < p.first || j >= recent ? 0xffffffffu : ordered(__ldcg(w + j)); };
-    // the least key that stays: digit by digit, `left` of those that share the digits so far
+    const int run = K > 0 ? 32 * K : ((ctx + C_WARPS - 1) / C_WARPS + 31) & ~31, from = warp * run, to = min(ctx, from + run), n = to > from ? (to - from + 31) / 32 : 0;
+    auto key = [&](int j) { return j >= to ? 0u : (j < p.first || j >= recent ? 0xffffffffu : ordered(__ldcg(w + j))); };
+    uint32_t held[K > 0 ? K : 1];
+    if constexpr (K > 0) {
+#pragma unroll
+        for (int i = 0; i < K; ++i) held[i] = key(from + 32 * i + lane);
+    }
+    // f(position, its key) for the run's positions, 32 at a time
+    auto each = [&](auto f) {
+        if constexpr (K > 0) {
+#pragma unroll
+            for (int i = 0; i < K; ++i)
+                if (i < n) f(from + 32 * i + lane, held[i]);
+        } else
+            for (int i = 0; i < n; ++i) f(from + 32 * i + lane, key(from + 32 * i + lane));
+    };
+    // the least key that stays: digit by digit, `need` of those that share the digits so far
     uint32_t least = 0;
     int need = count;
 #pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), width = pass == 2 ? 10 : 11;
-        const uint32_t above = pass == 0 ? 0u : 0xffffffffu << (shift + width);
-        for (int i = tid; i < C_BINS; i += C_THREADS) bins[i] = 0;
-        __syncthreads();
-        for (int j = tid; j < ctx; j += C_THREADS) {
-            const uint32_t x = key(j);
-            if ((x & above) == least) atomicAdd(&bins[(x >> shift) & ((1u << width) - 1u)], 1);
-        }
-        __syncthreads();
-        // the bin with the need-th from above: thread i has bins 2 i and 2 i + 1
-        const int hi = bins[2 * tid + 1], lo = bins[2 * tid], mine = hi + lo;
-        int sum = mine;                                       // of this lane and the ones after it
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        const uint32_t above = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
 #pragma unroll
-        for (int x = 1; x < 32; x <<= 1) {
-            const int got = __shfl_down_sync(0xffffffffu, sum, x);
-            if (lane + x < 32) sum += got;
-        }
-        if (lane == 0) part[warp] = sum;
+        for (int i = 0; i < C_BINS / C_WARPS; ++i) bins[warp + C_WARPS * i][lane] = 0;
         __syncthreads();
-        int after = 0;
-        for (int i = warp + 1; i < C_WARPS; ++i) after += part[i];
-        const int over_hi = after + sum - mine;               // keys in higher bins
-        if (over_hi < need && need <= over_hi + mine) {
-            const bool upper = need <= over_hi + hi;
-            found = 2 * tid + (upper ? 1 : 0);
-            left = need - over_hi - (upper ? 0 : hi);
+        each([&](int j, uint32_t x) {
+            if (j < to && (x & above) == least) atomicAdd(&bins[(x >> shift) & 255u][lane], 1);
+        });
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < C_BINS / C_WARPS; ++i) {
+            int x = bins[warp + C_WARPS * i][lane];
+#pragma unroll
+            for (int y = 16; y > 0; y >>= 1) x += __shfl_xor_sync(0xffffffffu, x, y);
+            if (lane == 0) sums[warp + C_WARPS * i] = x;
+        }
+        __syncthreads();
+        if (warp == 0) {                                      // the bin with the need-th from above: lane l has bins 8 l ... 8 l + 7
+            int mine[8], all = 0;
+#pragma unroll
+            for (int i = 7; i >= 0; --i) mine[i] = all += sums[8 * lane + i];         // of it and the lane's higher ones
+            int after = all;
+#pragma unroll
+            for (int x = 1; x < 32; x <<= 1) {
+                const int got = __shfl_down_sync(0xffffffffu, after, x);
+                if (lane + x < 32) after += got;
+            }
+            after -= all;                                     // keys in the bins of the lanes after this one
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int higher = after + (i < 7 ? mine[i + 1] : 0);
+                if (higher < need && need <= after + mine[i]) {
+                    found = 8 * lane + i;
+                    left = need - higher;
+                }
+            }
         }
         __syncthreads();
         least |= (uint32_t)found << shift;
         need = left;
     }
-    // a warp's run of positions, 32 at a time: those above the least, and the first `need` of its equals
-    const int run = ((ctx + C_WARPS - 1) / C_WARPS + 31) & ~31, from = warp * run, to = min(ctx, from + run);
+    // those above the least, and the first `need` of its equals
     int n_over = 0, n_same = 0;
-    for (int j = from; j < to; j += 32) {
-        const uint32_t x = j + lane < to ? key(j + lane) : 0u;
-        n_over += __popc(__ballot_sync(0xffffffffu, j + lane < to && x > least));
-        n_same += __popc(__ballot_sync(0xffffffffu, j + lane < to && x == least));
-    }
+    each([&](int j, uint32_t x) {
+        n_over += __popc(__ballot_sync(0xffffffffu, j < to && x > least));
+        n_same += __popc(__ballot_sync(0xffffffffu, j < to && x == least));
+    });
     if (lane == 0) { over[warp] = n_over; same[warp] = n_same; }
     __syncthreads();
     int at = 0, seen = 0;
@@ -100,15 +126,14 @@ __global__ void __launch_bounds__(C_THREADS) select_kernel(const __grid_constant
         at += over[i] + min(same[i], max(0, need - seen));
         seen += same[i];
     }
-    for (int j = from; j < to; j += 32) {
-        const uint32_t x = j + lane < to ? key(j + lane) : 0u;
-        const uint32_t eq = __ballot_sync(0xffffffffu, j + lane < to && x == least), below = (1u << lane) - 1u;
-        const bool stays = j + lane < to && (x > least || (x == least && seen + __popc(eq & below) < need));
+    each([&](int j, uint32_t x) {
+        const uint32_t eq = __ballot_sync(0xffffffffu, j < to && x == least), below = (1u << lane) - 1u;
+        const bool stays = j < to && (x > least || (x == least && seen + __popc(eq & below) < need));
         const uint32_t all = __ballot_sync(0xffffffffu, stays);
-        if (stays) kept[at + __popc(all & below)] = j + lane;
+        if (stays) kept[at + __popc(all & below)] = j;
         at += __popc(all);
         seen += __popc(eq);
-    }
+    });
 }
 
 constexpr int M_THREADS = 256, M_UNITS = 8, M_TILE = M_THREADS * M_UNITS, M_ARRAYS = 192, M_CLUSTER = 8;
@@ -253,7 +278,9 @@ extern "C" int pgk_select_rows(const float* weights, long weights_ld, const int3
     if (seqs == 0) return 0;
     PGK_REQUIRE(weights && seq_slots && context_lens && kept && counts, "select_rows failed: an array is missing");
     SelectParams p = {weights, weights_ld, seq_slots, context_lens, slots, kv_heads, budget, first, recent, max_context, kept, counts};
-    PGK_CUDA(launch_waiting(select_kernel, dim3(kv_heads, seqs), dim3(C_THREADS), 0, (cudaStream_t)stream, p));
+    const auto kernel = max_context <= 4 * C_THREADS ? select_kernel<4> : (max_context <= 8 * C_THREADS ? select_kernel<8> :
+                        (max_context <= 16 * C_THREADS ? select_kernel<16> : select_kernel<0>));
+    PGK_CUDA(launch_waiting(kernel, dim3(kv_heads, seqs), dim3(C_THREADS), 0, (cudaStream_t)stream, p));
     return 0;
 }
 
@@ -288,10 +315,10 @@ extern "C" int pgk_move_rows(void* const* host_arrays, const int32_t* host_row_b
         if (p.chunk < 1) p.chunk = 1;
         const int chunks = (p.n + p.chunk - 1) / p.chunk + (p.weights ? 1 : 0);
         PGK_REQUIRE((long long)chunks * kv_heads <= 65535, "move_rows failed: too many heads");
-        // blocks that share a head's rows: as many as there are SMs for, none with less than a tile
+        // blocks that share a head's rows: until there are twelve a SM, which even out (256 heads of 4096 rows, 1 / 2 / 4 / 8 blocks: 139 / 148 / 132 / 147 us), none with less than a tile
         const long long items = (long long)chunks * kv_heads * seqs;
         int blocks = 1;
-        while (blocks < M_CLUSTER && items * blocks * 2 <= 4 * sm_count() && (long long)width * (p.bytes / unit) > (long long)M_TILE * blocks) blocks *= 2;
+        while (blocks < M_CLUSTER && items * blocks * 2 <= 12 * sm_count() && (long long)width * (p.bytes / unit) > (long long)M_TILE * blocks) blocks *= 2;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(blocks, (unsigned)(chunks * kv_heads), (unsigned)seqs);
         cfg.blockDim = dim3(M_THREADS);

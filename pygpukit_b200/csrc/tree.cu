@@ -163,8 +163,8 @@ extern "C" int pgk_accept_tree(const void* logits, long ld, int dtype, int vocab
     if (!chosen && total > 0) {
         if (int rc = scratch_alloc(&ws, (size_t)total * 4, st)) return rc;
         const int size = dtype == 0 ? 4 : 2, wide = (uintptr_t)logits % 16 == 0 && ld * size % 16 == 0;
-        int blocks = 1;                                       // a row's: as many as there are SMs for, none with less than four rounds
-        while (blocks < A_CLUSTER && (long long)total * blocks * 2 <= 4 * sm_count() && (long long)vocab * size > 4ll * 16 * A_THREADS * blocks) blocks *= 2;
+        int blocks = 1;                                       // a row's: until there are 16 a SM, which even out, none with less than four rounds
+        while (blocks < A_CLUSTER && (long long)total * blocks <= 8 * sm_count() && (long long)vocab * size > 4ll * 16 * A_THREADS * blocks) blocks *= 2;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(blocks, total);
         cfg.blockDim = dim3(A_THREADS);

@@ -10,7 +10,7 @@ from .config import (GPT2_SPEC, LLAMA_SPEC, MIXTRAL_SPEC, MODEL_SPECS, QWEN2_SPE
                      ParallelMixerSpec, RotarySpec, YarnSpec,
                      layered_config_from_json)
 from .decode import (BeamSearch, DecodeBatch, DecodeJacobi, DecodeM1, DecodeM1Graph, DecodeSpeculative, DecodeStrategy,
-                     RaggedScheduler)
+                     DecodeTree, RaggedScheduler)
 from .layers import (MLP, Attention, BiasedRouterMoE, DeltaRuleMixer, GatedLinearMixer, GLAMixer, MatrixLSTMMixer, PolyNormRows, PreNormSeamBlock, SandwichBlock, CausalConvRows, LinearAttentionMixer, ParallelMixer, PreNormBlock, ActivatedRows, SquaredReluRows, GatedDenseRows, GroupedRouterMoE, LatentAttentionMixer, ParallelBlock, RowNorm, TokenSideInput, Linear, LinearBF16, LinearFP8, LinearNVF4, LinearRows, MoELayer, Norm, interleave_gate_up,
                      PagedAttentionMixer, PostNormBlock, TransformerBlock,
                      apply_rotary_pos_emb_numpy, precompute_freqs_cis)

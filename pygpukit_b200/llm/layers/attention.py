@@ -195,9 +195,10 @@ class Attention:
     # ---- decode
     def attend(self, x: GPUArray, position: int, context_len: int, *, qkv_buf: GPUArray | None = None,
                attn_buf: GPUArray | None = None, pos_buf: GPUArray | None = None,
-               ctx_buf: GPUArray | None = None, norm=None) -> GPUArray:
+               ctx_buf: GPUArray | None = None, norm=None, tree=None) -> GPUArray:
         """qkv projection -> QK-norm/RoPE/KV-write -> split-KV attention; returns [M, q_dim]
-        (the input of o_proj).  M rows = M consecutive positions of one sequence."""
+        (the input of o_proj).  M rows = M consecutive positions of one sequence, or with `tree` (a `decode.tree.TreeRows`) the
+        rows of a tree of drafts behind `position` cached ones, which see their ancestors only."""
         assert self._k_cache is not None, "Call init_fixed_cache first"
         M = x.shape[0]
         H, Hkv, hd = self.num_heads, self.num_kv_heads, self.head_dim
@@ -209,6 +210,18 @@ class Attention:
             attn_buf = GPUArray((M, H * hd), bfloat16)
         elif attn_buf.shape[0] != M:
             attn_buf = attn_buf.slice_rows(M)
+        if tree is not None:
+            kp, vp = self._kv_ptrs()
+            api.qk_norm_rope_kv_write_tree(qkv.device_ptr, None if self.q_norm is None else self.q_norm.weight.device_ptr,
+                                           None if self.k_norm is None else self.k_norm.weight.device_ptr,
+                                           float(self.q_norm.eps if self.q_norm is not None else 0.0), self._cos_dev.device_ptr,
+                                           self._sin_dev.device_ptr, kp, vp, M, H, Hkv, hd, self._max_cache_len, int(position), None,
+                                           tree.depths.device_ptr, _st())
+            # the cache of the sequence is one page of `_max_cache_len` positions
+            api.paged_attention(qkv.device_ptr, width, kp, vp, attn_buf.device_ptr, H * hd, 1, self._max_cache_len, tree.zero.device_ptr, 1, 1,
+                                tree.zero.device_ptr, tree.context.device_ptr, tree.starts.device_ptr, 1, M, M, int(context_len), H, Hkv, hd, 0.0,
+                                tree.masks.device_ptr, tree.masks.shape[1], None, 2, _st())
+            return attn_buf
         if M == 1 and hd == 128 and self.config.use_rope and _FUSED_BRACKET:
             # one launch: QK-norm + RoPE + KV write + split-KV attention (pgk_rope_sdpa_decode)
             kp, vp = self._kv_ptrs()

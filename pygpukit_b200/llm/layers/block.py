@@ -22,9 +22,9 @@ class TransformerBlock:
         self.comm = comm   # TensorParallel communicator or None
 
     def decode(self, hidden: GPUArray, position: int, context_len: int, bufs=None, pos_buf=None, ctx_buf=None,
-               multi: bool = False) -> GPUArray:
+               multi: bool = False, tree=None) -> GPUArray:
         """hidden [M, H] -> hidden [M, H], updated IN PLACE (M consecutive tokens of one sequence; multi = True: the
-        new tokens of M independent sequences, pos_buf / ctx_buf are then arrays of M)."""
+        new tokens of M independent sequences, pos_buf / ctx_buf are then arrays of M; tree: the rows of a tree of drafts)."""
         M = hidden.shape[0]
 
         def buf(name):
@@ -41,11 +41,11 @@ class TransformerBlock:
                                        norm=self.attn_norm if fuse else None)
         elif can_fuse_norm(self.attn_norm, hidden.shape[1]) and M <= 64:
             a = self.attn.attend(hidden, position, context_len, qkv_buf=buf("qkv_proj_out"), attn_buf=buf("attn_flat"),
-                                 pos_buf=pos_buf, ctx_buf=ctx_buf, norm=self.attn_norm)
+                                 pos_buf=pos_buf, ctx_buf=ctx_buf, norm=self.attn_norm, tree=tree)
         else:
             x = self.attn_norm(hidden, out=buf("norm_out"))
             a = self.attn.attend(x, position, context_len, qkv_buf=buf("qkv_proj_out"), attn_buf=buf("attn_flat"),
-                                 pos_buf=pos_buf, ctx_buf=ctx_buf)
+                                 pos_buf=pos_buf, ctx_buf=ctx_buf, tree=tree)
         if tp and self.comm.fuses_allreduce(self.attn.o_proj, M):
             self.attn.o_proj.forward_allreduce(a, hidden)          # GEMV + all-reduce + residual: one launch
         elif tp:

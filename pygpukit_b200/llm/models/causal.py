@@ -624,6 +624,71 @@ class CausalTransformerModel:
         stats = {"draft_count": len(draft), "accepted_count": sum(1 for a, d in zip(accepted, draft) if a == d)}
         return accepted, stats
 
+    # ------------------------------------------------------------------ trees of drafts
+    def decode_step_tree_lookahead(self, token_id: int, branches: tuple = (3, 2, 1), draft_layers: int = 8) -> tuple[list[int], dict]:
+        """One self-speculative step with a tree of drafts (net-new; the reference drafts chains): the early layers draft branches[0] tokens behind
+        `token_id`, branches[1] behind each of them and so on, the full model verifies the whole tree in ONE batched pass whose rows see
+        their ancestors only, and the longest run of drafts that are the model's greedy tokens is accepted, with the model's token behind it.  The
+        cache rows of the accepted drafts then move together, in every layer by one launch.  Call `set_lookahead_confirmed_pos(prefill_len)` after
+        the prefill.  The chosen drafts of a level and the accepted rows come back to the host (4 bytes each)."""
+        from ...ops.beam import beam_select
+        from ...ops.paged_rows import move_rows_paged
+        from ...ops.tree import accept_tree
+        from ..decode.tree import TreeRows, tree_size
+        if self.tp != 1:
+            raise NotImplementedError("self-speculative decode runs on one GPU (the draft needs the full lm_head)")
+        if not self.config.use_rope or self.position_embed is not None:
+            raise ValueError("trees of drafts need rotary positions")
+        b = self.buffers
+        n = tree_size(branches)
+        V, H = self._head.shape[0], self.config.hidden_size
+        if n > b.max_batch_size:
+            raise ValueError(f"a tree of {n} rows exceeds max_batch_size {b.max_batch_size} (init_decode)")
+        if max(branches) > min(V, 64):
+            raise ValueError(f"branches {tuple(branches)}: 64 drafts behind a row at most")
+        confirmed = self.get_lookahead_confirmed_pos()
+        if confirmed + n > self._max_seq:
+            raise ValueError(f"speculating {n} rows from position {confirmed} exceeds the fixed cache ({self._max_seq})")
+        self.reset_lookahead_all()
+        rows = getattr(self, "_tree_rows", None)
+        if rows is None or rows.most < n:
+            rows = self._tree_rows = TreeRows(max(n, b.max_batch_size))
+        self._enter(_st())
+        layers = self.blocks[:max(0, min(int(draft_layers), len(self.blocks)))]
+
+        def run(tokens, parents, blocks):
+            step = rows.step(tokens, parents, confirmed)
+            hidden = self._embed(tokens, len(tokens), confirmed, b)
+            for blk in blocks:
+                blk.decode(hidden, confirmed, confirmed + len(tokens), b, tree=step)
+            return hidden, step
+
+        # 1. draft level by level; the rows that are there run again with every level (few rows cost what one does)
+        tokens, parents, level = [int(token_id)], [-1], 1
+        for width in branches:
+            hidden, _ = run(tokens, parents, layers)
+            at = len(tokens) - level
+            last = GPUArray((level, H), bfloat16, ptr=hidden.device_ptr + 2 * H * at, source=hidden)
+            logits = self.get_logits(self._final(last, b))
+            _, _, picked = beam_select(logits, rows.scores(level), width)
+            picked = picked.to_numpy()
+            for i in range(level):
+                tokens += [int(t) for t in picked[i]]
+                parents += [at + i] * width
+            level *= width
+        # 2. verify the tree with the full model
+        hidden, step = run(tokens, parents, self.blocks)
+        logits = self.get_logits(self._final(hidden, b))
+        got, count, nxt = accept_tree(logits, step.tokens, step.parents, step.starts, n)
+        # 3. the accepted rows move together
+        arrays = [GPUArray((1, blk.attn.num_kv_heads, self._max_seq, blk.attn.head_dim), bfloat16, ptr=p, source=c)
+                  for blk in self.blocks for p, c in zip(blk.attn._kv_ptrs(), (blk.attn._k_cache, blk.attn._v_cache))]
+        move_rows_paged(arrays, step.zero.view((1, 1)), step.zero, got, count, starts=step.base)
+        path = [int(r) for r in got.to_numpy()[0] if r >= 0]
+        accepted = [tokens[r] for r in path[1:]] + [int(nxt.to_numpy()[0])]
+        self.commit_lookahead_all(len(path))
+        return accepted, {"draft_count": n - 1, "accepted_count": len(path) - 1}
+
     # ------------------------------------------------------------------ Jacobi decode
     def _argmax_tokens(self, hidden: GPUArray, scratch: GPUArray) -> list[int]:
         """greedy token of every row of final-normed hidden states: lm_head + row argmax on the device"""

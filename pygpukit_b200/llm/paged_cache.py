@@ -20,6 +20,8 @@ Shared pages: `assign` makes sequences into what others hold (the beams of a sea
 from one, some end).  Whole pages are shared and counted; a partly filled one goes to one of the takers and is copied for the others, as
 state rows are, by `ops.copy_rows`.  A sequence that was cut back into a shared page gets a copy of its own before it grows again.
 
+Rows that move: `keep_rows` cuts sequences to some of their positions, which move together in place (drafts of a tree that were accepted, evicted positions).
+
 Four bits: dtype "int4" keeps uint8 arrays `[pages, kv_heads, page_size, ops.int4_row_bytes(dim)]` for the operators of `ops/paged.py` (keys and
 values of one size, pages of a multiple of 16 positions, no pooled rows).  The models' layers do not read them: `LayeredCausalModel` refuses such a cache.
 
@@ -41,6 +43,7 @@ from ..core.factory import zeros
 from ..core.stream import current_stream_handle as _st
 from ..ops.beam import copy_rows
 from ..ops.paged import int4_row_bytes
+from ..ops.paged_rows import move_rows_paged
 
 
 _versions = itertools.count(1)
@@ -145,6 +148,22 @@ class PagePool:
             self._drop(p)
         del ent[1][keep:]
         ent[2] = length
+
+    def own_pages(self, seq_id, start: int) -> list:
+        """Pages of its own in the place of those from position `start` on that others hold too: (that one, the new one) each, to be copied."""
+        slot, pages, length, _ = self._seq[seq_id]
+        if not 0 <= start <= length:
+            raise ValueError(f"own_pages: position {start} outside 0..{length}")
+        pairs = []
+        for i in range(start // self.page_size, len(pages)):
+            if pages[i] in self._shared:
+                old, new = pages[i], self._new_page()
+                self._drop(old)
+                pages[i] = new
+                self.table[slot, i] = new
+                self.dirty = True
+                pairs.append((old, new))
+        return pairs
 
     def release(self, seq_id) -> None:
         slot, pages, _, _ = self._seq.pop(seq_id)
@@ -374,6 +393,40 @@ class PagedKVCache:
         if self.has_state and length != self.pool.length(seq_id):
             raise ValueError("PagedKVCache: a sequence with recurrent state cannot be cut back")
         self.pool.truncate(seq_id, length)
+
+    def keep_rows(self, keeps: dict) -> None:
+        """Cut sequences to some of their positions: {id: (start, rows)} leaves the positions before `start`, and behind them those at start + rows[0],
+        start + rows[1], ... (ascending numbers), in every layer; the sequence ends there.  Accepted drafts of a tree, say, or what is left when
+        positions are evicted.  Rows move in the order of the current stream (`ops.move_rows_paged`); keys stay turned by the positions that they had.  Pages that others
+        hold too are copied first."""
+        if self.int4 or self.has_state or any(self.pools):
+            raise ValueError("PagedKVCache: rows of four-bit pages, pooled rows and recurrent states do not move")
+        # everything is looked at before anything changes
+        for seq, (start, rows) in keeps.items():
+            length = self.pool.length(seq)
+            if not 0 <= start <= length or any(not 0 <= r < length - start for r in rows) or any(a >= b for a, b in zip(rows, rows[1:])):
+                raise ValueError(f"keep_rows: rows {list(rows)!r} behind position {start} of a sequence of {length} (ascending)")
+        moving = [(seq, start, rows) for seq, (start, rows) in keeps.items() if any(r != i for i, r in enumerate(rows))]
+        if moving:
+            pairs = [p for seq, start, _ in moving for p in self.pool.own_pages(seq, start)]
+            self._grown()
+            self._copy(self._page_arrays(), pairs)
+            table, arrays = self.page_table(), self._page_arrays()
+            S, width = len(moving), max(len(rows) for _, _, rows in moving)
+            host = np.full(S * (3 + width), -1, np.int32)
+            host[:S] = [self.pool.slot(seq) for seq, _, _ in moving]
+            host[S:2 * S] = [start for _, start, _ in moving]
+            host[2 * S:3 * S] = [len(rows) for _, _, rows in moving]
+            for i, (_, _, rows) in enumerate(moving):
+                host[3 * S + i * width:3 * S + i * width + len(rows)] = rows
+            dev = GPUArray((host.size,), int32)
+            api.upload(dev.device_ptr, host.ctypes.data, host.nbytes, _st())
+            slots, starts, counts = (dev._view(i * S, (S,)) for i in range(3))
+            at = dev._view(3 * S, (S, width))
+            for heads in sorted({a.shape[1] for a in arrays}):        # a call's arrays have one number of heads
+                move_rows_paged([a for a in arrays if a.shape[1] == heads], table, slots, at, counts, starts=starts)
+        for seq, (start, rows) in keeps.items():
+            self.pool.truncate(seq, start + len(rows))
 
     def sync_table(self) -> None:
         """Upload the page table when it changed since the last upload."""

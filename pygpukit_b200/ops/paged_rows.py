@@ -159,8 +159,8 @@ def move_rows_paged(arrays: "list[GPUArray]", page_table: GPUArray, slots: GPUAr
         if a._dtype is uint8 or a._dtype == uint8:
             raise ValueError(f"{name}: pages of bytes keep a position's row in two places")
     sizes = array("i", [a._shape[3] * a._dtype.itemsize for a in arrays])
-    if any(n % 2 for n in sizes):
-        raise ValueError(f"{name}: rows of an odd number of bytes, {dtype} {shape}")
+    if any(n % 2 or n > 4096 for n in sizes):
+        raise ValueError(f"{name}: rows of an even number of bytes up to 4096, got {dtype} {shape}")
     ptrs = array("Q", [a._ptr for a in arrays])
     if len(set(ptrs)) < len(ptrs):
         raise ValueError(f"{name}: an array is there twice")
