@@ -169,6 +169,25 @@ template <int DT> __device__ __forceinline__ uint32_t paged_pack2(float lo, floa
     } else
         return pack_bf16x2(lo, hi);
 }
+// Two weights (not negative) as one word.  bfloat16: rounded up from the half on by integers, since the conversion shares its unit with the exponentials: of a tile of 128 x 128
+// scores 512 cycles beside their 1024.  (A NaN may get lost; the row's sum has it.)
+template <int DT> __device__ __forceinline__ uint32_t paged_weights2(float a, float b) {
+    if constexpr (DT == 1) return paged_pack2<1>(a, b);
+    else return __byte_perm(__float_as_uint(a) + 0x8000u, __float_as_uint(b) + 0x8000u, 0x7632);
+}
+// the same as two terms: what is left of the first one's cut
+template <int DT> __device__ __forceinline__ void paged_weights2x2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    if constexpr (DT == 1) {
+        hi = paged_pack2<1>(a, b);
+        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        lo = paged_pack2<1>(a - back.x, b - back.y);
+    } else {
+        const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+        hi = __byte_perm(x, y, 0x7632);
+        const float u = a - __uint_as_float(x & 0xffff0000u), v = b - __uint_as_float(y & 0xffff0000u);
+        lo = __byte_perm(__float_as_uint(u) + 0x8000u, __float_as_uint(v) + 0x8000u, 0x7632);
+    }
+}
 template <int DT> __device__ __forceinline__ float paged_float(const void* base, size_t at) {
     if constexpr (DT == 0) return __ldcg((const float*)base + at);
     else if constexpr (DT == 1) return __half2float(__ushort_as_half(ld_act2((const uint16_t*)base + at)));
@@ -220,6 +239,43 @@ template <int N, typename F> __device__ __forceinline__ float reduce_lanes(float
 // 2^(s - m) for a reference that is not there yet (m = -infinity)
 __device__ __forceinline__ float paged_neg(float m) { return m == -INFINITY ? 0.f : -m; }
 
+// A tile of V in shared memory, `chunks` of 64 elements (128 bytes a key, `chunk` bytes each), keys j0 on, as a warp has fetched it in pieces of bp positions: the values of positions
+// [from, end) that are not finite become zeros -- true where there were any --, and what lies behind the end in the last piece as well (what was not fetched is zeros).
+template <int DT> __device__ __forceinline__ bool paged_fix_values(uint32_t tile, int chunks, uint32_t chunk, int j0, int from, int end, int bp, int lane) {
+    const int k0 = max(0, from - j0), k1 = min(128, end - j0);
+    auto unit = [&](uint32_t a, uint32_t (&x)[4]) {
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(a) : "memory");
+    };
+    auto put = [&](uint32_t a, const uint32_t (&x)[4]) {
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+    };
+    uint32_t most = 0;                                        // the largest magnitude says whether there are any
+#pragma unroll 4
+    for (int e = k0 * 8 + lane; e < k1 * 8; e += 32)
+        for (int c = 0; c < chunks; ++c) {
+            uint32_t x[4];
+            unit(tile + (uint32_t)c * chunk + (uint32_t)e * 16u, x);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) most = __vmaxu2(most, x[y] & 0x7fff7fffu);
+        }
+    const bool bad = __any_sync(0xffffffffu, paged_unfinite<DT>(most) != 0);
+    if (bad)
+        for (int e = k0 * 8 + lane; e < k1 * 8; e += 32)
+            for (int c = 0; c < chunks; ++c) {
+                const uint32_t a = tile + (uint32_t)c * chunk + (uint32_t)e * 16u;
+                uint32_t x[4];
+                unit(a, x);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) x[y] &= ~paged_unfinite<DT>(x[y]);
+                put(a, x);
+            }
+    const uint32_t none[4] = {0, 0, 0, 0};
+    const int z1 = bp ? min(128, (max(0, k1) + bp - 1) & ~(bp - 1)) : 0;
+    for (int e = max(0, k1) * 8 + lane; e < z1 * 8; e += 32)
+        for (int c = 0; c < chunks; ++c) put(tile + (uint32_t)c * chunk + (uint32_t)e * 16u, none);
+    return bad;
+}
+
 // A row's outputs d ... d + 3, rounded and written
 template <int DT> __device__ __forceinline__ void paged_put(const PagedParams& p, size_t at, float4 o) {
     if constexpr (DT == 0) {
@@ -234,19 +290,20 @@ template <int DT> __device__ __forceinline__ void paged_put(const PagedParams& p
     }
 }
 
-// What the cluster's blocks need to become one: shared memory beside the sums [ROWS][DN + 4]
-template <int ROWS> struct PagedFold {
-    float m[ROWS], l[ROWS];               // a block's references (log2) and sums
-    int bad;                              // whether a value of the step's rows that is not finite was taken as zero
-    float factor[PAGED_CLUSTER][ROWS];    // what a block's sums are multiplied by
-    long long at[ROWS];                   // where a row's outputs go, below 0: nowhere
+// What the cluster's blocks need to become one: shared memory beside the sums [PARTS][ROWS][DN + 4]; a block may have summed its keys in several parts
+template <int ROWS, int PARTS = 1> struct PagedFold {
+    float m[PARTS * ROWS], l[PARTS * ROWS];            // references (log2) and sums
+    int bad;                                           // whether a value of the step's rows that is not finite was taken as zero
+    float factor[PAGED_CLUSTER * PARTS][ROWS];         // what a part's sums are multiplied by
+    long long at[ROWS];                                // where a row's outputs go, below 0: nowhere
 };
 
 // The end of every kernel: block r of the cluster has every `splits`-th of its rows' pieces of four elements.  `bad`: values among the step's rows that are not finite were
 // taken as zero, since a weight of zero times them would reach rows that do not see them; the rows that do add them here.
-template <int ROWS, int UNIT, int DT, int DN>
-__device__ __forceinline__ void paged_fold(const PagedParams& p, const PagedBlock<ROWS, UNIT>& b, const float* sums, PagedFold<ROWS>& f) {
-    constexpr int PIECES = DN / 4;
+template <int ROWS, int UNIT, int DT, int DN, int PARTS = 1>
+__device__ __forceinline__ void paged_fold(const PagedParams& p, const PagedBlock<ROWS, UNIT>& b, const float* sums, PagedFold<ROWS, PARTS>& f) {
+    constexpr int PIECES = DN / 4, MOST = PAGED_CLUSTER * PARTS;
+    const int parts = p.splits * PARTS;
     if (p.splits > 1) paged_cluster_sync();
     else __syncthreads();
     bool bad = false;
@@ -254,29 +311,28 @@ __device__ __forceinline__ void paged_fold(const PagedParams& p, const PagedBloc
     for (int r = (int)threadIdx.x; r < ROWS; r += (int)blockDim.x) {
         const int x = b.f0 + r, i = x / p.rep, tok = b.first + i, h = b.head * p.rep + x - i * p.rep;
         const bool live = r < b.live && tok >= 0 && tok < p.tokens;
-        float top = -INFINITY, sum = 0.f, ms[PAGED_CLUSTER], ls[PAGED_CLUSTER];
-        const uint32_t m_at = smem_u32(&f.m[r]), l_at = smem_u32(&f.l[r]);
+        float top = -INFINITY, sum = 0.f, ms[MOST], ls[MOST];
 #pragma unroll
-        for (int s = 0; s < PAGED_CLUSTER; ++s) {
+        for (int s = 0; s < MOST; ++s) {
             ms[s] = -INFINITY;
             ls[s] = 0.f;
-            if (s < p.splits) {
-                ms[s] = paged_remote_float(paged_remote(m_at, s));
-                ls[s] = paged_remote_float(paged_remote(l_at, s));
+            if (s < parts) {
+                ms[s] = paged_remote_float(paged_remote(smem_u32(&f.m[s % PARTS * ROWS + r]), s / PARTS));
+                ls[s] = paged_remote_float(paged_remote(smem_u32(&f.l[s % PARTS * ROWS + r]), s / PARTS));
             }
         }
 #pragma unroll
-        for (int s = 0; s < PAGED_CLUSTER; ++s) top = fmaxf(top, ms[s]);
+        for (int s = 0; s < MOST; ++s) top = fmaxf(top, ms[s]);
 #pragma unroll
-        for (int s = 0; s < PAGED_CLUSTER; ++s) {
+        for (int s = 0; s < MOST; ++s) {
             ms[s] = ms[s] == -INFINITY ? ls[s] - ls[s] : exp2f(ms[s] - top);           // no maximum: nothing seen, or all NaN, which the sum knows
             sum = fmaf(ms[s], ls[s], sum);
         }
         const bool any = sum > 0.f || sum != sum;
         const float inv = any ? 1.f / sum : 0.f;
 #pragma unroll
-        for (int s = 0; s < PAGED_CLUSTER; ++s)
-            if (s < p.splits) f.factor[s][r] = ms[s] * inv;
+        for (int s = 0; s < MOST; ++s)
+            if (s < parts) f.factor[s][r] = ms[s] * inv;
         f.at[r] = live ? (long long)tok * p.o_ld + (long long)h * p.dim : -1ll;
         if (live && p.lse && b.split == 0) p.lse[(size_t)tok * p.heads + h] = any ? (top + log2f(sum)) * PAGED_LN2 : -INFINITY;
     }
@@ -287,7 +343,7 @@ __device__ __forceinline__ void paged_fold(const PagedParams& p, const PagedBloc
         const long long at = f.at[r];
         if (at < 0 || d >= p.dim) continue;
         float4 o;
-        if (p.splits == 1) {
+        if (parts == 1) {
             const float w = f.factor[0][r];
             const float4 v = *(const float4*)(sums + r * (DN + 4) + d);
             o = make_float4(w * v.x, w * v.y, w * v.z, w * v.w);
@@ -295,14 +351,14 @@ __device__ __forceinline__ void paged_fold(const PagedParams& p, const PagedBloc
             o = make_float4(0.f, 0.f, 0.f, 0.f);
             const uint32_t from = sums_at + (uint32_t)(r * (DN + 4) + d) * 4u;
 #pragma unroll 1
-            for (int s0 = 0; s0 < p.splits; s0 += 4) {                     // four loads on their way
+            for (int s0 = 0; s0 < parts; s0 += 4) {                        // four loads on their way
                 float4 v[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
-                    if (s0 + u < p.splits) v[u] = paged_remote_float4(paged_remote(from, s0 + u));
+                    if (s0 + u < parts) v[u] = paged_remote_float4(paged_remote(from + (uint32_t)((s0 + u) % PARTS * ROWS * (DN + 4)) * 4u, (s0 + u) / PARTS));
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
-                    if (s0 + u < p.splits) {
+                    if (s0 + u < parts) {
                         const float w = f.factor[s0 + u][r];
                         o.x = fmaf(w, v[u].x, o.x); o.y = fmaf(w, v[u].y, o.y); o.z = fmaf(w, v[u].z, o.z); o.w = fmaf(w, v[u].w, o.w);
                     }

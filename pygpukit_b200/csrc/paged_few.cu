@@ -203,42 +203,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) paged_few_kernel(const __grid_co
                 ok = all_wait(err, &land, landed);
                 landed ^= 1u;
                 if (!ok) return;
-                // values of the step's rows: is any not finite?  The largest magnitude of a lane's says
-                const int j0 = (b.ubeg + i) * W_KEYS, k0 = max(0, from - j0), k1 = min(W_KEYS, b.end - j0);
-                auto unit = [&](uint32_t a, uint32_t (&x)[4]) {
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(a) : "memory");
-                };
-                auto put = [&](uint32_t a, const uint32_t (&x)[4]) {
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
-                };
-                uint32_t most = 0;
-#pragma unroll 4
-                for (int e = k0 * 8 + lane; e < k1 * 8; e += 32)
-#pragma unroll
-                    for (int c = 0; c < C; ++c) {
-                        uint32_t x[4];
-                        unit(tile + (uint32_t)c * W_CHUNK + (uint32_t)e * 16u, x);
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) most = __vmaxu2(most, x[y] & 0x7fff7fffu);
-                    }
-                if (__any_sync(0xffffffffu, paged_unfinite<DT>(most) != 0)) {
-                    bad = true;
-                    for (int e = k0 * 8 + lane; e < k1 * 8; e += 32)
-                        for (int c = 0; c < C; ++c) {
-                            const uint32_t a = tile + (uint32_t)c * W_CHUNK + (uint32_t)e * 16u;
-                            uint32_t x[4];
-                            unit(a, x);
-#pragma unroll
-                            for (int y = 0; y < 4; ++y) x[y] &= ~paged_unfinite<DT>(x[y]);
-                            put(a, x);
-                        }
-                }
-                // what lies behind the end in the last copy (what was not copied is zeros)
-                const uint32_t none[4] = {0, 0, 0, 0};
-                const int z1 = cp.bp ? min(W_KEYS, (max(0, k1) + cp.bp - 1) & ~(cp.bp - 1)) : 0;
-                for (int e = max(0, k1) * 8 + lane; e < z1 * 8; e += 32)
-#pragma unroll
-                    for (int c = 0; c < C; ++c) put(tile + (uint32_t)c * W_CHUNK + (uint32_t)e * 16u, none);
+                bad |= paged_fix_values<DT>(tile, C, W_CHUNK, (b.ubeg + i) * W_KEYS, from, b.end, cp.bp, lane);
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[at.s]);
@@ -337,12 +302,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) paged_few_kernel(const __grid_co
                 const float a = ex2(fmaf(s[2 * e], p.scale_log2, nm[2 * e])), c = ex2(fmaf(s[2 * e + 1], p.scale_log2, nm[2 * e + 1]));
                 l[2 * e] += a;
                 l[2 * e + 1] += c;
-                hi[e] = paged_pack2<DT>(a, c);
-                if constexpr (DT == 1) {
-                    const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-                    lo[e] = paged_pack2<DT>(a - back.x, c - back.y);
-                } else
-                    lo[e] = pack_bf16x2(a - bf16lo(hi[e]), c - bf16hi(hi[e]));
+                paged_weights2x2<DT>(a, c, hi[e], lo[e]);
             }
             // the product that has read what was here: of the tile before, or the one before that
             if (i >= X::PBUF && !waited) {
