@@ -5,9 +5,18 @@
 // before context - n and, of the step's, those whose bit is set in its mask, or without masks the rows 0 ... i.  Slots, contexts, row starts and page numbers are
 // data of the device: whatever they say, nothing outside the arrays is touched.
 #pragma once
-#include "common.cuh"
+#include "tc_common.cuh"
 
 namespace pgk {
+
+// n / d = hi(n mul) >> shift for n < 2^31; mul 0: d = 1
+struct PagedDiv { uint32_t mul, shift; };
+inline PagedDiv paged_divisor(int d) {
+    if (d <= 1) return {0u, 0u};
+    uint32_t log = 0;                     // the least with d <= 2^log
+    while ((1ull << log) < (uint64_t)d) ++log;
+    return {(uint32_t)((1ull << (31 + log)) / (uint64_t)d + 1), log - 1};
+}
 
 struct PagedParams {
     const void* q; void* out;
@@ -21,9 +30,10 @@ struct PagedParams {
     const int32_t* masks;                 // [tokens][words], or NULL
     int words;
     float* lse;                           // [tokens][heads] natural logarithms, or NULL
+    float* partial;                       // NULL: the blocks that share a sequence's keys are a cluster; otherwise where each leaves its sums, [item][head][split][ROWS][DN + 4]
     float* weights; long weights_ld;      // paged_weigh.cu: [slots][kv_heads][weights_ld]
     bool wide_q, wide_o;                  // rows on 16-byte boundaries
-    uint32_t page_mul, page_shift;        // n / page_size = hi(n page_mul) >> page_shift for n < 2^31; page_mul 0: pages of one position
+    PagedDiv by_page, by_rep, by_seqs, by_splits;
 };
 
 // paged_tc.cu: whether it serves the call, and the call; paged_few.cu: what it does not; paged_f32.cu
@@ -32,7 +42,7 @@ int paged_tc(const PagedParams& p, int dtype, cudaStream_t st);
 int paged_few(const PagedParams& p, int dtype, cudaStream_t st);
 int paged_f32(const PagedParams& p, cudaStream_t st);
 
-constexpr int PAGED_CLUSTER = 16;         // blocks that share a sequence's keys, at most
+constexpr int PAGED_CLUSTER = 16, PAGED_APART = 32;       // blocks that share a sequence's keys, at most: of a cluster, and one by one
 
 // How many clusters of a kernel run at once: of eight blocks, one a SM, fewer than 148 / 8
 template <typename... KArgs>
@@ -53,22 +63,29 @@ inline cudaError_t clusters_at_once(int* out, void (*kernel)(KArgs...), int thre
     if (n > 0) *out = n;
     return cudaSuccess;
 }
-// Blocks of a cluster that share a sequence's tiles: rounds of clusters times (a block's tiles + what it costs besides, in tiles)
-inline int paged_clusters(const PagedParams& p, int keys, const int* at_once, int most, int ends) {
+// Blocks that share a sequence's tiles.  As a cluster, which folds through shared memory: rounds of clusters times (a block's tiles + what it costs besides, in tiles).  Or one by
+// one, which leave their sums in memory for another launch (about as much again): where clusters do not fill the SMs.  One sequence of 8 key heads, us: 1 row over 4096 keys, clusters
+// of 10 11.7 and 18 blocks apart 13.1; over 32000 36.2 and 33.6; 208 rows over 32000 in two tiles, clusters of 6 59 and 9 blocks apart 51.
+struct PagedSplit { int splits; bool apart; };
+inline PagedSplit paged_split(const PagedParams& p, int keys, const int* at_once, int most, int ends) {
     const int nt = (p.max_keys + keys - 1) / keys;
     const long long items = (long long)p.seqs * p.tiles * p.kv_heads;
     long long least = 0;
-    int best = 1;
+    PagedSplit best = {1, false};
     for (int s = 1; s <= most; ++s) {
         const long long cost = ((items + at_once[s] - 1) / at_once[s]) * ((nt + s - 1) / s + ends);
-        if (s == 1 || cost < least) { best = s; least = cost; }
+        if (s == 1 || cost < least) { best = {s, false}; least = cost; }
+    }
+    for (int s = 2; s <= PAGED_APART && items * s <= at_once[1]; ++s) {
+        const long long cost = (nt + s - 1) / s + 2 * ends;
+        if (cost < least) { best = {s, true}; least = cost; }
     }
     return best;
 }
 
 // blocks of a cluster along z, and the launch that waits for the kernel before it
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_clusters(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
+inline cudaError_t launch_clusters(void (*kernel)(KArgs...), dim3 grid, bool apart, int threads, size_t smem, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads);
@@ -80,7 +97,7 @@ inline cudaError_t launch_clusters(void (*kernel)(KArgs...), dim3 grid, int thre
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = 1;
     attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = grid.z;
+    attr[1].val.clusterDim.z = apart ? 1u : grid.z;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     count_launch();
@@ -91,7 +108,7 @@ inline cudaError_t launch_clusters(void (*kernel)(KArgs...), dim3 grid, int thre
 
 constexpr float PAGED_LOG2E = 1.4426950408889634f, PAGED_LN2 = 0.6931471805599453f, PAGED_LAZY = 8.f;
 
-__device__ __forceinline__ uint32_t paged_page_of(const PagedParams& p, uint32_t n) { return p.page_mul ? __umulhi(n, p.page_mul) >> p.page_shift : n; }
+__device__ __forceinline__ int paged_div(int n, PagedDiv d) { return d.mul ? (int)(__umulhi((uint32_t)n, d.mul) >> d.shift) : n; }       // n not negative
 
 // A block's rows -- ROWS of one sequence's, a token's query heads of one key head beside each other -- and the keys that they see between them, cut over the blocks of a
 // cluster in units of UNIT keys.
@@ -99,8 +116,9 @@ template <int ROWS, int UNIT> struct PagedBlock {
     int seq, head, split, slot, ctx, first, n_rows, f0, live, base, end, ubeg, uend;       // base: the position of the step's row 0
     const int32_t* table;
     __device__ __forceinline__ PagedBlock(const PagedParams& p, int item, int head_, int split_) : head(head_), split(split_) {
-        seq = item % p.seqs;
-        f0 = (p.tiles - 1 - item / p.seqs) * ROWS;
+        const int turn = paged_div(item, p.by_seqs);
+        seq = item - turn * p.seqs;
+        f0 = (p.tiles - 1 - turn) * ROWS;
         slot = __ldcg(p.seq_slots + seq);
         ctx = max(0, __ldcg(p.contexts + seq));
         first = p.starts ? __ldcg(p.starts + seq) : seq;
@@ -109,9 +127,9 @@ template <int ROWS, int UNIT> struct PagedBlock {
         const bool work = f0 < rows && (unsigned)slot < (unsigned)p.slots && ctx > 0;
         live = f0 < rows && (unsigned)slot < (unsigned)p.slots ? min(ROWS, rows - f0) : 0;
         base = ctx - n_rows;                                                             // may lie before position 0: those rows have no key
-        const int last = p.masks ? ctx : base + (f0 + max(live, 1) - 1) / p.rep + 1;      // behind the last key that a row sees
+        const int last = p.masks ? ctx : base + paged_div(f0 + max(live, 1) - 1, p.by_rep) + 1;      // behind the last key that a row sees
         end = work ? max(0, min(min(last, ctx), p.max_keys)) : 0;
-        const int nu = (end + UNIT - 1) / UNIT, per = (nu + p.splits - 1) / p.splits;
+        const int nu = (end + UNIT - 1) / UNIT, per = paged_div(nu + p.splits - 1, p.by_splits);
         ubeg = min(nu, split * per);
         uend = min(nu, ubeg + per);
         table = p.table + (work ? (size_t)slot * p.max_pages : 0);
@@ -119,12 +137,12 @@ template <int ROWS, int UNIT> struct PagedBlock {
     // the cache row (of dim elements) that holds position j of the head, or -1
     __device__ __forceinline__ int row_of(const PagedParams& p, int j) const {
         if (j < 0 || j >= end) return -1;
-        const uint32_t pg = paged_page_of(p, (uint32_t)j);
+        const int pg = paged_div(j, p.by_page);
         const int page = __ldcg(table + pg);
         if ((unsigned)page >= (unsigned)p.pages) return -1;
-        return (page * p.kv_heads + head) * p.page_size + (j - (int)(pg * (uint32_t)p.page_size));
+        return (page * p.kv_heads + head) * p.page_size + (j - pg * p.page_size);
     }
-    __device__ __forceinline__ int token(const PagedParams& p, int r) const { return first + (f0 + r) / p.rep; }
+    __device__ __forceinline__ int token(const PagedParams& p, int r) const { return first + paged_div(f0 + r, p.by_rep); }
 };
 
 // Whether step row i sees step row t
@@ -155,11 +173,6 @@ __device__ __forceinline__ uint32_t paged_remote(uint32_t at, uint32_t rank) {
 __device__ __forceinline__ float paged_remote_float(uint32_t at) {
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-    return v;
-}
-__device__ __forceinline__ float4 paged_remote_float4(uint32_t at) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
     return v;
 }
 template <int DT> __device__ __forceinline__ uint32_t paged_pack2(float lo, float hi) {
@@ -290,97 +303,185 @@ template <int DT> __device__ __forceinline__ void paged_put(const PagedParams& p
     }
 }
 
-// What the cluster's blocks need to become one: shared memory beside the sums [PARTS][ROWS][DN + 4]; a block may have summed its keys in several parts
-template <int ROWS, int PARTS = 1> struct PagedFold {
-    float m[PARTS * ROWS], l[PARTS * ROWS];            // references (log2) and sums
-    int bad;                                           // whether a value of the step's rows that is not finite was taken as zero
-    float factor[PAGED_CLUSTER * PARTS][ROWS];         // what a part's sums are multiplied by
-    long long at[ROWS];                                // where a row's outputs go, below 0: nowhere
+// Values among the step's rows that are not finite were taken as zero, since a weight of zero times them would reach rows that do not see them; a row that does adds them
+template <int ROWS, int UNIT, int DT>
+__device__ __noinline__ void paged_add_unfinite(const PagedParams& p, const PagedBlock<ROWS, UNIT>& b, int r, int d, float4& o) {
+    const int step = paged_div(b.f0 + r, p.by_rep);
+    for (int j = max(0, b.base); j < b.end; ++j) {
+        if (!paged_sees(p, b.first + step, step, j - b.base)) continue;
+        const int row = b.row_of(p, j);
+        if (row < 0) continue;
+        float* x = &o.x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float v = paged_float<DT>(p.v_data, (size_t)row * p.dim + d + e);
+            if (!(fabsf(v) < INFINITY)) x[e] += v;
+        }
+    }
+}
+
+// What a block says of its rows: references (log2) and sums, and whether a value of the step's rows that is not finite was taken as zero
+template <int ROWS> struct PagedFold {
+    float m[ROWS], l[ROWS];
+    int bad;
 };
 
-// The end of every kernel: block r of the cluster has every `splits`-th of its rows' pieces of four elements.  `bad`: values among the step's rows that are not finite were
-// taken as zero, since a weight of zero times them would reach rows that do not see them; the rows that do add them here.
-template <int ROWS, int UNIT, int DT, int DN, int PARTS = 1>
-__device__ __forceinline__ void paged_fold(const PagedParams& p, const PagedBlock<ROWS, UNIT>& b, const float* sums, PagedFold<ROWS, PARTS>& f) {
-    constexpr int PIECES = DN / 4, MOST = PAGED_CLUSTER * PARTS;
-    const int parts = p.splits * PARTS;
-    if (p.splits > 1) paged_cluster_sync();
-    else __syncthreads();
-    bool bad = false;
-    for (int s = 0; s < p.splits; ++s) bad |= __float_as_int(paged_remote_float(paged_remote(smem_u32(&f.bad), s))) != 0;
-    for (int r = (int)threadIdx.x; r < ROWS; r += (int)blockDim.x) {
-        const int x = b.f0 + r, i = x / p.rep, tok = b.first + i, h = b.head * p.rep + x - i * p.rep;
-        const bool live = r < b.live && tok >= 0 && tok < p.tokens;
-        float top = -INFINITY, sum = 0.f, ms[MOST], ls[MOST];
-#pragma unroll
-        for (int s = 0; s < MOST; ++s) {
-            ms[s] = -INFINITY;
-            ls[s] = 0.f;
-            if (s < parts) {
-                ms[s] = paged_remote_float(paged_remote(smem_u32(&f.m[s % PARTS * ROWS + r]), s / PARTS));
-                ls[s] = paged_remote_float(paged_remote(smem_u32(&f.l[s % PARTS * ROWS + r]), s / PARTS));
-            }
-        }
-#pragma unroll
-        for (int s = 0; s < MOST; ++s) top = fmaxf(top, ms[s]);
-#pragma unroll
-        for (int s = 0; s < MOST; ++s) {
-            ms[s] = ms[s] == -INFINITY ? ls[s] - ls[s] : exp2f(ms[s] - top);           // no maximum: nothing seen, or all NaN, which the sum knows
-            sum = fmaf(ms[s], ls[s], sum);
-        }
-        const bool any = sum > 0.f || sum != sum;
-        const float inv = any ? 1.f / sum : 0.f;
-#pragma unroll
-        for (int s = 0; s < MOST; ++s)
-            if (s < parts) f.factor[s][r] = ms[s] * inv;
-        f.at[r] = live ? (long long)tok * p.o_ld + (long long)h * p.dim : -1ll;
-        if (live && p.lse && b.split == 0) p.lse[(size_t)tok * p.heads + h] = any ? (top + log2f(sum)) * PAGED_LN2 : -INFINITY;
+// What a part's sums are multiplied by: without a maximum nothing was seen, or all was NaN, which the sum knows
+__device__ __forceinline__ float paged_factor(float m, float l, float top) { return m == -INFINITY ? l - l : ex2(m - top); }
+
+// The end of every kernel, whose block leaves its rows' sums at stage + r (DN + 4).  begin(), with all threads, when nothing of the shared memory is in use any more; join(), with
+// all threads, when sums, references and so on are there.  Row r belongs to block r % splits of the cluster, which gets it from all blocks and joins them (fetching from the
+// others as one goes waited for each load of a row and for a barrier before leaving: 7900 of a block's 17,000 cycles for a tree of 8 over 1000 keys; sent element by element 25
+// cycles a store).  Or the rows go to memory for paged_join_kernel.
+template <int ROWS, int UNIT, int DT, int DN> struct PagedOut {
+    static constexpr int LD = DN + 4, BYTES = (2 * ROWS + PAGED_CLUSTER - 1) * LD * 4;
+    const PagedParams& p;
+    const PagedBlock<ROWS, UNIT>& b;
+    const PagedFold<ROWS>& f;
+    float* const stage;
+    __device__ __forceinline__ PagedOut(const PagedParams& p_, const PagedBlock<ROWS, UNIT>& b_, const PagedFold<ROWS>& f_, float* stage_) : p(p_), b(b_), f(f_), stage(stage_) {}
+    __device__ __forceinline__ void begin() {
+        __syncthreads();
+        if (p.splits > 1 && !p.partial) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     }
-    __syncthreads();
-    const uint32_t sums_at = smem_u32(sums);
-    for (int i = b.split * (int)blockDim.x + (int)threadIdx.x; i < b.live * PIECES; i += p.splits * (int)blockDim.x) {
-        const int r = i / PIECES, d = (i - r * PIECES) * 4;
-        const long long at = f.at[r];
-        if (at < 0 || d >= p.dim) continue;
-        float4 o;
-        if (parts == 1) {
-            const float w = f.factor[0][r];
-            const float4 v = *(const float4*)(sums + r * (DN + 4) + d);
-            o = make_float4(w * v.x, w * v.y, w * v.z, w * v.w);
-        } else {
-            o = make_float4(0.f, 0.f, 0.f, 0.f);
-            const uint32_t from = sums_at + (uint32_t)(r * (DN + 4) + d) * 4u;
+    template <typename Then> __device__ __forceinline__ void join(Then then) {
+        const int tid = (int)threadIdx.x, threads = (int)blockDim.x, lane = tid & 31, warps = threads >> 5, slots = paged_div(ROWS + p.splits - 1, p.by_splits);
+        for (int r = tid; r < b.live; r += threads) *(float4*)(stage + r * LD + DN) = make_float4(f.m[r], f.l[r], f.bad ? 1.f : 0.f, 0.f);
+        __syncthreads();
+        then();                                    // the sums have been read
+        float* room = stage;
+        if (p.splits > 1) {
+            room += ROWS * LD;
+            float* const global = p.partial ? p.partial + ((size_t)(blockIdx.x * gridDim.y + blockIdx.y) * p.splits + b.split) * (ROWS * LD) : nullptr;
+            if (!global) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 #pragma unroll 1
-            for (int s0 = 0; s0 < parts; s0 += 4) {                        // four loads on their way
-                float4 v[4];
+            for (int r = tid >> 5; r < b.live; r += warps) {
+                const int slot = paged_div(r, p.by_splits);
+                const uint32_t to = paged_remote(smem_u32(room) + (uint32_t)((b.split * slots + slot) * LD) * 4u, global ? 0u : (uint32_t)(r - slot * p.splits));
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (s0 + u < parts) v[u] = paged_remote_float4(paged_remote(from + (uint32_t)((s0 + u) % PARTS * ROWS * (DN + 4)) * 4u, (s0 + u) / PARTS));
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (s0 + u < parts) {
-                        const float w = f.factor[s0 + u][r];
-                        o.x = fmaf(w, v[u].x, o.x); o.y = fmaf(w, v[u].y, o.y); o.z = fmaf(w, v[u].z, o.z); o.w = fmaf(w, v[u].w, o.w);
+                for (int c = 0; c < LD / 4; c += 32)
+                    if (c + lane < LD / 4) {
+                        const float4 v = *(const float4*)(stage + r * LD + 4 * (c + lane));
+                        if (global) __stcg((float4*)(global + r * LD) + c + lane, v);
+                        else asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" :: "r"(to + 16u * (uint32_t)(c + lane)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
                     }
             }
+            if (global) return;
+            paged_cluster_sync();
         }
-        if (bad) {
-            const int step = (b.f0 + r) / p.rep;
-            for (int j = max(0, b.base); j < b.end; ++j) {
-                if (!paged_sees(p, b.first + step, step, j - b.base)) continue;
-                const int row = b.row_of(p, j);
-                if (row < 0) continue;
-                float* x = &o.x;
+        // ---------------- rows split, split + splits, ...: a part's factor goes where its reference was; beside the first one's where the row goes (and whether values were
+        // taken as zero), and what all is multiplied by
+        const int mine = b.live > b.split ? paged_div(b.live - b.split + p.splits - 1, p.by_splits) : 0, ld = slots * LD;
+        for (int slot = tid; slot < mine; slot += threads) {
+            const int x = b.f0 + b.split + slot * p.splits, i = paged_div(x, p.by_rep), tok = b.first + i, h = b.head * p.rep + x - i * p.rep;
+            float* const tail = room + slot * LD + DN;
+            float top = -INFINITY, sum = 0.f, bad = 0.f;
+            for (int s0 = 0; s0 < p.splits; s0 += 4) {
+                float m[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float v = paged_float<DT>(p.v_data, (size_t)row * p.dim + d + e);
-                    if (!(fabsf(v) < INFINITY)) x[e] += v;
+                for (int u = 0; u < 4; ++u) m[u] = s0 + u < p.splits ? tail[(s0 + u) * ld] : -INFINITY;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) top = fmaxf(top, m[u]);
+            }
+            for (int s0 = 0; s0 < p.splits; s0 += 4) {
+                float4 v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = s0 + u < p.splits ? *(const float4*)(tail + (s0 + u) * ld) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const float w = paged_factor(v[u].x, v[u].y, top);
+                    sum = fmaf(v[u].y, w, sum);
+                    bad += v[u].z;
+                    if (s0 + u < p.splits) tail[(s0 + u) * ld] = w;
                 }
             }
+            const bool any = sum > 0.f || sum != sum, there = tok >= 0 && tok < p.tokens;
+            tail[1] = __int_as_float(there ? tok : -1);
+            tail[2] = __int_as_float(bad != 0.f ? ~h : h);
+            tail[3] = any ? 1.f / sum : 0.f;
+            if (p.lse && there) p.lse[(size_t)tok * p.heads + h] = any ? (top + log2f(sum)) * PAGED_LN2 : -INFINITY;
         }
-        paged_put<DT>(p, (size_t)at + d, o);
+        __syncthreads();
+#pragma unroll 2
+        for (int i = tid; i < mine * (DN / 4); i += threads) {
+            const int slot = i / (DN / 4), d = (i - slot * (DN / 4)) * 4;
+            const float* const from = room + slot * LD;
+            const float4 t = *(const float4*)(from + DN), first = *(const float4*)(from + d);
+            const int tok = __float_as_int(t.y), where = __float_as_int(t.z), h = where < 0 ? ~where : where;
+            if (d >= p.dim || tok < 0) continue;
+            float4 o = make_float4(t.x * first.x, t.x * first.y, t.x * first.z, t.x * first.w);
+#pragma unroll 4
+            for (int s = 1; s < p.splits; ++s) {
+                const float w = from[s * ld + DN];
+                const float4 v = *(const float4*)(from + s * ld + d);
+                o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
+            }
+            o.x *= t.w; o.y *= t.w; o.z *= t.w; o.w *= t.w;
+            if (where < 0) paged_add_unfinite<ROWS, UNIT, DT>(p, b, b.split + slot * p.splits, d, o);
+            paged_put<DT>(p, (size_t)tok * p.o_ld + (size_t)h * p.dim + d, o);
+        }
     }
-    if (p.splits > 1) paged_cluster_sync();        // nobody leaves while another reads
+};
+
+// What blocks that are no cluster have left becomes one: a warp a row
+template <int ROWS, int UNIT, int DT, int DN>
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedParams p) {
+    griddep_wait();
+    griddep_launch();
+    const PagedBlock<ROWS, UNIT> b(p, (int)blockIdx.x, (int)blockIdx.y, 0);
+    const int r = (int)blockIdx.z * 8 + (int)(threadIdx.x >> 5);
+    if (r >= b.live) return;
+    constexpr int LD = DN + 4;
+    const int lane = (int)threadIdx.x & 31, x = b.f0 + r, i = paged_div(x, p.by_rep), tok = b.first + i, h = b.head * p.rep + x - i * p.rep;
+    if (tok < 0 || tok >= p.tokens) return;
+    const float* const from = p.partial + ((size_t)(blockIdx.x * gridDim.y + blockIdx.y) * p.splits * ROWS + r) * LD;
+    const float4 tail = lane < p.splits ? __ldcg((const float4*)(from + (size_t)lane * (ROWS * LD) + DN)) : make_float4(-INFINITY, 0.f, 0.f, 0.f);   // lane s knows part s
+    const float top = warp_max(tail.x);
+    float w = paged_factor(tail.x, tail.y, top);
+    const float sum = warp_sum(tail.y * w);
+    const bool bad = __any_sync(0xffffffffu, tail.z != 0.f), any = sum > 0.f || sum != sum;
+    w *= any ? 1.f / sum : 0.f;
+    if (lane == 0 && p.lse) p.lse[(size_t)tok * p.heads + h] = any ? (top + log2f(sum)) * PAGED_LN2 : -INFINITY;
+#pragma unroll
+    for (int d = 4 * lane; d < (DN + 127) / 128 * 128; d += 128) {
+        const bool mine = d < p.dim;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int s0 = 0; s0 < p.splits; s0 += 8) {                        // eight loads on their way
+            float4 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = mine && s0 + u < p.splits ? __ldcg((const float4*)(from + (size_t)(s0 + u) * (ROWS * LD) + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float y = __shfl_sync(0xffffffffu, w, s0 + u);
+                o.x = fmaf(y, v[u].x, o.x); o.y = fmaf(y, v[u].y, o.y); o.z = fmaf(y, v[u].z, o.z); o.w = fmaf(y, v[u].w, o.w);
+            }
+        }
+        if (!mine) continue;
+        if (bad) paged_add_unfinite<ROWS, UNIT, DT>(p, b, r, d, o);
+        paged_put<DT>(p, (size_t)tok * p.o_ld + (size_t)h * p.dim + d, o);
+    }
+}
+
+// The launch of an attention kernel with the split that it takes, and of the join behind blocks that are no cluster
+template <int ROWS, int UNIT, int DT, int DN, typename Launch>
+int paged_launch(PagedParams p, PagedSplit split, cudaStream_t st, Launch launch) {
+    p.splits = split.splits;
+    p.by_splits = paged_divisor(p.splits);
+    const dim3 grid((unsigned)(p.seqs * p.tiles), p.kv_heads, p.splits);
+    void* ws = nullptr;
+    if (split.apart) {
+        if (int rc = scratch_alloc(&ws, (size_t)grid.x * grid.y * grid.z * ROWS * (DN + 4) * 4, st)) return rc;
+        p.partial = (float*)ws;
+    }
+    cudaError_t e = launch(p, grid, split.apart);
+    if (e == cudaSuccess && ws) {
+        const long long most = (long long)p.max_rows * p.rep;
+        e = launch_waiting(paged_join_kernel<ROWS, UNIT, DT, DN>, dim3(grid.x, grid.y, (unsigned)((most < ROWS ? most : ROWS) + 7) / 8), dim3(256), 0, st, p);
+    }
+    if (int rc = scratch_free(ws, st)) return rc;
+    PGK_CUDA(e);
+    return 0;
 }
 
 #endif  // __CUDACC__

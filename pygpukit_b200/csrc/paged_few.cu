@@ -37,7 +37,7 @@ template <int NR, int C> struct Few {
     static constexpr int ROOM = 218 * 1024 - 1024 - (int)(Q + PBUF * P), FIT = ROOM / (int)TILE, SLOTS = FIT < 8 ? FIT : 8;
     static constexpr int BYTES = SLOTS * (int)TILE + (int)(Q + PBUF * P) + 1024;
     static constexpr uint32_t COLUMNS = 2 * NR + DG * 2 * NR, TMEM = COLUMNS <= 64 ? 64 : (COLUMNS <= 128 ? 128 : (COLUMNS <= 256 ? 256 : 512));
-    static_assert(SLOTS >= 2 && COLUMNS <= 512 && NR * (DN + 4) * 4 <= SLOTS * (int)TILE);
+    static_assert(SLOTS >= 2 && COLUMNS <= 512 && (2 * NR + PAGED_CLUSTER - 1) * (DN + 4) * 4 <= BYTES - 1024);
 };
 
 __device__ __forceinline__ bool all_wait(int* err, uint64_t* bar, uint32_t parity) {
@@ -86,10 +86,13 @@ __global__ void __launch_bounds__(W_THREADS, 1) paged_few_kernel(const __grid_co
     const int quad = warp & 3, half = (warp >> 2) & 1, r0 = half * R;
 
     if (warp < W_SOFT) {
+        const int last = min(b.end, b.uend * W_KEYS), step = cp.bp ? cp.bp : 1;
+        int j = b.ubeg * W_KEYS + step * tid;
+        int page = j < last ? __ldcg(b.table + paged_div(j, p.by_page)) : 0;          // looked at behind the queries
         // ---------------- queries: rows of 128 bytes, 64 elements each, zeros behind the head's end
 #pragma unroll 4
         for (int i = tid; i < NR * C * 8; i += W_SOFT * 32) {
-            const int r = i / (C * 8), u = i - r * (C * 8), d = u * 8, x = b.f0 + r, row = x / p.rep, tok = b.first + row;
+            const int r = i / (C * 8), u = i - r * (C * 8), d = u * 8, x = b.f0 + r, row = paged_div(x, p.by_rep), tok = b.first + row;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (r < b.live && d < D && tok >= 0 && tok < p.tokens) {
                 const uint16_t* src = (const uint16_t*)p.q + (size_t)tok * p.q_ld + (size_t)(b.head * p.rep + x - row * p.rep) * D + d;
@@ -104,9 +107,8 @@ __global__ void __launch_bounds__(W_THREADS, 1) paged_few_kernel(const __grid_co
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
                          :: "r"(qs + (uint32_t)(u >> 3) * X::QCHUNK + (uint32_t)r * 128u + (uint32_t)(((u & 7) ^ (r & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
         }
-        const int last = min(b.end, b.uend * W_KEYS), step = cp.bp ? cp.bp : 1;
-        bool gone = false;
-        for (int j = b.ubeg * W_KEYS + step * tid; j < last; j += step * W_SOFT * 32) gone |= b.row_of(p, j) < 0;
+        bool gone = (unsigned)page >= (unsigned)p.pages;
+        for (j += step * W_SOFT * 32; j < last; j += step * W_SOFT * 32) gone |= b.row_of(p, j) < 0;
         if (gone) missing = 1;
         fence_proxy_async();
     }
@@ -230,7 +232,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) paged_few_kernel(const __grid_co
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
         const int clean = missing ? 0 : min(b.base, b.end);               // keys before this one are seen by all
         const int key = quad * 32 + lane, mine = r0 + (lane & (R - 1));    // the row whose reference the lane keeps
-        const int step_row = (b.f0 + mine) / p.rep, tok = b.first + step_row;
+        const int step_row = paged_div(b.f0 + mine, p.by_rep), tok = b.first + step_row;
         const bool live = mine < b.live && tok >= 0 && tok < p.tokens;
         float m_r = -INFINITY, nm[R], l[R];
 #pragma unroll
@@ -339,9 +341,9 @@ __global__ void __launch_bounds__(W_THREADS, 1) paged_few_kernel(const __grid_co
             f.l[mine] = (w.x + w.y) + (w.z + w.w);
         }
     }
-    __syncthreads();                               // nobody's tile is read or written any more
+    PagedOut<NR, W_KEYS, DT, X::DN> out(p, b, f, (float*)(smem + (ring - smem_u32(smem))));
+    out.begin();                                   // nobody's tile is read or written any more
     tc_fence_after();
-    float* const sums = (float*)(smem + (ring - smem_u32(smem)));  // [NR][DN + 4]
     if (warp < W_SOFT) {
 #pragma unroll 1
         for (int g = 0; g < X::DG; ++g) {
@@ -357,15 +359,16 @@ __global__ void __launch_bounds__(W_THREADS, 1) paged_few_kernel(const __grid_co
             }
             if (d < X::DN) {
 #pragma unroll
-                for (int r = 0; r < R; ++r) sums[(r0 + r) * (X::DN + 4) + d] = x[r] + y[r];
+                for (int r = 0; r < R; ++r)
+                    out.stage[(r0 + r) * out.LD + d] = x[r] + y[r];
             }
             __syncwarp();
         }
     }
     tc_fence_before();
-    __syncthreads();
-    if (warp == W_SOFT) tmem_dealloc(tmem, X::TMEM);
-    paged_fold<NR, W_KEYS, DT, X::DN>(p, b, sums, f);
+    out.join([&] {
+        if (warp == W_SOFT) tmem_dealloc(tmem, X::TMEM);
+    });
 }
 
 template <int NR, int C, int DT>
@@ -393,9 +396,9 @@ int launch_few(PagedParams p, cudaStream_t st) {
                     tma_map_bf16_2d(&vmap, p.v_data, (uint64_t)p.dim, (uint64_t)cp.rows, (uint64_t)p.dim * 2, 64, box),
                 "paged_attention failed: no tensor map of %d rows of %d elements", cp.rows, p.dim);
     p.tiles = (int)(((long long)p.max_rows * p.rep + NR - 1) / NR);
-    p.splits = paged_clusters(p, W_KEYS, at_once, PAGED_CLUSTER, 4);
-    PGK_CUDA(launch_clusters(kernel, dim3((unsigned)(p.seqs * p.tiles), p.kv_heads, p.splits), W_THREADS, (size_t)X::BYTES, st, kmap, vmap, p, cp));
-    return 0;
+    return paged_launch<NR, W_KEYS, DT, X::DN>(p, paged_split(p, W_KEYS, at_once, PAGED_CLUSTER, 4), st, [&](const PagedParams& q, dim3 grid, bool apart) {
+        return launch_clusters(kernel, grid, apart, W_THREADS, (size_t)X::BYTES, st, kmap, vmap, q, cp);
+    });
 }
 template <int C, int DT>
 int launch_few_rows(const PagedParams& p, cudaStream_t st) {

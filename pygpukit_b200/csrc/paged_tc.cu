@@ -9,9 +9,10 @@
 //     (two terms would be half as many products again).
 //   * only tiles that hold the step's rows, or the context's end, look at masks.  What lies behind the end is zeroed in V by the copying warp, and values of the step's
 //     rows that are not finite are taken as zero there (a weight of zero times them would reach rows that do not see them) and added in the end.
-// Bound by exponentials and products: of a tile 1024 cycles of the special unit and 1024 of the tensor cores.  (256 rows a block, two tiles of rows that take turns, has room for
-// four tiles of K and V only: 125 us where this takes 104, a step of 32 rows over 64000 keys.)
-// Blocks of a cluster share a sequence's keys and fold through distributed shared memory.
+// Bound by the copies: a SM takes in about 32 bytes a clock, 64 KB of a tile a microsecond, whatever the others do; its products and exponentials need half of that.  (256 rows
+// a block, two sets of rows over the same tiles, halves the copies, but has room for one tile of scores a set: 3500 cycles for what are 2 x 2000 here, and a longer way in and
+// out: 8 x 64 rows over 4100 keys 54 us where this takes 47.)
+// Blocks of a cluster share a sequence's keys.
 #include "paged.cuh"
 #include "tc_common.cuh"
 #include "tma.cuh"
@@ -37,7 +38,7 @@ template <int C> struct Tile {
     static constexpr uint32_t BYTES = C * T_CHUNK;
     // Half of a SM's shared memory at least: a block takes all of tensor memory, and two of unlike kernels on a SM, each of a cluster whose others wait for tensor memory
     // on the other's SMs, would wait for ever.
-    static constexpr int RING = T_SLOTS * (int)BYTES, FOLD = T_ROWS * (DN + 4) * 4, HALF = 116 * 1024, MOST = RING > FOLD ? RING : FOLD,
+    static constexpr int RING = T_SLOTS * (int)BYTES, FOLD = (2 * T_ROWS + PAGED_CLUSTER - 1) * (DN + 4) * 4, HALF = 116 * 1024, MOST = RING > FOLD ? RING : FOLD,
                          SMEM = (MOST > HALF ? MOST : HALF) + 1024;
 };
 
@@ -92,45 +93,58 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
     const PagedBlock<T_ROWS, T_KEYS> b(p, (int)blockIdx.x, (int)blockIdx.y, (int)blockIdx.z);
     const int n = b.uend - b.ubeg, steps = (D + 15) / 16;
     const int quad = warp & 3, side = (warp >> 2) & 1, row = quad * 32 + lane;
-    const int step_row = (b.f0 + row) / p.rep, tok = b.first + step_row;
+    const int step_row = paged_div(b.f0 + row, p.by_rep), tok = b.first + step_row;
     const bool live = warp < T_SOFT && row < b.live && tok >= 0 && tok < p.tokens;
 
-    if (warp < 4) {                                // queries to tensor memory, zeros behind the head's end
-        const uint16_t* const src = (const uint16_t*)p.q + (live ? (size_t)tok * p.q_ld + (size_t)(b.head * p.rep + b.f0 + row - step_row * p.rep) * D : 0);
-        uint32_t x[X::DN / 32][16];
-#pragma unroll
-        for (int c = 0; c < X::DN / 32; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                const int d = 32 * c + 8 * i;
-                if (live && d < D) {
-                    if (p.wide_q) v = ld_act16(src + d);
-                    else {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = (uint32_t)ld_act2(src + d + 2 * e) | (uint32_t)ld_act2(src + d + 2 * e + 1) << 16;
-                        v = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                }
-                x[c][4 * i] = v.x; x[c][4 * i + 1] = v.y; x[c][4 * i + 2] = v.z; x[c][4 * i + 3] = v.w;
-            }
-        __syncwarp();
-#pragma unroll
-        for (int c = 0; c < X::DN / 32; ++c) tmem_st16u(tmem + ((uint32_t)(quad * 32) << 16) + T_Q + (uint32_t)c * 16u, x[c]);
-        tmem_st_wait();
-    } else if (warp < T_SOFT) {
+    // Queries, zeros behind the head's end: rows as they lie through the ring's last place, which the copying warp has not come to, to tensor memory, a lane a row
+    if (warp < T_SOFT) {
         const int last = min(b.end, b.uend * T_KEYS);
-        bool gone = false;
-        for (int j = b.ubeg * T_KEYS + cp.bp * (tid - 128); j < last; j += cp.bp * 128) gone |= b.row_of(p, j) < 0;
+        int j = b.ubeg * T_KEYS + cp.bp * tid;
+        const int page = j < last ? __ldcg(b.table + paged_div(j, p.by_page)) : 0;    // looked at behind the queries
+        const uint32_t qs = ring + (T_SLOTS - 1) * X::BYTES;
+#pragma unroll
+        for (int i = tid; i < T_ROWS * C * 8; i += T_SOFT * 32) {
+            const int r = i / (C * 8), u = i - r * (C * 8), x = b.f0 + r, step = paged_div(x, p.by_rep), t = b.first + step;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < b.live && u * 8 < D && t >= 0 && t < p.tokens) {
+                const uint16_t* const src = (const uint16_t*)p.q + (size_t)t * p.q_ld + (size_t)(b.head * p.rep + x - step * p.rep) * D + u * 8;
+                if (p.wide_q) v = ld_act16(src);
+                else {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = (uint32_t)ld_act2(src + 2 * e) | (uint32_t)ld_act2(src + 2 * e + 1) << 16;
+                    v = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(qs + (uint32_t)r * (C * 128u) + (uint32_t)((u ^ (r & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+        }
+        bool gone = (unsigned)page >= (unsigned)p.pages;
+        for (j += cp.bp * T_SOFT * 32; j < last; j += cp.bp * T_SOFT * 32) gone |= b.row_of(p, j) < 0;
         if (gone) missing = 1;
-    }
-    if (warp <= T_SOFT) {                          // the copies are on their way meanwhile
-        tc_fence_before();
         __syncwarp();
-        asm volatile("bar.sync 9, %0;" :: "n"((T_SOFT + 1) * 32) : "memory");
-        tc_fence_after();
+        asm volatile("bar.sync 10, %0;" :: "n"(T_SOFT * 32) : "memory");
+        uint32_t x[X::DN / 4];                     // a half of the row
+#pragma unroll
+        for (int i = 0; i < C * 4; ++i) {
+            const uint32_t u = (uint32_t)(side * C * 4 + i);
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[4 * i]), "=r"(x[4 * i + 1]), "=r"(x[4 * i + 2]), "=r"(x[4 * i + 3])
+                         : "r"(qs + (uint32_t)row * (C * 128u) + ((u ^ (uint32_t)(row & 7)) << 4)) : "memory");
+        }
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < C; ++c) tmem_st16u(tmem + ((uint32_t)(quad * 32) << 16) + T_Q + (uint32_t)(side * C + c) * 16u, *(uint32_t (*)[16])(x + 16 * c));
+        tmem_st_wait();
+        fence_proxy_async();                       // the place goes back to the copies
+        tc_fence_before();
     }
+    // The copying warp comes when all other places are on their way.  (That the rest waits for it, instead of it alone for the queries, takes 46.5 us where 50 went by: 512 rows of
+    // eight sequences over 4100 keys.)
+    auto queries_there = [] {
+        __syncwarp();
+        asm volatile("bar.sync 9, %0;" :: "n"(T_THREADS) : "memory");
+        tc_fence_after();
+    };
+    if (warp <= T_SOFT) queries_there();
 
     if (warp == T_SOFT) {
         // ---------------- MMAs, from one thread.  The ring has K 0, K 1, V 0, K 2, V 1, ...
@@ -177,7 +191,7 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
     } else if (warp == T_SOFT + 1) {
         // ---------------- copies: lane l has piece l of a tile
         const int pieces = T_KEYS / cp.bp, from = min(b.base, b.end);      // from `from` on values are looked at
-        bool ok = true, bad = false;
+        bool ok = true, bad = false, met = false;
         int issued = 0;
         uint32_t landed = 0;
         RingPos at;
@@ -186,6 +200,10 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
             return r < 0 ? cp.rows : r;
         };
         auto fetch = [&](const CUtensorMap* map, int i, int at_row, bool fix) {
+            if (issued == T_SLOTS - 1 && !met) {
+                met = true;
+                queries_there();
+            }
             ok = ok && __all_sync(0xffffffffu, bar_wait(err, smem_u32(&empty[at.s]), at.round ^ 1u));
             if (!ok) return;
             const uint32_t bar = smem_u32(fix ? &land : &full[at.s]), tile = ring + at.s * X::BYTES;
@@ -216,6 +234,7 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
             r0 = r1;
             r1 = r2;
         }
+        if (!met) queries_there();
         if (bad) f.bad = 1;
         if (lane == 0)
             for (int j = max(0, issued - T_SLOTS); j < issued; ++j)       // whoever gave up: do not leave with copies in flight
@@ -314,15 +333,16 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
         half_m[side][row] = m;
         half_l[side][row] = l;
     }
-    __syncthreads();                               // nobody's tile is read or written any more
+    PagedOut<T_ROWS, T_KEYS, DT, X::DN> out(p, b, f, (float*)smem);
+    out.begin();                                   // nobody's tile is read or written any more
     tc_fence_after();
     if (tid < T_ROWS) {                            // references only grow: the larger one is the outputs'
         const float m0 = half_m[0][tid], m1 = half_m[1][tid], l0 = half_l[0][tid], l1 = half_l[1][tid], m = fmaxf(m0, m1);
         f.m[tid] = m;
         f.l[tid] = (m0 == -INFINITY ? l0 : l0 * exp2f(m0 - m)) + (m1 == -INFINITY ? l1 : l1 * exp2f(m1 - m));
     }
-    float* const sums = (float*)smem;              // [128][DN + 4]
     if (warp < T_SOFT) {
+        float* const to = out.stage + row * out.LD;
 #pragma unroll 1
         for (int c = side * (X::DN / 2); c < (side + 1) * (X::DN / 2); c += 16) {
             float o[16];
@@ -332,14 +352,15 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
                 for (int e = 0; e < 16; ++e) o[e] = 0.f;
             }
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) *(float4*)(sums + (size_t)row * (X::DN + 4) + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            for (int e = 0; e < 16; e += 4) *(float4*)(to + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             __syncwarp();
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == T_SOFT) tmem_dealloc(tmem, 512);
-    paged_fold<T_ROWS, T_KEYS, DT, X::DN>(p, b, sums, f);
+    out.join([&] {
+        if (warp == T_SOFT) tmem_dealloc(tmem, 512);
+    });
 }
 
 template <int C, int DT>
@@ -365,9 +386,9 @@ int launch_tiles(PagedParams p, cudaStream_t st) {
                     tma_map_bf16_2d(&vmap, p.v_data, (uint64_t)p.dim, (uint64_t)cp.rows, (uint64_t)p.dim * 2, 64, (uint32_t)cp.bp),
                 "paged_attention failed: no tensor map of %d rows of %d elements", cp.rows, p.dim);
     p.tiles = (int)(((long long)p.max_rows * p.rep + T_ROWS - 1) / T_ROWS);
-    p.splits = paged_clusters(p, T_KEYS, at_once, PAGED_CLUSTER, 4);
-    PGK_CUDA(launch_clusters(kernel, dim3((unsigned)(p.seqs * p.tiles), p.kv_heads, p.splits), T_THREADS, (size_t)X::SMEM, st, kmap, vmap, p, cp));
-    return 0;
+    return paged_launch<T_ROWS, T_KEYS, DT, X::DN>(p, paged_split(p, T_KEYS, at_once, PAGED_CLUSTER, 4), st, [&](const PagedParams& q, dim3 grid, bool apart) {
+        return launch_clusters(kernel, grid, apart, T_THREADS, (size_t)X::SMEM, st, kmap, vmap, q, cp);
+    });
 }
 
 }  // namespace

@@ -26,7 +26,7 @@ constexpr float H_NONE = -3e38f;
 __device__ __forceinline__ float row_neg(const PagedParams& p, const Keys& b, int r) {
     const int tok = b.token(p, r);
     if (r >= b.live || tok < 0 || tok >= p.tokens) return H_NONE;
-    const float z = __ldcg(p.lse + (size_t)tok * p.heads + b.head * p.rep + r % p.rep);
+    const float z = __ldcg(p.lse + (size_t)tok * p.heads + b.head * p.rep + r - paged_div(r, p.by_rep) * p.rep);
     return z == -INFINITY ? H_NONE : -z * PAGED_LOG2E;
 }
 __device__ __forceinline__ void add_weight(const PagedParams& p, const Keys& b, int j, float w) {
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(H_THREADS) paged_weigh_kernel(const __grid_con
             // ---------------- the batch's rows
 #pragma unroll 4
             for (int i = tid; i < groups * NR * C * 8; i += H_SOFT * 32) {
-                const int r = i / (C * 8), u = i - r * (C * 8), d = u * 8, x = f0 + r, row = x / p.rep, tok = b.first + row, g = r / NR, rr = r - g * NR;
+                const int r = i / (C * 8), u = i - r * (C * 8), d = u * 8, x = f0 + r, row = paged_div(x, p.by_rep), tok = b.first + row, g = r / NR, rr = r - g * NR;
                 uint4 v = make_uint4(0, 0, 0, 0);
                 if (x < b.live && d < D && tok >= 0 && tok < p.tokens) {
                     const uint16_t* src = (const uint16_t*)p.q + (size_t)tok * p.q_ld + (size_t)(b.head * p.rep + x - row * p.rep) * D + d;
@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(H_THREADS) paged_weigh_kernel(const __grid_con
                 for (int g = 0; g < groups; ++g, ++turn) {
                     uint32_t see = 0;
                     if (edge) {
-                        const int x = f0 + g * NR + r0 + (lane & (R - 1)), row = x / p.rep;
+                        const int x = f0 + g * NR + r0 + (lane & (R - 1)), row = paged_div(x, p.by_rep);
                         see = x < b.live && j0 < b.end ? paged_window(p, b.first + row, row, j0 - b.base) : 0u;
                     }
                     ok = ok && __all_sync(0xffffffffu, bar_wait(err, smem_u32(&sfull[turn & 1]), (uint32_t)(turn >> 1) & 1u));
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(G_THREADS) paged_weigh_f32_kernel(const __grid
     for (int f0 = 0; f0 < b.live; f0 += G_ROWS) {
         __syncthreads();
         for (int i = tid; i < G_ROWS * D; i += G_THREADS) {
-            const int r = i / D, f = f0 + r, row = f / p.rep, tok = b.first + row;
+            const int r = i / D, f = f0 + r, row = paged_div(f, p.by_rep), tok = b.first + row;
             qs[i] = f < b.live && tok >= 0 && tok < p.tokens ? __ldcg((const float*)p.q + (size_t)tok * p.q_ld + (size_t)(b.head * p.rep + f - row * p.rep) * D + (i - r * D)) : 0.f;
         }
         if (tid < G_ROWS) negs[tid] = row_neg(p, b, f0 + tid);
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(G_THREADS) paged_weigh_f32_kernel(const __grid
                 const float w = ex2(fmaf(s[r], p.scale_log2, negs[r0 + r]));
                 bool sees = true;
                 if (edge) {
-                    const int i = (f0 + r0 + r) / p.rep;
+                    const int i = paged_div(f0 + r0 + r, p.by_rep);
                     sees = rows >= 0 && (j < b.base || paged_sees(p, b.first + i, i, j - b.base));
                 }
                 if (sees) sum += w;
@@ -330,6 +330,7 @@ template <int NR, int C, int DT> int launch_weigh(PagedParams p, cudaStream_t st
         const long long cost = ((items * s + slots - 1) / slots) * ((nt + s - 1) / s + 3);
         if (s == 1 || cost < least) { p.splits = s; least = cost; }
     }
+    p.by_splits = paged_divisor(p.splits);
     PGK_CUDA(launch_waiting(paged_weigh_kernel<NR, C, DT>, dim3(p.splits, p.kv_heads, p.seqs), dim3(H_THREADS), (size_t)smem, st, kmap, p, cp));
     return 0;
 }
@@ -390,12 +391,9 @@ int paged_params(const char* fn, PagedParams* out, const void* q, long q_ld, con
     p.max_keys = max_context < max_pages * page_size ? max_context : max_pages * page_size;
     p.scale_log2 = (scale > 0.f ? scale : 1.f / sqrtf((float)dim)) * PAGED_LOG2E;
     p.masks = masks; p.words = mask_words;
-    if (page_size > 1) {                                      // log: the least with page_size <= 2^log
-        uint32_t log = 0;
-        while ((1ull << log) < (uint64_t)page_size) ++log;
-        p.page_shift = log - 1;
-        p.page_mul = (uint32_t)((1ull << (31 + log)) / (uint64_t)page_size + 1);
-    }
+    p.by_page = paged_divisor(page_size);
+    p.by_rep = paged_divisor(p.rep);
+    p.by_seqs = paged_divisor(p.seqs);
     const int size = dtype == 0 ? 4 : 2;
     p.wide_q = (uintptr_t)q % 16 == 0 && q_ld * size % 16 == 0;
     *out = p;

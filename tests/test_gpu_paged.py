@@ -128,6 +128,25 @@ def test_long_contexts_over_many_blocks(dtype, rows):
     s.check(s.run())
 
 
+@pytest.mark.parametrize("dtype,portions,Hq,H,D,ps,masks", [
+    ("bfloat16", [(17000, 1)], 8, 2, 128, 64, "chain"), ("float16", [(17003, 3)], 8, 2, 96, 16, "tree"), ("bfloat16", [(0, 0), (17000, 50), (5, 5), (300, 7)], 6, 1, 128, 64, "any"),
+    ("float16", [(9000, 140)], 2, 1, 64, 32, "tree"), ("bfloat16", [(9001, 20)], 4, 2, 80, 100, "tree"), ("bfloat16", [(6000, 2)], 2, 1, 256, 64, "tree"),
+    ("float32", [(6000, 2), (3, 3)], 4, 1, 128, 64, "any"), ("float32", [(6001, 5)], 4, 2, 64, 16, "tree"), ("float32", [(5000, 3)], 2, 1, 256, 64, "tree")])
+def test_long_contexts_over_blocks_that_are_no_cluster(dtype, portions, Hq, H, D, ps, masks):
+    s = Step(portions, Hq, H, D, ps, dtype, masks=masks, seed=8)
+    s.check(s.run())
+
+
+@pytest.mark.parametrize("dtype,rows,Hq,D", [("bfloat16", 3, 2, 128), ("float16", 70, 2, 128), ("float32", 3, 2, 64)])
+def test_values_that_are_not_finite_behind_a_long_context(dtype, rows, Hq, D):
+    s = Step([(17000, rows)], Hq, 1, D, 64, dtype, masks="tree", seed=4)
+    x = np.full((1, D), np.nan)
+    s.p.put(s.p.v, 0, [17000 - rows + 1], ref.rounded(x, dtype))
+    x[:, ::2] = -np.inf
+    s.p.put(s.p.v, 0, [17000 - 1], ref.rounded(x, dtype))
+    s.check(s.run())
+
+
 @pytest.mark.parametrize("rows", [1, 9, 40])
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
 def test_masks_make_what_no_masks_make(dtype, rows):
