@@ -234,17 +234,17 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 // the lanes' N values (a power of two up to 32) reduced over the warp: lane l ends with value l % N
-template <int N, typename F> __device__ __forceinline__ float reduce_lanes(float (&v)[N], int lane, F f) {
+template <int N, typename T, typename F> __device__ __forceinline__ T reduce_lanes(T (&v)[N], int lane, F f) {
 #pragma unroll
     for (int w = N / 2; w > 0; w >>= 1) {
         const bool up = lane & w;
 #pragma unroll
         for (int j = 0; j < w; ++j) {
-            const float got = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + w], w);
+            const T got = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + w], w);
             v[j] = f(up ? v[j + w] : v[j], got);
         }
     }
-    float x = v[0];
+    T x = v[0];
 #pragma unroll
     for (int w = N; w < 32; w <<= 1) x = f(x, __shfl_xor_sync(0xffffffffu, x, w));
     return x;

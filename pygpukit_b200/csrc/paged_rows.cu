@@ -3,11 +3,12 @@
 // Selection.  Of a sequence's positions the first, the recent and the ones of the largest weights stay, per key head, `budget` in all, in ascending order.  A block has one head, a
 // warp a run of its positions, a weight as an ordered 32-bit number in a register.  The least that stays is found in four digits of eight bits, a histogram each, in which every lane
 // has a column of its own: weights are alike in their upper digits, and a warp's 32 additions to one place would take turns.  Then a warp counts what stays of its run and writes it
-// behind what the warps before it have.  Bound by its passes' latencies, 4 bytes a position being little.
+// behind what the warps before it have.  A digit that nothing below the least shares ends the search.  Bound by its passes' latencies, 4 bytes a position being little: 2048 of 4096
+// positions of 8 heads 7.1 us, 4096 of 8192 of 128 heads 12.0.
 //
 // Moving.  Row start + i of a sequence becomes, in place, what row start + from[i] was, from[i] >= i.  What is written lies before everything that is still to be read, from[i'] >= i' > i,
 // but for the rows that are moved at the same time: a tile's rows are read by all of the cluster before any is written, and the next tile's are on their way
-// meanwhile.  Bound by memory.
+// meanwhile.  Bound by memory (2048 of 4096 rows of 128 heads and keys and values, 550 MB, 126 us) or, of few rows, by the chain from position to page to row: 4 rows in 16 layers 6.3 us.
 #include "paged.cuh"
 #include "../../include/pgk_b200.h"
 
@@ -36,7 +37,7 @@ template <int K>
 __global__ void __launch_bounds__(C_THREADS) select_kernel(const __grid_constant__ SelectParams p) {
     __shared__ int bins[C_BINS][32];
     __shared__ int sums[C_BINS], over[C_WARPS], same[C_WARPS];
-    __shared__ int found, left;
+    __shared__ int found, left, whole;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.x, seq = blockIdx.y;
     griddep_wait();
     griddep_launch();
@@ -81,13 +82,11 @@ __global__ void __launch_bounds__(C_THREADS) select_kernel(const __grid_constant
             if (j < to && (x & above) == least) atomicAdd(&bins[(x >> shift) & 255u][lane], 1);
         });
         __syncthreads();
+        int x[C_BINS / C_WARPS];
 #pragma unroll
-        for (int i = 0; i < C_BINS / C_WARPS; ++i) {
-            int x = bins[warp + C_WARPS * i][lane];
-#pragma unroll
-            for (int y = 16; y > 0; y >>= 1) x += __shfl_xor_sync(0xffffffffu, x, y);
-            if (lane == 0) sums[warp + C_WARPS * i] = x;
-        }
+        for (int i = 0; i < C_BINS / C_WARPS; ++i) x[i] = bins[warp + C_WARPS * i][lane];
+        const int sum = reduce_lanes<C_BINS / C_WARPS>(x, lane, [](int a, int b) { return a + b; });
+        if (lane < C_BINS / C_WARPS) sums[warp + C_WARPS * lane] = sum;
         __syncthreads();
         if (warp == 0) {                                      // the bin with the need-th from above: lane l has bins 8 l ... 8 l + 7
             int mine[8], all = 0;
@@ -106,12 +105,14 @@ __global__ void __launch_bounds__(C_THREADS) select_kernel(const __grid_constant
                 if (higher < need && need <= after + mine[i]) {
                     found = 8 * lane + i;
                     left = need - higher;
+                    whole = need == after + mine[i];
                 }
             }
         }
         __syncthreads();
         least |= (uint32_t)found << shift;
         need = left;
+        if (whole) break;                                     // all that share the digits stay; what they have behind them does not count
     }
     // those above the least, and the first `need` of its equals
     int n_over = 0, n_same = 0;
@@ -121,11 +122,8 @@ __global__ void __launch_bounds__(C_THREADS) select_kernel(const __grid_constant
     });
     if (lane == 0) { over[warp] = n_over; same[warp] = n_same; }
     __syncthreads();
-    int at = 0, seen = 0;
-    for (int i = 0; i < warp; ++i) {
-        at += over[i] + min(same[i], max(0, need - seen));
-        seen += same[i];
-    }
+    static_assert(C_WARPS == 32);
+    int seen = __reduce_add_sync(0xffffffffu, lane < warp ? same[lane] : 0), at = __reduce_add_sync(0xffffffffu, lane < warp ? over[lane] : 0) + min(seen, need);
     each([&](int j, uint32_t x) {
         const uint32_t eq = __ballot_sync(0xffffffffu, j < to && x == least), below = (1u << lane) - 1u;
         const bool stays = j < to && (x > least || (x == least && seen + __popc(eq & below) < need));
@@ -148,7 +146,7 @@ struct MoveParams {
     int width, by_head;                   // from [sequences][kv_heads if by_head][width]
     float* weights; long weights_ld;      // moved as well, [slots][kv_heads][weights_ld]; what is behind the last row up to the context becomes zero
     const int32_t* contexts;
-    uint32_t page_mul, page_shift;
+    PagedDiv by_page, by_units;
 };
 
 template <int V> struct Unit;
@@ -181,14 +179,14 @@ __global__ void __launch_bounds__(M_THREADS, 3) move_kernel(const __grid_constan
         const int32_t* const table = p.table + (there ? (size_t)slot * p.max_pages : 0);
         auto row_of = [&](long long j) {
             if (j < 0 || j >= (long long)p.max_pages * p.page_size) return -1;
-            const uint32_t pg = p.page_mul ? __umulhi((uint32_t)j, p.page_mul) >> p.page_shift : (uint32_t)j;
-            const int page = __ldcg(table + pg);
-            return (unsigned)page >= (unsigned)p.pages ? -1 : (page * p.kv_heads + head) * p.page_size + ((int)j - (int)(pg * (uint32_t)p.page_size));
+            const int pg = paged_div((int)j, p.by_page), page = __ldcg(table + pg);
+            return (unsigned)page >= (unsigned)p.pages ? -1 : (page * p.kv_heads + head) * p.page_size + ((int)j - pg * p.page_size);
         };
         const uint32_t units = (uint32_t)(p.bytes / V);
         // rows of a tile: of one array as many as it has units for, or all there are and as many arrays
         const int per = max(1, (int)(M_TILE / units)), rows = min(per, count), group = count <= per && blocks == 1 ? max(1, per / max(1, count)) : 1;
         const int tiles = rows > 0 ? (count + rows * blocks - 1) / (rows * blocks) : 0;
+        const uint32_t per_array = (1u << 22) / (uint32_t)max(1, rows) + 1u;                // exact for ar < 2^11
         auto look = [&](int tile) {
             const int i0 = (tile * blocks + rank) * rows;
             for (int r = tid; r < rows; r += M_THREADS) {
@@ -208,18 +206,19 @@ __global__ void __launch_bounds__(M_THREADS, 3) move_kernel(const __grid_constan
                 for (uint32_t c0 = 0; c0 < units; c0 += M_TILE) {
                     const uint32_t wide = min(units - c0, (uint32_t)M_TILE), total = wide * (uint32_t)rows * (uint32_t)n;
                     T x[M_UNITS];
-                    T* to[M_UNITS];
+                    T *to[M_UNITS], *at[M_UNITS];
 #pragma unroll
-                    for (int q = 0; q < M_UNITS; ++q) {
-                        const uint32_t e = (uint32_t)(q * M_THREADS + tid), ar = e / wide, c = c0 + (e - ar * wide), k = group > 1 ? ar / (uint32_t)rows : 0u;
-                        to[q] = nullptr;
-                        if (e >= total) continue;
-                        const int2 at = places[t & 1][ar - k * (uint32_t)rows];
-                        if (at.x < 0) continue;
+                    for (int q = 0; q < M_UNITS; ++q) {               // all addresses before the first load: no branch between
+                        const uint32_t e = (uint32_t)(q * M_THREADS + tid), ar = units > M_TILE ? 0u : (uint32_t)paged_div((int)e, p.by_units), c = c0 + (e - ar * wide);
+                        const uint32_t k = group > 1 ? min(__umulhi(ar << 10, per_array), (uint32_t)n - 1u) : 0u;         // ar / rows
+                        const int2 row = places[t & 1][min(ar - k * (uint32_t)rows, (uint32_t)M_TILE - 1u)];
                         T* const base = (T*)p.arrays[a0 + a + (int)k];
-                        x[q] = load_unit(base + (size_t)at.x * units + c);
-                        to[q] = base + (size_t)at.y * units + c;
+                        at[q] = base + (size_t)max(row.x, 0) * units + c;
+                        to[q] = e < total && row.x >= 0 ? base + (size_t)max(row.y, 0) * units + c : nullptr;
                     }
+#pragma unroll
+                    for (int q = 0; q < M_UNITS; ++q)
+                        if (to[q]) x[q] = load_unit(at[q]);
                     if (c0 + M_TILE >= units) {
                         if (t + 1 < tiles) look(t + 1);
                         else if (tiles % 2 == 0) look(0);         // for the next array; this tile is in the other buffer
@@ -297,12 +296,7 @@ extern "C" int pgk_move_rows(void* const* host_arrays, const int32_t* host_row_b
     p.table = page_table; p.pages = pages; p.page_size = page_size; p.slots = slots; p.max_pages = max_pages; p.kv_heads = kv_heads;
     p.seq_slots = seq_slots; p.starts = starts; p.from = from; p.counts = counts; p.width = width; p.by_head = by_head;
     p.weights_ld = weights_ld; p.contexts = context_lens;
-    if (page_size > 1) {
-        uint32_t log = 0;
-        while ((1ull << log) < (uint64_t)page_size) ++log;
-        p.page_shift = log - 1;
-        p.page_mul = (uint32_t)((1ull << (31 + log)) / (uint64_t)page_size + 1);
-    }
+    p.by_page = paged_divisor(page_size);
     const cudaStream_t st = (cudaStream_t)stream;
     for (int a = 0; a < n_arrays; ++a)
         PGK_REQUIRE(host_arrays[a] && host_row_bytes[a] > 0 && host_row_bytes[a] % 2 == 0, "move_rows failed: rows of %d bytes", host_row_bytes[a]);
@@ -310,12 +304,13 @@ extern "C" int pgk_move_rows(void* const* host_arrays, const int32_t* host_row_b
         uintptr_t low = (uintptr_t)p.bytes;
         for (int a = 0; a < p.n; ++a) low |= (uintptr_t)p.arrays[a];
         const int unit = low % 16 == 0 ? 16 : (low % 4 == 0 ? 4 : 2);
+        p.by_units = paged_divisor(p.bytes / unit);
         // arrays of a block: as many as leave four blocks a SM, where there are so many
         p.chunk = (int)((long long)p.n * kv_heads * seqs / (4 * sm_count()));
         if (p.chunk < 1) p.chunk = 1;
         const int chunks = (p.n + p.chunk - 1) / p.chunk + (p.weights ? 1 : 0);
         PGK_REQUIRE((long long)chunks * kv_heads <= 65535, "move_rows failed: too many heads");
-        // blocks that share a head's rows: until there are twelve a SM, which even out (256 heads of 4096 rows, 1 / 2 / 4 / 8 blocks: 139 / 148 / 132 / 147 us), none with less than a tile
+        // blocks that share a head's rows: until there are twelve a SM, which even out (256 heads of 4096 rows, 1 / 2 / 4 / 8 blocks, before the addresses came before the loads: 139 / 148 / 132 / 147 us; now 126 with 4), none with less than a tile
         const long long items = (long long)chunks * kv_heads * seqs;
         int blocks = 1;
         while (blocks < M_CLUSTER && items * blocks * 2 <= 12 * sm_count() && (long long)width * (p.bytes / unit) > (long long)M_TILE * blocks) blocks *= 2;
