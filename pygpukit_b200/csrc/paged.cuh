@@ -66,6 +66,7 @@ inline cudaError_t clusters_at_once(int* out, void (*kernel)(KArgs...), int thre
 // Blocks that share a sequence's tiles.  As a cluster, which folds through shared memory: rounds of clusters times (a block's tiles + what it costs besides, in tiles).  Or one by
 // one, which leave their sums in memory for another launch (about as much again): where clusters do not fill the SMs.  One sequence of 8 key heads, us: 1 row over 4096 keys, clusters
 // of 10 11.7 and 18 blocks apart 13.1; over 32000 36.2 and 33.6; 208 rows over 32000 in two tiles, clusters of 6 59 and 9 blocks apart 51.
+// Eight trees of 128 float32 rows over 4000 keys, 1 / 2 / 3 blocks: 379 / 316 / 360.
 struct PagedSplit { int splits; bool apart; };
 inline PagedSplit paged_split(const PagedParams& p, int keys, const int* at_once, int most, int ends) {
     const int nt = (p.max_keys + keys - 1) / keys;
@@ -73,11 +74,13 @@ inline PagedSplit paged_split(const PagedParams& p, int keys, const int* at_once
     long long least = 0;
     PagedSplit best = {1, false};
     for (int s = 1; s <= most; ++s) {
-        const long long cost = ((items + at_once[s] - 1) / at_once[s]) * ((nt + s - 1) / s + ends);
+        long long rounds = (8 * items + at_once[s] - 1) / at_once[s];                      // in eighths, whole ones up to two: then blocks no longer end together
+        if (rounds <= 16) rounds = (rounds + 7) & ~7ll;
+        const long long cost = rounds * ((nt + s - 1) / s + ends);
         if (s == 1 || cost < least) { best = {s, false}; least = cost; }
     }
     for (int s = 2; s <= PAGED_APART && items * s <= at_once[1]; ++s) {
-        const long long cost = (nt + s - 1) / s + 2 * ends;
+        const long long cost = 8 * ((nt + s - 1) / s + 2 * ends);
         if (cost < least) { best = {s, true}; least = cost; }
     }
     return best;
