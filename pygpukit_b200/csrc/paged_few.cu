@@ -388,7 +388,7 @@ int launch_few(PagedParams p, cudaStream_t st) {
     if (cp.bp > W_KEYS) cp.bp = W_KEYS;
     if (cp.bp < 8) cp.bp = 0;
     cp.rows = p.pages * p.kv_heads * p.page_size;
-    cp.err = wait_word(kWaitPaged);
+    cp.err = wait_word(kWaitPagedFew);
     PGK_REQUIRE(cp.err, "paged_attention failed: no pinned host memory");
     CUtensorMap kmap{}, vmap{};
     const uint32_t box = cp.bp ? (uint32_t)cp.bp : 1u;

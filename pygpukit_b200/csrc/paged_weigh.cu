@@ -317,7 +317,7 @@ template <int NR, int C, int DT> int launch_weigh(PagedParams p, cudaStream_t st
     cp.rows = p.pages * p.kv_heads * p.page_size;
     const long long groups = ((long long)p.max_rows * p.rep + NR - 1) / NR;
     cp.groups = (int)(groups < X::MOST ? groups : X::MOST);
-    cp.err = wait_word(kWaitPaged);
+    cp.err = wait_word(kWaitWeigh);
     PGK_REQUIRE(cp.err, "paged_weigh failed: no pinned host memory");
     CUtensorMap kmap{};
     PGK_REQUIRE(tma_encode_fn() && tma_map_bf16_2d(&kmap, p.k_data, (uint64_t)p.dim, (uint64_t)cp.rows, (uint64_t)p.dim * 2, 64, cp.bp ? (uint32_t)cp.bp : 1u),
