@@ -153,14 +153,17 @@ def move_rows_paged(arrays: "list[GPUArray]", page_table: GPUArray, slots: GPUAr
         raise ValueError(f"{name}: no arrays")
     pages, H, ps, _, n_slots, max_pages = _pages(name, arrays[0], page_table)
     shape, dtype = arrays[0]._shape, arrays[0]._dtype
-    for a in arrays:
-        if a._shape != shape and (len(a._shape) != 4 or a._shape[:3] != shape[:3] or a._shape[3] < 1):
+    sizes = array("i", [shape[3] * dtype.itemsize]) * len(arrays)
+    unlike = [i for i, a in enumerate(arrays) if a._shape != shape or a._dtype is not dtype]      # most calls have none
+    for i in (0, *unlike):
+        a = arrays[i]
+        if len(a._shape) != 4 or a._shape[:3] != shape[:3] or a._shape[3] < 1:
             raise ValueError(f"{name}: arrays [{pages}, {H}, {ps}, elements], got {a.shape}")
-        if a._dtype is uint8 or a._dtype == uint8:
+        if a._dtype == uint8:
             raise ValueError(f"{name}: pages of bytes keep a position's row in two places")
-    sizes = array("i", [a._shape[3] * a._dtype.itemsize for a in arrays])
-    if any(n % 2 or n > 4096 for n in sizes):
-        raise ValueError(f"{name}: rows of an even number of bytes up to 4096, got {dtype} {shape}")
+        sizes[i] = a._shape[3] * a._dtype.itemsize
+        if sizes[i] % 2 or sizes[i] > 4096:
+            raise ValueError(f"{name}: rows of an even number of bytes up to 4096, got {a._dtype} {a.shape}")
     ptrs = array("Q", [a._ptr for a in arrays])
     if len(set(ptrs)) < len(ptrs):
         raise ValueError(f"{name}: an array is there twice")
