@@ -4,6 +4,8 @@
 // 16-bit pages: scores S^T[128 keys, NR rows] = K Q^T by tcgen05 as in paged_few.cu, tiles of K through a ring, the step's rows in shared memory (as many as 64 KB hold at a
 // time); eight warps, a lane a key and half of the rows each, sum the weights as they come.  32-bit pages: multiply-adds, a lane a key.  A position's sum is one
 // thread's until it is added, so that the same call gives the same bits.  Decoding is bound by the bytes of the keys, windows of a prompt's last tokens by the exponentials.
+#include <type_traits>
+
 #include "paged.cuh"
 #include "tc_common.cuh"
 #include "tma.cuh"
@@ -197,28 +199,32 @@ __global__ void __launch_bounds__(H_THREADS) paged_weigh_kernel(const __grid_con
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sread[turn & 1]);
                     const float4* const neg = (const float4*)(negs + g * NR + r0);
-                    const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
-                    uint64_t sum2 = pair(sum, 0.f);
+                    auto add = [&](auto masked) {          // apart from each other: a branch at every weight is 1340 cycles for 64 rows
+                        const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
+                        uint64_t sum2 = pair(sum, 0.f);
 #pragma unroll
-                    for (int r = 0; r < R; r += 4) {
-                        const float4 x = neg[r / 4];
-                        float w[4];
-                        unpair(fma2(pair(s[r], s[r + 1]), scale2, pair(x.x, x.y)), w[0], w[1]);
-                        unpair(fma2(pair(s[r + 2], s[r + 3]), scale2, pair(x.z, x.w)), w[2], w[3]);
+                        for (int r = 0; r < R; r += 4) {
+                            const float4 x = neg[r / 4];
+                            float w[4];
+                            unpair(fma2(pair(s[r], s[r + 1]), scale2, pair(x.x, x.y)), w[0], w[1]);
+                            unpair(fma2(pair(s[r + 2], s[r + 3]), scale2, pair(x.z, x.w)), w[2], w[3]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            w[e] = ex2(w[e]);
-                            if (edge) {
-                                const uint32_t bits = __shfl_sync(0xffffffffu, see, r + e);
-                                if (!there || !((bits >> lane) & 1u)) w[e] = 0.f;
+                            for (int e = 0; e < 4; ++e) {
+                                w[e] = ex2(w[e]);
+                                if constexpr (masked.value) {
+                                    const uint32_t bits = __shfl_sync(0xffffffffu, see, r + e);
+                                    if (!there || !((bits >> lane) & 1u)) w[e] = 0.f;
+                                }
                             }
+                            sum2 = add2(sum2, pair(w[0], w[1]));
+                            sum2 = add2(sum2, pair(w[2], w[3]));
                         }
-                        sum2 = add2(sum2, pair(w[0], w[1]));
-                        sum2 = add2(sum2, pair(w[2], w[3]));
-                    }
-                    float u, v;
-                    unpair(sum2, u, v);
-                    sum = u + v;
+                        float u, v;
+                        unpair(sum2, u, v);
+                        sum = u + v;
+                    };
+                    if (edge) add(std::true_type{});
+                    else add(std::false_type{});
                 }
                 if (half == 1) other[i & 1][key] = sum;
                 asm volatile("bar.sync %0, 64;" :: "r"(1 + quad) : "memory");      // a key's two warps; two turns of places, so that none is overwritten unread
