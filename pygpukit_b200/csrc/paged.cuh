@@ -64,8 +64,8 @@ inline cudaError_t clusters_at_once(int* out, void (*kernel)(KArgs...), int thre
     return cudaSuccess;
 }
 // Blocks that share a sequence's tiles.  As a cluster, which folds through shared memory: rounds of clusters times (a block's tiles + what it costs besides, in tiles).  Or one by
-// one, which leave their sums in memory for another launch (about as much again): where clusters do not fill the SMs.  One sequence of 8 key heads, us: 1 row over 4096 keys, clusters
-// of 10 11.7 and 18 blocks apart 13.1; over 32000 36.2 and 33.6; 208 rows over 32000 in two tiles, clusters of 6 59 and 9 blocks apart 51.
+// one, which leave their sums in memory for another launch (half as much again): where clusters do not fill the SMs.  One sequence of 8 key heads, us: 1 row over 4096 keys, clusters
+// of 10 11.5 and 18 blocks apart 11.6; over 8000 15.2 and 13.6, over 32000 37 and 32; 208 rows over 32000 in two tiles, clusters of 6 54 and 9 blocks apart 45.
 // Eight trees of 128 float32 rows over 4000 keys, 1 / 2 / 3 blocks: 379 / 316 / 360.
 struct PagedSplit { int splits; bool apart; };
 inline PagedSplit paged_split(const PagedParams& p, int keys, const int* at_once, int most, int ends) {
@@ -80,7 +80,7 @@ inline PagedSplit paged_split(const PagedParams& p, int keys, const int* at_once
         if (s == 1 || cost < least) { best = {s, false}; least = cost; }
     }
     for (int s = 2; s <= PAGED_APART && items * s <= at_once[1]; ++s) {
-        const long long cost = 8 * ((nt + s - 1) / s + 2 * ends);
+        const long long cost = 8 * ((nt + s - 1) / s) + 12 * ends;
         if (cost < least) { best = {s, true}; least = cost; }
     }
     return best;
@@ -429,16 +429,22 @@ template <int ROWS, int UNIT, int DT, int DN> struct PagedOut {
 // What blocks that are no cluster have left becomes one: a warp a row
 template <int ROWS, int UNIT, int DT, int DN>
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedParams p) {
+    const PagedBlock<ROWS, UNIT> b(p, (int)blockIdx.x, (int)blockIdx.y, 0);          // what the kernel before has read as well: it is there
+    const int r = (int)blockIdx.z * 8 + (int)(threadIdx.x >> 5);
     griddep_wait();
     griddep_launch();
-    const PagedBlock<ROWS, UNIT> b(p, (int)blockIdx.x, (int)blockIdx.y, 0);
-    const int r = (int)blockIdx.z * 8 + (int)(threadIdx.x >> 5);
     if (r >= b.live) return;
-    constexpr int LD = DN + 4;
+    constexpr int LD = DN + 4, STEP = ROWS * LD;
     const int lane = (int)threadIdx.x & 31, x = b.f0 + r, i = paged_div(x, p.by_rep), tok = b.first + i, h = b.head * p.rep + x - i * p.rep;
     if (tok < 0 || tok >= p.tokens) return;
     const float* const from = p.partial + ((size_t)(blockIdx.x * gridDim.y + blockIdx.y) * p.splits * ROWS + r) * LD;
-    const float4 tail = lane < p.splits ? __ldcg((const float4*)(from + (size_t)lane * (ROWS * LD) + DN)) : make_float4(-INFINITY, 0.f, 0.f, 0.f);   // lane s knows part s
+    float4 v[8];                                                          // eight parts on their way, the first ones beside the references
+    auto load = [&](int d, int s0) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = d < p.dim && s0 + u < p.splits ? __ldcg((const float4*)(from + (size_t)(s0 + u) * STEP + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    const float4 tail = lane < p.splits ? __ldcg((const float4*)(from + (size_t)lane * STEP + DN)) : make_float4(-INFINITY, 0.f, 0.f, 0.f);       // lane s knows part s
+    load(4 * lane, 0);
     const float top = warp_max(tail.x);
     float w = paged_factor(tail.x, tail.y, top);
     const float sum = warp_sum(tail.y * w);
@@ -447,20 +453,17 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     if (lane == 0 && p.lse) p.lse[(size_t)tok * p.heads + h] = any ? (top + log2f(sum)) * PAGED_LN2 : -INFINITY;
 #pragma unroll
     for (int d = 4 * lane; d < (DN + 127) / 128 * 128; d += 128) {
-        const bool mine = d < p.dim;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-        for (int s0 = 0; s0 < p.splits; s0 += 8) {                        // eight loads on their way
-            float4 v[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = mine && s0 + u < p.splits ? __ldcg((const float4*)(from + (size_t)(s0 + u) * (ROWS * LD) + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s0 = 0; s0 < p.splits; s0 += 8) {
+            if (d >= 128 || s0 > 0) load(d, s0);
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                const float y = __shfl_sync(0xffffffffu, w, s0 + u);
+                const float y = __shfl_sync(0xffffffffu, w, (s0 + u) & 31);
                 o.x = fmaf(y, v[u].x, o.x); o.y = fmaf(y, v[u].y, o.y); o.z = fmaf(y, v[u].z, o.z); o.w = fmaf(y, v[u].w, o.w);
             }
         }
-        if (!mine) continue;
+        if (d >= p.dim) continue;
         if (bad) paged_add_unfinite<ROWS, UNIT, DT>(p, b, r, d, o);
         paged_put<DT>(p, (size_t)tok * p.o_ld + (size_t)h * p.dim + d, o);
     }
