@@ -43,6 +43,7 @@ int paged_few(const PagedParams& p, int dtype, cudaStream_t st);
 int paged_f32(const PagedParams& p, cudaStream_t st);
 
 constexpr int PAGED_CLUSTER = 16, PAGED_APART = 32;       // blocks that share a sequence's keys, at most: of a cluster, and one by one
+static_assert(PAGED_APART <= 32);          // a lane of the join has one
 
 // How many clusters of a kernel run at once: of eight blocks, one a SM, fewer than 148 / 8
 template <typename... KArgs>
