@@ -308,36 +308,6 @@ def test_outputs_over_queries_captured_and_repeated(dtype, rows):
             assert all(np.array_equal(u, v) for u, v in zip(s.read(x), want))
 
 
-@pytest.mark.parametrize("dtype,rows", [("bfloat16", 1), ("float16", 70), ("float32", 2)])
-def test_blocks_that_are_no_cluster_captured_side_by_side_and_over_queries(dtype, rows):
-    """two graphs of a call whose blocks leave their sums in memory, replayed at the same time; and outputs that take the queries' place"""
-    s = Step([(9000, rows), (3, min(rows, 3))], 4, 1, 128, 64, dtype, "tree" if rows > 1 else "chain", seed=23)
-    want = s.run()
-    s.check(want)
-    a = s.arrays()
-    a["out"] = a["q"]
-    s.call(a, weigh=False)
-    assert np.array_equal(s.read(a)[0], want[0])
-    sets, streams, graphs = [s.arrays() for _ in range(2)], [Stream() for _ in range(2)], []
-    for x, st in zip(sets, streams):
-        with use_stream(st):
-            s.call(x, weigh=False)
-            st.synchronize()
-            g = CudaGraph()
-            with g.capture(st):
-                for _ in range(3):
-                    s.call(x, weigh=False)
-            graphs.append(g)
-    for _ in range(4):
-        for g, st in zip(graphs, streams):
-            g.replay(st)
-    for st in streams:
-        st.synchronize()
-    for x in sets:
-        got = s.read(x)
-        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
-
-
 def test_a_fixed_cache_is_one_page():
     s = Step([(900, 5)], 8, 2, 128, 1000, "bfloat16", "tree", seed=18)
     s.check(s.run())
