@@ -307,20 +307,35 @@ template <int DT> __device__ __forceinline__ void paged_put(const PagedParams& p
     }
 }
 
-// Values among the step's rows that are not finite were taken as zero, since a weight of zero times them would reach rows that do not see them; a row that does adds them
+// The values that are not finite of the positions from `from` on that row r sees: where there are any, they are the row's element.  Among the step's rows they were taken as zero, since
+// a weight of zero times them would reach rows that do not see them; those before the step were multiplied, but an infinity times a weight's second term, or a weight that is
+// zero for being small, is a NaN.  (Element by element, since such values are rare.)
 template <int ROWS, int UNIT, int DT>
-__device__ __noinline__ void paged_add_unfinite(const PagedParams& p, const PagedBlock<ROWS, UNIT>& b, int r, int d, float4& o) {
+__device__ __noinline__ void paged_unfinite_values(const PagedParams& p, const PagedBlock<ROWS, UNIT>& b, int r, int d, int from, float4& o) {
     const int step = paged_div(b.f0 + r, p.by_rep);
-    for (int j = max(0, b.base); j < b.end; ++j) {
-        if (!paged_sees(p, b.first + step, step, j - b.base)) continue;
+    float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = max(0, from); j < b.end; ++j) {
+        if (j >= b.base && !paged_sees(p, b.first + step, step, j - b.base)) continue;
         const int row = b.row_of(p, j);
         if (row < 0) continue;
-        float* x = &o.x;
+        float* x = &u.x;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float v = paged_float<DT>(p.v_data, (size_t)row * p.dim + d + e);
             if (!(fabsf(v) < INFINITY)) x[e] += v;
         }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if ((&u.x)[e] != 0.f) (&o.x)[e] = (&u.x)[e];
+}
+// A row's outputs behind its factor 1 / sum (zero: it sees nothing).  bad: values of the step's rows were taken as zero
+template <int ROWS, int UNIT, int DT>
+__device__ __forceinline__ void paged_settle(const PagedParams& p, const PagedBlock<ROWS, UNIT>& b, int r, int d, bool bad, float factor, float4& o) {
+    if (factor == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);
+    else if (factor == factor) {                              // (a NaN among the scores is in all)
+        const bool fine = fabsf(o.x) < INFINITY && fabsf(o.y) < INFINITY && fabsf(o.z) < INFINITY && fabsf(o.w) < INFINITY;
+        if (bad || !fine) paged_unfinite_values<ROWS, UNIT, DT>(p, b, r, d, fine ? b.base : 0, o);
     }
 }
 
@@ -421,7 +436,7 @@ template <int ROWS, int UNIT, int DT, int DN> struct PagedOut {
                 o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
             }
             o.x *= t.w; o.y *= t.w; o.z *= t.w; o.w *= t.w;
-            if (where < 0) paged_add_unfinite<ROWS, UNIT, DT>(p, b, b.split + slot * p.splits, d, o);
+            paged_settle<ROWS, UNIT, DT>(p, b, b.split + slot * p.splits, d, where < 0, t.w, o);
             paged_put<DT>(p, (size_t)tok * p.o_ld + (size_t)h * p.dim + d, o);
         }
     }
@@ -450,7 +465,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     float w = paged_factor(tail.x, tail.y, top);
     const float sum = warp_sum(tail.y * w);
     const bool bad = __any_sync(0xffffffffu, tail.z != 0.f), any = sum > 0.f || sum != sum;
-    w *= any ? 1.f / sum : 0.f;
+    const float factor = any ? 1.f / sum : 0.f;
+    w *= factor;
     if (lane == 0 && p.lse) p.lse[(size_t)tok * p.heads + h] = any ? (top + log2f(sum)) * PAGED_LN2 : -INFINITY;
 #pragma unroll
     for (int d = 4 * lane; d < (DN + 127) / 128 * 128; d += 128) {
@@ -465,7 +481,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
             }
         }
         if (d >= p.dim) continue;
-        if (bad) paged_add_unfinite<ROWS, UNIT, DT>(p, b, r, d, o);
+        paged_settle<ROWS, UNIT, DT>(p, b, r, d, bad, factor, o);
         paged_put<DT>(p, (size_t)tok * p.o_ld + (size_t)h * p.dim + d, o);
     }
 }

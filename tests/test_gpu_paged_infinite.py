@@ -1,0 +1,62 @@
+"""Infinities in the keys and values of a paged cache, before the step and among its rows: attention and the weights by position against float64."""
+import numpy as np
+import pytest
+
+from tests import paged_ref as ref
+from tests.test_gpu_paged import Step
+
+pytestmark = pytest.mark.gpu
+
+
+def put(s, a, seq, j, head, elements, x):
+    """elements of position j of a sequence's key head"""
+    row = np.asarray(a[s.p.table[s.p.slots[seq], j // s.p.ps], :, j % s.p.ps]).copy()
+    row[head, elements] = ref.rounded(np.array([x]), s.dtype)[0]
+    s.p.put(a, seq, [j], [row])
+
+
+def checked(s):
+    got = s.run()
+    with np.errstate(invalid="ignore"):               # infinities that agree, subtracted
+        s.check(got)
+    return got
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("rows,D", [(1, 128), (9, 128), (40, 128), (40, 64), (3, 200), (1, 256)])
+@pytest.mark.parametrize("context", [150, 17000])
+def test_values_before_the_step(context, rows, D, dtype):
+    """an infinity is what every row of its key head has there, whatever its weight; two of unlike signs, or a NaN, are NaN; a finite value beside them stays one"""
+    s = Step([(context, rows), (99, rows)], 4, 2, D, 32, dtype, "tree" if rows > 1 else "chain", seed=21)
+    for j, e, x in ((3, 0, np.inf), (70, 5, -np.inf), (4, 9, np.inf), (60, 9, -np.inf), (31, 11, np.nan), (context - rows - 1, D - 1, -np.inf)):
+        put(s, s.p.v, 0, j, 1, e, x)
+    out = checked(s)[0]
+    assert (out[:rows, 2:, 0] == np.inf).all() and (out[:rows, 2:, [5, D - 1]] == -np.inf).all() and np.isnan(out[:rows, 2:, [9, 11]]).all()
+    assert np.isfinite(np.delete(out[:rows, 2:], [0, 5, 9, 11, D - 1], axis=2)).all() and np.isfinite(out[:rows, :2]).all() and np.isfinite(out[rows:]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("rows", [2, 9, 60])
+def test_values_before_the_step_and_among_its_rows(rows, dtype):
+    s = Step([(300, rows)], 4, 2, 128, 16, dtype, "tree", seed=22)
+    put(s, s.p.v, 0, 17, 0, 3, np.inf)
+    put(s, s.p.v, 0, 300 - rows + 1, 0, 3, -np.inf)    # the step's row 1: where it is seen both are, NaN
+    put(s, s.p.v, 0, 300 - 1, 0, 64, np.inf)
+    out = checked(s)[0]
+    sees = np.array([bool(m[1]) for m in s.masks])
+    assert np.isnan(out[sees][:, :2, 3]).all() and (out[~sees][:, :2, 3] == np.inf).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+def test_values_of_weights_that_are_zero(dtype):
+    """an infinite value whose weight is too small for 32 bits is seen all the same; where a row's scores are NaN it is NaN throughout"""
+    s = Step([(200, 2)], 4, 2, 128, 16, dtype, "chain", seed=23)
+    s.q[:] = ref.rounded(np.full(s.q.shape, 1.0), dtype)
+    for j in range(200):
+        put(s, s.p.k, 0, j, slice(None), slice(None), -12.0 if j == 30 else 12.0)      # scores -136 and 136: weights of e^-272
+    put(s, s.p.v, 0, 30, 1, 7, np.inf)
+    out = s.run()[0]
+    assert (out[:, 2:, 7] == np.inf).all() and np.isfinite(np.delete(out[:, 2:], 7, axis=2)).all() and np.isfinite(out[:, :2]).all()
+    put(s, s.p.k, 0, 31, 1, 0, np.nan)
+    out = s.run()[0]
+    assert np.isnan(out[:, 2:]).all() and np.isfinite(out[:, :2]).all()
