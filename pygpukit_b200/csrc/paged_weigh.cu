@@ -23,7 +23,7 @@ constexpr int G_WARPS = 4, G_THREADS = G_WARPS * 32, G_KEYS = G_WARPS * 32, G_RO
 using Keys = PagedBlock<H_ALL, H_KEYS>;
 static_assert(H_KEYS == G_KEYS);
 
-// minus a row's logarithm (log2); for rows that do not exist or see nothing a number that leaves no weight (a key's NaN is in the sums of the rows that see it all the same)
+// minus a row's logarithm (log2); for rows that see nothing a number that leaves no weight
 constexpr float H_NONE = -3e38f;
 __device__ __forceinline__ float row_neg(const PagedParams& p, const Keys& b, int r) {
     const int tok = b.token(p, r);
@@ -185,8 +185,10 @@ __global__ void __launch_bounds__(H_THREADS) paged_weigh_kernel(const __grid_con
                 const bool edge = j0 + 32 > clean, there = edge && missing ? b.row_of(p, j) >= 0 : j < b.end;
                 float sum = 0.f;
                 for (int g = 0; g < groups; ++g, ++turn) {
+                    const int rows = b.live - f0 - g * NR - r0;    // of this half's; where there are fewer than R, the rest's queries are zeros, which times an infinite key are NaN
+                    const bool mixed = edge || rows < R;
                     uint32_t see = 0;
-                    if (edge) {
+                    if (mixed) {
                         const int x = f0 + g * NR + r0 + (lane & (R - 1)), row = paged_div(x, p.by_rep);
                         see = x < b.live && j0 < b.end ? paged_window(p, b.first + row, row, j0 - b.base) : 0u;
                     }
@@ -198,6 +200,7 @@ __global__ void __launch_bounds__(H_THREADS) paged_weigh_kernel(const __grid_con
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sread[turn & 1]);
+                    if (rows <= 0) continue;
                     const float4* const neg = (const float4*)(negs + g * NR + r0);
                     auto add = [&](auto masked) {          // apart from each other: a branch at every weight is 1340 cycles for 64 rows
                         const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
@@ -223,7 +226,7 @@ __global__ void __launch_bounds__(H_THREADS) paged_weigh_kernel(const __grid_con
                         unpair(sum2, u, v);
                         sum = u + v;
                     };
-                    if (edge) add(std::true_type{});
+                    if (mixed) add(std::true_type{});
                     else add(std::false_type{});
                 }
                 if (half == 1) other[i & 1][key] = sum;
@@ -297,8 +300,8 @@ __global__ void __launch_bounds__(G_THREADS) paged_weigh_f32_kernel(const __grid
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float w = ex2(fmaf(s[r], p.scale_log2, negs[r0 + r]));
-                bool sees = true;
-                if (edge) {
+                bool sees = f0 + r0 + r < b.live;          // (other rows' queries are zeros: an infinite key makes NaN of them)
+                if (edge && sees) {
                     const int i = paged_div(f0 + r0 + r, p.by_rep);
                     sees = rows >= 0 && (j < b.base || paged_sees(p, b.first + i, i, j - b.base));
                 }

@@ -60,3 +60,39 @@ def test_values_of_weights_that_are_zero(dtype):
     put(s, s.p.k, 0, 31, 1, 0, np.nan)
     out = s.run()[0]
     assert np.isnan(out[:, 2:]).all() and np.isfinite(out[:, :2]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("rows,Hq", [(1, 8), (1, 32), (3, 2), (5, 14), (9, 16), (40, 6), (33, 2)])
+def test_keys_whose_scores_are_minus_infinity(rows, Hq, dtype):
+    """a key that is infinite where the queries are positive weighs nothing or all; rows that fill up a product have no part in it"""
+    s = Step([(300, rows), (70, rows)], Hq, 2, 128, 32, dtype, "tree" if rows > 1 else "chain", seed=24)
+    q = ref.floats(s.q, dtype)
+    q[..., 17] = 1.0
+    s.q = ref.rounded(q, dtype)
+    minus = (0, 5), (0, 200), (1, 1), (0, 300 - 1)
+    for seq, j in minus:
+        put(s, s.p.k, seq, j, slice(None), 17, -30000.0)
+    far = checked(s)                                   # scores that weigh nothing, either
+    for seq, j in minus:
+        put(s, s.p.k, seq, j, slice(None), 17, -np.inf)
+    out, lse, weights = got = s.run()
+    assert all(np.array_equal(x, y) for x, y in zip(got, far))
+    assert np.isfinite(out).all() and np.isfinite(lse).all() and np.isfinite(weights).all()
+    for seq, j in ((0, 5), (0, 200), (1, 1)):
+        assert np.array_equal(weights[s.p.slots[seq], :, j], s.weights[s.p.slots[seq], :, j])
+    put(s, s.p.k, 0, 9, 1, 17, np.inf)                 # a score of +infinity: the rows of its key head are NaN, and what they weigh
+    out, lse, weights = s.run()
+    assert np.isnan(out[:rows, Hq // 2:]).all() and np.isnan(lse[:rows, Hq // 2:]).all() and np.isfinite(out[:rows, :Hq // 2]).all() and np.isfinite(out[rows:]).all()
+    assert np.isnan(weights[s.p.slots[0], 1, :300 - rows]).all() and np.isfinite(weights[s.p.slots[0], 0]).all() and np.isfinite(weights[s.p.slots[1]]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+def test_a_key_that_only_the_next_sequence_would_see(dtype):
+    """three rows of one head: the fourth place's mask is the next sequence's"""
+    s = Step([(40, 3), (60, 6)], 2, 2, 128, 16, dtype, "tree", seed=25)
+    s.masks = [np.array([True, False, False]), np.array([True, True, False]), np.array([True, True, False])] + [np.ones(6, bool)] * 6
+    for x in (np.inf, np.nan):
+        put(s, s.p.k, 0, 39, slice(None), 4, x)        # the step's row 2, which none of the three sees
+        out, lse, weights = checked(s)
+        assert np.isfinite(out).all() and np.isfinite(lse).all() and np.isfinite(weights).all()
