@@ -27,6 +27,7 @@ struct PagedParams {
     const int32_t* seq_slots; const int32_t* contexts; const int32_t* starts;      // starts NULL: a row a sequence
     int seqs, tokens, max_rows, max_keys, heads, rep, tiles, splits;
     float scale_log2;                     // scale log2 e
+    float zero;                           // what a product is added to so that it is rounded: of a product and a sum alone the compiler makes one multiply-add
     const int32_t* masks;                 // [tokens][words], or NULL
     int words;
     float* lse;                           // [tokens][heads] natural logarithms, or NULL
@@ -111,6 +112,11 @@ inline cudaError_t launch_clusters(void (*kernel)(KArgs...), dim3 grid, bool apa
 #ifdef __CUDACC__
 
 constexpr float PAGED_LOG2E = 1.4426950408889634f, PAGED_LN2 = 0.6931471805599453f, PAGED_LAZY = 8.f;
+// A row's reference m from its largest score (log2).  A weight is 2^(x - m) with x, the score times the factor, rounded as m is: left exact in one multiply-add, the rounding of m would
+// be a factor of all weights of the row, 2^(2^-2) at 2^22 but 2^256 at 2^32.  (Two instructions for two scores where one would do: 8 x 64 rows over 4100 keys 49.5 -> 51.9 us, 13 rows of 16
+// sequences 25.6 -> 26.0, few rows as before; a second form of a tile behind a branch 52.4 and more.)  float16 weights go from 2^6 down, so that small ones keep their bits, and grow to 2^14; where a
+// reference has no bits for that, from 1.
+template <int DT> __device__ __forceinline__ float paged_reference(float top) { return DT == 1 && fabsf(top) < 4194304.f ? top - 6.f : top; }
 
 __device__ __forceinline__ int paged_div(int n, PagedDiv d) { return d.mul ? (int)(__umulhi((uint32_t)n, d.mul) >> d.shift) : n; }       // n not negative
 

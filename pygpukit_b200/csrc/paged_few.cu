@@ -53,7 +53,6 @@ __global__ void __launch_bounds__(W_THREADS, 1) paged_few_kernel(const __grid_co
                                                                  const __grid_constant__ PagedParams p, const __grid_constant__ FewCopies cp) {
     using X = Few<NR, C>;
     constexpr int R = X::R, SLOTS = X::SLOTS;
-    constexpr float TOP = DT == 1 ? 6.f : 0.f;                     // float16 weights: from 2^6 down, so that small ones keep their bits; they grow to 2^14
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS], land, sfull[2], pready[2], pvdone[2];        // a barrier each: of two tiles both may have come before the first is looked for
     __shared__ uint32_t tmem_base_s;
@@ -267,7 +266,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) paged_few_kernel(const __grid_co
             __syncwarp();
             asm volatile("bar.sync %0, 128;" :: "r"(1 + half) : "memory");
             const float4 w = *(const float4*)wmax[i & 1][mine];
-            const float mt = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)) * p.scale_log2 - TOP;
+            const float mt = paged_reference<DT>(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)) * p.scale_log2);
             const bool up = mt > m_r + PAGED_LAZY;                // (also the first finite maximum)
             bool waited = false;
             if (__any_sync(0xffffffffu, up)) {                    // the same in the half's four warps: its columns of O^T move along
@@ -298,10 +297,14 @@ __global__ void __launch_bounds__(W_THREADS, 1) paged_few_kernel(const __grid_co
                     tmem_st_wait();
                 }
             }
+            const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), zero2 = pair(p.zero, p.zero);
             uint32_t hi[R / 2], lo[R / 2];
 #pragma unroll
             for (int e = 0; e < R / 2; ++e) {
-                const float a = ex2(fmaf(s[2 * e], p.scale_log2, nm[2 * e])), c = ex2(fmaf(s[2 * e + 1], p.scale_log2, nm[2 * e + 1]));
+                float a, c;
+                unpair(add2(fma2(pair(s[2 * e], s[2 * e + 1]), scale2, zero2), pair(nm[2 * e], nm[2 * e + 1])), a, c);
+                a = ex2(a);
+                c = ex2(c);
                 l[2 * e] += a;
                 l[2 * e + 1] += c;
                 paged_weights2x2<DT>(a, c, hi[e], lo[e]);

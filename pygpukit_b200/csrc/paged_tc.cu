@@ -44,13 +44,13 @@ template <int C> struct Tile {
 
 // 32 weights 2^(s scale + neg) to TMEM column `to`; their sum is of the unrounded ones
 template <int DT>
-__device__ __forceinline__ void weights32(const float* s, float scale, float neg, uint32_t to, uint64_t& l) {
+__device__ __forceinline__ void weights32(const float* s, float scale, float zero, float neg, uint32_t to, uint64_t& l) {
     uint32_t y[16];
-    const uint64_t scale2 = pair(scale, scale), neg2 = pair(neg, neg);
+    const uint64_t scale2 = pair(scale, scale), zero2 = pair(zero, zero), neg2 = pair(neg, neg);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         float a, b;
-        unpair(fma2(pair(s[2 * e], s[2 * e + 1]), scale2, neg2), a, b);
+        unpair(add2(fma2(pair(s[2 * e], s[2 * e + 1]), scale2, zero2), neg2), a, b);
         a = ex2(a);
         b = ex2(b);
         l = add2(l, pair(a, b));
@@ -64,7 +64,6 @@ template <int C, int DT>
 __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                                                                 const __grid_constant__ PagedParams p, const __grid_constant__ Copies cp) {
     using X = Tile<C>;
-    constexpr float TOP = DT == 1 ? 6.f : 0.f;                     // as in paged_few.cu
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(8) uint64_t full[T_SLOTS], empty[T_SLOTS], land, sfull[2], pready[2], pvdone[2];
     __shared__ uint32_t tmem_base_s;
@@ -285,7 +284,7 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
 #pragma unroll
                 for (int e = 0; e < 64; ++e) t[e & 3] = fmaxf(t[e & 3], s[e]);
             }
-            const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * p.scale_log2 - TOP;
+            const float top = paged_reference<DT>(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * p.scale_log2);
             // the reference passes from the other side's warp, which has the tile before, and on to it
             float was = -INFINITY;
             if (i > 0) {
@@ -317,11 +316,11 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
             }
             const float neg = paged_neg(now);
             uint64_t l2 = pair(0.f, 0.f);
-            weights32<DT>(s, p.scale_log2, neg, at + 64u, l2);            // each half to where its scores were
-            weights32<DT>(s + 32, p.scale_log2, neg, at + 80u, l2);
+            weights32<DT>(s, p.scale_log2, p.zero, neg, at + 64u, l2);    // each half to where its scores were
+            weights32<DT>(s + 32, p.scale_log2, p.zero, neg, at + 80u, l2);
             load(0);
-            weights32<DT>(s, p.scale_log2, neg, at, l2);
-            weights32<DT>(s + 32, p.scale_log2, neg, at + 16u, l2);
+            weights32<DT>(s, p.scale_log2, p.zero, neg, at, l2);
+            weights32<DT>(s + 32, p.scale_log2, p.zero, neg, at + 16u, l2);
             float la, lb;
             unpair(l2, la, lb);
             l += la + lb;

@@ -96,3 +96,31 @@ def test_a_key_that_only_the_next_sequence_would_see(dtype):
         put(s, s.p.k, 0, 39, slice(None), 4, x)        # the step's row 2, which none of the three sees
         out, lse, weights = checked(s)
         assert np.isfinite(out).all() and np.isfinite(lse).all() and np.isfinite(weights).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("rows,D,context", [(1, 128, 300), (9, 128, 300), (40, 128, 300), (40, 64, 300), (3, 200, 300), (1, 128, 9000), (40, 128, 9000)])
+@pytest.mark.parametrize("most,sign", [(2.0 ** 21, 1), (2.0 ** 24, 1), (2.0 ** 25, -1), (2.0 ** 27, 1), (2.0 ** 30, -1), (2.0 ** 33, 1)])
+def test_scores_of_any_size(most, sign, rows, D, context, dtype):
+    """scores of c (1 - j / 64), j = 0 ... 31 in turns, of one product each, up to `most` or down from its negative: the difference of neighbours is far above a score's
+    rounding, so that the keys of the largest score share the weight"""
+    s = Step([(context, rows)], 4, 2, D, 32, dtype, "tree" if rows > 1 else "chain", seed=26)
+    rng = np.random.default_rng(7)
+    turn = rng.integers(0, 32, context)
+    turn[:8] = np.arange(8)                            # the largest, and what comes next, before the step
+    q, k = np.zeros(s.q.shape), np.zeros((context, 2, D))
+    scale = 2.0 ** -4                                  # most = scale q k
+    a = 2.0 ** np.ceil(np.log2(most / scale) / 2)
+    q[..., 3], k[..., 3] = a, sign * (most / scale / a) * (1 - sign * turn[:, None] / 64)
+    if max(a, np.abs(k).max()) > 60000 and dtype == "float16":
+        pytest.skip("no such float16 numbers")
+    s.q = ref.rounded(q, dtype)
+    s.p.put(s.p.k, 0, range(context), ref.rounded(k, dtype))
+    out, lse, weights = s.run(scale=scale)
+    want, want_lse, _, _, by = ref.attention(s.p, ref.floats(s.q, dtype), s.starts, s.masks, scale)
+    v = s.p.rows(s.p.v, 0, context)
+    # weights of 1 / n: each is one rounding off its type, sums are exact but for float32's; the output's rounding
+    spread = np.abs(v).max(axis=0)[np.arange(4) // 2][None]
+    e = ref.EPS[dtype]
+    assert np.isfinite(out).all() and (np.abs(out - want) <= (e + 2.0 ** -14) * spread).all()
+    assert (np.abs(lse - want_lse) <= 2.0 ** -22 * np.abs(want_lse)).all()
