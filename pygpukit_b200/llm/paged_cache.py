@@ -151,19 +151,43 @@ class PagePool:
 
     def own_pages(self, seq_id, start: int) -> list:
         """Pages of its own in the place of those from position `start` on that others hold too: (that one, the new one) each, to be copied."""
-        slot, pages, length, _ = self._seq[seq_id]
+        length = self._seq[seq_id][2]
         if not 0 <= start <= length:
             raise ValueError(f"own_pages: position {start} outside 0..{length}")
-        pairs = []
-        for i in range(start // self.page_size, len(pages)):
-            if pages[i] in self._shared:
-                old, new = pages[i], self._new_page()
-                self._drop(old)
-                pages[i] = new
-                self.table[slot, i] = new
-                self.dirty = True
-                pairs.append((old, new))
+        plan = self.plan_pages([(seq_id, start, length)])
+        pairs = self.pairs_of(plan)
+        self.take_pages(plan)
         return pairs
+
+    def plan_pages(self, ranges: list) -> list:
+        """Pages of their own for the (id, start, end) of `ranges`, the first sequence first, in the place of those of the positions start ... end - 1 that others hold
+        too: (id, number of the page in the sequence, new page) each, for `take_pages`.  No sequence changes; there are enough free pages then."""
+        held, plan = dict(self._shared), []
+        for seq_id, start, end in ranges:
+            pages = self._seq[seq_id][1]
+            for i in range(start // self.page_size, -(-end // self.page_size)):
+                n = held.get(pages[i], 1)
+                if n > 1:                              # the last of those that hold it keeps it
+                    held[pages[i]] = n - 1
+                    plan.append((seq_id, i))
+        if len(plan) > len(self._free_pages):
+            self._grow_pages(len(plan) - len(self._free_pages))
+        return [(*at, new) for at, new in zip(plan, heapq.nsmallest(len(plan), self._free_pages))]
+
+    def pairs_of(self, plan: list) -> list:
+        """(page, new page) of a plan, to be copied before it is taken"""
+        return [(self._seq[seq_id][1][i], new) for seq_id, i, new in plan]
+
+    def take_pages(self, plan: list) -> None:
+        """What `plan_pages` has planned, with nothing in between."""
+        for seq_id, i, new in plan:
+            slot, pages, _, _ = self._seq[seq_id]
+            if heapq.heappop(self._free_pages) != new:
+                raise RuntimeError("take_pages: pages were taken since they were planned")
+            self._drop(pages[i])
+            pages[i] = new
+            self.table[slot, i] = new
+            self.dirty = True
 
     def release(self, seq_id) -> None:
         slot, pages, _, _ = self._seq.pop(seq_id)
@@ -397,8 +421,9 @@ class PagedKVCache:
     def keep_rows(self, keeps: dict) -> None:
         """Cut sequences to some of their positions: {id: (start, rows)} leaves the positions before `start`, and behind them those at start + rows[0],
         start + rows[1], ... (ascending numbers), in every layer; the sequence ends there.  Accepted drafts of a tree, say, or what is left when
-        positions are evicted.  Rows move in the order of the current stream (`ops.move_rows_paged`); keys stay turned by the positions that they had.  Pages that others
-        hold too are copied first."""
+        positions are evicted, the same ones of all key heads.  Rows move in the order of the current stream (`ops.move_rows_paged`).  Pages that rows move into and that others
+        hold too are copied first; a call that fails for want of memory leaves every sequence as it was.  Keys stay turned by the positions that they had, while what is appended later is
+        numbered from the sequence's new length on: a program that evicts turned keys numbers its queries itself."""
         if self.int4 or self.has_state or any(self.pools):
             raise ValueError("PagedKVCache: rows of four-bit pages, pooled rows and recurrent states do not move")
         # everything is looked at before anything changes
@@ -408,9 +433,11 @@ class PagedKVCache:
                 raise ValueError(f"keep_rows: rows {list(rows)!r} behind position {start} of a sequence of {length} (ascending)")
         moving = [(seq, start, rows) for seq, (start, rows) in keeps.items() if any(r != i for i, r in enumerate(rows))]
         if moving:
-            pairs = [p for seq, start, _ in moving for p in self.pool.own_pages(seq, start)]
+            # pages that a row moves into: from the first row that is another one to the last
+            plan = self.pool.plan_pages([(seq, start + next(i for i, r in enumerate(rows) if r != i), start + len(rows)) for seq, start, rows in moving])
             self._grown()
-            self._copy(self._page_arrays(), pairs)
+            self._copy(self._page_arrays(), self.pool.pairs_of(plan))
+            self.pool.take_pages(plan)
             table, arrays = self.page_table(), self._page_arrays()
             S, width = len(moving), max(len(rows) for _, _, rows in moving)
             host = np.full(S * (3 + width), -1, np.int32)
