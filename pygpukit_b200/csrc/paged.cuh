@@ -5,6 +5,8 @@
 // before context - n and, of the step's, those whose bit is set in its mask, or without masks the rows 0 ... i.  Slots, contexts, row starts and page numbers are
 // data of the device: whatever they say, nothing outside the arrays is touched.
 #pragma once
+#include <mutex>
+
 #include "tc_common.cuh"
 
 namespace pgk {
@@ -46,7 +48,7 @@ int paged_f32(const PagedParams& p, cudaStream_t st);
 constexpr int PAGED_CLUSTER = 16, PAGED_APART = 32;       // blocks that share a sequence's keys, at most: of a cluster, and one by one
 static_assert(PAGED_APART <= 32);          // a lane of the join has one
 
-// How many clusters of a kernel run at once: of eight blocks, one a SM, fewer than 148 / 8
+// How many clusters of a kernel run at once: of eight blocks, one a SM, fewer than 148 / 8; 0: none of that size runs
 template <typename... KArgs>
 inline cudaError_t clusters_at_once(int* out, void (*kernel)(KArgs...), int threads, size_t smem, int blocks) {
     cudaLaunchConfig_t cfg = {};
@@ -59,12 +61,26 @@ inline cudaError_t clusters_at_once(int* out, void (*kernel)(KArgs...), int thre
     cfg.dynamicSmemBytes = smem;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    *out = 1;
-    int n = 0;
-    if (cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg)) return e;
-    if (n > 0) *out = n;
+    *out = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(out, kernel, &cfg);
+    if (e == cudaSuccess || blocks == 1) return e;
+    cudaGetLastError();
+    *out = 0;
     return cudaSuccess;
 }
+// What a launcher has asked once, by the first thread that comes: a call's split, and with it its bits, is the same in all
+struct PagedOccupancy {
+    std::mutex mutex;
+    bool asked = false;
+    int at_once[PAGED_CLUSTER + 1] = {};
+    template <typename F> cudaError_t once(F ask) {
+        std::lock_guard<std::mutex> lock(mutex);
+        if (asked) return cudaSuccess;
+        const cudaError_t e = ask(at_once);
+        asked = e == cudaSuccess;
+        return e;
+    }
+};
 // Blocks that share a sequence's tiles.  As a cluster, which folds through shared memory: rounds of clusters times (a block's tiles + what it costs besides, in tiles).  Or one by
 // one, which leave their sums in memory for another launch (half as much again): where clusters do not fill the SMs.  One sequence of 8 key heads, us: 1 row over 4096 keys, clusters
 // of 10 11.5 and 18 blocks apart 11.6; over 8000 15.2 and 13.6, over 32000 37 and 32; 208 rows over 32000 in two tiles, clusters of 6 54 and 9 blocks apart 45.
@@ -76,7 +92,9 @@ inline PagedSplit paged_split(const PagedParams& p, int keys, const int* at_once
     long long least = 0;
     PagedSplit best = {1, false};
     for (int s = 1; s <= most; ++s) {
-        long long rounds = (8 * items + at_once[s] - 1) / at_once[s];                      // in eighths, whole ones up to two: then blocks no longer end together
+        if (s > 1 && at_once[s] <= 0) continue;                                            // none of that size runs: its launch would fail
+        const int fit = at_once[s] > 0 ? at_once[s] : 1;
+        long long rounds = (8 * items + fit - 1) / fit;                                    // in eighths, whole ones up to two: then blocks no longer end together
         if (rounds <= 16) rounds = (rounds + 7) & ~7ll;
         const long long cost = rounds * ((nt + s - 1) / s + ends);
         if (s == 1 || cost < least) { best = {s, false}; least = cost; }

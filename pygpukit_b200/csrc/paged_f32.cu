@@ -299,22 +299,20 @@ __global__ void __launch_bounds__(W * 32, 1) paged_f32_kernel(const __grid_const
 
 template <int R, int E, int W>
 int launch_single(PagedParams p, cudaStream_t st) {
-    static bool configured = false;
-    if (!configured) {
-        PGK_CUDA(cudaFuncSetAttribute(paged_f32_kernel<R, E, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, Single<R, E, W>::bytes(64 * E)));
-        PGK_CUDA(cudaFuncSetAttribute(paged_f32_kernel<R, E, W>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        configured = true;
-    }
     const int smem = Single<R, E, W>::bytes(p.dim), kind = smem > 113 * 1024 ? 0 : (smem > 75 * 1024 ? 1 : 2);       // one, two, three blocks a SM
-    static int at_once[3][PAGED_CLUSTER + 1] = {};
-    if (at_once[kind][1] == 0)
-        for (int i = PAGED_CLUSTER; i >= 1; --i) {            // (the first one last: then all are there)
-            int n;
-            PGK_CUDA(clusters_at_once(&n, paged_f32_kernel<R, E, W>, W * 32, (size_t)smem, i));
-            at_once[kind][i] = kind ? n + n / 16 : n;         // a few more than fit run beside the others' second half: 96 of three blocks, 93 fit, 35 us, of two blocks 45
+    static PagedOccupancy fits[3];
+    PGK_CUDA(fits[kind].once([&](int* at_once) {
+        const auto kernel = paged_f32_kernel<R, E, W>;
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Single<R, E, W>::bytes(64 * E));
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        for (int i = 1; e == cudaSuccess && i <= PAGED_CLUSTER; ++i) {
+            e = clusters_at_once(&at_once[i], kernel, W * 32, (size_t)smem, i);
+            if (kind) at_once[i] += at_once[i] / 16;          // a few more than fit run beside the others' second half: 96 of three blocks, 93 fit, 35 us, of two blocks 45
         }
+        return e;
+    }));
     p.tiles = (int)(((long long)p.max_rows * p.rep + R - 1) / R);
-    return paged_launch<R, S_KEYS, 0, 64 * E>(p, paged_split(p, S_KEYS * W, at_once[kind], PAGED_CLUSTER, 2), st, [&](const PagedParams& q, dim3 grid, bool apart) {
+    return paged_launch<R, S_KEYS, 0, 64 * E>(p, paged_split(p, S_KEYS * W, fits[kind].at_once, PAGED_CLUSTER, 2), st, [&](const PagedParams& q, dim3 grid, bool apart) {
         return launch_clusters(paged_f32_kernel<R, E, W>, grid, apart, W * 32, (size_t)smem, st, q);
     });
 }

@@ -377,15 +377,14 @@ __global__ void __launch_bounds__(W_THREADS, 1) paged_few_kernel(const __grid_co
 template <int NR, int C, int DT>
 int launch_few(PagedParams p, cudaStream_t st) {
     using X = Few<NR, C>;
-    static bool configured = false;
-    static int at_once[PAGED_CLUSTER + 1] = {};
+    static PagedOccupancy fits;
     const auto kernel = paged_few_kernel<NR, C, DT>;
-    if (!configured) {
-        PGK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, X::BYTES));
-        PGK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        for (int i = 1; i <= PAGED_CLUSTER; ++i) PGK_CUDA(clusters_at_once(&at_once[i], kernel, W_THREADS, X::BYTES, i));
-        configured = true;
-    }
+    PGK_CUDA(fits.once([&](int* at_once) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, X::BYTES);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        for (int i = 1; e == cudaSuccess && i <= PAGED_CLUSTER; ++i) e = clusters_at_once(&at_once[i], kernel, W_THREADS, X::BYTES, i);
+        return e;
+    }));
     FewCopies cp = {};
     cp.bp = p.page_size & -p.page_size;
     if (cp.bp > W_KEYS) cp.bp = W_KEYS;
@@ -399,7 +398,7 @@ int launch_few(PagedParams p, cudaStream_t st) {
                     tma_map_bf16_2d(&vmap, p.v_data, (uint64_t)p.dim, (uint64_t)cp.rows, (uint64_t)p.dim * 2, 64, box),
                 "paged_attention failed: no tensor map of %d rows of %d elements", cp.rows, p.dim);
     p.tiles = (int)(((long long)p.max_rows * p.rep + NR - 1) / NR);
-    return paged_launch<NR, W_KEYS, DT, X::DN>(p, paged_split(p, W_KEYS, at_once, PAGED_CLUSTER, 4), st, [&](const PagedParams& q, dim3 grid, bool apart) {
+    return paged_launch<NR, W_KEYS, DT, X::DN>(p, paged_split(p, W_KEYS, fits.at_once, PAGED_CLUSTER, 4), st, [&](const PagedParams& q, dim3 grid, bool apart) {
         return launch_clusters(kernel, grid, apart, W_THREADS, (size_t)X::BYTES, st, kmap, vmap, q, cp);
     });
 }

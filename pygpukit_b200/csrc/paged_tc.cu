@@ -365,15 +365,14 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
 template <int C, int DT>
 int launch_tiles(PagedParams p, cudaStream_t st) {
     using X = Tile<C>;
-    static bool configured = false;
-    static int at_once[PAGED_CLUSTER + 1] = {};
+    static PagedOccupancy fits;
     const auto kernel = paged_tc_kernel<C, DT>;
-    if (!configured) {
-        PGK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM));
-        PGK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        for (int i = 1; i <= PAGED_CLUSTER; ++i) PGK_CUDA(clusters_at_once(&at_once[i], kernel, T_THREADS, X::SMEM, i));
-        configured = true;
-    }
+    PGK_CUDA(fits.once([&](int* at_once) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        for (int i = 1; e == cudaSuccess && i <= PAGED_CLUSTER; ++i) e = clusters_at_once(&at_once[i], kernel, T_THREADS, X::SMEM, i);
+        return e;
+    }));
     Copies cp = {};
     cp.bp = p.page_size & -p.page_size;
     if (cp.bp > T_KEYS) cp.bp = T_KEYS;
@@ -385,7 +384,7 @@ int launch_tiles(PagedParams p, cudaStream_t st) {
                     tma_map_bf16_2d(&vmap, p.v_data, (uint64_t)p.dim, (uint64_t)cp.rows, (uint64_t)p.dim * 2, 64, (uint32_t)cp.bp),
                 "paged_attention failed: no tensor map of %d rows of %d elements", cp.rows, p.dim);
     p.tiles = (int)(((long long)p.max_rows * p.rep + T_ROWS - 1) / T_ROWS);
-    return paged_launch<T_ROWS, T_KEYS, DT, X::DN>(p, paged_split(p, T_KEYS, at_once, PAGED_CLUSTER, 4), st, [&](const PagedParams& q, dim3 grid, bool apart) {
+    return paged_launch<T_ROWS, T_KEYS, DT, X::DN>(p, paged_split(p, T_KEYS, fits.at_once, PAGED_CLUSTER, 4), st, [&](const PagedParams& q, dim3 grid, bool apart) {
         return launch_clusters(kernel, grid, apart, T_THREADS, (size_t)X::SMEM, st, kmap, vmap, q, cp);
     });
 }
