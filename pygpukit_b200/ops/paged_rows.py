@@ -82,9 +82,11 @@ def sdpa_paged(Q: GPUArray, k_cache: GPUArray, v_cache: GPUArray, out: GPUArray,
     """Attention of many sequences' steps over the cache: decoded tokens, trees of drafted tokens (masks), portions of prompts.  Q, out [tokens, heads, dim].
 
     scale 0: 1 / sqrt(dim).  lse float32 [tokens, heads]: the natural logarithm of the sum of the scores' exponentials, -infinity for a row that sees nothing,
-    whose outputs are zeros.  out may be Q.  Scores, maxima and sums are float32; rows of 16 bits weigh the values by weights rounded to their type.
-    Heads of 64 to 128 elements on pages of a multiple of 8 positions run on the tensor cores' large tiles from 17 rows a sequence and key head on (a token's heads of
-    one key head are rows), 16-bit types; the longest step of a call decides for all of it."""
+    whose outputs are zeros.  out may be Q.  Scores, maxima and sums are float32.  An infinite value is the output of the rows that see it, whatever its weight.
+
+    16-bit types: from 33 rows a sequence and key head on (a token's heads of one key head are rows; the longest step of a call decides for all of it), heads of 64 to 128 elements on
+    pages of a multiple of 8 positions take tiles whose weights are rounded once, to the cache's type (half a unit of it: in the end 1.4 times the error of the output's own rounding).  Up to 32 rows, and
+    for other heads and pages, a weight is two terms of the type, and what is left is the output's rounding."""
     name = "sdpa_paged"
     code, T, Hq, args = _step(name, Q, k_cache, page_table, slots, context_lens, max_context, scale, row_starts, max_rows, masks)
     if v_cache._shape != k_cache._shape or not _is(v_cache, k_cache._dtype):
@@ -101,7 +103,8 @@ def weigh_paged(Q: GPUArray, k_cache: GPUArray, lse: GPUArray, weights: GPUArray
                 max_context: int, scale: float = 0.0, *, row_starts: "GPUArray | None" = None, max_rows: int = 1, masks: "GPUArray | None" = None) -> None:
     """Add the attention weights of a step to what the positions have: weights float32 [slots, kv_heads, positions] gains, at the sequence's slot, the sum over its
     rows and the query heads of the key head of exp(scale q . k - lse).  lse float32 [tokens, heads] is what `sdpa_paged` leaves with the same arguments
-    (rows at -infinity have no weights).  The same call gives the same bits unless two of its sequences have one slot."""
+    (rows at -infinity have no weights; lse is float32, and weights are off by a factor of e^(|lse| 2^-24) for its rounding: 6 % where scores are a million).  The same
+    call gives the same bits unless two of its sequences have one slot."""
     name = "weigh_paged"
     code, T, Hq, args = _step(name, Q, k_cache, page_table, slots, context_lens, max_context, scale, row_starts, max_rows, masks)
     if lse._shape != (T, Hq) or not _is(lse, float32):
