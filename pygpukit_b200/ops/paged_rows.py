@@ -24,6 +24,9 @@ from ._common import _st
 from .paged import _index, _is
 
 
+MOST_POSITIONS = 1 << 30          # of a slot's weights or of a list of rows: the kernels count in 32 bits
+
+
 def _pages(name: str, cache: GPUArray, page_table: GPUArray) -> tuple[int, int, int, int, int, int]:
     """(pages, kv_heads, page size, dim, slots, pages of a slot)"""
     if len(cache._shape) != 4:
@@ -34,6 +37,8 @@ def _pages(name: str, cache: GPUArray, page_table: GPUArray) -> tuple[int, int, 
     slots, max_pages = page_table._shape
     if min(pages, H, ps, D, slots, max_pages) < 1:
         raise ValueError(f"{name}: a cache without rows, {cache.shape}, or slots, {page_table.shape}")
+    if max(pages * H * ps, max_pages * ps, slots) >= 2 ** 31:
+        raise ValueError(f"{name}: a cache {cache.shape} behind {page_table.shape} pages (2^31 - 1 rows, and positions of a slot, at most)")
     return pages, H, ps, D, slots, max_pages
 
 
@@ -45,6 +50,8 @@ def _step(name: str, Q: GPUArray, k_cache: GPUArray, page_table: GPUArray, slots
         raise ValueError(f"{name} expects Q [tokens, heads, dim], got {Q.shape}")
     T, Hq, D = Q._shape
     pages, H, ps, dim, n_slots, max_pages = _pages(name, k_cache, page_table)
+    if T >= 2 ** 31:
+        raise ValueError(f"{name}: {T} rows")
     if dim != D or not _is(k_cache, Q._dtype):
         raise ValueError(f"{name}: a cache of {k_cache.dtype} {k_cache.shape} for queries of {Q.dtype} {Q.shape}")
     if D % 8 or D > 256:
@@ -124,6 +131,8 @@ def select_rows(weights: GPUArray, slots: GPUArray, context_lens: GPUArray, budg
     if len(weights._shape) != 3 or not _is(weights, float32) or min(weights._shape) < 1:
         raise ValueError(f"{name}: weights must be float32 [slots, kv_heads, positions], got {weights.dtype} {weights.shape}")
     n_slots, H, P = weights._shape
+    if P > MOST_POSITIONS or n_slots >= 2 ** 31:
+        raise ValueError(f"{name}: weights {weights.shape} ({MOST_POSITIONS} positions at most)")
     if len(slots._shape) != 1:
         raise ValueError(f"{name}: slots must be int32 [sequences], got {slots.dtype} {slots.shape}")
     S = slots._shape[0]
@@ -180,6 +189,8 @@ def move_rows_paged(arrays: "list[GPUArray]", page_table: GPUArray, slots: GPUAr
     by_head = len(rows._shape) == 3
     if not _is(rows, int32) or rows._shape[:-1] != ((S, H) if by_head else (S,)):
         raise ValueError(f"{name}: rows must be int32 [{S}, n] or [{S}, {H}, n], got {rows.dtype} {rows.shape}")
+    if rows._shape[-1] > MOST_POSITIONS:
+        raise ValueError(f"{name}: {rows._shape[-1]} rows of a sequence ({MOST_POSITIONS} at most)")
     if starts is not None:
         _index(name, "starts", starts, S)
     ld = 0

@@ -10,6 +10,7 @@ from ._common import _st
 from .paged import _index, _is
 
 MAX_TREE_ROWS = 4096
+MAX_MASK_WORDS = 1 << 18
 
 
 def _trees(name: str, parents: GPUArray, row_starts: GPUArray, max_rows: int) -> tuple[int, int]:
@@ -20,6 +21,8 @@ def _trees(name: str, parents: GPUArray, row_starts: GPUArray, max_rows: int) ->
         raise ValueError(f"{name}: row_starts must be int32 [sequences + 1], got {row_starts.dtype} {row_starts.shape}")
     if not 1 <= max_rows <= MAX_TREE_ROWS:
         raise ValueError(f"{name}: max_rows {max_rows} (1 ... {MAX_TREE_ROWS})")
+    if parents._shape[0] >= 2 ** 31:
+        raise ValueError(f"{name}: {parents._shape[0]} rows")
     return parents._shape[0], row_starts._shape[0] - 1
 
 
@@ -35,6 +38,8 @@ def tree_masks(parents: GPUArray, row_starts: GPUArray, max_rows: int, *, masks:
         masks = GPUArray((T, words), int32)
     elif len(masks._shape) != 2 or masks._shape[0] != T or masks._shape[1] < words or not _is(masks, int32):
         raise ValueError(f"{name}: masks must be int32 [{T}, {words} words], got {masks.dtype} {masks.shape}")
+    elif masks._shape[1] > MAX_MASK_WORDS:
+        raise ValueError(f"{name}: masks of {masks._shape[1]} words ({MAX_MASK_WORDS} at most)")
     if depths is None:
         depths = GPUArray((T,), int32)
     else:
@@ -61,6 +66,8 @@ def accept_tree(logits: GPUArray, tokens: GPUArray, parents: GPUArray, row_start
         if len(logits._shape) != 2 or logits._shape[0] != T or logits._shape[1] < 1:
             raise ValueError(f"{name}: logits must be [{T}, vocab], got {logits.shape}")
         V = logits._shape[1]
+        if V > 1 << 30:
+            raise ValueError(f"{name}: a vocabulary of {V} (2^30 at most)")
     if T > 65535:
         raise ValueError(f"{name}: {T} rows (65535 at most)")
     if out is None:
