@@ -5,13 +5,13 @@
 //   * one thread issues S = Q K^T, queries in tensor memory, and O += P V.  Products run in the order in which they were issued, so that the scores of tile i + 2 may
 //     follow the product that reads the weights of tile i in their place;
 //   * four warps, a lane a row, have the even tiles, four the odd ones: the maxima of one are looked for while the other's weights are formed.  A row's reference, which
-//     both share, moves when its maximum has grown by 2^8; it passes from tile to tile before the weights are formed.  A weight is rounded to the cache's type once
-//     (two terms would be half as many products again).
+//     both share, moves when its maximum has grown by 2^8; it passes from tile to tile before the weights are formed.  A weight is rounded to the cache's type once:
+//     outputs are off by 1.4 times what their own rounding makes.  (Two terms, half as many products again, leave only that: 8 x 64 rows over 4100 keys 49.6 -> 61 us.)
 //   * only tiles that hold the step's rows, or the context's end, look at masks.  What lies behind the end is zeroed in V by the copying warp, and values of the step's
 //     rows that are not finite are taken as zero there (a weight of zero times them would reach rows that do not see them) and added in the end.
 // Bound by the copies: a SM takes in about 32 bytes a clock, 64 KB of a tile a microsecond, whatever the others do; its products and exponentials need half of that.  (256 rows
 // a block, two sets of rows over the same tiles, halves the copies, but has room for one tile of scores a set: 3500 cycles for what are 2 x 2000 here, and a longer way in and
-// out: 8 x 64 rows over 4100 keys 54 us where this takes 47.)
+// out: 8 x 64 rows over 4100 keys 54 us where this took 47; it is 49.6 since scores of any size have weights, see paged_reference.)
 // Blocks of a cluster share a sequence's keys.
 #include "paged.cuh"
 #include "tc_common.cuh"
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(T_THREADS, 1) paged_tc_kernel(const __grid_con
         fence_proxy_async();                       // the place goes back to the copies
         tc_fence_before();
     }
-    // The copying warp comes when all other places are on their way.  (That the rest waits for it, instead of it alone for the queries, takes 46.5 us where 50 went by: 512 rows of
+    // The copying warp comes when all other places are on their way.  (That the rest waits for it, instead of it alone for the queries, took 46.5 us where 50 went by: 512 rows of
     // eight sequences over 4100 keys.)
     auto queries_there = [] {
         __syncwarp();
