@@ -876,7 +876,7 @@ int pgk_copy_rows(void* const* host_arrays, const int64_t* host_row_bytes, int n
  * page_table int32 [slots][max_pages]; dim a multiple of 8 up to 256, pages of any size.  Sequence s has rows row_starts[s] ... row_starts[s + 1] - 1 of q (row s
  * without row_starts), the last n of its context_lens[s] positions: step row t lies at position context - n + t.  Row i sees every position before
  * context - n and the step rows whose bits its mask has: masks int32 [tokens][mask_words], bit t % 32 of word t / 32; NULL: the rows 0 ... i.
- * max_rows and max_context bound the data.  Slots, positions and page numbers are data of the device: what they place outside the arrays is skipped.
+ * max_rows and max_context bound the data (select_rows: max_context, move_rows: width, accept_tree: vocab up to 2^31 - 2^16).  Slots, positions and page numbers are data of the device: what they place outside the arrays is skipped.
  *   attention: out[t][h] = softmax(scale q . k) v, zeros for rows that see nothing; lse (or NULL) float32 [tokens][heads], the natural logarithm of the
  *           scores' exponentials' sum, -infinity for such rows.  scale 0: 1 / sqrt(dim).  out may be q.
  *   weigh:  weights[slot][g][j] += sum over the sequence's rows and the heads h of g of exp(scale q . k_j - lse), weights float32 [slots][kv_heads][weights_ld].

@@ -45,6 +45,7 @@ int paged_tc(const PagedParams& p, int dtype, cudaStream_t st);
 int paged_few(const PagedParams& p, int dtype, cudaStream_t st);
 int paged_f32(const PagedParams& p, cudaStream_t st);
 
+constexpr int PAGED_MOST = 0x7fff0000;       // of what a kernel counts in steps of up to 2^15: the count behind the last stays in 32 bits
 constexpr int PAGED_CLUSTER = 16, PAGED_APART = 32;       // blocks that share a sequence's keys, at most: of a cluster, and one by one
 static_assert(PAGED_APART <= 32);          // a lane of the join has one
 

@@ -271,7 +271,7 @@ using namespace pgk;
 
 extern "C" int pgk_select_rows(const float* weights, long weights_ld, const int32_t* seq_slots, const int32_t* context_lens, int seqs, int slots, int kv_heads, int max_context,
                                int budget, int first, int recent, int32_t* kept, int32_t* counts, void* stream) {
-    PGK_REQUIRE(seqs >= 0 && seqs <= 65535 && slots > 0 && kv_heads > 0 && max_context >= 0 && max_context <= 1 << 30 && weights_ld >= max_context, "select_rows failed: %d sequences, %d slots of %d heads, %d of %ld positions",
+    PGK_REQUIRE(seqs >= 0 && seqs <= 65535 && slots > 0 && kv_heads > 0 && max_context >= 0 && max_context <= PAGED_MOST && weights_ld >= max_context, "select_rows failed: %d sequences, %d slots of %d heads, %d of %ld positions",
                 seqs, slots, kv_heads, max_context, weights_ld);
     PGK_REQUIRE(budget > 0 && first >= 0 && recent >= 0 && (long long)first + recent <= budget, "select_rows failed: a budget of %d with %d first and %d recent positions", budget, first, recent);
     if (seqs == 0) return 0;
@@ -286,7 +286,7 @@ extern "C" int pgk_select_rows(const float* weights, long weights_ld, const int3
 extern "C" int pgk_move_rows(void* const* host_arrays, const int32_t* host_row_bytes, int n_arrays, const int32_t* page_table, int pages, int page_size, int slots, int max_pages,
                              int kv_heads, const int32_t* seq_slots, const int32_t* starts, const int32_t* from, const int32_t* counts, int seqs, int width, int by_head, float* weights,
                              long weights_ld, const int32_t* context_lens, void* stream) {
-    PGK_REQUIRE(n_arrays >= 0 && pages > 0 && page_size > 0 && slots > 0 && max_pages > 0 && kv_heads > 0 && seqs >= 0 && seqs <= 65535 && width >= 0 && width <= 1 << 30 && weights_ld >= 0,
+    PGK_REQUIRE(n_arrays >= 0 && pages > 0 && page_size > 0 && slots > 0 && max_pages > 0 && kv_heads > 0 && seqs >= 0 && seqs <= 65535 && width >= 0 && width <= PAGED_MOST && weights_ld >= 0,
                 "move_rows failed: %d arrays of %d pages of %d positions, %d slots of %d pages, %d heads, %d sequences", n_arrays, pages, page_size, slots, max_pages, kv_heads, seqs);
     PGK_REQUIRE((long long)pages * kv_heads * page_size <= 0x7fffffffll && (long long)max_pages * page_size <= 0x7fffffffll && kv_heads <= 65535,
                 "move_rows failed: too many rows or heads");

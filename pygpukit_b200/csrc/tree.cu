@@ -155,7 +155,7 @@ extern "C" int pgk_tree_masks(const int32_t* parents, const int32_t* row_starts,
 extern "C" int pgk_accept_tree(const void* logits, long ld, int dtype, int vocab, const int32_t* chosen, const int32_t* tokens, const int32_t* parents, const int32_t* row_starts, int seqs,
                                int total, int max_rows, int32_t* rows, int32_t* counts, int32_t* next_tokens, void* stream) {
     PGK_REQUIRE(seqs >= 0 && total >= 0 && total <= 65535 && max_rows > 0 && max_rows <= 4096, "accept_tree failed: %d sequences of up to %d rows in %d", seqs, max_rows, total);
-    PGK_REQUIRE(chosen || (dtype >= 0 && dtype <= 2 && vocab > 0 && vocab <= 1 << 30 && ld >= vocab), "accept_tree failed: type %d, vocabulary %d in rows of %ld", dtype, vocab, ld);
+    PGK_REQUIRE(chosen || (dtype >= 0 && dtype <= 2 && vocab > 0 && vocab <= PAGED_MOST && ld >= vocab), "accept_tree failed: type %d, vocabulary %d in rows of %ld", dtype, vocab, ld);
     if (seqs == 0) return 0;
     PGK_REQUIRE((logits || chosen || total == 0) && tokens && parents && row_starts && rows && counts && next_tokens, "accept_tree failed: an array is missing");
     const cudaStream_t st = (cudaStream_t)stream;

@@ -24,7 +24,7 @@ from ._common import _st
 from .paged import _index, _is
 
 
-MOST_POSITIONS = 1 << 30          # of a slot's weights or of a list of rows: the kernels count in 32 bits
+MOST_POSITIONS = 2 ** 31 - 2 ** 16          # of a slot's weights or of a list of rows: the kernels count in 32 bits
 
 
 def _pages(name: str, cache: GPUArray, page_table: GPUArray) -> tuple[int, int, int, int, int, int]:

@@ -11,6 +11,7 @@ from .paged import _index, _is
 
 MAX_TREE_ROWS = 4096
 MAX_MASK_WORDS = 1 << 18
+MOST_VOCABULARY = 2 ** 31 - 2 ** 16
 
 
 def _trees(name: str, parents: GPUArray, row_starts: GPUArray, max_rows: int) -> tuple[int, int]:
@@ -66,8 +67,8 @@ def accept_tree(logits: GPUArray, tokens: GPUArray, parents: GPUArray, row_start
         if len(logits._shape) != 2 or logits._shape[0] != T or logits._shape[1] < 1:
             raise ValueError(f"{name}: logits must be [{T}, vocab], got {logits.shape}")
         V = logits._shape[1]
-        if V > 1 << 30:
-            raise ValueError(f"{name}: a vocabulary of {V} (2^30 at most)")
+        if V > MOST_VOCABULARY:
+            raise ValueError(f"{name}: a vocabulary of {V} ({MOST_VOCABULARY} at most)")
     if T > 65535:
         raise ValueError(f"{name}: {T} rows (65535 at most)")
     if out is None:
